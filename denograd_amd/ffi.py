@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libjsgrad_hip.so")
 
 F32, F16, BF16 = 0, 1, 2
 W_F32, W_F16, W_I8, W_NF4 = 0, 1, 2, 3
-PROF_KINDS = {"embed": 0, "rmsnorm": 1, "linear": 2, "qkv_rope": 3, "attn_decode": 4, "ffn_gate": 5, "argmax": 6, "decode_step": 7, "gemm": 8, "attn_prefill": 9, "attn_wo": 10, "read_probe": 11, "sample": 12}
+PROF_KINDS = {"embed": 0, "rmsnorm": 1, "linear": 2, "qkv_rope": 3, "attn_decode": 4, "ffn_gate": 5, "argmax": 6, "decode_step": 7, "gemm": 8, "attn_prefill": 9, "attn_wo": 10, "read_probe": 11, "sample": 12, "paged_rows": 13, "attn_paged": 14}
 
 
 class HipError(RuntimeError):
@@ -23,6 +23,14 @@ class HipError(RuntimeError):
 
 _vp, _i32, _f32, _sz, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
 _pp = C.POINTER(C.c_void_p)
+
+class PagesDesc(C.Structure):
+    """jsgrad_hip_pages_t"""
+    _fields_ = ([(n, C.c_int) for n in ("kind", "n_pages", "page_size", "n_kv_heads", "head_dim", "table_width")]
+                + [(n, C.c_void_p) for n in ("pages_k", "pages_v", "scales_k", "scales_v", "page_table")])
+
+
+_pages = C.POINTER(PagesDesc)    # an instance may be passed as it is
 
 # name -> (argtypes, restype); every entry point declared in include/jsgrad_hip.h
 SIGNATURES: dict[str, tuple[list, object]] = {
@@ -85,6 +93,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "jsgrad_hip_attn_batch_workspace_bytes": ([_i32, _i32, _i32, _i32], _sz),
     "jsgrad_hip_attn_decode_batch": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32], _i32),
     "jsgrad_hip_argmax_rows": ([_vp, _i32, _i32, _vp], _i32),
+    "jsgrad_hip_paged_write": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32], _i32),
+    "jsgrad_hip_paged_read": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp], _i32),
+    "jsgrad_hip_attn_paged_workspace_bytes": ([_i32, _i32, _i32], _sz),
+    "jsgrad_hip_attn_paged": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp], _i32),
     "jsgrad_hip_step_workspace_bytes": ([_i32, _i32, _i32], _sz),
     "jsgrad_hip_decode_step": ([_vp], _i32),
     "jsgrad_hip_step_status": ([_vp, C.POINTER(_i32)], _i32),

@@ -11,6 +11,7 @@ be captured once as a HIP graph (the role TinyJit's symbolic `start_pos` plays a
 from __future__ import annotations
 
 import ctypes as C
+from typing import TYPE_CHECKING
 
 import numpy as np
 
@@ -18,6 +19,9 @@ from . import ffi
 from .ffi import check
 from .nn import Embedding, Linear, RMSNorm, act_code
 from .tensor import Tensor
+
+if TYPE_CHECKING:
+    from .paged import PagedBatch
 
 
 def precompute_freqs_cis(dim: int, end: int, theta: float = 10000.0, dtype: str = "float32", device: str = "HIP") -> Tensor:
@@ -69,6 +73,23 @@ class Attention:
             check(lib.jsgrad_hip_attn_prefill(rows.q.ptr, ck, cv, rows.attn.ptr, bsz, seqlen, start_pos, self.n_heads, self.n_kv_heads, self.head_dim, self.max_context))
         check(lib.jsgrad_hip_gemm(self.wo.kind, self.wo.weight.ptr, sp(self.wo), self.dim, self.n_heads * self.head_dim, rows.attn.ptr, n, out.ptr, residual.ptr))
         return out
+
+    def call_paged(self, xn: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", residual: Tensor, out: Tensor, window: int = 0,
+                   sinks: int = 0) -> Tensor:
+        """The rows of a ragged batch over a paged cache: xn is the normed input; out = residual + wo(attention)."""
+        n = batch.rows
+        self._gemm(self.wq, xn, n, rows.q)
+        self._gemm(self.wk, xn, n, rows.k)
+        self._gemm(self.wv, xn, n, rows.v)
+        batch.write(layer, rows.k, rows.v, rows.q, freqs_cis, self.n_heads)
+        batch.attend(layer, rows.q, self.n_heads, rows.attn, window, sinks)
+        self._gemm(self.wo, rows.attn, n, out, residual)
+        return out
+
+    @staticmethod
+    def _gemm(l: Linear, x: Tensor, n: int, out: Tensor, residual: Tensor | None = None) -> None:
+        check(ffi.load().jsgrad_hip_gemm(l.kind, l.weight.ptr, l.scale.ptr if l.scale is not None else None, l.out_features, l.in_features, x.ptr, n, out.ptr,
+                                         residual.ptr if residual is not None else None))
 
     def call(self, x: Tensor, state: Tensor, freqs_cis: Tensor, norm: RMSNorm, ctx: "_Scratch") -> Tensor:
         """x: the block input row; returns x + wo(attention(norm(x))) in ctx.h2."""
@@ -135,12 +156,21 @@ class TransformerBlock:
 
     def call_rows(self, x: Tensor, bsz: int, seqlen: int, start_pos: int, state: Tensor, freqs_cis: Tensor, rows: "_RowScratch") -> Tensor:
         """TransformerBlock.call (llama.ts:124-127) on x [bsz*seqlen, dim]; the result is written back into x."""
-        n, attend, feed = bsz * seqlen, self.attention.call_rows, self.feed_forward.call_rows
+        n, attend = bsz * seqlen, self.attention.call_rows
         # only the two classes' own methods norm on their way: one of the caller's own, of a class or set on the object, takes its rows normed
         if getattr(attend, "__func__", None) is ATTENTION_ROWS:
             h = attend(x, bsz, seqlen, start_pos, state, freqs_cis, rows, x, rows.h2, self.attention_norm)
         else:
             h = attend(self._normed(x, self.attention_norm, rows, n), bsz, seqlen, start_pos, state, freqs_cis, rows, residual=x, out=rows.h2)
+        return self._feed_rows(h, n, rows, x)
+
+    def call_paged(self, x: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", window: int = 0, sinks: int = 0) -> Tensor:
+        """TransformerBlock.call (llama.ts:124-127) on the rows x of a ragged batch over a paged cache; the result is written back into x."""
+        h = self.attention.call_paged(self._normed(x, self.attention_norm, rows, batch.rows), layer, batch, freqs_cis, rows, x, rows.h2, window, sinks)
+        return self._feed_rows(h, batch.rows, rows, x)
+
+    def _feed_rows(self, h: Tensor, n: int, rows, x: Tensor) -> Tensor:
+        feed = self.feed_forward.call_rows
         if getattr(feed, "__func__", None) is FEED_FORWARD_ROWS:
             return feed(h, n, rows, h, x, self.ffn_norm)
         return feed(self._normed(h, self.ffn_norm, rows, n), n, rows, residual=h, out=x)
@@ -216,6 +246,25 @@ class _RowScratch:
 
     def fits(self, bsz: int, seqlen: int) -> bool:
         return bsz == self.bsz and bsz * seqlen <= self.n
+
+
+class _PagedScratch:
+    """Activations of a call on a paged cache: `rows` rows of `bsz` sequences (grown on demand, never shrunk)."""
+
+    def __init__(self, bsz: int, rows: int, m: "Transformer"):
+        self.bsz, self.n, f16 = bsz, rows, "float16"
+        hd, e = m.dim // m.n_heads, Tensor.empty
+        self.tokens = e((rows,), "int32", m.device)
+        self.h, self.h2, self.xn = (e((rows, m.dim), f16, m.device) for _ in range(3))
+        self.q, self.attn = (e((rows, m.n_heads * hd), f16, m.device) for _ in range(2))
+        self.k, self.v = (e((rows, m.n_kv_heads * hd), f16, m.device) for _ in range(2))
+        self.g = e((rows, m.hidden_dim), f16, m.device)
+        self.last = e((bsz, m.dim), f16, m.device)
+        self.logits = e((bsz, m.vocab_size), f16, m.device)
+        self.next_tokens = e((bsz,), "int32", m.device)
+
+    def fits(self, bsz: int, rows: int) -> bool:
+        return bsz <= self.bsz and rows <= self.n
 
 
 class _FusedStep:
@@ -325,6 +374,8 @@ class Transformer:
         self.fuse_attn_wo = fuse_attn_wo   # attention and wo of a layer as one launch, where the model qualifies
         self._fused: _FusedStep | None = None
         self._rows: _RowScratch | None = None
+        self._paged: _PagedScratch | None = None
+        self._paged_rope: Tensor | None = None
         # sampling (llama.ts:131-185): (temperature, top_k, top_p, alpha_f, alpha_p) of the current calls; greedy until told otherwise
         self._sampling = (0.0, 0, 0.0, 0.0, 0.0)
         self.alpha_counter: Tensor | None = None      # llama.ts:130: created on the first call with alpha_f or alpha_p (module-wide in the reference)
@@ -559,6 +610,48 @@ class Transformer:
             check(lib.jsgrad_hip_gemm_norm(out.kind, out.weight.ptr, out.scale.ptr if out.scale is not None else None, self.vocab_size, self.dim, last.ptr,
                                            self.norm.weight.ptr, self.norm.eps, rows.xn.ptr, bsz, rows.logits.ptr))
             check(lib.jsgrad_hip_argmax_rows(rows.logits.ptr, bsz, self.vocab_size, rows.next_tokens.ptr))
+        return Tensor(buffer=rows.next_tokens.lazydata.view(bsz, "int32", 0), shape=(bsz,), dtype="int32", device=self.device)
+
+    def forward_paged(self, cache, seqs, tokens, window: int = 0, sinks: int = 0) -> Tensor:
+        """Transformer.forward (llama.ts:201-213) for sequences of different lengths over a PagedCache: tokens[i] are the next token ids of sequence
+        seqs[i], a prompt, a part of one, or the one token that the call before returned.  Returns the greedy next token of every sequence, an int32
+        tensor in the order of seqs (Tensor.argmax of each, as forward_rows for several sequences).  window, sinks: as PagedBatch.attend has them.
+        A row of the model's own contiguous cache is neither read nor written.  fp16 activations; fp16 / int8 / NF4 weights."""
+        lib = ffi.load()
+        if self.dtype != "float16":
+            raise NotImplementedError("a paged cache is built for fp16 activations; float32 models take one position per call")
+        toks = [np.asarray(t, np.int32).reshape(-1) for t in tokens]
+        seqs = list(seqs)
+        if len(toks) != len(seqs) or any(t.size == 0 for t in toks):
+            raise ValueError(f"{len(seqs)} sequences take {len(seqs)} arrays of one token and more")
+        flat = np.concatenate(toks) if toks else np.zeros(0, np.int32)
+        if flat.size and (flat.min() < 0 or flat.max() >= self.vocab_size):
+            raise ValueError(f"token outside the vocabulary of {self.vocab_size}")
+        hd = self.dim // self.n_heads
+        if (cache.n_layers, cache.n_kv_heads, cache.head_dim) != (len(self.layers), self.n_kv_heads, hd):
+            raise ValueError(f"a cache of {cache.n_layers} layers of {cache.n_kv_heads} heads of {cache.head_dim}, the model has {len(self.layers)} of {self.n_kv_heads} of {hd}")
+        if any(cache.lengths[s] + t.size > 2 * self.max_context for s, t in zip(seqs, toks)):
+            raise ValueError(f"positions beyond {2 * self.max_context}, where the rotary table ends")
+        batch = cache.begin(seqs, [t.size for t in toks])
+        n, bsz = batch.rows, len(seqs)
+        if self._paged_rope is None or self._paged_rope.shape[1] < batch.width * cache.page_size:
+            # the table reaches to the end of the last page of any sequence that may come
+            self._paged_rope = precompute_freqs_cis(hd, 2 * self.max_context + cache.page_size, self.rope_theta, self.dtype, self.device)
+        if self._paged is None or not self._paged.fits(bsz, n):
+            self._paged = _PagedScratch(bsz, n, self)
+        rows, sp = self._paged, lambda l: l.scale.ptr if l.scale is not None else None
+        rows.tokens.lazydata.view(n, "int32", 0).ensure_allocated().copyin(flat)
+        emb = self.tok_embeddings
+        from .nn import _KIND
+        check(lib.jsgrad_hip_embed_rows(_KIND[emb.weight.dtype], emb.weight.ptr, sp(emb), rows.tokens.ptr, n, rows.h.ptr, self.dim, self.vocab_size))
+        for i, layer in enumerate(self.layers):
+            layer.call_paged(rows.h, i, batch, self._paged_rope, rows, window, sinks)
+        last = np.cumsum([t.size for t in toks]) - 1
+        for b in range(bsz):
+            check(lib.jsgrad_hip_copy(rows.last.ptr + b * self.dim * 2, rows.h.ptr + int(last[b]) * self.dim * 2, self.dim * 2))
+        out = self.output
+        check(lib.jsgrad_hip_gemm_norm(out.kind, out.weight.ptr, sp(out), self.vocab_size, self.dim, rows.last.ptr, self.norm.weight.ptr, self.norm.eps, rows.xn.ptr, bsz, rows.logits.ptr))
+        check(lib.jsgrad_hip_argmax_rows(rows.logits.ptr, bsz, self.vocab_size, rows.next_tokens.ptr))
         return Tensor(buffer=rows.next_tokens.lazydata.view(bsz, "int32", 0), shape=(bsz,), dtype="int32", device=self.device)
 
     def rows_logits(self) -> Tensor:

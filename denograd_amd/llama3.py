@@ -328,6 +328,26 @@ class Llama3:
         self.start_pos = pos
         return hist.numpy().T.copy()
 
+    def generate_paged(self, prompts, n_new: int, dtype: str = "float16", page_size: int = 64, window: int = 0, sinks: int = 0) -> np.ndarray:
+        """Prompts of any lengths at once, greedily, over a paged cache made for them: fp16 pages, or int8 ones of half the size.  With a window a
+        sequence keeps the pages that it still sees.  Returns int32 [number of prompts, n_new]."""
+        from .paged import PagedCache
+        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        if not prompts or any(p.size == 0 for p in prompts) or n_new < 1:
+            raise ValueError("one prompt and one new token at least, and no empty prompt")
+        m = self.model
+        n_pages = sum(-(-(p.size + n_new - 1) // page_size) for p in prompts)
+        cache = PagedCache(len(m.layers), m.n_kv_heads, m.dim // m.n_heads, n_pages, page_size, dtype, self.device)
+        seqs = [cache.add() for _ in prompts]
+        out, toks = np.empty((len(prompts), n_new), np.int32), prompts
+        for i in range(n_new):
+            toks = m.forward_paged(cache, seqs, toks, window, sinks).numpy()
+            out[:, i] = toks
+            if window:
+                for s in seqs:
+                    cache.slide(s, window, sinks)
+        return out
+
     def generate(self, prompt, n_new: int) -> np.ndarray:
         """Token-serial prefill, then n_new greedy tokens with the token fed back on the device (no per-token host
         sync); one read of the token history at the end."""

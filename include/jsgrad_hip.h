@@ -101,7 +101,7 @@ int jsgrad_hip_event_destroy(void *event);
 /* Per-kernel statistics (DEBUG>=2 of engine/realize.ts:168-178; ProfileRangeEvent, runtime/allocator.ts:147-151):
  * while enabled, every Llama kernel launched outside a graph capture is bracketed by an event pair.  `read` waits
  * for the stream and returns launch count and summed milliseconds of one kind since profiling was enabled. */
-enum { JSGRAD_PROF_EMBED = 0, JSGRAD_PROF_RMSNORM, JSGRAD_PROF_LINEAR, JSGRAD_PROF_QKV_ROPE, JSGRAD_PROF_ATTN, JSGRAD_PROF_FFN_GATE, JSGRAD_PROF_ARGMAX, JSGRAD_PROF_STEP, JSGRAD_PROF_GEMM, JSGRAD_PROF_ATTN_PREFILL, JSGRAD_PROF_ATTN_WO, JSGRAD_PROF_READ, JSGRAD_PROF_SAMPLE };
+enum { JSGRAD_PROF_EMBED = 0, JSGRAD_PROF_RMSNORM, JSGRAD_PROF_LINEAR, JSGRAD_PROF_QKV_ROPE, JSGRAD_PROF_ATTN, JSGRAD_PROF_FFN_GATE, JSGRAD_PROF_ARGMAX, JSGRAD_PROF_STEP, JSGRAD_PROF_GEMM, JSGRAD_PROF_ATTN_PREFILL, JSGRAD_PROF_ATTN_WO, JSGRAD_PROF_READ, JSGRAD_PROF_SAMPLE, JSGRAD_PROF_PAGED_ROWS, JSGRAD_PROF_ATTN_PAGED };
 int jsgrad_hip_profile(int enable);
 int jsgrad_hip_profile_read(int kind, int *host_out_count, double *host_out_total_ms);
 
@@ -255,6 +255,53 @@ int jsgrad_hip_attn_decode_batch(const void *q, const void *cache_k, const void 
 
 /* Tensor.argmax (tensor.ts:2314-2320) of every row of logits[rows][n]: tokens_out[rows]. */
 int jsgrad_hip_argmax_rows(const void *logits, int rows, int n, int32_t *tokens_out);
+
+/* ---------------------------------------------------------------------------------
+ * A paged KV cache and ragged batches: sequences of different lengths, each with its own number of new rows (a prompt or a part
+ * of one, one token, none), over pages of a pool.  Stands beside the contiguous cache of the calls above (models/llama.ts:61-97);
+ * pages, their int8 form, windows and sinks have no counterpart in the reference.  fp16 activations.
+ *
+ * A page holds page_size positions (a power of two from 16 to 256) of every kv head of one layer:
+ *   pages_k, pages_v   [n_pages][n_kv_heads][page_size][head_dim], fp16 or int8 (kind JSGRAD_W_F16 / JSGRAD_W_I8), 16-byte aligned
+ *   scales_k, scales_v float [n_pages][n_kv_heads][page_size] of int8 pages, 16-byte aligned: a row is code * scale; NULL for fp16
+ *   page_table         int32 [n_seqs][table_width]: the page of positions [i * page_size, (i + 1) * page_size) of the batch's sequence
+ * An entry that is no page of the pool (below 0, or n_pages and more) is a page that is not there: nothing is written to its positions and
+ * no query sees them, so that pages behind a window may be given away.  head_dim is 64 or 128.
+ *
+ * The batch: row_starts int32 [n_seqs + 1], rising from 0, and lengths int32 [n_seqs]: row i of the n = row_starts[b + 1] - row_starts[b]
+ * rows of sequence b is its position lengths[b] - n + i (lengths count the new rows).  `rows`: how many rows q, k, v and the outputs have;
+ * those behind row_starts[n_seqs] are left as they are.  These arrays and the table are read on the device: a captured graph replays with
+ * what they hold then.  No entry of them makes a call leave its buffers, and rows at positions below 0 or behind the table are neither
+ * written nor rotated, and see what the table has before them.
+ * --------------------------------------------------------------------------------- */
+typedef struct {
+  int kind, n_pages, page_size, n_kv_heads, head_dim, table_width;
+  void *pages_k, *pages_v, *scales_k, *scales_v;
+  const int32_t *page_table;
+} jsgrad_hip_pages_t;
+
+/* apply_rotary_emb + KV-cache assign (models/llama.ts:17-32,61-87) for the batch's rows of k and v [rows][n_kv_heads][head_dim] and of
+ * q [rows][n_heads][head_dim], whose rotated rows go to q_out (may be q; both NULL: no queries).  rope_table: [rope_rows][head_dim/2][2] as
+ * jsgrad_hip_rope_table makes it, of at least table_width * page_size positions; NULL: no rotation.  Sums are float.  int8 pages: scale =
+ * max |x| / 127 of a position's row of one head, code = rint(x / scale); a row of zeros has scale 1, one with a value that is not finite reads as
+ * NaN.  Two rows of a batch on one place of one page: either may be the one that stays. */
+int jsgrad_hip_paged_write(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q,
+                           const void *k, const void *v, const void *rope_table, int rope_rows, void *q_out, int n_heads);
+
+/* The batch's rows out of the pages: k_out, v_out [rows][n_kv_heads][head_dim], RN16(code * scale) of int8 pages, zeros where there is no
+ * page.  A whole sequence: as many rows as positions. */
+int jsgrad_hip_paged_read(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, void *k_out, void *v_out);
+
+/* scaled_dot_product_attention (tensor.ts:3920-3934) of the batch's rows q [rows][n_heads][head_dim] over the pages, grouped-query: the row at
+ * position p sees the positions j <= p that have a page and, with window > 0, j > p - window or j < sinks (the last `window` of them and the first
+ * `sinks`).  out [rows][n_heads][head_dim], not q; zeros for a row that sees nothing.  What a row does not see does not reach its result, also where
+ * it is not a number.  int8 pages count as code * scale in float.
+ * workspace: jsgrad_hip_attn_paged_workspace_bytes() bytes, 16-byte aligned, zero-filled once before first use; any number of calls of these heads,
+ * captured ones among them, may have the same one (they are ordered by the library's stream).  Results do not depend on the order in which
+ * blocks run.  The sizes of a batch alone, not of the sequences in it, decide which kernel runs: a row's sums may come in another order in another batch. */
+size_t jsgrad_hip_attn_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
+int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out,
+                          int n_heads, int window, int sinks, void *workspace);
 
 /* ---------------------------------------------------------------------------------
  * The whole decode step as ONE kernel.

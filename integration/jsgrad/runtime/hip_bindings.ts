@@ -66,6 +66,10 @@ const SYMBOLS = {
   jsgrad_hip_attn_batch_workspace_bytes: { parameters: [I, I, I, I], result: U }, // batch, n_heads, n_kv_heads, head_dim
   jsgrad_hip_attn_decode_batch: { parameters: [P, P, P, P, P, P, I, I, I, I, I], result: I }, // q, cache_k, cache_v, state, out, workspace, batch, n_heads, n_kv_heads, head_dim, max_context
   jsgrad_hip_argmax_rows: { parameters: [P, I, I, P], result: I }, // logits, rows, n, tokens_out
+  jsgrad_hip_paged_write: { parameters: [B, P, P, I, I, P, P, P, P, I, P, I], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, k, v, rope_table, rope_rows, q_out, n_heads
+  jsgrad_hip_paged_read: { parameters: [B, P, P, I, I, P, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, k_out, v_out
+  jsgrad_hip_attn_paged_workspace_bytes: { parameters: [I, I, I], result: U }, // n_heads, n_kv_heads, head_dim
+  jsgrad_hip_attn_paged: { parameters: [B, P, P, I, I, P, P, I, I, I, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, out, n_heads, window, sinks, workspace
   jsgrad_hip_step_workspace_bytes: { parameters: [I, I, I], result: U }, // n_heads, n_kv_heads, head_dim
   jsgrad_hip_decode_step: { parameters: [B], result: I }, // host_desc
   jsgrad_hip_step_status: { parameters: [P, B], result: I }, // workspace, host_out_error
@@ -107,7 +111,7 @@ export const check = (rc: number): void => {
 // include/jsgrad_hip.h: activation dtypes, weight formats, cast sources, profile kinds
 export const JSGRAD_F32 = 0, JSGRAD_F16 = 1, JSGRAD_BF16 = 2
 export const JSGRAD_W_F32 = 0, JSGRAD_W_F16 = 1, JSGRAD_W_I8 = 2, JSGRAD_W_NF4 = 3
-export const PROF = ['EMBED', 'RMSNORM', 'LINEAR', 'QKV_ROPE', 'ATTN', 'FFN_GATE', 'ARGMAX', 'STEP', 'GEMM', 'ATTN_PREFILL', 'ATTN_WO', 'READ', 'SAMPLE'] as const
+export const PROF = ['EMBED', 'RMSNORM', 'LINEAR', 'QKV_ROPE', 'ATTN', 'FFN_GATE', 'ARGMAX', 'STEP', 'GEMM', 'ATTN_PREFILL', 'ATTN_WO', 'READ', 'SAMPLE', 'PAGED_ROWS', 'ATTN_PAGED'] as const
 
 /** A device address as the number Deno's FFI passes for `pointer` parameters. */
 export type DevPtr = bigint
@@ -139,6 +143,20 @@ export type StepDesc = {
   tokens_cap: number
   h: DevPtr, h2: DevPtr, q: DevPtr, attn: DevPtr, g: DevPtr, logits: DevPtr
   workspace: DevPtr, trace?: DevPtr
+}
+export const PAGES_BYTES = 64
+export type PagesDesc = {
+  kind: number, n_pages: number, page_size: number, n_kv_heads: number, head_dim: number, table_width: number
+  pages_k: DevPtr, pages_v: DevPtr, scales_k?: DevPtr, scales_v?: DevPtr, page_table: DevPtr
+}
+/** The host descriptor handed to jsgrad_hip_paged_write / jsgrad_hip_paged_read / jsgrad_hip_attn_paged. */
+export const pack_pages = (d: PagesDesc): Uint8Array => {
+  const buf = new ArrayBuffer(PAGES_BYTES), v = new DataView(buf)
+  const ints = [d.kind, d.n_pages, d.page_size, d.n_kv_heads, d.head_dim, d.table_width]                                            // 0..24
+  for (let i = 0; i < ints.length; i++) v.setInt32(4 * i, ints[i], true)
+  const ptrs = [d.pages_k, d.pages_v, d.scales_k, d.scales_v, d.page_table]                                                        // 24..64
+  for (let i = 0; i < ptrs.length; i++) v.setBigUint64(24 + 8 * i, ptrs[i] ?? 0n, true)
+  return new Uint8Array(buf)
 }
 export const STEP_BYTES = 200
 /** The host descriptor handed to jsgrad_hip_decode_step / jsgrad_hip_stream_step. */
