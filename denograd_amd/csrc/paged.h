@@ -2,7 +2,7 @@
 // a host compiler takes it too (tests/test_paged_plan.py walks it over batches and tables with anything in them).
 //
 // row_starts, lengths and page_table are device memory that the host does not look at.  Whatever they hold, no address outside the buffers is made
-// of it: first rows are brought into [0, rows], a negative length counts as zero, and a position whose table entry is no page of the pool, or that
+// of it: first rows are brought into [0, rows], lengths into [0, 2^30], and a position whose table entry is no page of the pool, or that
 // lies behind the table, has no page: nothing is written there and no query sees it.
 #pragma once
 #include <stdint.h>
@@ -28,7 +28,7 @@ JSG_BOTH PagedSeq paged_seq(int start, int end, int len, int rows) {
   PagedSeq s;
   s.start = paged_clamp(start, 0, rows);
   s.n = paged_clamp(end, s.start, rows) - s.start;
-  s.len = len < 0 ? 0 : len;
+  s.len = paged_clamp(len, 0, 1 << 30);  // no table has more positions
   return s;
 }
 JSG_BOTH PagedSeq paged_seq(const PagedBatch &p, int b) { return paged_seq(p.row_starts[b], p.row_starts[b + 1], p.lengths[b], p.rows); }
@@ -44,6 +44,44 @@ JSG_BOTH int paged_page(const PagedBatch &p, int b, int pos) {
 // row of pages_k / pages_v ([n_pages][n_kv_heads][page_size] rows of head_dim) of a position on that page; scales have one value per row
 JSG_BOTH size_t paged_row(const PagedBatch &p, int n_kv_heads, int id, int g, int pos) {
   return (((size_t)id * n_kv_heads + g) << p.page_shift) + (size_t)(pos & ((1 << p.page_shift) - 1));
+}
+
+
+// ---- the work of an attention launch
+constexpr int PAGED_KEYS = 64;           // keys of a tile
+// Key tiles that rows at positions p_lo .. p_hi look at: [0, n_sink), then from t_lo on, n in all.
+struct PagedKeys {
+  int n_sink, t_lo, n;
+  JSG_BOTH int tile(int i) const { return i < n_sink ? i : t_lo + (i - n_sink); }
+};
+JSG_BOTH PagedKeys paged_keys(int p_lo, int p_hi, int room, int window, int sinks) {
+  PagedKeys k = {0, 0, 0};
+  const int hi = p_hi < room ? p_hi : room - 1, t_end = hi < 0 ? 0 : hi / PAGED_KEYS + 1;
+  if (window > 0 && p_lo >= window) k.t_lo = (p_lo - window + 1) / PAGED_KEYS;
+  if (window > 0 && sinks > 0) k.n_sink = paged_clamp((sinks - 1) / PAGED_KEYS + 1, 0, k.t_lo < t_end ? k.t_lo : t_end);
+  k.n = k.n_sink + (t_end > k.t_lo ? t_end - k.t_lo : 0);
+  return k;
+}
+// A sequence's share of a launch with blocks of q_rows (row, query head) pairs, the heads of a kv head side by side: q tiles, and the key tiles of the last one.
+struct PagedShare {
+  int q_tiles, key_tiles;
+};
+// rows * n_rep is below 2^30; div: x / n_rep
+template <typename Div> JSG_BOTH PagedShare paged_share(const PagedSeq &s, int n_rep, Div div, int q_rows, int room, int window, int sinks) {
+  PagedShare h;
+  h.q_tiles = (s.n * n_rep + q_rows - 1) / q_rows;
+  h.key_tiles = s.n > 0 ? paged_keys(paged_pos(s, div((h.q_tiles - 1) * q_rows)), paged_pos(s, s.n - 1), room, window, sinks).n : 0;
+  return h;
+}
+// Key tiles of a part where all parts of a launch have about the same: the launch's (q tile, key tile) pairs over `blocks`.  Items of key_tiles > target are cut into
+// ceil(key_tiles / target) parts and fewer, so that all parts of cut items together are fewer than 2 * blocks: each takes at least half a target's pairs.
+JSG_BOTH int paged_target(float pairs, int blocks, int least) {
+  const float t = pairs * (1.0001f / (float)blocks);           // a little more than the share, whatever the rounding of the sum
+  return t < (float)least ? least : t < 1e9f ? (int)t + 1 : 1000000000;
+}
+JSG_BOTH int paged_parts(int key_tiles, int target, int most) {
+  const int n = key_tiles <= target ? 1 : (key_tiles + target - 1) / target;
+  return n > most ? (most < 1 ? 1 : most) : n;
 }
 
 }  // namespace jsg

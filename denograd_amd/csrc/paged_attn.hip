@@ -3,6 +3,8 @@
 // Row i of a sequence sits at position p and sees the keys j <= p that have a page and, with a window, are among the last `window` of them or
 // among the first `sinks`: out = sum_j softmax_j(q . K_j / sqrt(HD)) V_j, zeros where it sees none.  Reference semantics of the sum:
 // scaled_dot_product_attention (/root/reference/jsgrad/tensor.ts:3920-3934); windows, sinks and pages have no counterpart there.
+#include <type_traits>
+
 #include "gemm.h"
 #include "paged.h"
 
@@ -16,57 +18,435 @@ struct PagedAttnArgs {
   const float *scales_k, *scales_v;
   const _Float16 *q;                     // [rows][H][HD]
   _Float16 *out;
-  int n_heads, n_kv_heads, window, sinks;
+  int n_heads, window, sinks;
+  Divisor n_rep, n_kv_heads;
   float scale_log2;                      // float(1 / sqrt(HD)) * log2(e)
+  int *counters;                         // zero, and zero again afterwards
+  float *ws;
 };
 
-// One wavefront per (row, query head): 64 keys at a time, a lane's score each, then their weighted V rows with a lane's features each.
-template <int HD, bool I8> __global__ __launch_bounds__(64) void attn_paged_kernel(PagedAttnArgs a) {
-  constexpr int F = HD / 64;
-  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, g = h / (a.n_heads / a.n_kv_heads);
-  int b = 0;
-  while (b < a.pb.n_seqs && a.pb.row_starts[b + 1] <= r) b++;
-  if (b >= a.pb.n_seqs) return;
-  const PagedSeq s = paged_seq(a.pb, b);
-  if (r < s.start) return;
-  const int p = paged_pos(s, r - s.start), top = min(p, paged_room(a.pb) - 1);
-  const size_t at = ((size_t)r * a.n_heads + h) * HD;
-  float m = -INFINITY, l = 0.0f, o[F];
-#pragma unroll
-  for (int f = 0; f < F; f++) o[f] = 0.0f;
-  for (int j0 = 0; j0 <= top; j0 += 64) {
-    const int j = j0 + lane;
-    const int id = j <= top && (a.window == 0 || j > p - a.window || j < a.sinks) ? paged_page(a.pb, b, j) : -1;
-    const size_t row = id >= 0 ? paged_row(a.pb, a.n_kv_heads, id, g, j) : 0;
-    float x = -INFINITY;
-    if (id >= 0) {
-      float sum = 0.0f;
-      for (int e = 0; e < HD; e++) {
-        const float kv = I8 ? (float)((const int8_t *)a.pages_k)[row * HD + e] : (float)((const _Float16 *)a.pages_k)[row * HD + e];
-        sum = fmaf((float)a.q[at + e], kv, sum);
-      }
-      x = sum * a.scale_log2 * (I8 ? a.scales_k[row] : 1.0f);
+// ---------------------------------------------------------------- which work a block has
+//
+// A launch's items are (sequence, q tile, kv head); a q tile is QROWS (position, query head) pairs of a kv head, row = position * n_rep + head.  Long
+// ones are cut along the keys, so that the parts of a launch have about the same number of key tiles whatever the lengths of its sequences are
+// (paged_target).  The host knows neither lengths nor row starts: every wavefront goes over them, a sequence to a lane, and finds its block's item.
+// Block numbers have the kv heads innermost: blocks are dealt to the eight XCDs in turn, so that with eight kv heads each XCD has one, all q tiles of which
+// share its K and V in that L2, and all XCDs have the same work.  The q tiles with the most keys come first within a sequence.
+struct PagedItem {
+  PagedSeq s;
+  int b, g, qt, part, parts, slot;       // slot: of part 0 in the workspace; part p's is slot + p * n_kv_heads
+};
+constexpr uint32_t PAGED_MOST = 1u << 29;  // more blocks than a launch has: sums stop there instead of wrapping
+
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {     // inclusive prefix sums over the lanes, saturating
+  auto add = [&](uint32_t o) { v = min(v + o, PAGED_MOST); };
+  add((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true));    // row_shr
+  add((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true));
+  add((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true));
+  add((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true));
+  add((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));   // row_bcast 15
+  add((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));   // row_bcast 31
+  return v;
+}
+
+// blocks: how many parts a launch is to have at least; least: key tiles of a part.  False: no item has this block.
+template <int QROWS> __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, int blocks, int least, PagedItem &it) {
+  const int lane = threadIdx.x & 63, room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
+  const uint32_t want = (uint32_t)a.n_kv_heads.div((int)blockIdx.x);
+  it.g = (int)blockIdx.x - (int)want * KV;
+  PagedSeq s;
+  PagedShare h;
+  auto look = [&](int b0) {
+    const int b = b0 + lane;
+    s = {0, 0, 0};
+    h = {0, 0};
+    if (b < a.pb.n_seqs) {
+      s = paged_seq(a.pb, b);
+      h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
     }
-    const float mx = fmaxf(m, wave_max(x));
-    if (mx == -INFINITY && __builtin_amdgcn_ballot_w64(id >= 0) == 0) continue;
-    const float w = id >= 0 ? __builtin_amdgcn_exp2f(x - mx) : 0.0f, f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
-    m = mx;
-    l = l * f0 + wave_sum(w);
-#pragma unroll
-    for (int f = 0; f < F; f++) o[f] *= f0;
-    for (int u = 0; u < 64; u++) {
-      if (__builtin_amdgcn_readlane(id, u) < 0) continue;
-      const float wu = readlane_f(w, u);
-      const size_t ru = ((size_t)(uint32_t)__builtin_amdgcn_readlane((int)(row >> 32), u) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, u);
-#pragma unroll
-      for (int f = 0; f < F; f++) {
-        const size_t e = ru * HD + f * 64 + lane;
-        o[f] = fmaf(wu, I8 ? (float)((const int8_t *)a.pages_v)[e] * a.scales_v[ru] : (float)((const _Float16 *)a.pages_v)[e], o[f]);
+  };
+  float pairs = 0.0f;
+  for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
+    look(b0);
+    pairs += (float)h.q_tiles * (float)h.key_tiles;
+  }
+  const int target = paged_target(wave_sum(pairs) * (float)KV, blocks, least);
+  uint32_t before = 0, slots = 0;
+  for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
+    if (a.pb.n_seqs > 64) look(b0);
+    const int parts = paged_parts(h.key_tiles, target, (int)__builtin_amdgcn_sqrtf((float)h.key_tiles));
+    const uint32_t mine = (uint32_t)min((uint64_t)h.q_tiles * parts, (uint64_t)PAGED_MOST);
+    const uint32_t upto = scan64(mine), cut = scan64(parts > 1 ? mine : 0);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(before + upto > want);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      it.b = b0 + l;
+      it.s = {of(s.start), of(s.n), of(s.len)};
+      it.parts = of(parts);
+      const int nth = (int)(want - before) - of((int)(upto - mine));
+      it.part = 0;
+      it.qt = of(h.q_tiles) - 1 - nth;
+      if (it.parts > 1) {
+        it.qt = of(h.q_tiles) - 1 - nth / it.parts;
+        it.part = nth % it.parts;
       }
+      it.slot = ((int)slots + of((int)(cut - (parts > 1 ? mine : 0))) + nth - it.part) * KV + it.g;
+      return true;
     }
+    before = min(before + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), PAGED_MOST);
+    slots = min(slots + (uint32_t)__builtin_amdgcn_readlane((int)cut, 63), PAGED_MOST);
+  }
+  return false;
+}
+
+// ---------------------------------------------------------------- chunks of new rows
+//
+// Block = 4 wavefronts = 128 (position, query head) pairs of one kv head of one sequence, keys in tiles of 64, as attn_prefill_kernel (prefill.hip) has it:
+// scores transposed, S^T = K . Q^T, so that a lane holds 32 scores of one query row per tile and its fp16 weights lie as the operand of O^T = V^T . P^T
+// wants them; V^T fragments by transposing LDS reads; one barrier per tile, tile t + 1 being asked for behind the barrier of tile t.
+// A page has 16 rows at least: the 16 rows of a tile that a wavefront brings lie on one page, whose number it asks for a tile ahead.
+// fp16 pages come by direct global-to-LDS loads.  int8 ones come through registers and become halves on their way into LDS (exact), once for the block;
+// K's scale multiplies the scores.  V's scale goes into the exponent, weight = exp2(score + log2(scale) - maximum of that), so that what is rounded to fp16 is at
+// most 1 and the largest contributions keep their bits whatever the scales are; the sum of the weights takes it out again, in float.
+// Tiles that hold keys which some row of the wavefront does not see (the diagonal, a window's edge, a missing page) take their V through a test: halves that are not
+// finite are left out of the product, where a weight of zero would not stop them, and added for the rows that see them.
+constexpr int PC_THREADS = 256, PC_QROWS = 128;
+constexpr int PC_BLOCKS = 512, PC_LEAST = 8;               // two blocks to a compute unit; a tile takes 0.8 us and folding a part as long
+constexpr int PC_SLOTS = 2 * PC_BLOCKS;
+
+template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn_paged_chunk_kernel(PagedAttnArgs a) {
+  constexpr int ROWB = HD * 2, PPR = HD / 8;                 // bytes and 16-byte pieces of a row of halves
+  constexpr int TILE = PAGED_KEYS * ROWB, BUF = 2 * TILE;    // K tile, then V tile
+  constexpr int LOADS = TILE / 1024 / 4;                     // a wavefront's loads per tile of K, and of V
+  constexpr int RPL = 64 / PPR;                              // rows per load
+  constexpr int NT = HD / 32;                                // 32-feature tiles of the output
+  constexpr int CPT = HD / 64;                               // 16-byte pieces of codes per thread and tile of K, and of V
+  __shared__ __align__(16) unsigned char lds[2 * BUF];
+  __shared__ __align__(16) float scl[2][3][PAGED_KEYS];      // I8: K's scale times scale_log2, log2 and reciprocal of V's
+  __shared__ __align__(16) int here[2][4];                   // whether the page of 16 rows is there
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lg = lane >> 5;
+  PagedItem it;
+  if (!paged_item<PC_QROWS>(a, PC_BLOCKS, PC_LEAST, it)) return;
+  const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d, room = paged_room(a.pb), g = it.g;
+  const int rows = it.s.n * n_rep, p0 = paged_pos(it.s, 0), q0 = it.qt * PC_QROWS, qw0 = q0 + wave * 32;
+  const PagedKeys keys = paged_keys(p0 + a.n_rep.div(q0), p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1), room, a.window, a.sinks);
+  int i_lo = 0, i_hi = keys.n;
+  if (it.parts > 1) {
+    const int per = (keys.n + it.parts - 1) / it.parts;
+    i_lo = min(it.part * per, keys.n);
+    i_hi = min(i_lo + per, keys.n);
+  }
+  // this wavefront's first and last position; rows past the end repeat the last one and are never stored
+  const int pos_lo = p0 + a.n_rep.div(min(qw0, rows - 1)), pos_hi = p0 + a.n_rep.div(min(qw0 + 31, rows - 1));
+  const bool q_valid = qw0 + l32 < rows;
+  const int qrow = min(qw0 + l32, rows - 1), qs = a.n_rep.div(qrow), qpos = p0 + qs;
+  const size_t q_off = ((size_t)(it.s.start + qs) * a.n_heads + g * n_rep + qrow - qs * n_rep) * HD;
+  const int sees_from = a.window ? qpos - a.window : -1, sees_to = a.window ? a.sinks : 0;   // keys <= qpos that are > sees_from or < sees_to
+
+  // where piece p of row r of a tile is kept: K by all pieces of a row, V by pairs of pieces (a transposing read takes 32 bytes of eight rows)
+  auto k_at = [](int r, int p) { return HD == 128 ? p ^ (r & 15) : p ^ (r & 7); };
+  auto v_at = [](int r, int p) { return HD == 128 ? p ^ ((r & 7) << 1) : p ^ (((r >> 1) & 3) << 1); };
+
+  // this wavefront's rows of a tile: 16 * wave and on
+  auto page_of = [&](int i) { return i < i_hi ? __builtin_amdgcn_readfirstlane(paged_page(a.pb, it.b, keys.tile(i) * PAGED_KEYS + wave * 16)) : -1; };
+  auto row_of = [&](int i, int id) { return paged_row(a.pb, KV, max(id, 0), g, keys.tile(i) * PAGED_KEYS + wave * 16); };   // a missing page: page 0, masked
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds + wave * LOADS * 1024;
+  const int lrow = lane / PPR, lp = lane % PPR;
+  auto issue = [&](int i, int id, int buf) {                 // fp16
+    const uint32_t to = lds0 + buf * BUF;
+    const size_t at = row_of(i, id) * ROWB;
+    const i4_t rk = dma_rsrc((const unsigned char *)a.pages_k + at), rv = dma_rsrc((const unsigned char *)a.pages_v + at);
+#pragma unroll
+    for (int j = 0; j < LOADS; j++) {
+      const int r = j * RPL + lrow;
+      dma16(rk, (uint32_t)r * ROWB + k_at(wave * 16 + r, lp) * 16, 0, to + j * 1024);
+      dma16(rv, (uint32_t)r * ROWB + v_at(wave * 16 + r, lp) * 16, 0, to + TILE + j * 1024);
+    }
+    if (lane == 0) here[buf][wave] = id >= 0;
+  };
+  u4_t kc[CPT], vc[CPT];                                     // int8: this thread's codes and scale on their way
+  float sc = 1.0f;
+  const int crow = lane >> 2, cp = (lane & 3) * CPT;         // row and first piece of codes
+  auto load = [&](int i, int id) {
+    const size_t row = row_of(i, id);
+#pragma unroll
+    for (int c = 0; c < CPT; c++) {
+      kc[c] = *as_global<u4_t>((const int8_t *)a.pages_k + (row + crow) * HD + (cp + c) * 16);
+      vc[c] = *as_global<u4_t>((const int8_t *)a.pages_v + (row + crow) * HD + (cp + c) * 16);
+    }
+    sc = *as_global<float>((lane & 16 ? a.scales_v : a.scales_k) + row + (lane & 15));
+  };
+  auto store = [&](int id, int buf) {
+    unsigned char *const kt = lds + buf * BUF, *const vt = kt + TILE;
+    const int r = wave * 16 + crow;
+#pragma unroll
+    for (int c = 0; c < CPT; c++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        u4_t k, v;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          uint32_t lo, hi;
+          i8x4_to_h2x2(kc[c][2 * h + e], lo, hi);
+          k[2 * e] = lo; k[2 * e + 1] = hi;
+          i8x4_to_h2x2(vc[c][2 * h + e], lo, hi);
+          v[2 * e] = lo; v[2 * e + 1] = hi;
+        }
+        const int p = (cp + c) * 2 + h;
+        *(u4_t *)(kt + r * ROWB + k_at(r, p) * 16) = k;
+        *(u4_t *)(vt + r * ROWB + v_at(r, p) * 16) = v;
+      }
+    if (lane < 16) scl[buf][0][wave * 16 + lane] = sc * a.scale_log2;
+    else if (lane < 32) {
+      // A scale that is not a number makes the weights so, for the rows that see it.  Its reciprocal meets weights of zero as well, there and where
+      // nothing was ever written, and has to be finite.
+      scl[buf][1][wave * 16 + lane - 16] = __builtin_amdgcn_logf(sc);
+      scl[buf][2][wave * 16 + lane - 16] = sc >= 1e-38f && sc < INFINITY ? 1.0f / sc : 1.0f;
+    }
+    if (lane == 0) here[buf][wave] = id >= 0;
+  };
+
+  int id = page_of(i_lo), id_next = page_of(i_lo + 1);
+  if (i_lo < i_hi) {
+    if constexpr (I8) load(i_lo, id);
+    else issue(i_lo, id, 0);
+  }
+  // query row fragments: chunk c covers features [16c, 16c+16), the lane half picks 8 of them
+  h8_t qf[HD / 16];
+  {
+    const _Float16 *qp = a.q + q_off + lg * 8;
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++) qf[c] = *(const h8_t *)(qp + c * 16);
   }
 #pragma unroll
-  for (int f = 0; f < F; f++) a.out[at + f * 64 + lane] = (_Float16)(l == 0.0f ? 0.0f : o[f] / l);
+  for (int c = 0; c < HD / 16; c++) asm volatile("" : "+v"(qf[c]));   // waited for here, in front of the loop
+  if constexpr (I8)
+    if (i_lo < i_hi) store(id, 0);
+
+  f16_t o_acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o_acc[t][r] = 0.0f;
+  // the maximum starts finite: a part of the keys may hold none that a row sees, and -inf minus -inf is not a number
+  float m_run = -1e30f, l_run = 0.0f;
+  const float unit = I8 ? 1.0f : a.scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
+
+  // K fragment of key l32 (+ 32): chunk 2c + lg of its row; V: lane -> row (lane / 4 % 4) of its half's four keys, 8 bytes
+  const unsigned char *const kp = lds + l32 * ROWB;
+  const int vrow = 4 * lg + ((lane >> 2) & 3), vcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;   // byte column inside 64 (32 features)
+
+  for (int i = i_lo, buf = 0; i < i_hi; i++, buf ^= 1) {
+    if constexpr (!I8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();                                            // tile i is there, everyone is done with tile i - 1
+    id = id_next;
+    if (i + 1 < i_hi) {
+      if constexpr (I8) load(i + 1, id);
+      else issue(i + 1, id, buf ^ 1);
+      id_next = page_of(i + 2);
+    }
+    const int k0 = keys.tile(i) * PAGED_KEYS;
+    // every key of the tile is masked for this wavefront (uniform)
+    if (!(k0 > pos_hi || (a.window && k0 + PAGED_KEYS - 1 <= pos_lo - a.window && k0 >= a.sinks))) {
+      const int4 hv = *(const int4 *)here[buf];
+      const int pm = __builtin_amdgcn_readfirstlane(hv.x | hv.y << 1 | hv.z << 2 | hv.w << 3);
+      const bool masked = k0 + PAGED_KEYS - 1 > pos_lo || pm != 15 || (a.window && k0 <= pos_hi - a.window && k0 + PAGED_KEYS > a.sinks);
+      auto sees = [&](int key) { return key <= qpos && (key > sees_from || key < sees_to); };
+
+      // S^T tile: 64 keys x 32 query rows
+      f16_t s[2];
+#pragma unroll
+      for (int tk = 0; tk < 2; tk++) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[tk][r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+          const h8_t kf = *(const h8_t *)(kp + buf * BUF + tk * 32 * ROWB + k_at(l32, 2 * c + lg) * 16);
+          s[tk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], s[tk], 0, 0, 0);
+        }
+      }
+      // accumulator r of s[tk] is key k0 + tk*32 + 8*(r/4) + 4*lg + r%4 for query row l32
+      f4_t inv_v[2][4];
+      if constexpr (I8) {
+#pragma unroll
+        for (int tk = 0; tk < 2; tk++)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; r4++) {
+            const int at = tk * 32 + 8 * r4 + 4 * lg;
+            const f4_t ks = *(const f4_t *)&scl[buf][0][at], lv = *(const f4_t *)&scl[buf][1][at];
+            inv_v[tk][r4] = *(const f4_t *)&scl[buf][2][at];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[tk][r4 * 4 + e] = __builtin_fmaf(s[tk][r4 * 4 + e], ks[e], lv[e]);
+          }
+      }
+      if (masked) {
+#pragma unroll
+        for (int tk = 0; tk < 2; tk++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int key = k0 + tk * 32 + 8 * (r / 4) + 4 * lg + (r % 4);
+            if (!sees(key) || !(pm >> (tk * 2 + r / 8) & 1)) s[tk][r] = -INFINITY;
+          }
+      }
+      float mx = m_run;
+#pragma unroll
+      for (int tk = 0; tk < 2; tk++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[tk][r]), s[tk][r + 1]);
+      mx = max_xor32(mx);
+      // the sums are rescaled when some row's maximum has moved (uniform branch), so that the largest weight of a row is 1 and its fp16 rounding exact
+      if (__builtin_amdgcn_ballot_w64(mx > m_run)) {
+        const float alpha = __builtin_amdgcn_exp2f((m_run - mx) * unit);   // first visible tile: 0
+        m_run = mx;
+        l_run *= alpha;
+#pragma unroll
+        for (int td = 0; td < NT; td++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
+      }
+      const float mxs = m_run * unit;
+      float psum[2] = {0.0f, 0.0f};
+      h8_t pf[2][2];
+#pragma unroll
+      for (int tk = 0; tk < 2; tk++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const float p = __builtin_amdgcn_exp2f(I8 ? s[tk][r] - mxs : __builtin_fmaf(s[tk][r], unit, -mxs));
+          if constexpr (I8) psum[tk] = __builtin_fmaf(p, inv_v[tk][r / 4][r % 4], psum[tk]);
+          else psum[tk] += p;
+          pf[tk][r / 8][r % 8] = (_Float16)p;
+        }
+      l_run += psum[0] + psum[1];
+
+      // O^T += V^T . P^T : k-slot s' of lane half lg in step (tk, hs) is key tk*32 + hs*16 + 8*(s'/4) + 4*lg + s'%4
+      const unsigned char *const vt = lds + buf * BUF + TILE;
+      auto weigh = [&](auto test) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int tk = 0; tk < 2; tk++)
+#pragma unroll
+          for (int hs = 0; hs < 2; hs++)
+#pragma unroll
+            for (int td = 0; td < NT; td++) {
+              s4_t v[2];
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const int r = tk * 32 + hs * 16 + 8 * e + vrow, c = td * 64 + vcol;
+                v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vt + r * ROWB + v_at(r, c >> 4) * 16 + (c & 15)));
+              }
+              h8_t vf = __builtin_bit_cast(h8_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+              if constexpr (decltype(test)::value) {
+                u4_t w = __builtin_bit_cast(u4_t, vf);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  const uint32_t t = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // the sign bit of halves that are not finite
+                  bad |= t;
+                  w[e] &= ~(t | (t - (t >> 15)));
+                }
+                vf = __builtin_bit_cast(h8_t, w);
+              }
+              o_acc[td] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[tk][hs], o_acc[td], 0, 0, 0);
+            }
+        return bad;
+      };
+      if (!I8 && masked) {
+        if (__builtin_amdgcn_ballot_w64(weigh(std::true_type()) != 0)) {
+          for (int key = 0; key < PAGED_KEYS; key++) {
+            const bool seen = sees(k0 + key) && (pm >> (key >> 4) & 1);
+#pragma unroll
+            for (int td = 0; td < NT; td++)
+#pragma unroll
+              for (int r4 = 0; r4 < 4; r4++) {
+                const uint2 w = *(const uint2 *)(vt + key * ROWB + v_at(key, td * 4 + r4) * 16 + lg * 8);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  const uint32_t h = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
+                  if (seen && (h & 0x7c00u) == 0x7c00u) o_acc[td][r4 * 4 + e] += (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+                }
+              }
+          }
+        }
+      } else {
+        weigh(std::false_type());
+      }
+    }
+    if constexpr (I8)
+      if (i + 1 < i_hi) store(id, buf ^ 1);
+  }
+
+  if (it.parts > 1) {
+    // Sums cross compute units on different XCDs: device-scope stores and loads (cache policy 16), counted once they are
+    // acknowledged (the offset in the vector register, see sum_parts in gemm_tile.hip).
+    constexpr int VALS = (HD / 2 + 4) * 64;                   // floats of one wavefront: O^T, then (m, l)
+    const uint32_t slot = (uint32_t)VALS * 4 * 4, step = (uint32_t)KV * slot;
+    const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.ws + ((size_t)it.slot * 4 + wave) * VALS, (uint32_t)(it.parts - 1) * step + VALS * 4);
+    const uint32_t mine = (uint32_t)it.part * step + lane * 16;
+#pragma unroll
+    for (int td = 0; td < NT; td++)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; r4++) {
+        const f4_t v = {o_acc[td][r4 * 4], o_acc[td][r4 * 4 + 1], o_acc[td][r4 * 4 + 2], o_acc[td][r4 * 4 + 3]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), rw, mine + (td * 4 + r4) * 1024, 0, 16);
+      }
+    const f4_t ml = {m_run, l_run, 0.0f, 0.0f};
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, ml), rw, mine + NT * 4 * 1024, 0, 16);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int old = 0;
+    if (lane == 0) old = __hip_atomic_fetch_add(&a.counters[it.slot * 4 + wave], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    old = __builtin_amdgcn_readfirstlane(old);
+    if (old != it.parts - 1) return;
+    if (lane == 0) __hip_atomic_store(&a.counters[it.slot * 4 + wave], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+    // two parts per round trip; past the last part the last one again, with weight zero
+    m_run = -1e30f;
+    l_run = 0.0f;
+#pragma unroll
+    for (int td = 0; td < NT; td++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o_acc[td][r] = 0.0f;
+    for (int f = 0; f < it.parts; f += 2) {
+      f4_t w[2], v[2][NT * 4];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const uint32_t from = (uint32_t)min(f + u, it.parts - 1) * step + lane * 16;
+        w[u] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + NT * 4 * 1024, 0, 16));
+#pragma unroll
+        for (int j = 0; j < NT * 4; j++) v[u][j] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + j * 1024, 0, 16));
+      }
+      const float m = fmaxf(m_run, fmaxf(w[0][0], w[1][0]));
+      const float e = __builtin_amdgcn_exp2f((m_run - m) * unit);
+      const float e0 = __builtin_amdgcn_exp2f((w[0][0] - m) * unit);   // a part without a visible key: 0
+      const float e1 = f + 1 < it.parts ? __builtin_amdgcn_exp2f((w[1][0] - m) * unit) : 0.0f;
+      m_run = m;
+      l_run = l_run * e + (w[0][1] * e0 + w[1][1] * e1);
+#pragma unroll
+      for (int j = 0; j < NT * 4; j++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) o_acc[j / 4][(j % 4) * 4 + x] = o_acc[j / 4][(j % 4) * 4 + x] * e + (v[0][j][x] * e0 + v[1][j][x] * e1);
+    }
+  }
+
+  const float l = add_xor32(l_run), inv = l == 0.0f ? 0.0f : 1.0f / l;   // 0: the row sees nothing
+  _Float16 *op = a.out + q_off;
+#pragma unroll
+  for (int td = 0; td < NT; td++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      // a lane half holds four of every eight neighbouring features; the halves exchange, so that each has all eight of every other group
+      uint32_t w[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const h2_t h = {(_Float16)(o_acc[td][(2 * j + u) * 4 + 2 * e] * inv), (_Float16)(o_acc[td][(2 * j + u) * 4 + 2 * e + 1] * inv)};
+          w[u][e] = __builtin_bit_cast(uint32_t, h);
+        }
+      const auto lo = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const auto hi = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      const u4_t v = {lo[0], hi[0], lo[1], hi[1]};
+      if (q_valid) *(u4_t *)(op + td * 32 + 16 * j + 8 * lg) = v;
+    }
 }
 
 }  // namespace jsg
@@ -76,8 +456,9 @@ using namespace jsg;
 extern "C" {
 
 size_t jsgrad_hip_attn_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-  (void)n_heads, (void)n_kv_heads, (void)head_dim;
-  return 256;
+  // counters, then the sums of cut items, one slot for every part
+  (void)n_heads, (void)n_kv_heads;
+  return (size_t)PC_SLOTS * 4 * sizeof(int) + (size_t)PC_SLOTS * 4 * (head_dim / 2 + 4) * 64 * sizeof(float);
 }
 
 int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out,
@@ -85,24 +466,35 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   const char *who = "jsgrad_hip_attn_paged";
   PagedAttnArgs a = {};
   if (int e = paged_check(who, host_pages, row_starts, lengths, n_seqs, rows, &a.pb)) return e;
+  const int KV = host_pages->n_kv_heads, HD = host_pages->head_dim;
   JSG_REQUIRE(q && out && workspace, "%s: null pointer argument", who);
   JSG_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)workspace % 16 == 0, "%s: q, out and workspace must be 16-byte aligned", who);
   JSG_REQUIRE(q != out, "%s: out must not be q", who);
-  JSG_REQUIRE(n_heads > 0 && n_heads <= 65535 && n_heads % host_pages->n_kv_heads == 0, "%s: n_heads %d / n_kv_heads %d", who, n_heads, host_pages->n_kv_heads);
+  JSG_REQUIRE(n_heads > 0 && n_heads <= 65535 && n_heads % KV == 0, "%s: n_heads %d / n_kv_heads %d", who, n_heads, KV);
   JSG_REQUIRE(window >= 0 && sinks >= 0, "%s: window %d, sinks %d", who, window, sinks);
+  const int n_rep = n_heads / KV;
+  JSG_REQUIRE((size_t)rows * n_rep < (size_t)1 << 30, "%s: %d rows of %d heads", who, rows, n_heads);
   JSG_READY();
   a.pages_k = host_pages->pages_k; a.pages_v = host_pages->pages_v;
   a.scales_k = (const float *)host_pages->scales_k; a.scales_v = (const float *)host_pages->scales_v;
   a.q = (const _Float16 *)q; a.out = (_Float16 *)out;
-  a.n_heads = n_heads; a.n_kv_heads = host_pages->n_kv_heads;
-  a.window = window; a.sinks = sinks;
-  a.scale_log2 = (float)(1.0 / sqrt((double)host_pages->head_dim)) * 1.4426950408889634f;
-  const dim3 grid(rows, n_heads), block(64);
+  a.n_heads = n_heads;
+  a.n_rep = divisor(n_rep); a.n_kv_heads = divisor(KV);
+  a.window = window < 1 << 30 ? window : 1 << 30;             // no position is further: everything
+  a.sinks = sinks < 1 << 30 ? sinks : 1 << 30;
+  a.scale_log2 = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
+  a.counters = (int *)workspace;
+  a.ws = (float *)((char *)workspace + (size_t)PC_SLOTS * 4 * sizeof(int));
+  const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS;
+  // as many blocks as there may be items and parts: every sequence fills its last q tile at worst, and what is no longer than the least part is not cut
+  const size_t blocks = (size_t)KV * ((size_t)rows * n_rep / PC_QROWS + (n_seqs < rows ? n_seqs : rows)) + (room_tiles > PC_LEAST ? PC_SLOTS : 0);
+  JSG_REQUIRE(blocks < PAGED_MOST, "%s: %d rows of %d heads", who, rows, n_heads);
+  const dim3 grid((unsigned)blocks), block(PC_THREADS);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
-  if (host_pages->head_dim == 64 && i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_kernel<64, true>), grid, block, 0, a);
-  else if (host_pages->head_dim == 64) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_kernel<64, false>), grid, block, 0, a);
-  else if (i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_kernel<128, true>), grid, block, 0, a);
-  else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_kernel<128, false>), grid, block, 0, a);
+  if (HD == 64 && i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<64, true>), grid, block, 0, a);
+  else if (HD == 64) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<64, false>), grid, block, 0, a);
+  else if (i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<128, true>), grid, block, 0, a);
+  else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<128, false>), grid, block, 0, a);
   return 0;
 }
 

@@ -9,9 +9,6 @@
 
 namespace jsg {
 
-typedef float f16_t __attribute__((ext_vector_type(16)));
-typedef short s4_t __attribute__((ext_vector_type(4)));
-
 // ---------------------------------------------------------------- causal attention, S new positions
 //
 // Block = 4 wavefronts = 128 query rows of one kv head of one sequence: its n_rep query heads side by side, row = position *
@@ -34,23 +31,6 @@ typedef short s4_t __attribute__((ext_vector_type(4)));
 constexpr int PF_THREADS = 256, PF_QROWS = 128, PF_KEYS = 64;
 constexpr int PF_COUNTERS = 4096;
 static __device__ int pf_counters[PF_COUNTERS];
-
-// x / d for 0 <= x < 2^30: a division in full is 30 instructions that wait for each other, and a block of a short prompt has eight
-// of them in front of its one tile (57 positions, 24 heads of 128: 5.6 us, 5.5 without).
-struct Divisor {
-  uint32_t d, mul, shift;
-  __device__ int div(int x) const { return mul ? (int)(__umulhi((uint32_t)x, mul) >> shift) : x; }
-};
-static Divisor divisor(uint32_t d) {
-  Divisor r = {d, 0, 0};
-  if (d == 1) return r;
-  int s = 1;
-  while ((1u << s) < d) s++;
-  const int n = s < 2 ? 32 : 30 + s;                          // mul = ceil(2^n / d) <= 2^31, off by less than d <= 2^s
-  r.mul = (uint32_t)((((uint64_t)1 << n) + d - 1) / d);
-  r.shift = n - 32;
-  return r;
-}
 
 struct PrefillAttnArgs {
   const _Float16 *q;                 // [B*S][H*HD]
