@@ -73,8 +73,8 @@ template <typename Div> JSG_BOTH PagedShare paged_share(const PagedSeq &s, int n
   h.key_tiles = s.n > 0 ? paged_keys(paged_pos(s, div((h.q_tiles - 1) * q_rows)), paged_pos(s, s.n - 1), room, window, sinks).n : 0;
   return h;
 }
-// Key tiles of a part where all parts of a launch have about the same: the launch's (q tile, key tile) pairs over `blocks`.  Items of key_tiles > target are cut into
-// ceil(key_tiles / target) parts and fewer, so that all parts of cut items together are fewer than 2 * blocks: each takes at least half a target's pairs.
+// Key tiles of a part where `blocks` parts have the same share of the launch's pairs of a q tile and a key tile.  An item of key_tiles > target, for a target of that and more,
+// is cut into ceil(key_tiles / target) parts or fewer; the parts of cut items are fewer than 2 * blocks, as each has half a target's pairs at least.
 JSG_BOTH int paged_target(float pairs, int blocks, int least) {
   const float t = pairs * (1.0001f / (float)blocks);           // a little more than the share, whatever the rounding of the sum
   return t < (float)least ? least : t < 1e9f ? (int)t + 1 : 1000000000;

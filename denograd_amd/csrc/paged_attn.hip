@@ -20,6 +20,7 @@ struct PagedAttnArgs {
   _Float16 *out;
   int n_heads, window, sinks;
   Divisor n_rep, n_kv_heads;
+  int blocks, least;                     // how the keys are cut: paged_target
   float scale_log2;                      // float(1 / sqrt(HD)) * log2(e)
   int *counters;                         // zero, and zero again afterwards
   float *ws;
@@ -49,8 +50,8 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {     // inclusive prefix
   return v;
 }
 
-// blocks: how many parts a launch is to have at least; least: key tiles of a part.  False: no item has this block.
-template <int QROWS> __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, int blocks, int least, PagedItem &it) {
+// most(key tiles): parts of an item.  False: no item has this block.
+template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, Most most, PagedItem &it) {
   const int lane = threadIdx.x & 63, room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
   const uint32_t want = (uint32_t)a.n_kv_heads.div((int)blockIdx.x);
   it.g = (int)blockIdx.x - (int)want * KV;
@@ -65,16 +66,29 @@ template <int QROWS> __device__ __forceinline__ bool paged_item(const PagedAttnA
       h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
     }
   };
-  float pairs = 0.0f;
+  float pairs = 0.0f, items = 0.0f;
   for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
     look(b0);
     pairs += (float)h.q_tiles * (float)h.key_tiles;
+    items += (float)h.q_tiles;
   }
-  const int target = paged_target(wave_sum(pairs) * (float)KV, blocks, least);
+  pairs = wave_sum(pairs) * (float)KV;
+  items = wave_sum(items) * (float)KV;
+  // A share of the pairs each.  An item has up to one part more than its pairs make whole, so that all come to blocks + items and less.  Few items: a larger share of the
+  // pairs makes up for that.  More: the first of some larger shares with which the parts are no more than the blocks; or twice the share, where nothing else is.
+  const int share = paged_target(pairs, a.blocks, a.least);
+  int target = 2 * share;
+  if (items * 16.0f <= (float)a.blocks) target = share + share / 16;
+  else if (a.pb.n_seqs <= 64 && items < (float)a.blocks)
+    for (int t = share; t < 2 * share; t += (share + 3) / 4)
+      if (wave_sum((float)h.q_tiles * (float)paged_parts(h.key_tiles, t, most(h.key_tiles))) * (float)KV <= (float)a.blocks) {
+        target = t;
+        break;
+      }
   uint32_t before = 0, slots = 0;
   for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
     if (a.pb.n_seqs > 64) look(b0);
-    const int parts = paged_parts(h.key_tiles, target, (int)__builtin_amdgcn_sqrtf((float)h.key_tiles));
+    const int parts = paged_parts(h.key_tiles, target, most(h.key_tiles));
     const uint32_t mine = (uint32_t)min((uint64_t)h.q_tiles * parts, (uint64_t)PAGED_MOST);
     const uint32_t upto = scan64(mine), cut = scan64(parts > 1 ? mine : 0);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(before + upto > want);
@@ -128,7 +142,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lg = lane >> 5;
   PagedItem it;
-  if (!paged_item<PC_QROWS>(a, PC_BLOCKS, PC_LEAST, it)) return;
+  if (!paged_item<PC_QROWS>(a, [](int tiles) { return (int)__builtin_amdgcn_sqrtf((float)tiles); }, it)) return;
   const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d, room = paged_room(a.pb), g = it.g;
   const int rows = it.s.n * n_rep, p0 = paged_pos(it.s, 0), q0 = it.qt * PC_QROWS, qw0 = q0 + wave * 32;
   const PagedKeys keys = paged_keys(p0 + a.n_rep.div(q0), p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1), room, a.window, a.sinks);
@@ -449,6 +463,341 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
     }
 }
 
+// ---------------------------------------------------------------- one or a few new rows
+//
+// Block = 4 wavefronts, 16 (position, query head) pairs of one kv head of one sequence.  Bound by memory: each wavefront walks its own steps of 32 keys, K rows to registers as
+// they are the matrix operand, V rows through registers into the wavefront's own LDS, from where the transposing reads take them; the next step's K rows are asked
+// for as soon as the scores are made, its V rows as soon as those are in LDS, and nothing is waited for but that.  The wavefronts meet once, at the end.
+// The matrix instruction's 16 columns are the rows, so that a lane has four scores of each 16 keys of one row, and its weights are the operand of O^T = V^T . P^T as they lie.
+// Parts of an item are merged by the last of its blocks to arrive.
+constexpr int PF_THREADS = 256, PF_QROWS = 16;
+constexpr int PF_BLOCKS = 512, PF_LEAST = 2;
+constexpr int PF_SLOTS = 2 * PF_BLOCKS, PF_MOST = 64;      // parts of an item: a lane for each
+
+template <int HD, bool I8> struct PagedFew {
+  static constexpr int NW = 4, KEYS = 32, ROWB = HD * 2;
+  static constexpr int VROW = ROWB + 32;                     // bytes between V rows in LDS: eight banks further each, so that the reads of 16 rows by 32 bytes meet all banks alike
+  static constexpr int NT = HD / 16, KS = HD / 32;           // 16-feature tiles of the output, matrix instructions per 16 keys
+  static constexpr int OROW = HD + 4;                        // floats between rows of a wavefront's sums in LDS
+  static constexpr int GK = KS / (I8 ? 2 : 1), LPR = HD / (I8 ? 16 : 8), GV = LPR / 4;   // 16-byte loads of 16 keys' K and V; lanes per V row
+  static constexpr int SLOT = PF_QROWS * (HD + 4);           // floats of a part: the rows' sums, then (m, l, -, -) of each
+  struct Smem {
+    union {
+      unsigned char v[KEYS * VROW];
+      float o[PF_QROWS * OROW];
+    } wave[NW];
+    float m[NW][PF_QROWS], l[NW][PF_QROWS];
+    float w[PF_QROWS][PF_MOST], inv[PF_QROWS];
+    f4_t fold[PF_THREADS];
+    int is_last;
+  };
+  // Must be called by every thread of the block (it contains barriers).
+  static __device__ void item(const PagedAttnArgs &a, const PagedItem &it, Smem &sm) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+    const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d, room = paged_room(a.pb), g = it.g;
+    const int rows = it.s.n * n_rep, p0 = paged_pos(it.s, 0), q0 = it.qt * PF_QROWS, nr = min(PF_QROWS, rows - q0);
+    const int pos_lo = p0 + a.n_rep.div(q0), pos_hi = p0 + a.n_rep.div(q0 + nr - 1);
+    const PagedKeys keys = paged_keys(pos_lo, pos_hi, room, a.window, a.sinks);
+    int i_lo = 0, i_hi = keys.n;
+    if (it.parts > 1) {
+      const int per = (keys.n + it.parts - 1) / it.parts;
+      i_lo = min(it.part * per, keys.n);
+      i_hi = min(i_lo + per, keys.n);
+    }
+    auto out_row = [&](int r) {                              // of pair q0 + r
+      const int qs = a.n_rep.div(q0 + r);
+      return ((size_t)(it.s.start + qs) * a.n_heads + g * n_rep + q0 + r - qs * n_rep) * HD;
+    };
+    const int qpos = p0 + a.n_rep.div(q0 + min(l16, nr - 1));  // columns past the end repeat the last row and are never stored
+    const int sees_from = a.window ? qpos - a.window : -1, sees_to = a.window ? a.sinks : 0;
+    auto sees = [&](int key) { return key <= qpos && (key > sees_from || key < sees_to); };
+
+    auto key_of = [&](int st) { return keys.tile(st >> 1) * PAGED_KEYS + (st & 1) * KEYS; };
+    const int st_end = 2 * i_hi;
+    u4_t kr[2][GK], vr[2][GV];
+    f4_t ks[2], vs[2];
+    int id[2], next[2];
+    auto ids = [&](int st, int *to) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) to[h] = st < st_end ? __builtin_amdgcn_readfirstlane(paged_page(a.pb, it.b, key_of(st) + 16 * h)) : -1;
+    };
+    auto load_k = [&](int st, const int *page) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const size_t row = paged_row(a.pb, KV, max(page[h], 0), g, key_of(st) + 16 * h);   // a missing page: page 0, masked
+#pragma unroll
+        for (int c = 0; c < GK; c++)
+          kr[h][c] = *as_global<u4_t>((const unsigned char *)a.pages_k + (row + l16) * (I8 ? HD : ROWB) + (lq + 4 * c) * 16);
+        if constexpr (I8) ks[h] = *as_global<f4_t>(a.scales_k + row + 4 * lq);
+      }
+    };
+    auto load_v = [&](int st, const int *page) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const size_t row = paged_row(a.pb, KV, max(page[h], 0), g, key_of(st) + 16 * h);
+#pragma unroll
+        for (int c = 0; c < GV; c++)
+          vr[h][c] = *as_global<u4_t>((const unsigned char *)a.pages_v + (row + c * (64 / LPR) + lane / LPR) * (I8 ? HD : ROWB) + lane % LPR * 16);
+        if constexpr (I8) vs[h] = *as_global<f4_t>(a.scales_v + row + 4 * lq);
+      }
+    };
+
+    int st = 2 * i_lo + wave;
+    ids(st, id);
+    if (st < st_end) {
+      load_k(st, id);
+      load_v(st, id);
+    }
+    h8_t qf[KS];                                             // the features that the K fragments have: fp16 8 (4 s + lq) .., int8 16 (lq + 4 c) + 8 u .., s = 2 c + u
+    {
+      const _Float16 *const qp = a.q + out_row(min(l16, nr - 1));
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[s] = *(const h8_t *)(qp + (I8 ? 16 * (lq + 4 * (s / 2)) + 8 * (s % 2) : 8 * (4 * s + lq)));
+    }
+    f4_t o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) o[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = -1e30f, l_run = 0.0f;                      // finite: a step may hold no key that a row sees
+    const float unit = I8 ? 1.0f : a.scale_log2;
+    unsigned char *const vl = sm.wave[wave].v;
+
+    auto step = [&](auto more) {
+      ids(st + NW, next);
+      const int k0 = key_of(st);
+      f4_t s[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        s[h] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < GK; c++)
+#pragma unroll
+          for (int u = 0; u < KS / GK; u++) {
+            u4_t k = kr[h][c];
+            if constexpr (I8) {
+              uint32_t w[4];
+              i8x4_to_h2x2(kr[h][c][2 * u], w[0], w[1]);
+              i8x4_to_h2x2(kr[h][c][2 * u + 1], w[2], w[3]);
+              k = u4_t{w[0], w[1], w[2], w[3]};
+            }
+            s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, k), qf[c * (KS / GK) + u], s[h], 0, 0, 0);
+          }
+      }
+      if constexpr (I8) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) ks[h] *= a.scale_log2;
+      }
+      const f4_t kscale[2] = {ks[0], ks[1]};
+      if constexpr (decltype(more)::value) load_k(st + NW, next);
+      f4_t inv_v[2];
+      if constexpr (I8) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            // as in the chunk kernel: the scale of V in the exponent, its reciprocal finite whatever lies in a place that no row sees
+            const float v = vs[h][e];
+            s[h][e] = __builtin_fmaf(s[h][e], kscale[h][e], __builtin_amdgcn_logf(v));
+            inv_v[h][e] = v >= 1e-38f && v < INFINITY ? __builtin_amdgcn_rcpf(v) : 1.0f;
+          }
+      }
+      // value r of s[h] is key k0 + 16 h + 4 lq + r of row l16
+      const bool masked = k0 + KEYS - 1 > pos_lo || (id[0] | id[1]) < 0 || (a.window && k0 <= pos_hi - a.window && k0 + KEYS > a.sinks);
+      if (masked) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (!sees(k0 + 16 * h + 4 * lq + r) || id[h] < 0) s[h][r] = -INFINITY;
+      }
+      float mx = m_run;
+#pragma unroll
+      for (int h = 0; h < 2; h++) mx = fmaxf(fmaxf(fmaxf(mx, s[h][0]), fmaxf(s[h][1], s[h][2])), s[h][3]);
+      mx = max_xor32(max_xor16(mx));
+      if (__builtin_amdgcn_ballot_w64(mx > m_run)) {
+        const float alpha = __builtin_amdgcn_exp2f((m_run - mx) * unit);
+        m_run = mx;
+        l_run *= alpha;
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[t] *= alpha;
+      }
+      const float mxs = m_run * unit;
+      h8_t pf;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float p = __builtin_amdgcn_exp2f(I8 ? s[h][r] - mxs : __builtin_fmaf(s[h][r], unit, -mxs));
+          l_run = I8 ? __builtin_fmaf(p, inv_v[h][r], l_run) : l_run + p;
+          pf[4 * h + r] = (_Float16)p;
+        }
+      uint32_t bad = 0;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int c = 0; c < GV; c++) {
+          const int r = 16 * h + c * (64 / LPR) + lane / LPR, piece = lane % LPR;
+          if constexpr (I8) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              uint32_t w[4];
+              i8x4_to_h2x2(vr[h][c][2 * u], w[0], w[1]);
+              i8x4_to_h2x2(vr[h][c][2 * u + 1], w[2], w[3]);
+              *(u4_t *)(vl + r * VROW + (2 * piece + u) * 16) = u4_t{w[0], w[1], w[2], w[3]};
+            }
+          } else {
+            *(u4_t *)(vl + r * VROW + piece * 16) = vr[h][c];
+#pragma unroll
+            for (int e = 0; e < 4; e++) bad |= (vr[h][c][e] & 0x7fff7fffu) + 0x04000400u;   // bits 15 and 31: a half that is not finite
+          }
+        }
+      if constexpr (decltype(more)::value) load_v(st + NW, next);
+      auto weigh = [&](auto clean) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          s4_t v[2];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int r = 16 * h + 4 * lq + (l16 >> 2), c = t * 32 + (l16 & 3) * 8;
+            v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vl + r * VROW + c));
+          }
+          u4_t w = __builtin_bit_cast(u4_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (decltype(clean)::value) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t x = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+              w[e] &= ~(x | (x - (x >> 15)));
+            }
+          }
+          o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w), pf, o[t], 0, 0, 0);
+        }
+      };
+      if (I8 || !__builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0)) {
+        weigh(std::false_type());
+      } else {
+        // halves that are not finite: left out of the product, where a weight of zero would not stop them, and added for the rows that see them
+        weigh(std::true_type());
+        for (int key = 0; key < KEYS; key++) {
+          const bool seen = sees(k0 + key) && id[key >> 4] >= 0;
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            const uint2 w = *(const uint2 *)(vl + key * VROW + t * 32 + 8 * lq);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t x = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
+              o[t][e] += seen && (x & 0x7c00u) == 0x7c00u ? (float)__builtin_bit_cast(_Float16, (uint16_t)x) : 0.0f;
+            }
+          }
+        }
+      }
+      id[0] = next[0];
+      id[1] = next[1];
+    };
+    // the last step by itself: behind a branch around its loads every wait would be for all of them
+    if (st < st_end) {
+      for (; st + NW < st_end; st += NW) step(std::true_type());
+      step(std::false_type());
+    }
+
+    // the block's wavefronts: value r of o[t] is feature 16 t + 4 lq + r of row l16
+    l_run = add_xor32(add_xor16(l_run));
+#pragma unroll
+    for (int t = 0; t < NT; t++) *(f4_t *)&sm.wave[wave].o[l16 * OROW + t * 16 + 4 * lq] = o[t];
+    if (lq == 0) { sm.m[wave][l16] = m_run; sm.l[wave][l16] = l_run; }
+    lds_barrier();
+    auto block_sum = [&](int r, int c, f4_t &sum, float &M, float &L) {   // features 4 c .. of row r
+      M = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
+      sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const float e = __builtin_amdgcn_exp2f((sm.m[w][r] - M) * unit);
+        L = __builtin_fmaf(sm.l[w][r], e, L);
+        const f4_t v = *(const f4_t *)&sm.wave[w].o[r * OROW + 4 * c];
+#pragma unroll
+        for (int x = 0; x < 4; x++) sum[x] = __builtin_fmaf(v[x], e, sum[x]);
+      }
+    };
+    auto put = [&](int r, int c, f4_t sum, float inv) {
+      const h2_t lo = {(_Float16)(sum[0] * inv), (_Float16)(sum[1] * inv)}, hi = {(_Float16)(sum[2] * inv), (_Float16)(sum[3] * inv)};
+      *(uint2 *)(a.out + out_row(r) + 4 * c) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+    };
+    const int pieces = nr * (HD / 4);
+    if (it.parts == 1) {
+      for (int i = tid; i < pieces; i += PF_THREADS) {
+        f4_t sum;
+        float M, L;
+        block_sum(i / (HD / 4), i % (HD / 4), sum, M, L);
+        put(i / (HD / 4), i % (HD / 4), sum, L == 0.0f ? 0.0f : 1.0f / L);   // 0: the row sees nothing
+      }
+      return;
+    }
+    // Parts: sums through memory at device scope (cache policy 16), counted once they are acknowledged; the last block of the item folds them in order.
+    const uint32_t part_bytes = (uint32_t)KV * SLOT * 4;
+    const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.ws + (size_t)it.slot * SLOT, (uint32_t)(it.parts - 1) * part_bytes + SLOT * 4);
+    for (int i = tid; i < pieces; i += PF_THREADS) {
+      f4_t sum;
+      float M, L;
+      const int r = i / (HD / 4), c = i % (HD / 4);
+      block_sum(r, c, sum, M, L);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, sum), rw, (uint32_t)it.part * part_bytes + i * 16, 0, 16);
+      if (c == 0) {
+        const f4_t ml = {M, L, 0.0f, 0.0f};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, ml), rw, (uint32_t)it.part * part_bytes + (PF_QROWS * HD + r * 4) * 4, 0, 16);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) sm.is_last = __hip_atomic_fetch_add(&a.counters[it.slot], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.parts - 1;
+    __syncthreads();
+    if (!sm.is_last) return;
+    if (tid == 0) __hip_atomic_store(&a.counters[it.slot], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+    // weights of the parts: a wavefront per row, a part per lane
+    for (int r = wave; r < nr; r += NW) {
+      const f4_t ml = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, (uint32_t)min(lane, it.parts - 1) * part_bytes + (PF_QROWS * HD + r * 4) * 4, 0, 16));
+      const float m = lane < it.parts ? ml[0] : -1e30f, M = wave_max(m), e = lane < it.parts ? __builtin_amdgcn_exp2f((m - M) * unit) : 0.0f;
+      const float L = wave_sum(lane < it.parts ? ml[1] * e : 0.0f);
+      sm.w[r][lane] = e;
+      if (lane == 0) sm.inv[r] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+    lds_barrier();
+    // a thread per four features of a row; where those are fewer than threads, groups of threads share the parts
+    const int groups = pieces < PF_THREADS ? PF_THREADS / pieces : 1, mine = groups > 1 ? tid / pieces : 0;
+    for (int i0 = groups > 1 ? tid - mine * pieces : tid; i0 < pieces; i0 += PF_THREADS) {
+      const int r = i0 / (HD / 4), c = i0 % (HD / 4);
+      f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (mine < groups)
+        for (int f = mine; f < it.parts; f += groups * 8) {
+          f4_t v[8];
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            v[u] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, (uint32_t)min(f + u * groups, it.parts - 1) * part_bytes + i0 * 16, 0, 16));
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            if (f + u * groups < it.parts)
+#pragma unroll
+              for (int x = 0; x < 4; x++) sum[x] = __builtin_fmaf(v[u][x], sm.w[r][f + u * groups], sum[x]);
+        }
+      if (groups == 1) put(r, c, sum, sm.inv[r]);
+      else sm.fold[tid] = sum;
+    }
+    if (groups > 1) {
+      lds_barrier();
+      if (tid < pieces) {
+        f4_t sum = sm.fold[tid];
+        for (int u = 1; u < groups; u++) sum += sm.fold[tid + u * pieces];
+        put(tid / (HD / 4), tid % (HD / 4), sum, sm.inv[tid / (HD / 4)]);
+      }
+    }
+  }
+};
+
+template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4 : I8 ? 3 : 2) void attn_paged_few_kernel(PagedAttnArgs a) {
+  typedef PagedFew<HD, I8> A;
+  __shared__ typename A::Smem sm;
+  PagedItem it;
+  if (paged_item<PF_QROWS>(a, [](int tiles) { return min(PF_MOST, (int)(2.0f * __builtin_amdgcn_sqrtf((float)tiles))); }, it)) A::item(a, it, sm);
+}
+
 }  // namespace jsg
 
 using namespace jsg;
@@ -456,8 +805,9 @@ using namespace jsg;
 extern "C" {
 
 size_t jsgrad_hip_attn_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-  // counters, then the sums of cut items, one slot for every part
+  // counters, then the sums of cut items, one slot for every part: those of chunks are the larger ones
   (void)n_heads, (void)n_kv_heads;
+  static_assert(PF_SLOTS * PF_QROWS <= PC_SLOTS * 4 * 32 && PF_SLOTS <= PC_SLOTS * 4, "the few-row kernel's parts fit where the chunk kernel's do");
   return (size_t)PC_SLOTS * 4 * sizeof(int) + (size_t)PC_SLOTS * 4 * (head_dim / 2 + 4) * 64 * sizeof(float);
 }
 
@@ -485,16 +835,26 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   a.scale_log2 = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
   a.counters = (int *)workspace;
   a.ws = (float *)((char *)workspace + (size_t)PC_SLOTS * 4 * sizeof(int));
+  // As many blocks as there may be items and parts: every sequence fills its last q tile at worst, and what is no longer than the least part is not cut.
   const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS;
-  // as many blocks as there may be items and parts: every sequence fills its last q tile at worst, and what is no longer than the least part is not cut
-  const size_t blocks = (size_t)KV * ((size_t)rows * n_rep / PC_QROWS + (n_seqs < rows ? n_seqs : rows)) + (room_tiles > PC_LEAST ? PC_SLOTS : 0);
+  auto most_blocks = [&](int q_rows, int least, int slots) { return (size_t)KV * ((size_t)rows * n_rep / q_rows + (n_seqs < rows ? n_seqs : rows)) + (room_tiles > least ? slots : 0); };
+  const bool few = (size_t)rows * n_rep <= (size_t)PF_QROWS * n_seqs;
+  a.blocks = !few ? PC_BLOCKS : HD == 128 && host_pages->kind == JSGRAD_W_F16 ? PF_BLOCKS / 2 : PF_BLOCKS;
+  a.least = few ? PF_LEAST : PC_LEAST;
+  const size_t blocks = few ? most_blocks(PF_QROWS, PF_LEAST, PF_SLOTS) : most_blocks(PC_QROWS, PC_LEAST, PC_SLOTS);
   JSG_REQUIRE(blocks < PAGED_MOST, "%s: %d rows of %d heads", who, rows, n_heads);
-  const dim3 grid((unsigned)blocks), block(PC_THREADS);
+  const dim3 grid((unsigned)blocks);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
-  if (HD == 64 && i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<64, true>), grid, block, 0, a);
-  else if (HD == 64) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<64, false>), grid, block, 0, a);
-  else if (i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<128, true>), grid, block, 0, a);
-  else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_paged_chunk_kernel<128, false>), grid, block, 0, a);
+#define JSG_PAGED(KERNEL, THREADS)                                                                    \
+  do {                                                                                                \
+    if (HD == 64 && i8) JSG_LAUNCH(PROF_ATTN_PAGED, (KERNEL<64, true>), grid, dim3(THREADS), 0, a);     \
+    else if (HD == 64) JSG_LAUNCH(PROF_ATTN_PAGED, (KERNEL<64, false>), grid, dim3(THREADS), 0, a);     \
+    else if (i8) JSG_LAUNCH(PROF_ATTN_PAGED, (KERNEL<128, true>), grid, dim3(THREADS), 0, a);           \
+    else JSG_LAUNCH(PROF_ATTN_PAGED, (KERNEL<128, false>), grid, dim3(THREADS), 0, a);                  \
+  } while (0)
+  if (few) JSG_PAGED(attn_paged_few_kernel, PF_THREADS);
+  else JSG_PAGED(attn_paged_chunk_kernel, PC_THREADS);
+#undef JSG_PAGED
   return 0;
 }
 

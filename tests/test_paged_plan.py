@@ -60,7 +60,7 @@ int main() {
         pairs += (float)h.q_tiles * (float)h.key_tiles;
         if (h.key_tiles > longest) longest = h.key_tiles;
       }
-      const int target = paged_target(pairs * (float)KV, sh.blocks, sh.least);
+      const int target = paged_target(pairs * (float)KV, sh.blocks, sh.least) * range(8, 16) / 8;
       int64_t slots = 0, blocks = 0;
       for (int b = 0; b < p.n_seqs; b++) {
         const PagedSeq s = paged_seq(p, b);
