@@ -114,6 +114,14 @@ template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(c
   return false;
 }
 
+// paged_page for a position that all lanes share: through the scalar cache, sixteen entries to a line, and without a place among the vector loads, whose
+// results come in order, so that a page number asked for behind a tile's loads would be there only after the tile is.
+__device__ __forceinline__ int page_uniform(const PagedBatch &p, int b, int pos) {
+  if (pos < 0 || pos >= paged_room(p)) return -1;
+  const int id = *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(p.table + (size_t)b * p.width + (pos >> p.page_shift));
+  return id >= 0 && id < p.n_pages ? id : -1;
+}
+
 // ---------------------------------------------------------------- chunks of new rows
 //
 // Block = 4 wavefronts = 128 (position, query head) pairs of one kv head of one sequence, keys in tiles of 64, as attn_prefill_kernel (prefill.hip) has it:
@@ -128,6 +136,9 @@ template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(c
 constexpr int PC_THREADS = 256, PC_QROWS = 128;
 constexpr int PC_BLOCKS = 512, PC_LEAST = 8;               // two blocks to a compute unit; a tile takes 0.8 us and folding a part as long
 constexpr int PC_SLOTS = 2 * PC_BLOCKS;
+// A row's weights are exp2(score - M) with a whole number M, which moves up only when a score is more than PC_SLACK above it: they are 2^7 and less, and their fp16 rounding is
+// relative to themselves all the same.  Sums are rescaled for nearly no tile then, and exactly, by a power of two.
+constexpr float PC_SLACK = 6.0f;
 
 template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn_paged_chunk_kernel(PagedAttnArgs a) {
   constexpr int ROWB = HD * 2, PPR = HD / 8;                 // bytes and 16-byte pieces of a row of halves
@@ -164,7 +175,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
   auto v_at = [](int r, int p) { return HD == 128 ? p ^ ((r & 7) << 1) : p ^ (((r >> 1) & 3) << 1); };
 
   // this wavefront's rows of a tile: 16 * wave and on
-  auto page_of = [&](int i) { return i < i_hi ? __builtin_amdgcn_readfirstlane(paged_page(a.pb, it.b, keys.tile(i) * PAGED_KEYS + wave * 16)) : -1; };
+  auto page_of = [&](int i) { return i < i_hi ? page_uniform(a.pb, it.b, keys.tile(i) * PAGED_KEYS + wave * 16) : -1; };
   auto row_of = [&](int i, int id) { return paged_row(a.pb, KV, max(id, 0), g, keys.tile(i) * PAGED_KEYS + wave * 16); };   // a missing page: page 0, masked
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds + wave * LOADS * 1024;
   const int lrow = lane / PPR, lp = lane % PPR;
@@ -252,142 +263,168 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
   const unsigned char *const kp = lds + l32 * ROWB;
   const int vrow = 4 * lg + ((lane >> 2) & 3), vcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;   // byte column inside 64 (32 features)
 
-  for (int i = i_lo, buf = 0; i < i_hi; i++, buf ^= 1) {
+  // A tile that every row of the block sees whole, or one with the tests; returns after the next tile has been asked for and this one used.
+  const int blk_lo = p0 + a.n_rep.div(q0), blk_hi = p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1);
+  int i = i_lo, buf = 0, pm = 0;
+  auto begin = [&]() {                                       // tile i is there, everyone is done with tile i - 1; whether all of the block sees all of it
     if constexpr (!I8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();                                            // tile i is there, everyone is done with tile i - 1
+    lds_barrier();
     id = id_next;
     if (i + 1 < i_hi) {
       if constexpr (I8) load(i + 1, id);
       else issue(i + 1, id, buf ^ 1);
       id_next = page_of(i + 2);
     }
+    const int4 hv = *(const int4 *)here[buf];
+    pm = __builtin_amdgcn_readfirstlane(hv.x | hv.y << 1 | hv.z << 2 | hv.w << 3);
     const int k0 = keys.tile(i) * PAGED_KEYS;
-    // every key of the tile is masked for this wavefront (uniform)
-    if (!(k0 > pos_hi || (a.window && k0 + PAGED_KEYS - 1 <= pos_lo - a.window && k0 >= a.sinks))) {
-      const int4 hv = *(const int4 *)here[buf];
-      const int pm = __builtin_amdgcn_readfirstlane(hv.x | hv.y << 1 | hv.z << 2 | hv.w << 3);
-      const bool masked = k0 + PAGED_KEYS - 1 > pos_lo || pm != 15 || (a.window && k0 <= pos_hi - a.window && k0 + PAGED_KEYS > a.sinks);
-      auto sees = [&](int key) { return key <= qpos && (key > sees_from || key < sees_to); };
-
-      // S^T tile: 64 keys x 32 query rows
-      f16_t s[2];
+    return k0 + PAGED_KEYS - 1 <= blk_lo && pm == 15 && !(a.window && k0 <= blk_hi - a.window && k0 + PAGED_KEYS > a.sinks);
+  };
+  auto end = [&]() {
+    if constexpr (I8)
+      if (i + 1 < i_hi) store(id, buf ^ 1);
+    i++;
+    buf ^= 1;
+  };
+  auto tile = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    const int k0 = keys.tile(i) * PAGED_KEYS;
+    auto sees = [&](int key) { return (key <= qpos) & ((key > sees_from) | (key < sees_to)); };
+    // S^T tile: 64 keys x 32 query rows
+    f16_t s[2];
 #pragma unroll
-      for (int tk = 0; tk < 2; tk++) {
+    for (int tk = 0; tk < 2; tk++) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[tk][r] = 0.0f;
+      for (int r = 0; r < 16; r++) s[tk][r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++) {
-          const h8_t kf = *(const h8_t *)(kp + buf * BUF + tk * 32 * ROWB + k_at(l32, 2 * c + lg) * 16);
-          s[tk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], s[tk], 0, 0, 0);
-        }
+      for (int c = 0; c < HD / 16; c++) {
+        const h8_t kf = *(const h8_t *)(kp + buf * BUF + tk * 32 * ROWB + k_at(l32, 2 * c + lg) * 16);
+        s[tk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], s[tk], 0, 0, 0);
       }
-      // accumulator r of s[tk] is key k0 + tk*32 + 8*(r/4) + 4*lg + r%4 for query row l32
-      f4_t inv_v[2][4];
-      if constexpr (I8) {
-#pragma unroll
-        for (int tk = 0; tk < 2; tk++)
-#pragma unroll
-          for (int r4 = 0; r4 < 4; r4++) {
-            const int at = tk * 32 + 8 * r4 + 4 * lg;
-            const f4_t ks = *(const f4_t *)&scl[buf][0][at], lv = *(const f4_t *)&scl[buf][1][at];
-            inv_v[tk][r4] = *(const f4_t *)&scl[buf][2][at];
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[tk][r4 * 4 + e] = __builtin_fmaf(s[tk][r4 * 4 + e], ks[e], lv[e]);
-          }
-      }
-      if (masked) {
-#pragma unroll
-        for (int tk = 0; tk < 2; tk++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int key = k0 + tk * 32 + 8 * (r / 4) + 4 * lg + (r % 4);
-            if (!sees(key) || !(pm >> (tk * 2 + r / 8) & 1)) s[tk][r] = -INFINITY;
-          }
-      }
-      float mx = m_run;
+    }
+    // accumulator r of s[tk] is key k0 + tk*32 + 8*(r/4) + 4*lg + r%4 for query row l32
+    f4_t inv_v[2][4];
+    if constexpr (I8) {
 #pragma unroll
       for (int tk = 0; tk < 2; tk++)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[tk][r]), s[tk][r + 1]);
-      mx = max_xor32(mx);
-      // the sums are rescaled when some row's maximum has moved (uniform branch), so that the largest weight of a row is 1 and its fp16 rounding exact
-      if (__builtin_amdgcn_ballot_w64(mx > m_run)) {
-        const float alpha = __builtin_amdgcn_exp2f((m_run - mx) * unit);   // first visible tile: 0
-        m_run = mx;
-        l_run *= alpha;
+        for (int r4 = 0; r4 < 4; r4++) {
+          const int at = tk * 32 + 8 * r4 + 4 * lg;
+          const f4_t ks = *(const f4_t *)&scl[buf][0][at], lv = *(const f4_t *)&scl[buf][1][at];
+          inv_v[tk][r4] = *(const f4_t *)&scl[buf][2][at];
 #pragma unroll
-        for (int td = 0; td < NT; td++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
-      }
-      const float mxs = m_run * unit;
-      float psum[2] = {0.0f, 0.0f};
-      h8_t pf[2][2];
+          for (int e = 0; e < 4; e++) s[tk][r4 * 4 + e] = __builtin_fmaf(s[tk][r4 * 4 + e], ks[e], lv[e]);
+        }
+    }
+    if constexpr (!WHOLE) {
 #pragma unroll
       for (int tk = 0; tk < 2; tk++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          const float p = __builtin_amdgcn_exp2f(I8 ? s[tk][r] - mxs : __builtin_fmaf(s[tk][r], unit, -mxs));
-          if constexpr (I8) psum[tk] = __builtin_fmaf(p, inv_v[tk][r / 4][r % 4], psum[tk]);
-          else psum[tk] += p;
-          pf[tk][r / 8][r % 8] = (_Float16)p;
+          const int key = k0 + tk * 32 + 8 * (r / 4) + 4 * lg + (r % 4);
+          s[tk][r] = sees(key) & ((pm >> (tk * 2 + r / 8) & 1) != 0) ? s[tk][r] : -INFINITY;
         }
-      l_run += psum[0] + psum[1];
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int r = 1; r < 31; r += 2) mx = fmaxf(fmaxf(mx, s[r / 16][r % 16]), s[(r + 1) / 16][(r + 1) % 16]);
+    mx = max_xor32(fmaxf(mx, s[1][15])) * unit;
+    if (__builtin_amdgcn_ballot_w64(mx > m_run + PC_SLACK)) {
+      const float m = fmaxf(m_run, __builtin_ceilf(mx)), alpha = __builtin_amdgcn_exp2f(m_run - m);   // first visible tile: 0
+      m_run = m;
+      l_run *= alpha;
+#pragma unroll
+      for (int td = 0; td < NT; td++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
+    }
+    float psum[2] = {0.0f, 0.0f};
+    h8_t pf[2][2];
+#pragma unroll
+    for (int tk = 0; tk < 2; tk++)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        float p[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) p[e] = __builtin_amdgcn_exp2f(I8 ? s[tk][r + e] - m_run : __builtin_fmaf(s[tk][r + e], unit, -m_run));
+        const h2_t h = {(_Float16)p[0], (_Float16)p[1]};
+        pf[tk][r / 8][r % 8] = h[0];
+        pf[tk][r / 8][r % 8 + 1] = h[1];
+        // fp16 pages: the sum is of the rounded weights, which multiply V.  int8: of the float ones; a weight that a small scale makes vanish as a half still counts.
+        if constexpr (I8) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) psum[e] = __builtin_fmaf(p[e], inv_v[tk][r / 4][(r + e) % 4], psum[e]);
+        } else {
+          psum[tk] = __builtin_amdgcn_fdot2(h, h2_t{(_Float16)1.0f, (_Float16)1.0f}, psum[tk], false);
+        }
+      }
+    l_run += psum[0] + psum[1];
 
-      // O^T += V^T . P^T : k-slot s' of lane half lg in step (tk, hs) is key tk*32 + hs*16 + 8*(s'/4) + 4*lg + s'%4
-      const unsigned char *const vt = lds + buf * BUF + TILE;
-      auto weigh = [&](auto test) {
-        uint32_t bad = 0;
+    // O^T += V^T . P^T : k-slot s' of lane half lg in step (tk, hs) is key tk*32 + hs*16 + 8*(s'/4) + 4*lg + s'%4
+    const unsigned char *const vt = lds + buf * BUF + TILE;
+    uint32_t bad = 0;
 #pragma unroll
-        for (int tk = 0; tk < 2; tk++)
+    for (int tk = 0; tk < 2; tk++)
 #pragma unroll
-          for (int hs = 0; hs < 2; hs++)
+      for (int hs = 0; hs < 2; hs++)
 #pragma unroll
-            for (int td = 0; td < NT; td++) {
-              s4_t v[2];
+        for (int td = 0; td < NT; td++) {
+          s4_t v[2];
 #pragma unroll
-              for (int e = 0; e < 2; e++) {
-                const int r = tk * 32 + hs * 16 + 8 * e + vrow, c = td * 64 + vcol;
-                v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vt + r * ROWB + v_at(r, c >> 4) * 16 + (c & 15)));
-              }
-              h8_t vf = __builtin_bit_cast(h8_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-              if constexpr (decltype(test)::value) {
-                u4_t w = __builtin_bit_cast(u4_t, vf);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  const uint32_t t = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // the sign bit of halves that are not finite
-                  bad |= t;
-                  w[e] &= ~(t | (t - (t >> 15)));
-                }
-                vf = __builtin_bit_cast(h8_t, w);
-              }
-              o_acc[td] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[tk][hs], o_acc[td], 0, 0, 0);
-            }
-        return bad;
-      };
-      if (!I8 && masked) {
-        if (__builtin_amdgcn_ballot_w64(weigh(std::true_type()) != 0)) {
-          for (int key = 0; key < PAGED_KEYS; key++) {
-            const bool seen = sees(k0 + key) && (pm >> (key >> 4) & 1);
-#pragma unroll
-            for (int td = 0; td < NT; td++)
-#pragma unroll
-              for (int r4 = 0; r4 < 4; r4++) {
-                const uint2 w = *(const uint2 *)(vt + key * ROWB + v_at(key, td * 4 + r4) * 16 + lg * 8);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                  const uint32_t h = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
-                  if (seen && (h & 0x7c00u) == 0x7c00u) o_acc[td][r4 * 4 + e] += (float)__builtin_bit_cast(_Float16, (uint16_t)h);
-                }
-              }
+          for (int e = 0; e < 2; e++) {
+            const int r = tk * 32 + hs * 16 + 8 * e + vrow, c = td * 64 + vcol;
+            v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vt + r * ROWB + v_at(r, c >> 4) * 16 + (c & 15)));
           }
+          h8_t vf = __builtin_bit_cast(h8_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (!I8 && !WHOLE) {
+            u4_t w = __builtin_bit_cast(u4_t, vf);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t t = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // the sign bit of halves that are not finite
+              bad |= t;
+              w[e] &= ~(t | (t - (t >> 15)));
+            }
+            vf = __builtin_bit_cast(h8_t, w);
+          }
+          o_acc[td] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[tk][hs], o_acc[td], 0, 0, 0);
         }
-      } else {
-        weigh(std::false_type());
+    if constexpr (!I8 && !WHOLE) {
+      if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+        for (int key = 0; key < PAGED_KEYS; key++) {
+          const bool seen = sees(k0 + key) && (pm >> (key >> 4) & 1);
+#pragma unroll
+          for (int td = 0; td < NT; td++)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; r4++) {
+              const uint2 w = *(const uint2 *)(vt + key * ROWB + v_at(key, td * 4 + r4) * 16 + lg * 8);
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const uint32_t h = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
+                o_acc[td][r4 * 4 + e] += seen && (h & 0x7c00u) == 0x7c00u ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : 0.0f;
+              }
+            }
+        }
       }
     }
-    if constexpr (I8)
-      if (i + 1 < i_hi) store(id, buf ^ 1);
+  };
+  // every key of the tile is masked for this wavefront (uniform)
+  auto idle = [&]() {
+    const int k0 = keys.tile(i) * PAGED_KEYS;
+    return k0 > pos_hi || (a.window && k0 + PAGED_KEYS - 1 <= pos_lo - a.window && k0 >= a.sinks);
+  };
+  // Two loops, and each with its own copy of the accumulators' life: in one loop with both kinds of tiles they are copied twice a tile.
+  bool whole = i < i_hi && begin();
+  while (i < i_hi) {
+    while (i < i_hi && whole) {
+      tile(std::true_type());
+      end();
+      if (i < i_hi) whole = begin();
+    }
+    while (i < i_hi && !whole) {
+      if (!idle()) tile(std::false_type());
+      end();
+      if (i < i_hi) whole = begin();
+    }
   }
 
   if (it.parts > 1) {
@@ -429,9 +466,9 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
         for (int j = 0; j < NT * 4; j++) v[u][j] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + j * 1024, 0, 16));
       }
       const float m = fmaxf(m_run, fmaxf(w[0][0], w[1][0]));
-      const float e = __builtin_amdgcn_exp2f((m_run - m) * unit);
-      const float e0 = __builtin_amdgcn_exp2f((w[0][0] - m) * unit);   // a part without a visible key: 0
-      const float e1 = f + 1 < it.parts ? __builtin_amdgcn_exp2f((w[1][0] - m) * unit) : 0.0f;
+      const float e = __builtin_amdgcn_exp2f(m_run - m);
+      const float e0 = __builtin_amdgcn_exp2f(w[0][0] - m);   // a part without a visible key: 0
+      const float e1 = f + 1 < it.parts ? __builtin_amdgcn_exp2f(w[1][0] - m) : 0.0f;
       m_run = m;
       l_run = l_run * e + (w[0][1] * e0 + w[1][1] * e1);
 #pragma unroll
@@ -510,7 +547,7 @@ template <int HD, bool I8> struct PagedFew {
     };
     const int qpos = p0 + a.n_rep.div(q0 + min(l16, nr - 1));  // columns past the end repeat the last row and are never stored
     const int sees_from = a.window ? qpos - a.window : -1, sees_to = a.window ? a.sinks : 0;
-    auto sees = [&](int key) { return key <= qpos && (key > sees_from || key < sees_to); };
+    auto sees = [&](int key) { return (key <= qpos) & ((key > sees_from) | (key < sees_to)); };
 
     auto key_of = [&](int st) { return keys.tile(st >> 1) * PAGED_KEYS + (st & 1) * KEYS; };
     const int st_end = 2 * i_hi;
@@ -519,7 +556,7 @@ template <int HD, bool I8> struct PagedFew {
     int id[2], next[2];
     auto ids = [&](int st, int *to) {
 #pragma unroll
-      for (int h = 0; h < 2; h++) to[h] = st < st_end ? __builtin_amdgcn_readfirstlane(paged_page(a.pb, it.b, key_of(st) + 16 * h)) : -1;
+      for (int h = 0; h < 2; h++) to[h] = st < st_end ? page_uniform(a.pb, it.b, key_of(st) + 16 * h) : -1;
     };
     auto load_k = [&](int st, const int *page) {
 #pragma unroll
@@ -607,7 +644,7 @@ template <int HD, bool I8> struct PagedFew {
         for (int h = 0; h < 2; h++)
 #pragma unroll
           for (int r = 0; r < 4; r++)
-            if (!sees(k0 + 16 * h + 4 * lq + r) || id[h] < 0) s[h][r] = -INFINITY;
+            s[h][r] = sees(k0 + 16 * h + 4 * lq + r) & (id[h] >= 0) ? s[h][r] : -INFINITY;
       }
       float mx = m_run;
 #pragma unroll
