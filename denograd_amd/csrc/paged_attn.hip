@@ -20,10 +20,10 @@ struct PagedAttnArgs {
   _Float16 *out;
   int n_heads, window, sinks;
   Divisor n_rep, n_kv_heads;
-  int blocks, least;                     // how the keys are cut: paged_target
+  int few_blocks;                        // of the few-row items: what their pairs are shared among
   float scale_log2;                      // float(1 / sqrt(HD)) * log2(e)
-  int *counters;                         // zero, and zero again afterwards
-  float *ws;
+  int *counters, *few_counters;          // zero, and zero again afterwards
+  float *ws, *few_ws;
 };
 
 // ---------------------------------------------------------------- which work a block has
@@ -50,11 +50,13 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {     // inclusive prefix
   return v;
 }
 
-// most(key tiles): parts of an item.  False: no item has this block.
-template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, Most most, PagedItem &it) {
+// The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head: blocks, least: see paged_target; most(key tiles): parts of an
+// item.  False, and id less these items' blocks, where it is none of them.
+template <int QROWS, typename Most>
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, int &id, int from, int to, int blocks, int least, Most most, PagedItem &it) {
   const int lane = threadIdx.x & 63, room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
-  const uint32_t want = (uint32_t)a.n_kv_heads.div((int)blockIdx.x);
-  it.g = (int)blockIdx.x - (int)want * KV;
+  const uint32_t want = (uint32_t)a.n_kv_heads.div(id);
+  it.g = id - (int)want * KV;
   PagedSeq s;
   PagedShare h;
   auto look = [&](int b0) {
@@ -63,7 +65,7 @@ template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(c
     h = {0, 0};
     if (b < a.pb.n_seqs) {
       s = paged_seq(a.pb, b);
-      h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
+      if (s.n * n_rep >= from && s.n * n_rep <= to) h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
     }
   };
   float pairs = 0.0f, items = 0.0f;
@@ -76,12 +78,12 @@ template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(c
   items = wave_sum(items) * (float)KV;
   // A share of the pairs each.  An item has up to one part more than its pairs make whole, so that all come to blocks + items and less.  Few items: a larger share of the
   // pairs makes up for that.  More: the first of some larger shares with which the parts are no more than the blocks; or twice the share, where nothing else is.
-  const int share = paged_target(pairs, a.blocks, a.least);
+  const int share = paged_target(pairs, blocks, least);
   int target = 2 * share;
-  if (items * 16.0f <= (float)a.blocks) target = share + share / 16;
-  else if (a.pb.n_seqs <= 64 && items < (float)a.blocks)
+  if (items * 16.0f <= (float)blocks) target = share + share / 16;
+  else if (a.pb.n_seqs <= 64 && items < (float)blocks)
     for (int t = share; t < 2 * share; t += (share + 3) / 4)
-      if (wave_sum((float)h.q_tiles * (float)paged_parts(h.key_tiles, t, most(h.key_tiles))) * (float)KV <= (float)a.blocks) {
+      if (wave_sum((float)h.q_tiles * (float)paged_parts(h.key_tiles, t, most(h.key_tiles))) * (float)KV <= (float)blocks) {
         target = t;
         break;
       }
@@ -111,6 +113,7 @@ template <int QROWS, typename Most> __device__ __forceinline__ bool paged_item(c
     before = min(before + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), PAGED_MOST);
     slots = min(slots + (uint32_t)__builtin_amdgcn_readlane((int)cut, 63), PAGED_MOST);
   }
+  id -= (int)before * KV;
   return false;
 }
 
@@ -134,371 +137,393 @@ __device__ __forceinline__ int page_uniform(const PagedBatch &p, int b, int pos)
 // Tiles that hold keys which some row of the wavefront does not see (the diagonal, a window's edge, a missing page) take their V through a test: halves that are not
 // finite are left out of the product, where a weight of zero would not stop them, and added for the rows that see them.
 constexpr int PC_THREADS = 256, PC_QROWS = 128;
-constexpr int PC_BLOCKS = 512, PC_LEAST = 8;               // two blocks to a compute unit; a tile takes 0.8 us and folding a part as long
+constexpr int PC_BLOCKS = 512, PC_LEAST = 4;               // two blocks to a compute unit; a tile takes 1.5 us, and a part some 5 us of its own
 constexpr int PC_SLOTS = 2 * PC_BLOCKS;
 // A row's weights are exp2(score - M) with a whole number M, which moves up only when a score is more than PC_SLACK above it: they are 2^7 and less, and their fp16 rounding is
 // relative to themselves all the same.  Sums are rescaled for nearly no tile then, and exactly, by a power of two.
 constexpr float PC_SLACK = 6.0f;
 
-template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn_paged_chunk_kernel(PagedAttnArgs a) {
-  constexpr int ROWB = HD * 2, PPR = HD / 8;                 // bytes and 16-byte pieces of a row of halves
-  constexpr int TILE = PAGED_KEYS * ROWB, BUF = 2 * TILE;    // K tile, then V tile
-  constexpr int LOADS = TILE / 1024 / 4;                     // a wavefront's loads per tile of K, and of V
-  constexpr int RPL = 64 / PPR;                              // rows per load
-  constexpr int NT = HD / 32;                                // 32-feature tiles of the output
-  constexpr int CPT = HD / 64;                               // 16-byte pieces of codes per thread and tile of K, and of V
-  __shared__ __align__(16) unsigned char lds[2 * BUF];
-  __shared__ __align__(16) float scl[2][3][PAGED_KEYS];      // I8: K's scale times scale_log2, log2 and reciprocal of V's
-  __shared__ __align__(16) int here[2][4];                   // whether the page of 16 rows is there
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lg = lane >> 5;
-  PagedItem it;
-  if (!paged_item<PC_QROWS>(a, [](int tiles) { return (int)__builtin_amdgcn_sqrtf((float)tiles); }, it)) return;
-  const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d, room = paged_room(a.pb), g = it.g;
-  const int rows = it.s.n * n_rep, p0 = paged_pos(it.s, 0), q0 = it.qt * PC_QROWS, qw0 = q0 + wave * 32;
-  const PagedKeys keys = paged_keys(p0 + a.n_rep.div(q0), p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1), room, a.window, a.sinks);
-  int i_lo = 0, i_hi = keys.n;
-  if (it.parts > 1) {
-    const int per = (keys.n + it.parts - 1) / it.parts;
-    i_lo = min(it.part * per, keys.n);
-    i_hi = min(i_lo + per, keys.n);
-  }
-  // this wavefront's first and last position; rows past the end repeat the last one and are never stored
-  const int pos_lo = p0 + a.n_rep.div(min(qw0, rows - 1)), pos_hi = p0 + a.n_rep.div(min(qw0 + 31, rows - 1));
-  const bool q_valid = qw0 + l32 < rows;
-  const int qrow = min(qw0 + l32, rows - 1), qs = a.n_rep.div(qrow), qpos = p0 + qs;
-  const size_t q_off = ((size_t)(it.s.start + qs) * a.n_heads + g * n_rep + qrow - qs * n_rep) * HD;
-  const int sees_from = a.window ? qpos - a.window : -1, sees_to = a.window ? a.sinks : 0;   // keys <= qpos that are > sees_from or < sees_to
-
-  // where piece p of row r of a tile is kept: K by all pieces of a row, V by pairs of pieces (a transposing read takes 32 bytes of eight rows)
-  auto k_at = [](int r, int p) { return HD == 128 ? p ^ (r & 15) : p ^ (r & 7); };
-  auto v_at = [](int r, int p) { return HD == 128 ? p ^ ((r & 7) << 1) : p ^ (((r >> 1) & 3) << 1); };
-
-  // this wavefront's rows of a tile: 16 * wave and on
-  auto page_of = [&](int i) { return i < i_hi ? page_uniform(a.pb, it.b, keys.tile(i) * PAGED_KEYS + wave * 16) : -1; };
-  auto row_of = [&](int i, int id) { return paged_row(a.pb, KV, max(id, 0), g, keys.tile(i) * PAGED_KEYS + wave * 16); };   // a missing page: page 0, masked
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds + wave * LOADS * 1024;
-  const int lrow = lane / PPR, lp = lane % PPR;
-  auto issue = [&](int i, int id, int buf) {                 // fp16
-    const uint32_t to = lds0 + buf * BUF;
-    const size_t at = row_of(i, id) * ROWB;
-    const i4_t rk = dma_rsrc((const unsigned char *)a.pages_k + at), rv = dma_rsrc((const unsigned char *)a.pages_v + at);
-#pragma unroll
-    for (int j = 0; j < LOADS; j++) {
-      const int r = j * RPL + lrow;
-      dma16(rk, (uint32_t)r * ROWB + k_at(wave * 16 + r, lp) * 16, 0, to + j * 1024);
-      dma16(rv, (uint32_t)r * ROWB + v_at(wave * 16 + r, lp) * 16, 0, to + TILE + j * 1024);
-    }
-    if (lane == 0) here[buf][wave] = id >= 0;
+template <int HD, bool I8> struct PagedChunk {
+  static constexpr int ROWB = HD * 2, PPR = HD / 8;                 // bytes and 16-byte pieces of a row of halves
+  static constexpr int TILE = PAGED_KEYS * ROWB, BUF = 2 * TILE;    // K tile, then V tile
+  static constexpr int LOADS = TILE / 1024 / 4;                     // a wavefront's loads per tile of K, and of V
+  static constexpr int RPL = 64 / PPR;                              // rows per load
+  static constexpr int NT = HD / 32;                                // 32-feature tiles of the output
+  static constexpr int CPT = HD / 64;                               // 16-byte pieces of codes per thread and tile of K, and of V
+  struct Smem {
+    __align__(16) unsigned char tiles[2 * BUF];
+    float scl[2][3][PAGED_KEYS];                             // I8: K's scale times scale_log2, log2 and reciprocal of V's
   };
-  u4_t kc[CPT], vc[CPT];                                     // int8: this thread's codes and scale on their way
-  float sc = 1.0f;
-  const int crow = lane >> 2, cp = (lane & 3) * CPT;         // row and first piece of codes
-  auto load = [&](int i, int id) {
-    const size_t row = row_of(i, id);
-#pragma unroll
-    for (int c = 0; c < CPT; c++) {
-      kc[c] = *as_global<u4_t>((const int8_t *)a.pages_k + (row + crow) * HD + (cp + c) * 16);
-      vc[c] = *as_global<u4_t>((const int8_t *)a.pages_v + (row + crow) * HD + (cp + c) * 16);
+
+  // Must be called by every thread of the block (it contains barriers).
+  static __device__ void item(const PagedAttnArgs &a, const PagedItem &it, Smem &sm) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lg = lane >> 5;
+    unsigned char *const lds = sm.tiles;
+    auto &scl = sm.scl;
+    const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d, room = paged_room(a.pb), g = it.g;
+    const int rows = it.s.n * n_rep, p0 = paged_pos(it.s, 0), q0 = it.qt * PC_QROWS, qw0 = q0 + wave * 32;
+    const PagedKeys keys = paged_keys(p0 + a.n_rep.div(q0), p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1), room, a.window, a.sinks);
+    int i_lo = 0, i_hi = keys.n;
+    if (it.parts > 1) {
+      const int per = (keys.n + it.parts - 1) / it.parts;
+      i_lo = min(it.part * per, keys.n);
+      i_hi = min(i_lo + per, keys.n);
     }
-    sc = *as_global<float>((lane & 16 ? a.scales_v : a.scales_k) + row + (lane & 15));
-  };
-  auto store = [&](int id, int buf) {
-    unsigned char *const kt = lds + buf * BUF, *const vt = kt + TILE;
-    const int r = wave * 16 + crow;
+    // this wavefront's first and last position; rows past the end repeat the last one and are never stored
+    const int pos_lo = p0 + a.n_rep.div(min(qw0, rows - 1)), pos_hi = p0 + a.n_rep.div(min(qw0 + 31, rows - 1));
+    const bool q_valid = qw0 + l32 < rows;
+    const int qrow = min(qw0 + l32, rows - 1), qs = a.n_rep.div(qrow), qpos = p0 + qs;
+    const size_t q_off = ((size_t)(it.s.start + qs) * a.n_heads + g * n_rep + qrow - qs * n_rep) * HD;
+    const int sees_from = a.window ? qpos - a.window : -1, sees_to = a.window ? a.sinks : 0;   // keys <= qpos that are > sees_from or < sees_to
+
+    // where piece p of row r of a tile is kept: K by all pieces of a row, V by pairs of pieces (a transposing read takes 32 bytes of eight rows)
+    auto k_at = [](int r, int p) { return HD == 128 ? p ^ (r & 15) : p ^ (r & 7); };
+    auto v_at = [](int r, int p) { return HD == 128 ? p ^ ((r & 7) << 1) : p ^ (((r >> 1) & 3) << 1); };
+
+    // this wavefront's rows of a tile: 16 * wave and on
+    auto page_of = [&](int i) { return i < i_hi ? page_uniform(a.pb, it.b, keys.tile(i) * PAGED_KEYS + wave * 16) : -1; };
+    auto row_of = [&](int i, int id) { return paged_row(a.pb, KV, max(id, 0), g, keys.tile(i) * PAGED_KEYS + wave * 16); };   // a missing page: page 0, masked
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds + wave * LOADS * 1024;
+    const int lrow = lane / PPR, lp = lane % PPR;
+    auto issue = [&](int i, int id, int buf) {                 // fp16
+      const uint32_t to = lds0 + buf * BUF;
+      const size_t at = row_of(i, id) * ROWB;
+      const i4_t rk = dma_rsrc((const unsigned char *)a.pages_k + at), rv = dma_rsrc((const unsigned char *)a.pages_v + at);
 #pragma unroll
-    for (int c = 0; c < CPT; c++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        u4_t k, v;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          uint32_t lo, hi;
-          i8x4_to_h2x2(kc[c][2 * h + e], lo, hi);
-          k[2 * e] = lo; k[2 * e + 1] = hi;
-          i8x4_to_h2x2(vc[c][2 * h + e], lo, hi);
-          v[2 * e] = lo; v[2 * e + 1] = hi;
-        }
-        const int p = (cp + c) * 2 + h;
-        *(u4_t *)(kt + r * ROWB + k_at(r, p) * 16) = k;
-        *(u4_t *)(vt + r * ROWB + v_at(r, p) * 16) = v;
+      for (int j = 0; j < LOADS; j++) {
+        const int r = j * RPL + lrow;
+        dma16(rk, (uint32_t)r * ROWB + k_at(wave * 16 + r, lp) * 16, 0, to + j * 1024);
+        dma16(rv, (uint32_t)r * ROWB + v_at(wave * 16 + r, lp) * 16, 0, to + TILE + j * 1024);
       }
-    if (lane < 16) scl[buf][0][wave * 16 + lane] = sc * a.scale_log2;
-    else if (lane < 32) {
-      // A scale that is not a number makes the weights so, for the rows that see it.  Its reciprocal meets weights of zero as well, there and where
-      // nothing was ever written, and has to be finite.
-      scl[buf][1][wave * 16 + lane - 16] = __builtin_amdgcn_logf(sc);
-      scl[buf][2][wave * 16 + lane - 16] = sc >= 1e-38f && sc < INFINITY ? 1.0f / sc : 1.0f;
-    }
-    if (lane == 0) here[buf][wave] = id >= 0;
-  };
-
-  int id = page_of(i_lo), id_next = page_of(i_lo + 1);
-  if (i_lo < i_hi) {
-    if constexpr (I8) load(i_lo, id);
-    else issue(i_lo, id, 0);
-  }
-  // query row fragments: chunk c covers features [16c, 16c+16), the lane half picks 8 of them
-  h8_t qf[HD / 16];
-  {
-    const _Float16 *qp = a.q + q_off + lg * 8;
+    };
+    u4_t kc[CPT], vc[CPT];                                     // int8: this thread's codes and scale on their way
+    float sc = 1.0f;
+    const int crow = lane >> 2, cp = (lane & 3) * CPT;         // row and first piece of codes
+    auto load = [&](int i, int id) {
+      const size_t row = row_of(i, id);
 #pragma unroll
-    for (int c = 0; c < HD / 16; c++) qf[c] = *(const h8_t *)(qp + c * 16);
-  }
-#pragma unroll
-  for (int c = 0; c < HD / 16; c++) asm volatile("" : "+v"(qf[c]));   // waited for here, in front of the loop
-  if constexpr (I8)
-    if (i_lo < i_hi) store(id, 0);
-
-  f16_t o_acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; t++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) o_acc[t][r] = 0.0f;
-  // the maximum starts finite: a part of the keys may hold none that a row sees, and -inf minus -inf is not a number
-  float m_run = -1e30f, l_run = 0.0f;
-  const float unit = I8 ? 1.0f : a.scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
-
-  // K fragment of key l32 (+ 32): chunk 2c + lg of its row; V: lane -> row (lane / 4 % 4) of its half's four keys, 8 bytes
-  const unsigned char *const kp = lds + l32 * ROWB;
-  const int vrow = 4 * lg + ((lane >> 2) & 3), vcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;   // byte column inside 64 (32 features)
-
-  // A tile that every row of the block sees whole, or one with the tests; returns after the next tile has been asked for and this one used.
-  const int blk_lo = p0 + a.n_rep.div(q0), blk_hi = p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1);
-  int i = i_lo, buf = 0, pm = 0;
-  auto begin = [&]() {                                       // tile i is there, everyone is done with tile i - 1; whether all of the block sees all of it
-    if constexpr (!I8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();
-    id = id_next;
-    if (i + 1 < i_hi) {
-      if constexpr (I8) load(i + 1, id);
-      else issue(i + 1, id, buf ^ 1);
-      id_next = page_of(i + 2);
-    }
-    const int4 hv = *(const int4 *)here[buf];
-    pm = __builtin_amdgcn_readfirstlane(hv.x | hv.y << 1 | hv.z << 2 | hv.w << 3);
-    const int k0 = keys.tile(i) * PAGED_KEYS;
-    return k0 + PAGED_KEYS - 1 <= blk_lo && pm == 15 && !(a.window && k0 <= blk_hi - a.window && k0 + PAGED_KEYS > a.sinks);
-  };
-  auto end = [&]() {
-    if constexpr (I8)
-      if (i + 1 < i_hi) store(id, buf ^ 1);
-    i++;
-    buf ^= 1;
-  };
-  auto tile = [&](auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    const int k0 = keys.tile(i) * PAGED_KEYS;
-    auto sees = [&](int key) { return (key <= qpos) & ((key > sees_from) | (key < sees_to)); };
-    // S^T tile: 64 keys x 32 query rows
-    f16_t s[2];
-#pragma unroll
-    for (int tk = 0; tk < 2; tk++) {
-#pragma unroll
-      for (int r = 0; r < 16; r++) s[tk][r] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < HD / 16; c++) {
-        const h8_t kf = *(const h8_t *)(kp + buf * BUF + tk * 32 * ROWB + k_at(l32, 2 * c + lg) * 16);
-        s[tk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], s[tk], 0, 0, 0);
+      for (int c = 0; c < CPT; c++) {
+        kc[c] = *as_global<u4_t>((const int8_t *)a.pages_k + (row + crow) * HD + (cp + c) * 16);
+        vc[c] = *as_global<u4_t>((const int8_t *)a.pages_v + (row + crow) * HD + (cp + c) * 16);
       }
-    }
-    // accumulator r of s[tk] is key k0 + tk*32 + 8*(r/4) + 4*lg + r%4 for query row l32
-    f4_t inv_v[2][4];
-    if constexpr (I8) {
+      sc = *as_global<float>((lane & 16 ? a.scales_v : a.scales_k) + row + (lane & 15));
+    };
+    auto store = [&](int buf) {
+      unsigned char *const kt = lds + buf * BUF, *const vt = kt + TILE;
+      const int r = wave * 16 + crow;
 #pragma unroll
-      for (int tk = 0; tk < 2; tk++)
+      for (int c = 0; c < CPT; c++)
 #pragma unroll
-        for (int r4 = 0; r4 < 4; r4++) {
-          const int at = tk * 32 + 8 * r4 + 4 * lg;
-          const f4_t ks = *(const f4_t *)&scl[buf][0][at], lv = *(const f4_t *)&scl[buf][1][at];
-          inv_v[tk][r4] = *(const f4_t *)&scl[buf][2][at];
-#pragma unroll
-          for (int e = 0; e < 4; e++) s[tk][r4 * 4 + e] = __builtin_fmaf(s[tk][r4 * 4 + e], ks[e], lv[e]);
-        }
-    }
-    if constexpr (!WHOLE) {
-#pragma unroll
-      for (int tk = 0; tk < 2; tk++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int key = k0 + tk * 32 + 8 * (r / 4) + 4 * lg + (r % 4);
-          s[tk][r] = sees(key) & ((pm >> (tk * 2 + r / 8) & 1) != 0) ? s[tk][r] : -INFINITY;
-        }
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int r = 1; r < 31; r += 2) mx = fmaxf(fmaxf(mx, s[r / 16][r % 16]), s[(r + 1) / 16][(r + 1) % 16]);
-    mx = max_xor32(fmaxf(mx, s[1][15])) * unit;
-    if (__builtin_amdgcn_ballot_w64(mx > m_run + PC_SLACK)) {
-      const float m = fmaxf(m_run, __builtin_ceilf(mx)), alpha = __builtin_amdgcn_exp2f(m_run - m);   // first visible tile: 0
-      m_run = m;
-      l_run *= alpha;
-#pragma unroll
-      for (int td = 0; td < NT; td++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
-    }
-    float psum[2] = {0.0f, 0.0f};
-    h8_t pf[2][2];
-#pragma unroll
-    for (int tk = 0; tk < 2; tk++)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        float p[2];
-#pragma unroll
-        for (int e = 0; e < 2; e++) p[e] = __builtin_amdgcn_exp2f(I8 ? s[tk][r + e] - m_run : __builtin_fmaf(s[tk][r + e], unit, -m_run));
-        const h2_t h = {(_Float16)p[0], (_Float16)p[1]};
-        pf[tk][r / 8][r % 8] = h[0];
-        pf[tk][r / 8][r % 8 + 1] = h[1];
-        // fp16 pages: the sum is of the rounded weights, which multiply V.  int8: of the float ones; a weight that a small scale makes vanish as a half still counts.
-        if constexpr (I8) {
-#pragma unroll
-          for (int e = 0; e < 2; e++) psum[e] = __builtin_fmaf(p[e], inv_v[tk][r / 4][(r + e) % 4], psum[e]);
-        } else {
-          psum[tk] = __builtin_amdgcn_fdot2(h, h2_t{(_Float16)1.0f, (_Float16)1.0f}, psum[tk], false);
-        }
-      }
-    l_run += psum[0] + psum[1];
-
-    // O^T += V^T . P^T : k-slot s' of lane half lg in step (tk, hs) is key tk*32 + hs*16 + 8*(s'/4) + 4*lg + s'%4
-    const unsigned char *const vt = lds + buf * BUF + TILE;
-    uint32_t bad = 0;
-#pragma unroll
-    for (int tk = 0; tk < 2; tk++)
-#pragma unroll
-      for (int hs = 0; hs < 2; hs++)
-#pragma unroll
-        for (int td = 0; td < NT; td++) {
-          s4_t v[2];
+        for (int h = 0; h < 2; h++) {
+          u4_t k, v;
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const int r = tk * 32 + hs * 16 + 8 * e + vrow, c = td * 64 + vcol;
-            v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vt + r * ROWB + v_at(r, c >> 4) * 16 + (c & 15)));
+            uint32_t lo, hi;
+            i8x4_to_h2x2(kc[c][2 * h + e], lo, hi);
+            k[2 * e] = lo; k[2 * e + 1] = hi;
+            i8x4_to_h2x2(vc[c][2 * h + e], lo, hi);
+            v[2 * e] = lo; v[2 * e + 1] = hi;
           }
-          h8_t vf = __builtin_bit_cast(h8_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-          if constexpr (!I8 && !WHOLE) {
-            u4_t w = __builtin_bit_cast(u4_t, vf);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const uint32_t t = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // the sign bit of halves that are not finite
-              bad |= t;
-              w[e] &= ~(t | (t - (t >> 15)));
-            }
-            vf = __builtin_bit_cast(h8_t, w);
-          }
-          o_acc[td] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[tk][hs], o_acc[td], 0, 0, 0);
+          const int p = (cp + c) * 2 + h;
+          *(u4_t *)(kt + r * ROWB + k_at(r, p) * 16) = k;
+          *(u4_t *)(vt + r * ROWB + v_at(r, p) * 16) = v;
         }
-    if constexpr (!I8 && !WHOLE) {
-      if (__builtin_amdgcn_ballot_w64(bad != 0)) {
-        for (int key = 0; key < PAGED_KEYS; key++) {
-          const bool seen = sees(k0 + key) && (pm >> (key >> 4) & 1);
+      if (lane < 16) scl[buf][0][wave * 16 + lane] = sc * a.scale_log2;
+      else if (lane < 32) {
+        // A scale that is not a number makes the weights so, for the rows that see it.  Its reciprocal meets weights of zero as well, there and where
+        // nothing was ever written, and has to be finite.
+        scl[buf][1][wave * 16 + lane - 16] = __builtin_amdgcn_logf(sc);
+        scl[buf][2][wave * 16 + lane - 16] = sc >= 1e-38f && sc < INFINITY ? 1.0f / sc : 1.0f;
+      }
+    };
+
+    int id = page_of(i_lo), id_next = page_of(i_lo + 1);
+    if (i_lo < i_hi) {
+      if constexpr (I8) load(i_lo, id);
+      else issue(i_lo, id, 0);
+    }
+    // whether some page of these tiles is not there
+    bool holes = false;
+    for (int n = i_lo * 4 + lane; n < i_hi * 4; n += 64) holes |= paged_page(a.pb, it.b, keys.tile(n >> 2) * PAGED_KEYS + (n & 3) * 16) < 0;
+    holes = __builtin_amdgcn_ballot_w64(holes) != 0;
+    // query row fragments: chunk c covers features [16c, 16c+16), the lane half picks 8 of them
+    h8_t qf[HD / 16];
+    {
+      const _Float16 *qp = a.q + q_off + lg * 8;
+#pragma unroll
+      for (int c = 0; c < HD / 16; c++) qf[c] = *(const h8_t *)(qp + c * 16);
+    }
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++) asm volatile("" : "+v"(qf[c]));   // waited for here, in front of the loop
+    if constexpr (I8)
+      if (i_lo < i_hi) store(0);
+
+    f16_t o_acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o_acc[t][r] = 0.0f;
+    // the maximum starts finite: a part of the keys may hold none that a row sees, and -inf minus -inf is not a number
+    float m_run = -1e30f, l_run = 0.0f;
+    const float unit = I8 ? 1.0f : a.scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
+
+    // K fragment of key l32 (+ 32): chunk 2c + lg of its row; V: lane -> row (lane / 4 % 4) of its half's four keys, 8 bytes
+    const unsigned char *const kp = lds + l32 * ROWB;
+    const int vrow = 4 * lg + ((lane >> 2) & 3), vcol = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;   // byte column inside 64 (32 features)
+
+    // A tile that every row of the block sees whole, or one with the tests; returns after the next tile has been asked for and this one used.
+    const int blk_lo = p0 + a.n_rep.div(q0), blk_hi = p0 + a.n_rep.div(min(q0 + PC_QROWS, rows) - 1);
+    int i = i_lo, buf = 0;
+    auto begin = [&]() {                                       // tile i is there, everyone is done with tile i - 1; whether all of the block sees all of it
+      if constexpr (!I8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      lds_barrier();
+      id = id_next;
+      if (i + 1 < i_hi) {
+        if constexpr (I8) load(i + 1, id);
+        else issue(i + 1, id, buf ^ 1);
+        id_next = page_of(i + 2);
+      }
+      const int k0 = keys.tile(i) * PAGED_KEYS;
+      return k0 + PAGED_KEYS - 1 <= blk_lo && !holes && !(a.window && k0 <= blk_hi - a.window && k0 + PAGED_KEYS > a.sinks);
+    };
+    auto end = [&]() {
+      if constexpr (I8)
+        if (i + 1 < i_hi) store(buf ^ 1);
+      i++;
+      buf ^= 1;
+    };
+    auto tile = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      const int k0 = keys.tile(i) * PAGED_KEYS;
+      auto sees = [&](int key) { return (key <= qpos) & ((key > sees_from) | (key < sees_to)); };
+      const unsigned char *const kt = kp + buf * BUF, *const vt = lds + buf * BUF + TILE;
+      h8_t pf[2][2];
+      uint32_t bad = 0;
+      int pm = 15;                                           // which of the tile's four pages of 16 rows are there
+      if (!WHOLE && holes) {
+        pm = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) pm |= (page_uniform(a.pb, it.b, k0 + 16 * u) >= 0) << u;
+      }
+      // scores of 32 keys: accumulator r is key k0 + tk*32 + 8*(r/4) + 4*lg + r%4 for query row l32
+      auto score = [&](int tk) {
+        f16_t s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+          const h8_t kf = *(const h8_t *)(kt + tk * 32 * ROWB + k_at(l32, 2 * c + lg) * 16);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[c], s, 0, 0, 0);
+        }
+        return s;
+      };
+      auto finish = [&](f16_t &s, int tk) {
+        if constexpr (I8) {
+#pragma unroll
+          for (int r4 = 0; r4 < 4; r4++) {
+            const int at = tk * 32 + 8 * r4 + 4 * lg;
+            const f4_t ks = *(const f4_t *)&scl[buf][0][at], lv = *(const f4_t *)&scl[buf][1][at];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[r4 * 4 + e] = __builtin_fmaf(s[r4 * 4 + e], ks[e], lv[e]);
+          }
+        }
+        if constexpr (!WHOLE) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int key = k0 + tk * 32 + 8 * (r / 4) + 4 * lg + (r % 4);
+            s[r] = sees(key) & ((pm >> (tk * 2 + r / 8) & 1) != 0) ? s[r] : -INFINITY;
+          }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
+        mx = max_xor32(fmaxf(mx, s[15])) * unit;
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + PC_SLACK)) {
+          const float m = fmaxf(m_run, __builtin_ceilf(mx)), alpha = __builtin_amdgcn_exp2f(m_run - m);   // first visible keys: 0
+          m_run = m;
+          l_run *= alpha;
 #pragma unroll
           for (int td = 0; td < NT; td++)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; r4++) {
-              const uint2 w = *(const uint2 *)(vt + key * ROWB + v_at(key, td * 4 + r4) * 16 + lg * 8);
+            for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
+          if (tk == 1) {
+            const _Float16 h = (_Float16)alpha;
+#pragma unroll
+            for (int u = 0; u < 2; u++) pf[0][u] *= h8_t{h, h, h, h, h, h, h, h};
+          }
+        }
+      };
+      auto weights = [&](const f16_t &s, int tk) {
+        float psum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+          f4_t inv_v;
+          if constexpr (I8) inv_v = *(const f4_t *)&scl[buf][2][tk * 32 + 8 * r4 + 4 * lg];
+#pragma unroll
+          for (int e2 = 0; e2 < 4; e2 += 2) {
+            const int r = r4 * 4 + e2;
+            float p[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) p[e] = __builtin_amdgcn_exp2f(I8 ? s[r + e] - m_run : __builtin_fmaf(s[r + e], unit, -m_run));
+            const h2_t h = {(_Float16)p[0], (_Float16)p[1]};
+            pf[tk][r / 8][r % 8] = h[0];
+            pf[tk][r / 8][r % 8 + 1] = h[1];
+            // fp16 pages: the sum is of the rounded weights, which multiply V.  int8: of the float ones; a weight that a small scale makes vanish as a half still counts.
+            if constexpr (I8) {
+#pragma unroll
+              for (int e = 0; e < 2; e++) psum[e] = __builtin_fmaf(p[e], inv_v[e2 + e], psum[e]);
+            } else {
+              psum[r4 & 1] = __builtin_amdgcn_fdot2(h, h2_t{(_Float16)1.0f, (_Float16)1.0f}, psum[r4 & 1], false);
+            }
+          }
+        }
+        l_run += psum[0] + psum[1];
+      };
+      auto weigh = [&](int tk) {
+#pragma unroll
+        for (int hs = 0; hs < 2; hs++)
+#pragma unroll
+          for (int td = 0; td < NT; td++) {
+            s4_t v[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int r = tk * 32 + hs * 16 + 8 * e + vrow, c = td * 64 + vcol;
+              v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vt + r * ROWB + v_at(r, c >> 4) * 16 + (c & 15)));
+            }
+            h8_t vf = __builtin_bit_cast(h8_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            if constexpr (!I8 && !WHOLE) {
+              u4_t w = __builtin_bit_cast(u4_t, vf);
 #pragma unroll
               for (int e = 0; e < 4; e++) {
-                const uint32_t h = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
-                o_acc[td][r4 * 4 + e] += seen && (h & 0x7c00u) == 0x7c00u ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : 0.0f;
+                const uint32_t t = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // the sign bit of halves that are not finite
+                bad |= t;
+                w[e] &= ~(t | (t - (t >> 15)));
               }
+              vf = __builtin_bit_cast(h8_t, w);
             }
+            o_acc[td] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[tk][hs], o_acc[td], 0, 0, 0);
+          }
+      };
+      f16_t s0 = score(0);
+      finish(s0, 0);
+      f16_t s1 = score(1);
+      weights(s0, 0);
+      finish(s1, 1);
+      weigh(0);
+      weights(s1, 1);
+      weigh(1);
+      if constexpr (!I8 && !WHOLE) {
+        if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+          for (int key = 0; key < PAGED_KEYS; key++) {
+            const bool seen = sees(k0 + key) && (pm >> (key >> 4) & 1);
+#pragma unroll
+            for (int td = 0; td < NT; td++)
+#pragma unroll
+              for (int r4 = 0; r4 < 4; r4++) {
+                const uint2 w = *(const uint2 *)(vt + key * ROWB + v_at(key, td * 4 + r4) * 16 + lg * 8);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  const uint32_t h = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
+                  o_acc[td][r4 * 4 + e] += seen && (h & 0x7c00u) == 0x7c00u ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : 0.0f;
+                }
+              }
+          }
         }
       }
+    };
+    // every key of the tile is masked for this wavefront (uniform)
+    auto idle = [&]() {
+      const int k0 = keys.tile(i) * PAGED_KEYS;
+      return k0 > pos_hi || (a.window && k0 + PAGED_KEYS - 1 <= pos_lo - a.window && k0 >= a.sinks);
+    };
+    // Two loops, and each with its own copy of the accumulators' life: in one loop with both kinds of tiles they are copied twice a tile.
+    bool whole = i < i_hi && begin();
+    while (i < i_hi) {
+      while (i < i_hi && whole) {
+        tile(std::true_type());
+        end();
+        if (i < i_hi) whole = begin();
+      }
+      while (i < i_hi && !whole) {
+        if (!idle()) tile(std::false_type());
+        end();
+        if (i < i_hi) whole = begin();
+      }
     }
-  };
-  // every key of the tile is masked for this wavefront (uniform)
-  auto idle = [&]() {
-    const int k0 = keys.tile(i) * PAGED_KEYS;
-    return k0 > pos_hi || (a.window && k0 + PAGED_KEYS - 1 <= pos_lo - a.window && k0 >= a.sinks);
-  };
-  // Two loops, and each with its own copy of the accumulators' life: in one loop with both kinds of tiles they are copied twice a tile.
-  bool whole = i < i_hi && begin();
-  while (i < i_hi) {
-    while (i < i_hi && whole) {
-      tile(std::true_type());
-      end();
-      if (i < i_hi) whole = begin();
-    }
-    while (i < i_hi && !whole) {
-      if (!idle()) tile(std::false_type());
-      end();
-      if (i < i_hi) whole = begin();
-    }
-  }
 
-  if (it.parts > 1) {
-    // Sums cross compute units on different XCDs: device-scope stores and loads (cache policy 16), counted once they are
-    // acknowledged (the offset in the vector register, see sum_parts in gemm_tile.hip).
-    constexpr int VALS = (HD / 2 + 4) * 64;                   // floats of one wavefront: O^T, then (m, l)
-    const uint32_t slot = (uint32_t)VALS * 4 * 4, step = (uint32_t)KV * slot;
-    const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.ws + ((size_t)it.slot * 4 + wave) * VALS, (uint32_t)(it.parts - 1) * step + VALS * 4);
-    const uint32_t mine = (uint32_t)it.part * step + lane * 16;
+    if (it.parts > 1) {
+      // Sums cross compute units on different XCDs: device-scope stores and loads (cache policy 16), counted once they are
+      // acknowledged (the offset in the vector register, see sum_parts in gemm_tile.hip).
+      constexpr int VALS = (HD / 2 + 4) * 64;                   // floats of one wavefront: O^T, then (m, l)
+      const uint32_t slot = (uint32_t)VALS * 4 * 4, step = (uint32_t)KV * slot;
+      const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.ws + ((size_t)it.slot * 4 + wave) * VALS, (uint32_t)(it.parts - 1) * step + VALS * 4);
+      const uint32_t mine = (uint32_t)it.part * step + lane * 16;
+#pragma unroll
+      for (int td = 0; td < NT; td++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+          const f4_t v = {o_acc[td][r4 * 4], o_acc[td][r4 * 4 + 1], o_acc[td][r4 * 4 + 2], o_acc[td][r4 * 4 + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), rw, mine + (td * 4 + r4) * 1024, 0, 16);
+        }
+      const f4_t ml = {m_run, l_run, 0.0f, 0.0f};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, ml), rw, mine + NT * 4 * 1024, 0, 16);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      int old = 0;
+      if (lane == 0) old = __hip_atomic_fetch_add(&a.counters[it.slot * 4 + wave], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      old = __builtin_amdgcn_readfirstlane(old);
+      if (old != it.parts - 1) return;
+      if (lane == 0) __hip_atomic_store(&a.counters[it.slot * 4 + wave], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+      // two parts per round trip; past the last part the last one again, with weight zero
+      m_run = -1e30f;
+      l_run = 0.0f;
+#pragma unroll
+      for (int td = 0; td < NT; td++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o_acc[td][r] = 0.0f;
+      for (int f = 0; f < it.parts; f += 2) {
+        f4_t w[2], v[2][NT * 4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const uint32_t from = (uint32_t)min(f + u, it.parts - 1) * step + lane * 16;
+          w[u] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + NT * 4 * 1024, 0, 16));
+#pragma unroll
+          for (int j = 0; j < NT * 4; j++) v[u][j] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + j * 1024, 0, 16));
+        }
+        const float m = fmaxf(m_run, fmaxf(w[0][0], w[1][0]));
+        const float e = __builtin_amdgcn_exp2f(m_run - m);
+        const float e0 = __builtin_amdgcn_exp2f(w[0][0] - m);   // a part without a visible key: 0
+        const float e1 = f + 1 < it.parts ? __builtin_amdgcn_exp2f(w[1][0] - m) : 0.0f;
+        m_run = m;
+        l_run = l_run * e + (w[0][1] * e0 + w[1][1] * e1);
+#pragma unroll
+        for (int j = 0; j < NT * 4; j++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) o_acc[j / 4][(j % 4) * 4 + x] = o_acc[j / 4][(j % 4) * 4 + x] * e + (v[0][j][x] * e0 + v[1][j][x] * e1);
+      }
+    }
+
+    const float l = add_xor32(l_run), inv = l == 0.0f ? 0.0f : 1.0f / l;   // 0: the row sees nothing
+    _Float16 *op = a.out + q_off;
 #pragma unroll
     for (int td = 0; td < NT; td++)
 #pragma unroll
-      for (int r4 = 0; r4 < 4; r4++) {
-        const f4_t v = {o_acc[td][r4 * 4], o_acc[td][r4 * 4 + 1], o_acc[td][r4 * 4 + 2], o_acc[td][r4 * 4 + 3]};
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), rw, mine + (td * 4 + r4) * 1024, 0, 16);
+      for (int j = 0; j < 2; j++) {
+        // a lane half holds four of every eight neighbouring features; the halves exchange, so that each has all eight of every other group
+        uint32_t w[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const h2_t h = {(_Float16)(o_acc[td][(2 * j + u) * 4 + 2 * e] * inv), (_Float16)(o_acc[td][(2 * j + u) * 4 + 2 * e + 1] * inv)};
+            w[u][e] = __builtin_bit_cast(uint32_t, h);
+          }
+        const auto lo = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+        const u4_t v = {lo[0], hi[0], lo[1], hi[1]};
+        if (q_valid) *(u4_t *)(op + td * 32 + 16 * j + 8 * lg) = v;
       }
-    const f4_t ml = {m_run, l_run, 0.0f, 0.0f};
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, ml), rw, mine + NT * 4 * 1024, 0, 16);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    int old = 0;
-    if (lane == 0) old = __hip_atomic_fetch_add(&a.counters[it.slot * 4 + wave], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    old = __builtin_amdgcn_readfirstlane(old);
-    if (old != it.parts - 1) return;
-    if (lane == 0) __hip_atomic_store(&a.counters[it.slot * 4 + wave], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
-    // two parts per round trip; past the last part the last one again, with weight zero
-    m_run = -1e30f;
-    l_run = 0.0f;
-#pragma unroll
-    for (int td = 0; td < NT; td++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) o_acc[td][r] = 0.0f;
-    for (int f = 0; f < it.parts; f += 2) {
-      f4_t w[2], v[2][NT * 4];
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const uint32_t from = (uint32_t)min(f + u, it.parts - 1) * step + lane * 16;
-        w[u] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + NT * 4 * 1024, 0, 16));
-#pragma unroll
-        for (int j = 0; j < NT * 4; j++) v[u][j] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, from + j * 1024, 0, 16));
-      }
-      const float m = fmaxf(m_run, fmaxf(w[0][0], w[1][0]));
-      const float e = __builtin_amdgcn_exp2f(m_run - m);
-      const float e0 = __builtin_amdgcn_exp2f(w[0][0] - m);   // a part without a visible key: 0
-      const float e1 = f + 1 < it.parts ? __builtin_amdgcn_exp2f(w[1][0] - m) : 0.0f;
-      m_run = m;
-      l_run = l_run * e + (w[0][1] * e0 + w[1][1] * e1);
-#pragma unroll
-      for (int j = 0; j < NT * 4; j++)
-#pragma unroll
-        for (int x = 0; x < 4; x++) o_acc[j / 4][(j % 4) * 4 + x] = o_acc[j / 4][(j % 4) * 4 + x] * e + (v[0][j][x] * e0 + v[1][j][x] * e1);
-    }
   }
-
-  const float l = add_xor32(l_run), inv = l == 0.0f ? 0.0f : 1.0f / l;   // 0: the row sees nothing
-  _Float16 *op = a.out + q_off;
-#pragma unroll
-  for (int td = 0; td < NT; td++)
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      // a lane half holds four of every eight neighbouring features; the halves exchange, so that each has all eight of every other group
-      uint32_t w[2][2];
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const h2_t h = {(_Float16)(o_acc[td][(2 * j + u) * 4 + 2 * e] * inv), (_Float16)(o_acc[td][(2 * j + u) * 4 + 2 * e + 1] * inv)};
-          w[u][e] = __builtin_bit_cast(uint32_t, h);
-        }
-      const auto lo = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-      const auto hi = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-      const u4_t v = {lo[0], hi[0], lo[1], hi[1]};
-      if (q_valid) *(u4_t *)(op + td * 32 + 16 * j + 8 * lg) = v;
-    }
-}
+};
 
 // ---------------------------------------------------------------- one or a few new rows
 //
@@ -770,7 +795,7 @@ template <int HD, bool I8> struct PagedFew {
     }
     // Parts: sums through memory at device scope (cache policy 16), counted once they are acknowledged; the last block of the item folds them in order.
     const uint32_t part_bytes = (uint32_t)KV * SLOT * 4;
-    const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.ws + (size_t)it.slot * SLOT, (uint32_t)(it.parts - 1) * part_bytes + SLOT * 4);
+    const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.few_ws + (size_t)it.slot * SLOT, (uint32_t)(it.parts - 1) * part_bytes + SLOT * 4);
     for (int i = tid; i < pieces; i += PF_THREADS) {
       f4_t sum;
       float M, L;
@@ -784,10 +809,10 @@ template <int HD, bool I8> struct PagedFew {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (tid == 0) sm.is_last = __hip_atomic_fetch_add(&a.counters[it.slot], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.parts - 1;
+    if (tid == 0) sm.is_last = __hip_atomic_fetch_add(&a.few_counters[it.slot], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.parts - 1;
     __syncthreads();
     if (!sm.is_last) return;
-    if (tid == 0) __hip_atomic_store(&a.counters[it.slot], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+    if (tid == 0) __hip_atomic_store(&a.few_counters[it.slot], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
     // weights of the parts: a wavefront per row, a part per lane
     for (int r = wave; r < nr; r += NW) {
       const f4_t ml = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, (uint32_t)min(lane, it.parts - 1) * part_bytes + (PF_QROWS * HD + r * 4) * 4, 0, 16));
@@ -828,11 +853,32 @@ template <int HD, bool I8> struct PagedFew {
   }
 };
 
+// Parts cost their merge: as many as the root of the tiles, some more.  (us, 64 rows behind 1936, heads of 128, least part and most parts 8 tiles, sqrt(t) | 4, sqrt(t) | 4, sqrt(2 t): 22.8 | 21.5 |
+// 20.5; 57 behind 1024 18.4 | 17.1 | 17.3; one row behind 8000, heads of 64, 1 | 2 | 4 sqrt(t) / 2 .. 64 parts: 17.9 | 14.7 | 12.1, 2 sqrt(t) 10.5, 64 parts 14.1.)
+__device__ __forceinline__ int chunk_parts(int tiles) { return (int)__builtin_amdgcn_sqrtf(2.0f * (float)tiles); }
+__device__ __forceinline__ int few_parts(int tiles) { return min(PF_MOST, (int)(2.0f * __builtin_amdgcn_sqrtf((float)tiles))); }
+
+// Every sequence by the few-row blocks: 16 pairs and fewer per sequence and kv head, on the whole.
 template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4 : I8 ? 3 : 2) void attn_paged_few_kernel(PagedAttnArgs a) {
   typedef PagedFew<HD, I8> A;
   __shared__ typename A::Smem sm;
   PagedItem it;
-  if (paged_item<PF_QROWS>(a, [](int tiles) { return min(PF_MOST, (int)(2.0f * __builtin_amdgcn_sqrtf((float)tiles))); }, it)) A::item(a, it, sm);
+  int id = blockIdx.x;
+  if (paged_item<PF_QROWS>(a, id, 1, 0x7fffffff, a.few_blocks, PF_LEAST, few_parts, it)) A::item(a, it, sm);
+}
+
+// Chunks, and beside them the sequences that have a few rows: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
+// block for every compute unit, and the chunks' blocks beside them, as many again.  us, 512 rows behind 1792 and 30 sequences of up to 2304 with one each, heads of 128, fp16 | int8: chunks
+// alone 38 | 50, the others alone 40 | 25; chunks first, two blocks to a unit 84 | 71; the others first 66 | 71, and one block of each to a unit 57 | 64.
+template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn_paged_chunk_kernel(PagedAttnArgs a) {
+  __shared__ union {
+    typename PagedChunk<HD, I8>::Smem chunk;
+    typename PagedFew<HD, I8>::Smem few;
+  } sm;
+  PagedItem it;
+  int id = blockIdx.x;
+  if (paged_item<PF_QROWS>(a, id, 1, PF_QROWS, PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
+  else if (paged_item<PC_QROWS>(a, id, PF_QROWS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
 }
 
 }  // namespace jsg
@@ -841,11 +887,13 @@ using namespace jsg;
 
 extern "C" {
 
+// counters of chunks (one for each of a block's wavefronts) and of few-row items, then the sums of cut items, one slot for every part
+static size_t counter_bytes() { return ((size_t)PC_SLOTS * 4 + PF_SLOTS) * sizeof(int); }
+static size_t chunk_sums(int head_dim) { return (size_t)PC_SLOTS * 4 * (head_dim / 2 + 4) * 64; }
+static size_t few_sums(int head_dim) { return (size_t)PF_SLOTS * PF_QROWS * (head_dim + 4); }
 size_t jsgrad_hip_attn_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
-  // counters, then the sums of cut items, one slot for every part: those of chunks are the larger ones
   (void)n_heads, (void)n_kv_heads;
-  static_assert(PF_SLOTS * PF_QROWS <= PC_SLOTS * 4 * 32 && PF_SLOTS <= PC_SLOTS * 4, "the few-row kernel's parts fit where the chunk kernel's do");
-  return (size_t)PC_SLOTS * 4 * sizeof(int) + (size_t)PC_SLOTS * 4 * (head_dim / 2 + 4) * 64 * sizeof(float);
+  return counter_bytes() + (chunk_sums(head_dim) + few_sums(head_dim)) * sizeof(float);
 }
 
 int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out,
@@ -871,17 +919,19 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   a.sinks = sinks < 1 << 30 ? sinks : 1 << 30;
   a.scale_log2 = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
   a.counters = (int *)workspace;
-  a.ws = (float *)((char *)workspace + (size_t)PC_SLOTS * 4 * sizeof(int));
+  a.few_counters = a.counters + PC_SLOTS * 4;
+  a.ws = (float *)((char *)workspace + counter_bytes());
+  a.few_ws = a.ws + chunk_sums(HD);
+  // 64 KB on their way to a compute unit are enough: one block of fp16 rows of 128, else two
+  const bool i8 = host_pages->kind == JSGRAD_W_I8;
+  a.few_blocks = HD == 128 && !i8 ? PF_BLOCKS / 2 : PF_BLOCKS;
   // As many blocks as there may be items and parts: every sequence fills its last q tile at worst, and what is no longer than the least part is not cut.
-  const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS;
-  auto most_blocks = [&](int q_rows, int least, int slots) { return (size_t)KV * ((size_t)rows * n_rep / q_rows + (n_seqs < rows ? n_seqs : rows)) + (room_tiles > least ? slots : 0); };
   const bool few = (size_t)rows * n_rep <= (size_t)PF_QROWS * n_seqs;
-  a.blocks = !few ? PC_BLOCKS : HD == 128 && host_pages->kind == JSGRAD_W_F16 ? PF_BLOCKS / 2 : PF_BLOCKS;
-  a.least = few ? PF_LEAST : PC_LEAST;
-  const size_t blocks = few ? most_blocks(PF_QROWS, PF_LEAST, PF_SLOTS) : most_blocks(PC_QROWS, PC_LEAST, PC_SLOTS);
+  const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS;
+  const size_t blocks = (size_t)KV * ((size_t)rows * n_rep / (few ? PF_QROWS : PC_QROWS) + (n_seqs < rows ? n_seqs : rows)) +
+                        (!few && room_tiles > PC_LEAST ? PC_SLOTS : 0) + (room_tiles > PF_LEAST ? PF_SLOTS : 0);
   JSG_REQUIRE(blocks < PAGED_MOST, "%s: %d rows of %d heads", who, rows, n_heads);
   const dim3 grid((unsigned)blocks);
-  const bool i8 = host_pages->kind == JSGRAD_W_I8;
 #define JSG_PAGED(KERNEL, THREADS)                                                                    \
   do {                                                                                                \
     if (HD == 64 && i8) JSG_LAUNCH(PROF_ATTN_PAGED, (KERNEL<64, true>), grid, dim3(THREADS), 0, a);     \

@@ -191,6 +191,18 @@ def test_attention_of_a_ragged_batch(hip, kind, hd, H, KV, page, news, lens, win
 
 
 @pytest.mark.parametrize("kind", ["float16", "int8"])
+@pytest.mark.parametrize("hd,H,KV,news,lens", [(64, 8, 2, [1], [300]), (128, 8, 2, [1, 1], [70, 200]), (64, 8, 2, [3, 0, 40], [3, 9, 700]), (128, 4, 4, [16], [90]), (128, 4, 4, [17, 16], [90, 400]),
+                                                (64, 34, 2, [1, 1], [200, 50])])
+def test_a_batch_filled_up_with_rows_that_no_sequence_has(hip, kind, hd, H, KV, news, lens):
+    """As a captured graph's batch is: many more rows than the sequences have, and sequences with none; both kinds of blocks in a launch."""
+    rng = np.random.default_rng(hd + len(news))
+    c = Case(rng, kind, hd, KV, 16, news + [0] * 5, lens + [0, 7, 0, 100, 1], extra_rows=200).device()
+    q = rng.standard_normal((c.rows, H, hd)).astype(np.float16)
+    ref, tol = attention(c, q, H)
+    compare(run_attention(hip, c, q, H, 0, 0, times=2), ref, tol, int(c.starts[-1]))
+
+
+@pytest.mark.parametrize("kind", ["float16", "int8"])
 @pytest.mark.parametrize("hd,news,lens", [(64, [1, 1], [900, 64]), (128, [90, 1], [400, 33])])
 def test_large_scores_and_values_of_every_size(hip, kind, hd, news, lens):
     """Scores up to several hundred: one key has all the weight.  Values over eight orders of magnitude, those of int8 pages with scales as far apart."""
@@ -255,7 +267,8 @@ def test_pages_that_are_not_there(hip, kind):
 @pytest.mark.parametrize("kind,hd,H,KV,news,lens,window,sinks", [
     ("float16", 128, 8, 2, [1], [20011], 0, 0), ("int8", 64, 8, 2, [1, 1], [9000, 30], 0, 0), ("int8", 128, 8, 2, [3], [9000], 0, 0), ("float16", 64, 4, 2, [60], [6000], 0, 0),
     ("int8", 128, 32, 8, [100, 1, 1, 1], [2500, 4000, 5, 1200], 0, 0), ("float16", 64, 8, 2, [1], [20000], 9000, 100), ("float16", 128, 32, 8, [1] * 70, list(range(1, 1401, 20)), 0, 0),
-    ("int8", 64, 32, 8, [1] * 140, list(range(1, 1401, 10)), 0, 0), ("float16", 64, 8, 8, [2] * 65 + [40], list(range(2, 132, 2)) + [700], 0, 0),
+    ("int8", 64, 32, 8, [1] * 140, list(range(1, 1401, 10)), 0, 0), ("float16", 128, 32, 8, [300] + [1, 2, 4] * 7, [3000] + list(range(50, 2150, 100)), 0, 0),
+    ("int8", 128, 8, 2, [1, 900, 4, 40] + [1] * 66, [9000, 900, 4, 3000] + [77] * 66, 500, 70), ("float16", 64, 8, 8, [2] * 65 + [40], list(range(2, 132, 2)) + [700], 0, 0),
 ])
 def test_long_contexts_and_many_sequences(hip, kind, hd, H, KV, news, lens, window, sinks):
     """Keys in parts and their merge; more sequences than a wavefront has lanes.  A few rows and heads against float64, everything twice on one workspace."""
