@@ -13,6 +13,8 @@
 
 namespace jsg {
 
+constexpr int PR_THREADS = 256, PR_ROWS = 8;
+
 struct PagedArgs {
   PagedBatch pb;
   void *pages[2];                        // k, v
@@ -21,9 +23,10 @@ struct PagedArgs {
   _Float16 *y[3];                        // k, v, q rows out
   const _Float16 *rope;                  // [positions][HD/2][2] or null
   int n_kv_heads, n_heads;               // n_heads 0: no q
+  Divisor pieces;                        // of a row that is read: 8 elements of a head each
 };
 
-// Sequence of row r: the last one that begins at or before it.  Called by whole wavefronts with a uniform r: 64 first rows at a time.
+// Sequence of row r: the first one that ends behind it.  Called by whole wavefronts with a uniform r: 64 first rows at a time.
 __device__ __forceinline__ int paged_find(const PagedBatch &pb, int r) {
   const int lane = threadIdx.x & 63;
   for (int b0 = 0;; b0 += 64) {
@@ -42,8 +45,9 @@ template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
   return v;
 }
 
-// One block per row of the batch, a thread per 8 elements of a head: its heads are n_kv_heads of k, as many of v, then n_heads of q.
-template <int HD, bool I8> __global__ __launch_bounds__(256) void paged_write_kernel(PagedArgs a) {
+// Bound by memory: 32768 rows of 32 and 8 heads of 128, fp16 159 us = 5.1 TB/s, int8 170 (the quotients are divided out, so that a code is the nearest one: fp16 rows have many
+// that lie in the middle).  One block per row of the batch, a thread per 8 elements of a head: its heads are n_kv_heads of k, as many of v, then n_heads of q.
+template <int HD, bool I8> __global__ __launch_bounds__(PR_THREADS) void paged_write_kernel(PagedArgs a) {
   constexpr int G = HD / 8;
   const int r = blockIdx.x, KV = a.n_kv_heads, heads = 2 * KV + a.n_heads;
   const int b = paged_find(a.pb, r);
@@ -52,7 +56,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(256) void paged_write_ke
   const int pos = paged_pos(s, r - s.start);
   if (r < s.start || pos < 0 || pos >= paged_room(a.pb)) return;
   const int id = paged_page(a.pb, b, pos);
-  for (int i = threadIdx.x; i < heads * G; i += 256) {        // heads * G is a multiple of G: the lanes of a head stay together
+  for (int i = threadIdx.x; i < heads * G; i += PR_THREADS) {        // heads * G is a multiple of G: the lanes of a head stay together
     const int h = i / G, e0 = i % G * 8, which = h < KV ? 0 : h < 2 * KV ? 1 : 2, n = which == 2 ? a.n_heads : KV, g = h - which * KV;
     const h8_t x = *(const h8_t *)(a.x[which] + ((size_t)r * n + g) * HD + e0);
     float f[8];
@@ -94,7 +98,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(256) void paged_write_ke
 }
 
 // The same rows back: RN16(code * scale), zeros where there is no page.
-template <int HD, bool I8> __global__ __launch_bounds__(256) void paged_read_kernel(PagedArgs a) {
+template <int HD, bool I8> __global__ __launch_bounds__(PR_THREADS) void paged_read_kernel(PagedArgs a) {
   constexpr int G = HD / 8;
   const int r = blockIdx.x, KV = a.n_kv_heads;
   const int b = paged_find(a.pb, r);
@@ -103,7 +107,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(256) void paged_read_ker
   const int pos = paged_pos(s, r - s.start);
   if (r < s.start) return;
   const int id = paged_page(a.pb, b, pos);
-  for (int i = threadIdx.x; i < 2 * KV * G; i += 256) {
+  for (int i = threadIdx.x; i < 2 * KV * G; i += PR_THREADS) {
     const int h = i / G, e0 = i % G * 8, which = h < KV ? 0 : 1, g = h - which * KV;
     h8_t o = {};
     if (id >= 0) {
@@ -118,6 +122,86 @@ template <int HD, bool I8> __global__ __launch_bounds__(256) void paged_read_ker
       }
     }
     *(h8_t *)(a.y[which] + ((size_t)r * KV + g) * HD + e0) = o;
+  }
+}
+
+// Where a block's rows are.
+struct PagedRows {
+  size_t row[PR_ROWS];                   // of the pages, kv head 0
+  int pos[PR_ROWS];                      // -1: no sequence has the row, or its position lies outside the table
+  int id[PR_ROWS];                       // -1: no page
+};
+
+// Filled by a wavefront for itself: the sequences' arrays, one to a lane and 64 at a time, then a lane per row.  Two round trips to memory, the page numbers being the second.
+__device__ __forceinline__ void paged_rows(const PagedBatch &pb, int n_kv_heads, int r0, int n, PagedRows &to) {
+  const int lane = threadIdx.x & 63;
+  int b = -1, pos = -1;
+  for (int b0 = 0, done = 0; b0 < pb.n_seqs && done < n; b0 += 64) {
+    PagedSeq s = {0, 0, 0};
+    int end = 0x7fffffff;                                    // lanes past the last sequence
+    if (b0 + lane < pb.n_seqs) {
+      end = pb.row_starts[b0 + lane + 1];
+      s = paged_seq(pb.row_starts[b0 + lane], end, pb.lengths[b0 + lane], pb.rows);
+    }
+    for (; done < n; done++) {                               // the first sequence that ends behind the row
+      const uint64_t behind = __builtin_amdgcn_ballot_w64(end > r0 + done);
+      if (!behind) break;                                    // in the next 64
+      const int l = __builtin_ctzll(behind), start = __builtin_amdgcn_readlane(s.start, l), rows = __builtin_amdgcn_readlane(s.n, l);
+      const int at = r0 + done - start;
+      if (lane == done && at >= 0 && at < rows) {
+        b = b0 + l;
+        pos = __builtin_amdgcn_readlane(s.len, l) - rows + at;
+      }
+    }
+  }
+  if (lane < n) {
+    const bool in = b >= 0 && pos >= 0 && pos < paged_room(pb);
+    const int id = in ? paged_page(pb, b, pos) : -1;
+    to.pos[lane] = in ? pos : b >= 0 ? -2 : -1;              // -2: a sequence's row all the same, which is read as zeros
+    to.id[lane] = id;
+    to.row[lane] = id >= 0 ? paged_row(pb, n_kv_heads, id, 0, pos) : 0;
+  }
+}
+
+// PR_ROWS rows to a block, for batches with blocks enough all the same: more loads behind each look-up.
+template <int HD, bool I8> __global__ __launch_bounds__(PR_THREADS) void paged_read_rows_kernel(PagedArgs a) {
+  constexpr int G = HD / 8, U = 4;
+  __shared__ PagedRows all[PR_THREADS / 64];
+  PagedRows &at = all[threadIdx.x >> 6];
+  const int r0 = blockIdx.x * PR_ROWS, n_rows = min(PR_ROWS, a.pb.rows - r0), KV = a.n_kv_heads, total = n_rows * (int)a.pieces.d;
+  paged_rows(a.pb, KV, r0, n_rows, at);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // of this wavefront, in order
+  for (int i0 = threadIdx.x; i0 < total; i0 += U * PR_THREADS) {
+    h8_t v[U];
+    uint2 c[U];
+    float scale[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = min(i0 + u * PR_THREADS, total - 1), r = a.pieces.div(i), h = (i - r * (int)a.pieces.d) / G, which = h < KV ? 0 : 1;
+      // a row without a page asks for the first one's
+      const size_t row = at.row[r] + (at.id[r] >= 0 ? (size_t)(h - which * KV) << a.pb.page_shift : 0);
+      if constexpr (I8) {
+        c[u] = *(const uint2 *)((const int8_t *)a.pages[which] + row * HD + i % G * 8);
+        scale[u] = a.scales[which][row];
+      } else {
+        v[u] = *(const h8_t *)((const _Float16 *)a.pages[which] + row * HD + i % G * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * PR_THREADS, r = a.pieces.div(min(i, total - 1)), h = (i - r * (int)a.pieces.d) / G, which = h < KV ? 0 : 1;
+      if (i >= total || at.pos[r] == -1) continue;
+      h8_t o = {};
+      if (at.id[r] >= 0) {
+        if constexpr (I8) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) o[e] = mul_rn16((float)(int8_t)((e < 4 ? c[u].x : c[u].y) >> (8 * (e & 3))), scale[u]);
+        } else {
+          o = v[u];
+        }
+      }
+      *(h8_t *)(a.y[which] + ((size_t)(r0 + r) * KV + h - which * KV) * HD + i % G * 8) = o;
+    }
   }
 }
 
@@ -165,7 +249,7 @@ int jsgrad_hip_paged_write(const jsgrad_hip_pages_t *host_pages, const int32_t *
   a.y[2] = (_Float16 *)q_out;
   a.rope = (const _Float16 *)rope_table;
   a.n_kv_heads = host_pages->n_kv_heads; a.n_heads = q ? n_heads : 0;
-  const dim3 grid(rows), block(256);
+  const dim3 grid(rows), block(PR_THREADS);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
   if (host_pages->head_dim == 64 && i8) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<64, true>), grid, block, 0, a);
   else if (host_pages->head_dim == 64) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<64, false>), grid, block, 0, a);
@@ -185,12 +269,20 @@ int jsgrad_hip_paged_read(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   a.scales[0] = (float *)host_pages->scales_k; a.scales[1] = (float *)host_pages->scales_v;
   a.y[0] = (_Float16 *)k_out; a.y[1] = (_Float16 *)v_out;
   a.n_kv_heads = host_pages->n_kv_heads;
-  const dim3 grid(rows), block(256);
-  const bool i8 = host_pages->kind == JSGRAD_W_I8;
-  if (host_pages->head_dim == 64 && i8) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_read_kernel<64, true>), grid, block, 0, a);
-  else if (host_pages->head_dim == 64) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_read_kernel<64, false>), grid, block, 0, a);
-  else if (i8) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_read_kernel<128, true>), grid, block, 0, a);
-  else JSG_LAUNCH(PROF_PAGED_ROWS, (paged_read_kernel<128, false>), grid, block, 0, a);
+  a.pieces = divisor(2 * a.n_kv_heads * (host_pages->head_dim / 8));
+  // us, a row to a block | eight, 8 kv heads of 128: int8 2000 rows 4.8 | 6.5, 4096 6.8 | 8.0, fp16 9000 12.9 | 13.5, 32768 47.5 | 43.5 (6.2 TB/s), int8 32768 48 | 34.5 (5.9)
+  const bool i8 = host_pages->kind == JSGRAD_W_I8, several = rows > 12288;
+  const dim3 grid(several ? (rows + PR_ROWS - 1) / PR_ROWS : rows), block(PR_THREADS);
+#define JSG_READ(HD, I8)                                                                             \
+  do {                                                                                               \
+    if (several) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_read_rows_kernel<HD, I8>), grid, block, 0, a);     \
+    else JSG_LAUNCH(PROF_PAGED_ROWS, (paged_read_kernel<HD, I8>), grid, block, 0, a);                  \
+  } while (0)
+  if (host_pages->head_dim == 64 && i8) JSG_READ(64, true);
+  else if (host_pages->head_dim == 64) JSG_READ(64, false);
+  else if (i8) JSG_READ(128, true);
+  else JSG_READ(128, false);
+#undef JSG_READ
   return 0;
 }
 

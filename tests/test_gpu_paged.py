@@ -73,6 +73,32 @@ def test_rows_written_and_read_back(hip, kind, hd, H, KV, page, news, lens):
         assert np.all(read[n:] == 7)
 
 
+@pytest.mark.parametrize("kind,hd,KV,page,news,lens", [
+    ("float16", 64, 2, 16, [12800], [13000]), ("int8", 128, 2, 32, [5000, 0, 3, 8000, 1], [5000, 3, 3, 9000, 77]), ("int8", 64, 3, 256, [100] * 130 + [0] * 9, [120] * 130 + [5] * 9),
+    ("float16", 128, 1, 16, [1] * 20 + [12500] + [2] * 70, [9] * 20 + [12500] + [600] * 70),
+])
+def test_many_rows_read(hip, kind, hd, KV, page, news, lens):
+    """More than 12288 rows: eight to a block, of one sequence or several, some without a page, some that no sequence has."""
+    rng = np.random.default_rng(hd + KV)
+    c = Case(rng, kind, hd, KV, page, news, lens, extra_rows=13)
+    c.table[0, c.width // 2] = c.n_pages + 5
+    c.table[-1, 0] = -9
+    c.device()
+    out = [Tensor.full((c.rows + 1, KV, hd), 7.0, "float16") for _ in range(2)]
+    check(hip.jsgrad_hip_paged_read(*c.batch, out[0].ptr, out[1].ptr))
+    place = [c.places(b, l - m, l) for b, (m, l) in enumerate(zip(news, lens))]
+    ids, slots = (np.concatenate([p[i] for p in place]) for i in (0, 1))
+    n = int(c.starts[-1])
+    for name, t in zip("kv", out):
+        got = t.numpy()
+        if kind == "int8":
+            codes, scales = (c.ck, c.sk) if name == "k" else (c.cv, c.sv)
+            want = (codes[ids, :, slots].astype(np.float32) * scales[ids, :, slots][..., None]).astype(np.float16)
+        else:
+            want = getattr(c, name)[ids, :, slots]
+        assert np.array_equal(got[:n], np.where((ids < 0)[:, None, None], np.float16(0), want)) and np.all(got[n:] == 7)
+
+
 def test_a_write_without_rotation_queries_or_pages(hip):
     """No rope table: rows as they are.  No q: only the cache.  q_out may be q.  Rows without a page leave no trace and read as zeros; their queries are
     rotated all the same where the table has the position."""
