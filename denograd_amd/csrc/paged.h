@@ -74,13 +74,14 @@ template <typename Div> JSG_BOTH PagedShare paged_share(const PagedSeq &s, int n
   return h;
 }
 // Key tiles of a part where `blocks` parts have the same share of the launch's pairs of a q tile and a key tile.  An item of key_tiles > target, for a target of that and more,
-// is cut into ceil(key_tiles / target) parts or fewer; the parts of cut items are fewer than 2 * blocks, as each has half a target's pairs at least.
+// is cut into ceil(key_tiles / target) parts, one more at most, or fewer; the parts of cut items are no more than 2 * blocks, as each has half a target's pairs at least.
 JSG_BOTH int paged_target(float pairs, int blocks, int least) {
-  const float t = pairs * (1.0001f / (float)blocks);           // a little more than the share, whatever the rounding of the sum
+  const float t = pairs * (1.002f / (float)blocks);            // a little more than the share, for the rounding here and in the next
   return t < (float)least ? least : t < 1e9f ? (int)t + 1 : 1000000000;
 }
-JSG_BOTH int paged_parts(int key_tiles, int target, int most) {
-  const int n = key_tiles <= target ? 1 : (key_tiles + target - 1) / target;
+// inv: 1.0f / target
+JSG_BOTH int paged_parts(int key_tiles, int target, float inv, int most) {
+  const int n = key_tiles <= target ? 1 : (int)((float)(key_tiles - 1) * inv + 1e-3f) + 1;
   return n > most ? (most < 1 ? 1 : most) : n;
 }
 

@@ -50,23 +50,25 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {     // inclusive prefix
   return v;
 }
 
+// 64 sequences, one to a lane.
+__device__ __forceinline__ PagedSeq lane_seq(const PagedBatch &p, int b0) {
+  const int b = b0 + (threadIdx.x & 63);
+  return b < p.n_seqs ? paged_seq(p, b) : PagedSeq{0, 0, 0};
+}
+
 // The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head: blocks, least: see paged_target; most(key tiles): parts of an
 // item.  False, and id less these items' blocks, where it is none of them.
 template <int QROWS, typename Most>
-__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, int &id, int from, int to, int blocks, int least, Most most, PagedItem &it) {
-  const int lane = threadIdx.x & 63, room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSeq &first, int &id, int from, int to, int blocks, int least, Most most, PagedItem &it) {
+  const int room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
   const uint32_t want = (uint32_t)a.n_kv_heads.div(id);
   it.g = id - (int)want * KV;
   PagedSeq s;
   PagedShare h;
   auto look = [&](int b0) {
-    const int b = b0 + lane;
-    s = {0, 0, 0};
+    s = b0 ? lane_seq(a.pb, b0) : first;
     h = {0, 0};
-    if (b < a.pb.n_seqs) {
-      s = paged_seq(a.pb, b);
-      if (s.n * n_rep >= from && s.n * n_rep <= to) h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
-    }
+    if (s.n * n_rep >= from && s.n * n_rep <= to) h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
   };
   float pairs = 0.0f, items = 0.0f;
   for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
@@ -80,19 +82,20 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, int &id, int 
   // pairs makes up for that.  More: the first of some larger shares with which the parts are no more than the blocks; or twice the share, where nothing else is.
   const int share = paged_target(pairs, blocks, least);
   int target = 2 * share;
+  auto cut = [&](int t) { return paged_parts(h.key_tiles, t, __builtin_amdgcn_rcpf((float)t), most(h.key_tiles)); };
   if (items * 16.0f <= (float)blocks) target = share + share / 16;
   else if (a.pb.n_seqs <= 64 && items < (float)blocks)
     for (int t = share; t < 2 * share; t += (share + 3) / 4)
-      if (wave_sum((float)h.q_tiles * (float)paged_parts(h.key_tiles, t, most(h.key_tiles))) * (float)KV <= (float)blocks) {
+      if (wave_sum((float)h.q_tiles * (float)cut(t)) * (float)KV <= (float)blocks) {
         target = t;
         break;
       }
   uint32_t before = 0, slots = 0;
   for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
     if (a.pb.n_seqs > 64) look(b0);
-    const int parts = paged_parts(h.key_tiles, target, most(h.key_tiles));
+    const int parts = cut(target);
     const uint32_t mine = (uint32_t)min((uint64_t)h.q_tiles * parts, (uint64_t)PAGED_MOST);
-    const uint32_t upto = scan64(mine), cut = scan64(parts > 1 ? mine : 0);
+    const uint32_t upto = scan64(mine), held = scan64(parts > 1 ? mine : 0);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(before + upto > want);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -107,11 +110,11 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, int &id, int 
         it.qt = of(h.q_tiles) - 1 - nth / it.parts;
         it.part = nth % it.parts;
       }
-      it.slot = ((int)slots + of((int)(cut - (parts > 1 ? mine : 0))) + nth - it.part) * KV + it.g;
+      it.slot = ((int)slots + of((int)(held - (parts > 1 ? mine : 0))) + nth - it.part) * KV + it.g;
       return true;
     }
     before = min(before + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), PAGED_MOST);
-    slots = min(slots + (uint32_t)__builtin_amdgcn_readlane((int)cut, 63), PAGED_MOST);
+    slots = min(slots + (uint32_t)__builtin_amdgcn_readlane((int)held, 63), PAGED_MOST);
   }
   id -= (int)before * KV;
   return false;
@@ -157,6 +160,7 @@ template <int HD, bool I8> struct PagedChunk {
 
   // Must be called by every thread of the block (it contains barriers).
   static __device__ void item(const PagedAttnArgs &a, const PagedItem &it, Smem &sm) {
+    const float scale_log2 = a.scale_log2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lg = lane >> 5;
     unsigned char *const lds = sm.tiles;
     auto &scl = sm.scl;
@@ -198,6 +202,7 @@ template <int HD, bool I8> struct PagedChunk {
     };
     u4_t kc[CPT], vc[CPT];                                     // int8: this thread's codes and scale on their way
     float sc = 1.0f;
+    const float *const scales_k = a.scales_k, *const scales_v = a.scales_v;
     const int crow = lane >> 2, cp = (lane & 3) * CPT;         // row and first piece of codes
     auto load = [&](int i, int id) {
       const size_t row = row_of(i, id);
@@ -206,7 +211,7 @@ template <int HD, bool I8> struct PagedChunk {
         kc[c] = *as_global<u4_t>((const int8_t *)a.pages_k + (row + crow) * HD + (cp + c) * 16);
         vc[c] = *as_global<u4_t>((const int8_t *)a.pages_v + (row + crow) * HD + (cp + c) * 16);
       }
-      sc = *as_global<float>((lane & 16 ? a.scales_v : a.scales_k) + row + (lane & 15));
+      sc = *as_global<float>((lane & 16 ? scales_v : scales_k) + row + (lane & 15));
     };
     auto store = [&](int buf) {
       unsigned char *const kt = lds + buf * BUF, *const vt = kt + TILE;
@@ -228,12 +233,12 @@ template <int HD, bool I8> struct PagedChunk {
           *(u4_t *)(kt + r * ROWB + k_at(r, p) * 16) = k;
           *(u4_t *)(vt + r * ROWB + v_at(r, p) * 16) = v;
         }
-      if (lane < 16) scl[buf][0][wave * 16 + lane] = sc * a.scale_log2;
+      if (lane < 16) scl[buf][0][wave * 16 + lane] = sc * scale_log2;
       else if (lane < 32) {
         // A scale that is not a number makes the weights so, for the rows that see it.  Its reciprocal meets weights of zero as well, there and where
         // nothing was ever written, and has to be finite.
         scl[buf][1][wave * 16 + lane - 16] = __builtin_amdgcn_logf(sc);
-        scl[buf][2][wave * 16 + lane - 16] = sc >= 1e-38f && sc < INFINITY ? 1.0f / sc : 1.0f;
+        scl[buf][2][wave * 16 + lane - 16] = sc >= 1e-38f && sc < INFINITY ? __builtin_amdgcn_rcpf(sc) : 1.0f;
       }
     };
 
@@ -265,7 +270,7 @@ template <int HD, bool I8> struct PagedChunk {
       for (int r = 0; r < 16; r++) o_acc[t][r] = 0.0f;
     // the maximum starts finite: a part of the keys may hold none that a row sees, and -inf minus -inf is not a number
     float m_run = -1e30f, l_run = 0.0f;
-    const float unit = I8 ? 1.0f : a.scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
+    const float unit = I8 ? 1.0f : scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
 
     // K fragment of key l32 (+ 32): chunk 2c + lg of its row; V: lane -> row (lane / 4 % 4) of its half's four keys, 8 bytes
     const unsigned char *const kp = lds + l32 * ROWB;
@@ -357,24 +362,20 @@ template <int HD, bool I8> struct PagedChunk {
         float psum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int r4 = 0; r4 < 4; r4++) {
-          f4_t inv_v;
-          if constexpr (I8) inv_v = *(const f4_t *)&scl[buf][2][tk * 32 + 8 * r4 + 4 * lg];
+          const f4_t inv_v = I8 ? *(const f4_t *)&scl[buf][2][tk * 32 + 8 * r4 + 4 * lg] : f4_t{1.0f, 1.0f, 1.0f, 1.0f};
+          float p[4];
 #pragma unroll
-          for (int e2 = 0; e2 < 4; e2 += 2) {
-            const int r = r4 * 4 + e2;
-            float p[2];
+          for (int e = 0; e < 4; e++) p[e] = __builtin_amdgcn_exp2f(I8 ? s[r4 * 4 + e] - m_run : __builtin_fmaf(s[r4 * 4 + e], unit, -m_run));
 #pragma unroll
-            for (int e = 0; e < 2; e++) p[e] = __builtin_amdgcn_exp2f(I8 ? s[r + e] - m_run : __builtin_fmaf(s[r + e], unit, -m_run));
-            const h2_t h = {(_Float16)p[0], (_Float16)p[1]};
-            pf[tk][r / 8][r % 8] = h[0];
-            pf[tk][r / 8][r % 8 + 1] = h[1];
-            // fp16 pages: the sum is of the rounded weights, which multiply V.  int8: of the float ones; a weight that a small scale makes vanish as a half still counts.
-            if constexpr (I8) {
+          for (int e = 0; e < 4; e++) pf[tk][r4 / 2][r4 % 2 * 4 + e] = (_Float16)p[e];
+          // fp16 pages: the sum is of the rounded weights, which multiply V.  int8: of the float ones; a weight that a small scale makes vanish as a half still counts.
+          if constexpr (I8) {
 #pragma unroll
-              for (int e = 0; e < 2; e++) psum[e] = __builtin_fmaf(p[e], inv_v[e2 + e], psum[e]);
-            } else {
-              psum[r4 & 1] = __builtin_amdgcn_fdot2(h, h2_t{(_Float16)1.0f, (_Float16)1.0f}, psum[r4 & 1], false);
-            }
+            for (int e = 0; e < 4; e++) psum[e & 1] = __builtin_fmaf(p[e], inv_v[e], psum[e & 1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+              psum[r4 & 1] = __builtin_amdgcn_fdot2(h2_t{(_Float16)p[e], (_Float16)p[e + 1]}, h2_t{(_Float16)1.0f, (_Float16)1.0f}, psum[r4 & 1], false);
           }
         }
         l_run += psum[0] + psum[1];
@@ -555,6 +556,7 @@ template <int HD, bool I8> struct PagedFew {
   };
   // Must be called by every thread of the block (it contains barriers).
   static __device__ void item(const PagedAttnArgs &a, const PagedItem &it, Smem &sm) {
+    const float scale_log2 = a.scale_log2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
     const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d, room = paged_room(a.pb), g = it.g;
     const int rows = it.s.n * n_rep, p0 = paged_pos(it.s, 0), q0 = it.qt * PF_QROWS, nr = min(PF_QROWS, rows - q0);
@@ -620,7 +622,7 @@ template <int HD, bool I8> struct PagedFew {
 #pragma unroll
     for (int t = 0; t < NT; t++) o[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -1e30f, l_run = 0.0f;                      // finite: a step may hold no key that a row sees
-    const float unit = I8 ? 1.0f : a.scale_log2;
+    const float unit = I8 ? 1.0f : scale_log2;
     unsigned char *const vl = sm.wave[wave].v;
 
     auto step = [&](auto more) {
@@ -646,7 +648,7 @@ template <int HD, bool I8> struct PagedFew {
       }
       if constexpr (I8) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) ks[h] *= a.scale_log2;
+        for (int h = 0; h < 2; h++) ks[h] *= scale_log2;
       }
       const f4_t kscale[2] = {ks[0], ks[1]};
       if constexpr (decltype(more)::value) load_k(st + NW, next);
@@ -739,7 +741,7 @@ template <int HD, bool I8> struct PagedFew {
         // halves that are not finite: left out of the product, where a weight of zero would not stop them, and added for the rows that see them
         weigh(std::true_type());
         for (int key = 0; key < KEYS; key++) {
-          const bool seen = sees(k0 + key) && id[key >> 4] >= 0;
+          const bool seen = sees(k0 + key) && (key < 16 ? id[0] : id[1]) >= 0;
 #pragma unroll
           for (int t = 0; t < NT; t++) {
             const uint2 w = *(const uint2 *)(vl + key * VROW + t * 32 + 8 * lq);
@@ -863,8 +865,9 @@ template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4
   typedef PagedFew<HD, I8> A;
   __shared__ typename A::Smem sm;
   PagedItem it;
+  const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
-  if (paged_item<PF_QROWS>(a, id, 1, 0x7fffffff, a.few_blocks, PF_LEAST, few_parts, it)) A::item(a, it, sm);
+  if (paged_item<PF_QROWS>(a, first, id, 1, 0x7fffffff, a.few_blocks, PF_LEAST, few_parts, it)) A::item(a, it, sm);
 }
 
 // Chunks, and beside them the sequences that have a few rows: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
@@ -876,9 +879,10 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
     typename PagedFew<HD, I8>::Smem few;
   } sm;
   PagedItem it;
+  const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
-  if (paged_item<PF_QROWS>(a, id, 1, PF_QROWS, PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
-  else if (paged_item<PC_QROWS>(a, id, PF_QROWS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
+  if (paged_item<PF_QROWS>(a, first, id, 1, PF_QROWS, PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
+  else if (paged_item<PC_QROWS>(a, first, id, PF_QROWS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
 }
 
 }  // namespace jsg

@@ -65,8 +65,8 @@ int main() {
       for (int b = 0; b < p.n_seqs; b++) {
         const PagedSeq s = paged_seq(p, b);
         const PagedShare h = paged_share(s, n_rep, div, sh.q_rows, room, window, sinks);
-        const int parts = paged_parts(h.key_tiles, target, (int)sqrtf((float)h.key_tiles) * (round % 2 ? 1 : 100));
-        assert(parts >= 1);
+        const int parts = paged_parts(h.key_tiles, target, 1.0f / (float)target, (int)sqrtf((float)h.key_tiles) * (round % 2 ? 1 : 100));
+        assert(parts >= 1 && (parts == 1 || h.key_tiles > target) && parts <= (h.key_tiles - 1) / target + 2);
         blocks += (int64_t)KV * h.q_tiles * parts;
         if (parts > 1) slots += (int64_t)KV * h.q_tiles * parts, cut_items++;
         assert(parts == 1 || (room + PAGED_KEYS - 1) / PAGED_KEYS > sh.least);
