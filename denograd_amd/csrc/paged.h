@@ -31,6 +31,8 @@ JSG_BOTH PagedSeq paged_seq(int start, int end, int len, int rows) {
   s.len = paged_clamp(len, 0, 1 << 30);  // no table has more positions
   return s;
 }
+// Whether first rows fall here.  Where they do not, the sequences share the rows out among them, and a grid made for `rows` rows has blocks for all.
+JSG_BOTH bool paged_falls(const PagedBatch &p, int b) { return paged_clamp(p.row_starts[b + 1], 0, p.rows) < paged_clamp(p.row_starts[b], 0, p.rows); }
 JSG_BOTH PagedSeq paged_seq(const PagedBatch &p, int b) { return paged_seq(p.row_starts[b], p.row_starts[b + 1], p.lengths[b], p.rows); }
 // position of row i of a sequence: below zero where there are more new rows than positions
 JSG_BOTH int paged_pos(const PagedSeq &s, int i) { return s.len - s.n + i; }

@@ -1,6 +1,6 @@
 // Rows into and out of a paged KV cache: rotary embedding + write (fp16, or int8 with a float scale per position and head), and the read back.
 //
-// Reference semantics of what is written: apply_rotary_emb and the cache assign (/root/reference/jsgrad/models/llama.ts:17-32,61-87); the pages,
+// Reference semantics of what is written: apply_rotary_emb and the cache assign (jsgrad/models/llama.ts:17-32,61-87); the pages,
 // their int8 form and ragged batches have no counterpart there.
 //
 // int8, for the row x of one position and head (keys behind the rotation, in float): scale = max |x| / 127, code = rint(x / scale), so that code * scale is

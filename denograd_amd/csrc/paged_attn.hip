@@ -2,7 +2,7 @@
 //
 // Row i of a sequence sits at position p and sees the keys j <= p that have a page and, with a window, are among the last `window` of them or
 // among the first `sinks`: out = sum_j softmax_j(q . K_j / sqrt(HD)) V_j, zeros where it sees none.  Reference semantics of the sum:
-// scaled_dot_product_attention (/root/reference/jsgrad/tensor.ts:3920-3934); windows, sinks and pages have no counterpart there.
+// scaled_dot_product_attention (jsgrad/tensor.ts:3920-3934); windows, sinks and pages have no counterpart there.
 #include <type_traits>
 
 #include "gemm.h"
@@ -50,10 +50,13 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {     // inclusive prefix
   return v;
 }
 
-// 64 sequences, one to a lane.
+// 64 sequences, one to a lane; n is -1 where first rows fall.
 __device__ __forceinline__ PagedSeq lane_seq(const PagedBatch &p, int b0) {
   const int b = b0 + (threadIdx.x & 63);
-  return b < p.n_seqs ? paged_seq(p, b) : PagedSeq{0, 0, 0};
+  if (b >= p.n_seqs) return {0, 0, 0};
+  PagedSeq s = paged_seq(p, b);
+  if (paged_falls(p, b)) s.n = -1;
+  return s;
 }
 
 // The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head: blocks, least: see paged_target; most(key tiles): parts of an
@@ -71,11 +74,14 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSe
     if (s.n * n_rep >= from && s.n * n_rep <= to) h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
   };
   float pairs = 0.0f, items = 0.0f;
+  bool falls = false;
   for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
     look(b0);
+    falls |= s.n < 0;
     pairs += (float)h.q_tiles * (float)h.key_tiles;
     items += (float)h.q_tiles;
   }
+  if (__builtin_amdgcn_ballot_w64(falls)) return false;      // no batch: there may be more parts than blocks, and what counts them would not get back to zero
   pairs = wave_sum(pairs) * (float)KV;
   items = wave_sum(items) * (float)KV;
   // A share of the pairs each.  An item has up to one part more than its pairs make whole, so that all come to blocks + items and less.  Few items: a larger share of the
@@ -336,7 +342,7 @@ template <int HD, bool I8> struct PagedChunk {
 #pragma unroll
           for (int r = 0; r < 16; r++) {
             const int key = k0 + tk * 32 + 8 * (r / 4) + 4 * lg + (r % 4);
-            s[r] = sees(key) & ((pm >> (tk * 2 + r / 8) & 1) != 0) ? s[r] : -INFINITY;
+            s[r] = (sees(key) & ((pm >> (tk * 2 + r / 8) & 1) != 0)) ? s[r] : -INFINITY;
           }
         }
         float mx = s[0];
@@ -671,7 +677,7 @@ template <int HD, bool I8> struct PagedFew {
         for (int h = 0; h < 2; h++)
 #pragma unroll
           for (int r = 0; r < 4; r++)
-            s[h][r] = sees(k0 + 16 * h + 4 * lq + r) & (id[h] >= 0) ? s[h][r] : -INFINITY;
+            s[h][r] = (sees(k0 + 16 * h + 4 * lq + r) & (id[h] >= 0)) ? s[h][r] : -INFINITY;
       }
       float mx = m_run;
 #pragma unroll

@@ -271,8 +271,8 @@ int jsgrad_hip_argmax_rows(const void *logits, int rows, int n, int32_t *tokens_
  * The batch: row_starts int32 [n_seqs + 1], rising from 0, and lengths int32 [n_seqs]: row i of the n = row_starts[b + 1] - row_starts[b]
  * rows of sequence b is its position lengths[b] - n + i (lengths count the new rows).  `rows`: how many rows q, k, v and the outputs have;
  * those behind row_starts[n_seqs] are left as they are.  These arrays and the table are read on the device: a captured graph replays with
- * what they hold then.  No entry of them makes a call leave its buffers, and rows at positions below 0 or behind the table are neither
- * written nor rotated, and see what the table has before them.
+ * what they hold then.  No entry of them makes a call leave its buffers; where row_starts fall, attention writes nothing.  Rows at
+ * positions below 0 or behind the table are neither written nor rotated; they see what the table has before them.
  * --------------------------------------------------------------------------------- */
 typedef struct {
   int kind, n_pages, page_size, n_kv_heads, head_dim, table_width;
@@ -298,7 +298,7 @@ int jsgrad_hip_paged_read(const jsgrad_hip_pages_t *host_pages, const int32_t *r
  * it is not a number.  int8 pages count as code * scale in float.
  * workspace: jsgrad_hip_attn_paged_workspace_bytes() bytes, 16-byte aligned, zero-filled once before first use; any number of calls of these heads,
  * captured ones among them, may have the same one (they are ordered by the library's stream).  Results do not depend on the order in which
- * blocks run.  The sizes of a batch alone, not of the sequences in it, decide which kernel runs: a row's sums may come in another order in another batch. */
+ * blocks run.  How the work is cut goes by the whole batch: a row's sums may come in another order in another batch, also beside other sequences. */
 size_t jsgrad_hip_attn_paged_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
 int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out,
                           int n_heads, int window, int sinks, void *workspace);

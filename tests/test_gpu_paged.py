@@ -290,6 +290,23 @@ def test_pages_that_are_not_there(hip, kind):
         assert not got[21:].any()
 
 
+def test_row_starts_that_fall_leave_the_workspace_as_it_was(hip):
+    """512 sequences that all claim rows 0 to 3, and a long one behind them: a grid made for four rows has blocks for a part of that one's parts alone.
+    Nothing is written, and the next call on this workspace gives what it would have."""
+    rng = np.random.default_rng(12)
+    c = Case(rng, "float16", 64, 2, 64, [0] * 1025, [20] * 1024 + [2000])
+    c.starts, c.rows = np.array([0, 4] * 513, np.int32), 4
+    c.device()
+    ws, q, out = Tensor.zeros((hip.jsgrad_hip_attn_paged_workspace_bytes(4, 2, 64),), "uint8"), Tensor.zeros((4, 4, 64), "float16"), Tensor.full((4, 4, 64), 7.0, "float16")
+    check(hip.jsgrad_hip_attn_paged(*c.batch, q.ptr, out.ptr, 4, 0, 0, ws.ptr))
+    assert np.all(out.numpy() == 7)
+    for news in ([1], [300]):
+        good = Case(rng, "float16", 64, 2, 64, news, [2000]).device()
+        x = rng.standard_normal((good.rows, 4, 64)).astype(np.float16)
+        ref, tol = attention(good, x, 4)
+        compare(run_attention(hip, good, x, 4, 0, 0, ws), ref, tol, good.rows)
+
+
 @pytest.mark.parametrize("kind,hd,H,KV,news,lens,window,sinks", [
     ("float16", 128, 8, 2, [1], [20011], 0, 0), ("int8", 64, 8, 2, [1, 1], [9000, 30], 0, 0), ("int8", 128, 8, 2, [3], [9000], 0, 0), ("float16", 64, 4, 2, [60], [6000], 0, 0),
     ("int8", 128, 32, 8, [100, 1, 1, 1], [2500, 4000, 5, 1200], 0, 0), ("float16", 64, 8, 2, [1], [20000], 9000, 100), ("float16", 128, 32, 8, [1] * 70, list(range(1, 1401, 20)), 0, 0),

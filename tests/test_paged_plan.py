@@ -125,3 +125,42 @@ def test_indices_and_shares_of_any_batch(tmp_path):
     assert r.returncode == 0, r.stderr[-2000:]
     rows_seen, cut = (int(v) for v in r.stdout.split())
     assert rows_seen > 100000 and cut > 1000
+
+
+FALLS = r'''
+#include <stdio.h>
+#include <stdlib.h>
+#include <vector>
+#include "paged.h"
+using namespace jsg;
+int main() {
+  srand(1);
+  int fell = 0;
+  for (int round = 0; round < 20000; round++) {
+    PagedBatch p = {};
+    p.n_seqs = rand() % 9 + 1;
+    p.rows = rand() % 20 + 1;
+    std::vector<int32_t> starts(p.n_seqs + 1), lens(p.n_seqs, 5);
+    for (int b = 0; b <= p.n_seqs; b++) starts[b] = rand() % 3 ? (b ? starts[b - 1] : 0) + rand() % 4 : rand() % 6 == 0 ? (int32_t)((uint32_t)rand() * 2u) : rand() % 30;
+    p.row_starts = starts.data(); p.lengths = lens.data();
+    long all = 0;
+    bool falls = false;
+    for (int b = 0; b < p.n_seqs; b++) {
+      all += paged_seq(p, b).n;
+      falls |= paged_falls(p, b);
+      if (paged_falls(p, b) && starts[b + 1] >= starts[b]) return 1;
+    }
+    if (!falls && all > p.rows) return 2;
+    fell += falls;
+  }
+  return fell > 1000 && fell < 19000 ? 0 : 3;
+}
+'''
+
+
+def test_rows_are_shared_out_where_row_starts_do_not_fall(tmp_path):
+    """Which the grid of an attention launch rests on; a batch whose first rows fall is not worked on."""
+    src = tmp_path / "falls.cpp"
+    src.write_text(FALLS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined,address", "-fno-sanitize-recover=all", "-I", os.path.join(ROOT, "denograd_amd", "csrc"), str(src), "-o", str(tmp_path / "falls")], check=True)
+    assert subprocess.run([str(tmp_path / "falls")]).returncode == 0
