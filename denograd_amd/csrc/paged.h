@@ -49,6 +49,8 @@ JSG_BOTH size_t paged_row(const PagedBatch &p, int n_kv_heads, int id, int g, in
 }
 
 
+constexpr int PAGED_GRID = 1 << 24;      // a launch has fewer blocks of 256 threads: it counts its threads in 32 bits
+
 // ---- the work of an attention launch
 constexpr int PAGED_KEYS = 64;           // keys of a tile
 // Key tiles that rows at positions p_lo .. p_hi look at: [0, n_sink), then from t_lo on, n in all.

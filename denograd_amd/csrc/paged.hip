@@ -215,7 +215,7 @@ int paged_check(const char *who, const jsgrad_hip_pages_t *pg, const int32_t *ro
   JSG_REQUIRE(pg->page_size >= 16 && pg->page_size <= 256 && (pg->page_size & (pg->page_size - 1)) == 0, "%s: page_size %d (a power of two from 16 to 256)", who, pg->page_size);
   JSG_REQUIRE(pg->n_kv_heads > 0 && pg->n_kv_heads <= 1024 && pg->n_pages > 0, "%s: n_kv_heads %d, n_pages %d", who, pg->n_kv_heads, pg->n_pages);
   JSG_REQUIRE(pg->table_width > 0 && pg->table_width <= (1 << 30) / pg->page_size, "%s: table_width %d", who, pg->table_width);
-  JSG_REQUIRE(n_seqs > 0 && n_seqs <= 65535 && rows > 0 && rows <= 1 << 24, "%s: %d sequences, %d rows", who, n_seqs, rows);
+  JSG_REQUIRE(n_seqs > 0 && n_seqs <= 65535 && rows > 0 && rows < PAGED_GRID, "%s: %d sequences, %d rows", who, n_seqs, rows);
   JSG_REQUIRE((uintptr_t)pg->pages_k % 16 == 0 && (uintptr_t)pg->pages_v % 16 == 0, "%s: pages must be 16-byte aligned", who);
   JSG_REQUIRE(pg->kind == JSGRAD_W_F16 || ((uintptr_t)pg->scales_k % 16 == 0 && (uintptr_t)pg->scales_v % 16 == 0), "%s: scales must be 16-byte aligned", who);
   JSG_REQUIRE((uintptr_t)row_starts % 4 == 0 && (uintptr_t)lengths % 4 == 0 && (uintptr_t)pg->page_table % 4 == 0, "%s: row_starts, lengths and page_table must be 4-byte aligned", who);

@@ -37,7 +37,7 @@ struct PagedItem {
   PagedSeq s;
   int b, g, qt, part, parts, slot;       // slot: of part 0 in the workspace; part p's is slot + p * n_kv_heads
 };
-constexpr uint32_t PAGED_MOST = 1u << 29;  // more blocks than a launch has: sums stop there instead of wrapping
+constexpr uint32_t PAGED_MOST = 1u << 29;  // more than PAGED_GRID: sums stop there instead of wrapping
 
 __device__ __forceinline__ uint32_t scan64(uint32_t v) {     // inclusive prefix sums over the lanes, saturating
   auto add = [&](uint32_t o) { v = min(v + o, PAGED_MOST); };
@@ -919,7 +919,6 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   JSG_REQUIRE(window >= 0 && sinks >= 0, "%s: window %d, sinks %d", who, window, sinks);
   const int n_rep = n_heads / KV;
   JSG_REQUIRE((size_t)rows * n_rep < (size_t)1 << 30, "%s: %d rows of %d heads", who, rows, n_heads);
-  JSG_READY();
   a.pages_k = host_pages->pages_k; a.pages_v = host_pages->pages_v;
   a.scales_k = (const float *)host_pages->scales_k; a.scales_v = (const float *)host_pages->scales_v;
   a.q = (const _Float16 *)q; a.out = (_Float16 *)out;
@@ -940,7 +939,8 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS;
   const size_t blocks = (size_t)KV * ((size_t)rows * n_rep / (few ? PF_QROWS : PC_QROWS) + (n_seqs < rows ? n_seqs : rows)) +
                         (!few && room_tiles > PC_LEAST ? PC_SLOTS : 0) + (room_tiles > PF_LEAST ? PF_SLOTS : 0);
-  JSG_REQUIRE(blocks < PAGED_MOST, "%s: %d rows of %d heads", who, rows, n_heads);
+  JSG_REQUIRE(blocks < (size_t)PAGED_GRID, "%s: %d rows of %d heads", who, rows, n_heads);
+  JSG_READY();
   const dim3 grid((unsigned)blocks);
 #define JSG_PAGED(KERNEL, THREADS)                                                                    \
   do {                                                                                                \

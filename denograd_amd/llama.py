@@ -620,6 +620,8 @@ class Transformer:
         lib = ffi.load()
         if self.dtype != "float16":
             raise NotImplementedError("a paged cache is built for fp16 activations; float32 models take one position per call")
+        if window < 0 or sinks < 0:
+            raise ValueError(f"window {window}, sinks {sinks}")
         toks = [np.asarray(t, np.int32).reshape(-1) for t in tokens]
         seqs = list(seqs)
         if len(toks) != len(seqs) or any(t.size == 0 for t in toks):

@@ -1,6 +1,6 @@
 """A paged KV cache: sequences of different lengths in pages of one pool, in fp16 or quantised to int8 as they are written.
 
-Stands beside the contiguous cache of `llama.Attention` (/root/reference/jsgrad/models/llama.ts:78-87), which holds equally long sequences at one
+Stands beside the contiguous cache of `llama.Attention` (jsgrad/models/llama.ts:78-87), which holds equally long sequences at one
 position and reserves max_context positions for each.  `PageTable` is the bookkeeping, on the host alone; `PagedCache` has the pools of every
 layer and the calls on them; `PagedBatch` is one ragged batch: which sequences, how many new rows of each.  `Transformer.forward_paged`
 runs a model on it.
@@ -69,6 +69,8 @@ class PagedCache(PageTable):
         super().__init__(n_pages, page_size)
         if dtype not in ("float16", "int8"):
             raise ValueError(f"pages are float16 or int8, not {dtype}")
+        if n_layers < 1 or not 0 < n_kv_heads <= 1024 or head_dim not in (64, 128):
+            raise ValueError(f"{n_layers} layers of {n_kv_heads} heads of {head_dim}: one layer and more, 1 to 1024 heads of 64 or 128")
         self.n_layers, self.n_kv_heads, self.head_dim, self.dtype, self.device = n_layers, n_kv_heads, head_dim, dtype, device
         rows = (2, n_pages, n_kv_heads, page_size)
         self.pools = [Tensor.zeros((*rows, head_dim), dtype, device) for _ in range(n_layers)]       # k, then v
@@ -78,10 +80,11 @@ class PagedCache(PageTable):
         self._ws: dict[int, Tensor] = {}
 
     def begin(self, seqs, counts) -> "PagedBatch":
-        """A batch of counts[i] new rows of seqs[i], with pages for them.  The batch before it is over: they share the arrays that the device reads."""
-        seqs = list(seqs)
-        if not seqs or not sum(counts):
-            raise ValueError("a batch has one row at least")
+        """A batch of counts[i] new rows of seqs[i], with pages for them.  The batch before it is over: they share the arrays that the device
+        reads, which move when a batch needs more room than any before it (a captured graph is of no more use then)."""
+        seqs, counts = list(seqs), [int(c) for c in counts]
+        if not 0 < len(seqs) <= 65535 or not 0 < sum(counts) < 1 << 24:
+            raise ValueError(f"a batch has 1 to 65535 sequences and fewer than 2^24 rows, one at least: {len(seqs)} with {sum(counts)}")
         self.grow(seqs, counts)
         width = max(1, max(len(self.pages[s]) for s in seqs))
         n = len(seqs)

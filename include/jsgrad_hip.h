@@ -263,15 +263,15 @@ int jsgrad_hip_argmax_rows(const void *logits, int rows, int n, int32_t *tokens_
  *
  * A page holds page_size positions (a power of two from 16 to 256) of every kv head of one layer:
  *   pages_k, pages_v   [n_pages][n_kv_heads][page_size][head_dim], fp16 or int8 (kind JSGRAD_W_F16 / JSGRAD_W_I8), 16-byte aligned
- *   scales_k, scales_v float [n_pages][n_kv_heads][page_size] of int8 pages, 16-byte aligned: a row is code * scale, scale > 0; NULL for fp16
+ *   scales_k, scales_v float [n_pages][n_kv_heads][page_size] of int8 pages, 16-byte aligned: a row is code * scale, scale 1e-38 and more; NULL for fp16
  *   page_table         int32 [n_seqs][table_width]: the page of positions [i * page_size, (i + 1) * page_size) of the batch's sequence
  * An entry that is no page of the pool (below 0, or n_pages and more) is a page that is not there: nothing is written to its positions and
  * no query sees them, so that pages behind a window may be given away.  head_dim is 64 or 128.
  *
  * The batch: row_starts int32 [n_seqs + 1], rising from 0, and lengths int32 [n_seqs]: row i of the n = row_starts[b + 1] - row_starts[b]
- * rows of sequence b is its position lengths[b] - n + i (lengths count the new rows).  `rows`: how many rows q, k, v and the outputs have;
- * those behind row_starts[n_seqs] are left as they are.  These arrays and the table are read on the device: a captured graph replays with
- * what they hold then.  No entry of them makes a call leave its buffers; where row_starts fall, attention writes nothing.  Rows at
+ * rows of sequence b is its position lengths[b] - n + i (lengths count the new rows).  `rows`: how many rows q, k, v and the outputs have,
+ * fewer than 2^24; those behind row_starts[n_seqs] are left as they are.  These arrays and the table are read on the device: a captured graph
+ * replays with what they hold then.  No entry of them makes a call leave its buffers; where row_starts fall, attention writes nothing.  Rows at
  * positions below 0 or behind the table are neither written nor rotated; they see what the table has before them.
  * --------------------------------------------------------------------------------- */
 typedef struct {

@@ -135,6 +135,16 @@ def test_calls_that_are_refused_change_nothing(hip):
         batch.read(0)
 
 
+def test_windows_and_sinks_below_zero_are_refused_in_front_of_the_first_layer(hip):
+    _, llm = model()
+    cache = cache_for(llm, 4)
+    s = cache.add()
+    for more in (dict(window=-1), dict(sinks=-1)):
+        with pytest.raises(ValueError, match="window"):
+            llm.model.forward_paged(cache, [s], [np.arange(3, dtype=np.int32)], **more)
+        assert cache.lengths[s] == 0 and len(cache.free) == 4
+
+
 def test_captured_calls_replay_with_what_the_arrays_hold_then(hip):
     """Write and attention of one step recorded once; lengths move on between the replays, with eager calls of another batch on the same workspace between."""
     rng = np.random.default_rng(5)

@@ -9,7 +9,7 @@ import pytest
 
 from denograd_amd import ffi
 from denograd_amd.ffi import check
-from denograd_amd.paged import PageTable
+from denograd_amd.paged import PagedCache, PageTable
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 cpu_only = pytest.mark.skipif(os.path.exists("/dev/kfd"), reason="the addresses are made up")
@@ -72,6 +72,19 @@ def test_what_each_call_refuses_of_its_own():
                        (dict(window=-1), "window -1"), (dict(sinks=-1), "sinks -1"), (dict(q=A + 8), "aligned"), (dict(ws=A + 8), "aligned")):
         with pytest.raises(ffi.HipError, match=says):
             attend(desc(), **more)
+
+
+@cpu_only
+def test_more_rows_than_a_launch_has_blocks_are_refused():
+    """A grid's threads are counted in 32 bits, 256 to a block: fewer than 2^24 blocks."""
+    for call in (write, read, attend):
+        with pytest.raises(ffi.HipError, match="16777216 rows"):
+            call(desc(), rows=1 << 24)
+        with pytest.raises(ffi.HipError, match="jsgrad_hip_init has not been called"):
+            call(desc(), rows=(1 << 24) - 1)
+    # 2^25 pairs of each of 64 kv heads in q tiles of 128: 2^24 blocks, and those of the parts
+    with pytest.raises(ffi.HipError, match="2097152 rows of 1024 heads"):
+        attend(desc(n_kv_heads=64), rows=1 << 21, heads=1024)
 
 
 def test_descriptor_layout(tmp_path):
@@ -141,3 +154,16 @@ def test_page_table_refuses():
         t.slide(s, 0)
     with pytest.raises(MemoryError, match="5 pages are needed and 4 of 4 are free"):
         t.grow([s], [65])
+
+
+def test_paged_cache_refuses():
+    for args in ((1, 2, 96, 4), (1, 2, 64, 0), (0, 2, 64, 4), (1, 0, 64, 4), (1, 1025, 64, 4), (1, 2, 64, 4, 24), (1, 2, 64, 4, 16, "float32")):
+        with pytest.raises(ValueError):
+            PagedCache(*args)
+    cache = PagedCache.__new__(PagedCache)                # the bookkeeping alone: these come before anything on a device
+    PageTable.__init__(cache, 4, 16)
+    s = cache.add()
+    for seqs, counts in (([], []), ([s], [0]), ([s], [1 << 24]), ([s] * 65536, [1] * 65536), ([s], [1, 1]), ([s, s], [1, 1])):
+        with pytest.raises(ValueError):
+            cache.begin(seqs, counts)
+    assert cache.lengths[s] == 0 and len(cache.free) == 4
