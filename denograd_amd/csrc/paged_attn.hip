@@ -21,6 +21,7 @@ struct PagedAttnArgs {
   int n_heads, window, sinks;
   Divisor n_rep, n_kv_heads;
   int few_blocks;                        // of the few-row items: what their pairs are shared among
+  bool all_few;                          // the launch has blocks enough for few-row items of all its rows
   float scale_log2;                      // float(1 / sqrt(HD)) * log2(e)
   int *counters, *few_counters;          // zero, and zero again afterwards
   float *ws, *few_ws;
@@ -124,6 +125,16 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSe
   }
   id -= (int)before * KV;
   return false;
+}
+
+// Pairs of a q tile and a key tile in this batch, all heads.
+template <int QROWS> __device__ __forceinline__ float paged_pairs(const PagedAttnArgs &a, const PagedSeq &first) {
+  float pairs = 0.0f;
+  for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
+    const PagedShare h = paged_share(b0 ? lane_seq(a.pb, b0) : first, (int)a.n_rep.d, [&](int x) { return a.n_rep.div(x); }, QROWS, paged_room(a.pb), a.window, a.sinks);
+    pairs += (float)h.q_tiles * (float)h.key_tiles;
+  }
+  return wave_sum(pairs) * (float)a.n_kv_heads.d;
 }
 
 // paged_page for a position that all lanes share: through the scalar cache, sixteen entries to a line, and without a place among the vector loads, whose
@@ -542,6 +553,15 @@ template <int HD, bool I8> struct PagedChunk {
 constexpr int PF_THREADS = 256, PF_QROWS = 16;
 constexpr int PF_BLOCKS = 512, PF_LEAST = 2;
 constexpr int PF_SLOTS = 2 * PF_BLOCKS, PF_MOST = 64;      // parts of an item: a lane for each
+// Which sequences these blocks take.  A tile of 64 keys costs a compute unit 0.56 us for 16 pairs here and 1.4 for a chunk of 128 (int8 0.45 and 1.8; heads of 64 0.28 and 0.9,
+// 0.33 and 1.2), so that of up to 32 pairs their rows come cheaper: us, 16 pairs | 32 pairs, heads of 128, fp16 and int8: 30 sequences of up to 2300 with 32 pairs each 45 | 51 and
+// 49 | 34, behind 512 rows of another 72 | 67 and 87 | 75, four of 16000 76 | 60 and 80 | 49; 64 pairs: 30 sequences with 48 each 46 | 60 and 51 | 46.
+constexpr int PF_PAIRS = 32;
+// And a batch with little work has all of its rows here: a few keys on each of many compute units are done before a chunk's blocks have started and merged.
+// us, one sequence, 32 heads of 128 over 8, chunks | these, new rows behind so many (tiles of 16 pairs and 64 keys): fp16, 64 behind 1024 (2176) 17.9 | 14.8, 128 behind 1024
+// (4608) 18.4 | 15.7, 10 behind 16000 (6024) 41 | 29, 256 behind 500 (6144) 18.7 | 21.0, 64 behind 4000 (8192) 25.6 | 28.9; int8, 10240 28.2 | 26.6, 16640 40 | 42; heads of 64,
+// 10240 16.9 | 15.4, 16640 23.2 | 26.6.
+template <int HD, bool I8> constexpr float PF_ALL = HD == 128 && !I8 ? 6100.0f : 12288.0f;
 
 template <int HD, bool I8> struct PagedFew {
   static constexpr int NW = 4, KEYS = 32, ROWB = HD * 2;
@@ -866,7 +886,7 @@ template <int HD, bool I8> struct PagedFew {
 __device__ __forceinline__ int chunk_parts(int tiles) { return (int)__builtin_amdgcn_sqrtf(2.0f * (float)tiles); }
 __device__ __forceinline__ int few_parts(int tiles) { return min(PF_MOST, (int)(2.0f * __builtin_amdgcn_sqrtf((float)tiles))); }
 
-// Every sequence by the few-row blocks: 16 pairs and fewer per sequence and kv head, on the whole.
+// Every sequence by the few-row blocks: PF_PAIRS and fewer per sequence and kv head, on the whole, or little work all in all.
 template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4 : I8 ? 3 : 2) void attn_paged_few_kernel(PagedAttnArgs a) {
   typedef PagedFew<HD, I8> A;
   __shared__ typename A::Smem sm;
@@ -876,7 +896,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4
   if (paged_item<PF_QROWS>(a, first, id, 1, 0x7fffffff, a.few_blocks, PF_LEAST, few_parts, it)) A::item(a, it, sm);
 }
 
-// Chunks, and beside them the sequences that have a few rows: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
+// Chunks, and beside them the sequences that have PF_PAIRS and fewer: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
 // block for every compute unit, and the chunks' blocks beside them, as many again.  us, 512 rows behind 1792 and 30 sequences of up to 2304 with one each, heads of 128, fp16 | int8: chunks
 // alone 38 | 50, the others alone 40 | 25; chunks first, two blocks to a unit 84 | 71; the others first 66 | 71, and one block of each to a unit 57 | 64.
 template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn_paged_chunk_kernel(PagedAttnArgs a) {
@@ -887,8 +907,9 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
   PagedItem it;
   const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
-  if (paged_item<PF_QROWS>(a, first, id, 1, PF_QROWS, PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
-  else if (paged_item<PC_QROWS>(a, first, id, PF_QROWS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
+  const bool all = a.all_few && paged_pairs<PF_QROWS>(a, first) <= PF_ALL<HD, I8>;
+  if (paged_item<PF_QROWS>(a, first, id, 1, all ? 0x7fffffff : PF_PAIRS, all ? a.few_blocks : PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
+  else if (!all && paged_item<PC_QROWS>(a, first, id, PF_PAIRS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
 }
 
 }  // namespace jsg
@@ -934,11 +955,16 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   // 64 KB on their way to a compute unit are enough: one block of fp16 rows of 128, else two
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
   a.few_blocks = HD == 128 && !i8 ? PF_BLOCKS / 2 : PF_BLOCKS;
-  // As many blocks as there may be items and parts: every sequence fills its last q tile at worst, and what is no longer than the least part is not cut.
-  const bool few = (size_t)rows * n_rep <= (size_t)PF_QROWS * n_seqs;
-  const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS;
-  const size_t blocks = (size_t)KV * ((size_t)rows * n_rep / (few ? PF_QROWS : PC_QROWS) + (n_seqs < rows ? n_seqs : rows)) +
-                        (!few && room_tiles > PC_LEAST ? PC_SLOTS : 0) + (room_tiles > PF_LEAST ? PF_SLOTS : 0);
+  // As many blocks as there may be items and parts: every sequence fills its last q tile at worst, PF_PAIRS make several of the small ones, and what is no longer than the least
+  // part is not cut.  Where that is enough for items of PF_QROWS pairs alone, the device decides whether there are others (PF_ALL), for a table with much more room than the
+  // sequences fill; one without says so here, and the launch is of the smaller kernel (10 to 64 new rows alone, fp16 7.5 | 5.1 us).
+  const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS, seqs = n_seqs < rows ? n_seqs : rows;
+  const size_t few_items = KV * ((size_t)rows * n_rep / PF_QROWS + seqs), few_slots = room_tiles > PF_LEAST ? PF_SLOTS : 0;
+  const size_t items = KV * ((size_t)rows * n_rep / PC_QROWS + (size_t)(PF_PAIRS / PF_QROWS) * seqs), slots = few_slots + (room_tiles > PC_LEAST ? PC_SLOTS : 0);
+  const float all = HD == 64 ? (i8 ? PF_ALL<64, true> : PF_ALL<64, false>) : i8 ? PF_ALL<128, true> : PF_ALL<128, false>;
+  const bool few = (size_t)rows * n_rep <= (size_t)PF_PAIRS * n_seqs || (double)few_items * room_tiles <= all;
+  const size_t blocks = few ? few_items + few_slots : items + slots;
+  a.all_few = few_items + few_slots <= blocks;
   JSG_REQUIRE(blocks < (size_t)PAGED_GRID, "%s: %d rows of %d heads", who, rows, n_heads);
   JSG_READY();
   const dim3 grid((unsigned)blocks);

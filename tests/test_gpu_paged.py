@@ -290,6 +290,91 @@ def test_pages_that_are_not_there(hip, kind):
         assert not got[21:].any()
 
 
+def in_chunks(c, H):
+    """Room for more rows and positions than the batch has, as in a captured graph: a launch for so many has chunks for the sequences with more than a few rows."""
+    c.rows += 24000 // H
+    c.table = np.pad(c.table, ((0, 0), (0, -(-1100 // c.page))), constant_values=-1)
+    c.width = c.table.shape[1]
+    return c.device()
+
+
+def padded(c, q):
+    return np.concatenate([q, np.zeros((c.rows - q.shape[0], *q.shape[1:]), np.float16)])
+
+
+@pytest.mark.parametrize("kind,hd,H,KV,page,news,lens,window,sinks", [a for a in ATTN if max(a[5]) * a[2] > 32 * a[3]])
+def test_attention_of_a_ragged_batch_in_chunks(hip, kind, hd, H, KV, page, news, lens, window, sinks):
+    rng = np.random.default_rng(hd * 7 + H + page + sum(lens))
+    c = in_chunks(Case(rng, kind, hd, KV, page, news, lens), H)
+    q = padded(c, rng.standard_normal((int(c.starts[-1]), H, hd)).astype(np.float16))
+    ref, tol = attention(c, q, H, window, sinks)
+    compare(run_attention(hip, c, q, H, window, sinks, times=2), ref, tol, int(c.starts[-1]))
+
+
+@pytest.mark.parametrize("kind", ["float16", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_large_scores_and_values_of_every_size_in_chunks(hip, kind, hd):
+    rng = np.random.default_rng(hd)
+    news, lens = [90, 1, 40], [400, 33, 40]
+    c = Case(rng, kind, hd, 2, 16, news, lens)
+    size = (10.0 ** rng.uniform(-5, 3, c.v.shape[:3]))[..., None]
+    c = in_chunks(Case(np.random.default_rng(hd), kind, hd, 2, 16, news, lens, k=(c.k * np.float16(6)).astype(np.float16), v=(c.v * size).astype(np.float16)), 4)
+    q = padded(c, (rng.standard_normal((131, 4, hd)) * 4).astype(np.float16))
+    ref, tol = attention(c, q, 4)
+    compare(run_attention(hip, c, q, 4, 0, 0), ref, tol, 131)
+
+
+@pytest.mark.parametrize("kind", ["float16", "int8"])
+@pytest.mark.parametrize("hd,H,news,lens,window,sinks", [(64, 4, [70, 1], [300, 77], 0, 0), (128, 4, [33, 60], [130, 500], 40, 3), (128, 6, [140], [140], 0, 0)])
+def test_what_a_row_does_not_see_does_not_reach_it_in_chunks(hip, kind, hd, H, news, lens, window, sinks):
+    """Places that no row of the batch sees, and keys behind a row of its own chunk."""
+    rng = np.random.default_rng(hd + H)
+    c = Case(rng, kind, hd, 2, 16, news, lens)
+    mine = np.zeros(c.k.shape[:3], bool)
+    for b, (n, l) in enumerate(zip(news, lens)):
+        ids, slots = c.places(b, 0, l)
+        if window:
+            j = np.arange(l)
+            ids, slots = ids[(j > l - n - window) | (j < sinks)], slots[(j > l - n - window) | (j < sinks)]
+        mine[ids, :, slots] = True
+    k, v = c.k.copy(), c.v.copy()
+    k[~mine], v[~mine] = np.nan, np.inf
+    many = lambda: in_chunks(Case(np.random.default_rng(hd + H), kind, hd, 2, 16, news, lens, k=k, v=v), H)
+    c2, n = many(), sum(news)
+    q = padded(c2, rng.standard_normal((n, H, hd)).astype(np.float16))
+    ref, tol = attention(c2, q, H, window, sinks)
+    got = run_attention(hip, c2, q, H, window, sinks)
+    assert np.isfinite(ref[:n]).all()
+    compare(got, ref, tol, n)
+    # a row in the middle of the first chunk is not a number: the rows before it are what they are without it, it and those that see it are not numbers
+    at = news[0] // 2
+    ids, slots = c.places(0, lens[0] - news[0] + at, lens[0] - news[0] + at + 1)
+    k[ids[0], :, slots[0]], v[ids[0], :, slots[0]] = np.nan, np.nan
+    again = run_attention(hip, many(), q, H, window, sinks)
+    compare(again, ref, tol, at)
+    assert np.isnan(again[at:at + 1]).all() and (window or np.isnan(again[at:news[0]]).all())
+    # infinite values reach those that see them
+    k[ids[0], :, slots[0]], v[ids[0], :, slots[0]] = c.k[ids[0], :, slots[0]], np.inf
+    if kind == "float16":
+        again = run_attention(hip, many(), q, H, window, sinks)
+        compare(again, ref, tol, at)
+        assert not np.isfinite(again[at:at + 1]).any()
+
+
+@pytest.mark.parametrize("kind", ["float16", "int8"])
+def test_pages_that_are_not_there_in_chunks(hip, kind):
+    rng = np.random.default_rng(9)
+    c = Case(rng, kind, 64, 2, 16, [50, 1, 20, 30], [200, 150, 40, 30])
+    c.table[0, 2:5], c.table[1, 0], c.table[2, :], c.table[3, 0] = [-1, c.n_pages, -2 ** 31], 2 ** 31 - 1, -1, -7
+    in_chunks(c, 4)
+    q = padded(c, rng.standard_normal((101, 4, 64)).astype(np.float16))
+    for window, sinks in ((0, 0), (30, 4)):
+        ref, tol = attention(c, q, 4, window, sinks)
+        got = run_attention(hip, c, q, 4, window, sinks, times=2)
+        compare(got, ref, tol, 101)
+        assert not got[51:71].any() and not got[71:87].any() and got[87:101].any()
+
+
 def test_row_starts_that_fall_leave_the_workspace_as_it_was(hip):
     """512 sequences that all claim rows 0 to 3, and a long one behind them: a grid made for four rows has blocks for a part of that one's parts alone.
     Nothing is written, and the next call on this workspace gives what it would have."""
