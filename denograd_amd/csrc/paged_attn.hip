@@ -197,9 +197,10 @@ template <int HD, bool I8> struct PagedChunk {
     const size_t q_off = ((size_t)(it.s.start + qs) * a.n_heads + g * n_rep + qrow - qs * n_rep) * HD;
     const int sees_from = a.window ? qpos - a.window : -1, sees_to = a.window ? a.sinks : 0;   // keys <= qpos that are > sees_from or < sees_to
 
-    // where piece p of row r of a tile is kept: K by all pieces of a row, V by pairs of pieces (a transposing read takes 32 bytes of eight rows)
-    auto k_at = [](int r, int p) { return HD == 128 ? p ^ (r & 15) : p ^ (r & 7); };
-    auto v_at = [](int r, int p) { return HD == 128 ? p ^ ((r & 7) << 1) : p ^ (((r >> 1) & 3) << 1); };
+    // where piece p of row r of a tile is kept.  A quarter of the lanes reads a piece of sixteen rows of K, half of them 64 bytes of four rows of V, and a quarter writes (int8)
+    // four pieces, of different 64 bytes, of four rows: each goes over all 64 banks.
+    auto k_at = [](int r, int p) { return HD == 128 ? p ^ (r & 15) : p ^ ((r >> 1) & 7); };
+    auto v_at = [](int r, int p) { return HD == 128 ? p ^ ((r & 3) * 5) : p ^ (((r >> 1) & 1) * 5); };
 
     // this wavefront's rows of a tile: 16 * wave and on
     auto page_of = [&](int i) { return i < i_hi ? page_uniform(a.pb, it.b, keys.tile(i) * PAGED_KEYS + wave * 16) : -1; };
