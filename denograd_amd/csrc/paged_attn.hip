@@ -127,14 +127,18 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSe
   return false;
 }
 
-// Pairs of a q tile and a key tile in this batch, all heads.
-template <int QROWS> __device__ __forceinline__ float paged_pairs(const PagedAttnArgs &a, const PagedSeq &first) {
+// Whether no sequence has more than `few` (position, query head) pairs per kv head, or, with room for that (a.all_few), the batch is of no more than `little` pairs of a q
+// tile and a key tile, all heads.
+template <int QROWS> __device__ __forceinline__ bool paged_little(const PagedAttnArgs &a, const PagedSeq &first, int few, float little) {
   float pairs = 0.0f;
+  bool more = false;
   for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
-    const PagedShare h = paged_share(b0 ? lane_seq(a.pb, b0) : first, (int)a.n_rep.d, [&](int x) { return a.n_rep.div(x); }, QROWS, paged_room(a.pb), a.window, a.sinks);
+    const PagedSeq s = b0 ? lane_seq(a.pb, b0) : first;
+    const PagedShare h = paged_share(s, (int)a.n_rep.d, [&](int x) { return a.n_rep.div(x); }, QROWS, paged_room(a.pb), a.window, a.sinks);
     pairs += (float)h.q_tiles * (float)h.key_tiles;
+    more |= s.n * (int)a.n_rep.d > few;
   }
-  return wave_sum(pairs) * (float)a.n_kv_heads.d;
+  return !__builtin_amdgcn_ballot_w64(more) || (a.all_few && wave_sum(pairs) * (float)a.n_kv_heads.d <= little);
 }
 
 // paged_page for a position that all lanes share: through the scalar cache, sixteen entries to a line, and without a place among the vector loads, whose
@@ -893,7 +897,7 @@ template <int HD, bool I8> struct PagedFew {
 __device__ __forceinline__ int chunk_parts(int tiles) { return (int)__builtin_amdgcn_sqrtf(2.0f * (float)tiles); }
 __device__ __forceinline__ int few_parts(int tiles) { return min(PF_MOST, (int)(2.0f * __builtin_amdgcn_sqrtf((float)tiles))); }
 
-// Every sequence by the few-row blocks: PF_PAIRS and fewer per sequence and kv head, on the whole, or little work all in all.
+// Every sequence by the few-row blocks: one new row each, on the whole, or little work all in all.
 template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4 : I8 ? 3 : 2) void attn_paged_few_kernel(PagedAttnArgs a) {
   typedef PagedFew<HD, I8> A;
   __shared__ typename A::Smem sm;
@@ -914,7 +918,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
   PagedItem it;
   const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
-  const bool all = a.all_few && paged_pairs<PF_QROWS>(a, first) <= PF_ALL<HD, I8>;
+  const bool all = paged_little<PF_QROWS>(a, first, PF_PAIRS, PF_ALL<HD, I8>);
   if (paged_item<PF_QROWS>(a, first, id, 1, all ? 0x7fffffff : PF_PAIRS, all ? a.few_blocks : PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
   else if (!all && paged_item<PC_QROWS>(a, first, id, PF_PAIRS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
 }
@@ -963,13 +967,14 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
   a.few_blocks = HD == 128 && !i8 ? PF_BLOCKS / 2 : PF_BLOCKS;
   // As many blocks as there may be items and parts: every sequence fills its last q tile at worst, PF_PAIRS make several of the small ones, and what is no longer than the least
-  // part is not cut.  Where that is enough for items of PF_QROWS pairs alone, the device decides whether there are others (PF_ALL), for a table with much more room than the
-  // sequences fill; one without says so here, and the launch is of the smaller kernel (10 to 64 new rows alone, fp16 7.5 | 5.1 us).
+  // part is not cut.  Where that is enough for items of PF_QROWS pairs alone, the device decides whether there are others (PF_ALL, and whether any sequence has more than
+  // PF_PAIRS).  Where rows or the table's room say so, the launch is of the smaller kernel: us, chunk kernel | that, 10 to 64 new rows alone, fp16 7.5 | 5.1, 100 sequences of up to 1500
+  // with one row each, int8 47 | 40.  More rows than sequences do not: 300 rows behind 3700 and 63 sequences with one, fp16 99 | 142, 200 behind 1000 75 | 80.
   const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS, seqs = n_seqs < rows ? n_seqs : rows;
   const size_t few_items = KV * ((size_t)rows * n_rep / PF_QROWS + seqs), few_slots = room_tiles > PF_LEAST ? PF_SLOTS : 0;
   const size_t items = KV * ((size_t)rows * n_rep / PC_QROWS + (size_t)(PF_PAIRS / PF_QROWS) * seqs), slots = few_slots + (room_tiles > PC_LEAST ? PC_SLOTS : 0);
   const float all = HD == 64 ? (i8 ? PF_ALL<64, true> : PF_ALL<64, false>) : i8 ? PF_ALL<128, true> : PF_ALL<128, false>;
-  const bool few = (size_t)rows * n_rep <= (size_t)PF_PAIRS * n_seqs || (double)few_items * room_tiles <= all;
+  const bool few = rows <= n_seqs || (double)few_items * room_tiles <= all;
   const size_t blocks = few ? few_items + few_slots : items + slots;
   a.all_few = few_items + few_slots <= blocks;
   JSG_REQUIRE(blocks < (size_t)PAGED_GRID, "%s: %d rows of %d heads", who, rows, n_heads);

@@ -375,6 +375,21 @@ def test_pages_that_are_not_there_in_chunks(hip, kind):
         assert not got[51:71].any() and not got[71:87].any() and got[87:101].any()
 
 
+@pytest.mark.parametrize("kind,hd", [("float16", 64), ("int8", 128)])
+@pytest.mark.parametrize("news,lens", [([2] * 70, list(range(2, 702, 10))), ([8] * 5, [8, 9, 200, 500, 64]), ([1] * 65 + [9], [30] * 65 + [400]), ([2] * 40 + [300], [50] * 40 + [900]),
+                                       ([17, 0, 0, 1], [1000, 0, 3, 40])])
+def test_which_blocks_a_batch_has_is_found_on_the_device(hip, kind, hd, news, lens):
+    """Around 32 pairs to a sequence, and more sequences than lanes, under a table with room for much more than they fill."""
+    rng = np.random.default_rng(len(news) + hd)
+    c = Case(rng, kind, hd, 2, 16, news, lens)
+    c.table = np.pad(c.table, ((0, 0), (0, 5000)), constant_values=-1)
+    c.width = c.table.shape[1]
+    c.device()
+    q = rng.standard_normal((c.rows, 8, hd)).astype(np.float16)
+    ref, tol = attention(c, q, 8)
+    compare(run_attention(hip, c, q, 8, 0, 0, times=2), ref, tol, c.rows)
+
+
 def test_row_starts_that_fall_leave_the_workspace_as_it_was(hip):
     """512 sequences that all claim rows 0 to 3, and a long one behind them: a grid made for four rows has blocks for a part of that one's parts alone.
     Nothing is written, and the next call on this workspace gives what it would have."""
