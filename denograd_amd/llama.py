@@ -75,21 +75,21 @@ class Attention:
         return out
 
     def call_paged(self, xn: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", residual: Tensor, out: Tensor, window: int = 0,
-                   sinks: int = 0) -> Tensor:
-        """The rows of a ragged batch over a paged cache: xn is the normed input; out = residual + wo(attention)."""
-        n = batch.rows
-        self._gemm(self.wq, xn, n, rows.q)
-        self._gemm(self.wk, xn, n, rows.k)
-        self._gemm(self.wv, xn, n, rows.v)
+                   sinks: int = 0, norm: RMSNorm | None = None) -> Tensor:
+        """The rows of a ragged batch over a paged cache: xn is the normed input, or what norm is to be applied to; out = residual + wo(attention)."""
+        lib, n = ffi.load(), batch.rows
+        sp = lambda l: l.scale.ptr if l.scale is not None else None
+        weights = (self.wq.kind, self.wq.weight.ptr, sp(self.wq), self.wk.weight.ptr, sp(self.wk), self.wv.weight.ptr, sp(self.wv), xn.ptr)
+        # plain rows of q, k and v: n sequences at position 0, which turns nothing, of caches of one position each
+        rest = (n, 1, 0, rows.turn.ptr, rows.q.ptr, rows.k.ptr, rows.v.ptr, self.dim, self.n_heads, self.n_kv_heads, self.head_dim, 1)
+        if norm is None:
+            check(lib.jsgrad_hip_gemm_qkv_rope(*weights, *rest))
+        else:
+            check(lib.jsgrad_hip_gemm_qkv_rope_norm(*weights, norm.weight.ptr, norm.eps, rows.xn.ptr, *rest))
         batch.write(layer, rows.k, rows.v, rows.q, freqs_cis, self.n_heads)
         batch.attend(layer, rows.q, self.n_heads, rows.attn, window, sinks)
-        self._gemm(self.wo, rows.attn, n, out, residual)
+        check(lib.jsgrad_hip_gemm(self.wo.kind, self.wo.weight.ptr, sp(self.wo), self.dim, self.n_heads * self.head_dim, rows.attn.ptr, n, out.ptr, residual.ptr))
         return out
-
-    @staticmethod
-    def _gemm(l: Linear, x: Tensor, n: int, out: Tensor, residual: Tensor | None = None) -> None:
-        check(ffi.load().jsgrad_hip_gemm(l.kind, l.weight.ptr, l.scale.ptr if l.scale is not None else None, l.out_features, l.in_features, x.ptr, n, out.ptr,
-                                         residual.ptr if residual is not None else None))
 
     def call(self, x: Tensor, state: Tensor, freqs_cis: Tensor, norm: RMSNorm, ctx: "_Scratch") -> Tensor:
         """x: the block input row; returns x + wo(attention(norm(x))) in ctx.h2."""
@@ -140,7 +140,7 @@ class FeedForward:
         return out
 
 
-ATTENTION_ROWS, FEED_FORWARD_ROWS = Attention.call_rows, FeedForward.call_rows
+ATTENTION_ROWS, ATTENTION_PAGED, FEED_FORWARD_ROWS = Attention.call_rows, Attention.call_paged, FeedForward.call_rows
 
 
 class TransformerBlock:
@@ -166,7 +166,11 @@ class TransformerBlock:
 
     def call_paged(self, x: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", window: int = 0, sinks: int = 0) -> Tensor:
         """TransformerBlock.call (llama.ts:124-127) on the rows x of a ragged batch over a paged cache; the result is written back into x."""
-        h = self.attention.call_paged(self._normed(x, self.attention_norm, rows, batch.rows), layer, batch, freqs_cis, rows, x, rows.h2, window, sinks)
+        attend = self.attention.call_paged
+        if getattr(attend, "__func__", None) is ATTENTION_PAGED:
+            h = attend(x, layer, batch, freqs_cis, rows, x, rows.h2, window, sinks, self.attention_norm)
+        else:
+            h = attend(self._normed(x, self.attention_norm, rows, batch.rows), layer, batch, freqs_cis, rows, x, rows.h2, window, sinks)
         return self._feed_rows(h, batch.rows, rows, x)
 
     def _feed_rows(self, h: Tensor, n: int, rows, x: Tensor) -> Tensor:
@@ -258,6 +262,7 @@ class _PagedScratch:
         self.h, self.h2, self.xn = (e((rows, m.dim), f16, m.device) for _ in range(3))
         self.q, self.attn = (e((rows, m.n_heads * hd), f16, m.device) for _ in range(2))
         self.k, self.v = (e((rows, m.n_kv_heads * hd), f16, m.device) for _ in range(2))
+        self.turn = Tensor(np.tile(np.array([1, 0], np.float16), hd // 2), device=m.device)      # cos and sin of position 0
         self.g = e((rows, m.hidden_dim), f16, m.device)
         self.last = e((bsz, m.dim), f16, m.device)
         self.logits = e((bsz, m.vocab_size), f16, m.device)
@@ -648,11 +653,13 @@ class Transformer:
         check(lib.jsgrad_hip_embed_rows(_KIND[emb.weight.dtype], emb.weight.ptr, sp(emb), rows.tokens.ptr, n, rows.h.ptr, self.dim, self.vocab_size))
         for i, layer in enumerate(self.layers):
             layer.call_paged(rows.h, i, batch, self._paged_rope, rows, window, sinks)
-        last = np.cumsum([t.size for t in toks]) - 1
-        for b in range(bsz):
-            check(lib.jsgrad_hip_copy(rows.last.ptr + b * self.dim * 2, rows.h.ptr + int(last[b]) * self.dim * 2, self.dim * 2))
+        last = rows.h
+        if n > bsz:
+            last = rows.last
+            for b, i in enumerate(np.cumsum([t.size for t in toks]) - 1):
+                check(lib.jsgrad_hip_copy(last.ptr + b * self.dim * 2, rows.h.ptr + int(i) * self.dim * 2, self.dim * 2))
         out = self.output
-        check(lib.jsgrad_hip_gemm_norm(out.kind, out.weight.ptr, sp(out), self.vocab_size, self.dim, rows.last.ptr, self.norm.weight.ptr, self.norm.eps, rows.xn.ptr, bsz, rows.logits.ptr))
+        check(lib.jsgrad_hip_gemm_norm(out.kind, out.weight.ptr, sp(out), self.vocab_size, self.dim, last.ptr, self.norm.weight.ptr, self.norm.eps, rows.xn.ptr, bsz, rows.logits.ptr))
         check(lib.jsgrad_hip_argmax_rows(rows.logits.ptr, bsz, self.vocab_size, rows.next_tokens.ptr))
         return Tensor(buffer=rows.next_tokens.lazydata.view(bsz, "int32", 0), shape=(bsz,), dtype="int32", device=self.device)
 

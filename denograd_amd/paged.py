@@ -7,6 +7,8 @@ runs a model on it.
 """
 from __future__ import annotations
 
+from math import prod
+
 import numpy as np
 
 from . import ffi
@@ -113,20 +115,24 @@ class PagedBatch:
         self.cache, self.n_seqs, self.rows, self.width = cache, n_seqs, rows, width
         cache._batches += 1
         self._number = cache._batches
+        self._layers: dict[int, tuple] = {}                   # what the calls on a layer take
 
     def _args(self, layer: int) -> tuple:
         if self._number != self.cache._batches:
             raise RuntimeError("another batch has begun on this cache")
+        if layer in self._layers:
+            return self._layers[layer]
         c, plan = self.cache, self.cache._plan.ptr
         pool, scales = c.pools[layer], c.scales[layer]
         half = pool.nbytes // 2
         sp = (scales.ptr, scales.ptr + scales.nbytes // 2) if scales is not None else (None, None)
         desc = ffi.PagesDesc(ffi.W_I8 if c.dtype == "int8" else ffi.W_F16, c.n_pages, c.page_size, c.n_kv_heads, c.head_dim, self.width,
                              pool.ptr, pool.ptr + half, *sp, plan + 4 * (2 * self.n_seqs + 1))
-        return desc, plan, plan + 4 * (self.n_seqs + 1), self.n_seqs, self.rows
+        self._layers[layer] = desc, plan, plan + 4 * (self.n_seqs + 1), self.n_seqs, self.rows
+        return self._layers[layer]
 
     def _check(self, what: str, t: Tensor, heads: int) -> None:
-        if t.dtype != "float16" or t.numel < self.rows * heads * self.cache.head_dim:
+        if t.dtype != "float16" or prod(t.shape) < self.rows * heads * self.cache.head_dim:
             raise ValueError(f"{what}: {self.rows} float16 rows of {heads} heads of {self.cache.head_dim} are wanted, got {t.dtype} {t.shape}")
 
     def write(self, layer: int, k: Tensor, v: Tensor, q: Tensor | None = None, freqs_cis: Tensor | None = None, n_heads: int = 0, q_out: Tensor | None = None) -> Tensor | None:
@@ -137,10 +143,11 @@ class PagedBatch:
             q_out = q if q_out is None else q_out
             self._check("q", q, n_heads)
             self._check("q_out", q_out, n_heads)
-        if freqs_cis is not None and (freqs_cis.dtype != "float16" or freqs_cis.numel % self.cache.head_dim):
+        positions, odd = divmod(prod(freqs_cis.shape), self.cache.head_dim) if freqs_cis is not None else (0, 0)
+        if freqs_cis is not None and (freqs_cis.dtype != "float16" or odd):
             raise ValueError(f"freqs_cis: float16 rows of {self.cache.head_dim} are wanted, got {freqs_cis.dtype} {freqs_cis.shape}")
         p = lambda t: t.ptr if t is not None else None
-        check(ffi.load().jsgrad_hip_paged_write(*self._args(layer), p(q), k.ptr, v.ptr, p(freqs_cis), freqs_cis.numel // self.cache.head_dim if freqs_cis is not None else 0,
+        check(ffi.load().jsgrad_hip_paged_write(*self._args(layer), p(q), k.ptr, v.ptr, p(freqs_cis), positions,
                                                 p(q_out) if q is not None else None, n_heads))
         return q_out if q is not None else None
 

@@ -135,6 +135,26 @@ def test_calls_that_are_refused_change_nothing(hip):
         batch.read(0)
 
 
+def test_an_attention_of_the_callers_own_takes_its_rows_normed(hip):
+    """As with several rows (TransformerBlock.call_rows).  The norm's squares are added in another order then: the tolerance of the whole-model tests."""
+    _, llm = model()
+    prompts = [np.arange(n, dtype=np.int32) for n in (9, 1, 30)]
+    def run():
+        cache = cache_for(llm)
+        seqs = [cache.add() for _ in prompts]
+        llm.model.forward_paged(cache, seqs, prompts)
+        return logits(llm.model, 3)
+    want, seen = run(), []
+    for layer in llm.model.layers:
+        def own(xn, *args, attention=layer.attention, norm=layer.attention_norm):
+            seen.append((xn, norm))
+            return type(attention).call_paged(attention, xn, *args)
+        layer.attention.call_paged = own
+    got = run()
+    assert len(seen) == len(llm.model.layers) and all(x is llm.model._paged.xn for x, _ in seen)
+    assert np.max(np.abs(got - want)) <= 1e-2 * np.abs(want).max()
+
+
 def test_windows_and_sinks_below_zero_are_refused_in_front_of_the_first_layer(hip):
     _, llm = model()
     cache = cache_for(llm, 4)
