@@ -60,10 +60,10 @@ __device__ __forceinline__ PagedSeq lane_seq(const PagedBatch &p, int b0) {
   return s;
 }
 
-// The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head: blocks, least: see paged_target; most(key tiles): parts of an
-// item.  False, and id less these items' blocks, where it is none of them.
-template <int QROWS, typename Most>
-__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSeq &first, int &id, int from, int to, int blocks, int least, Most most, PagedItem &it) {
+// The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head: blocks_of(pairs of a q tile and a key tile, q tiles), least: see
+// paged_target; most(key tiles): parts of an item.  False, and id less these items' blocks, where it is none of them.
+template <int QROWS, typename Blocks, typename Most>
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSeq &first, int &id, int from, int to, Blocks blocks_of, int least, Most most, PagedItem &it) {
   const int room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
   const uint32_t want = (uint32_t)a.n_kv_heads.div(id);
   it.g = id - (int)want * KV;
@@ -87,7 +87,7 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSe
   items = wave_sum(items) * (float)KV;
   // A share of the pairs each.  An item has up to one part more than its pairs make whole, so that all come to blocks + items and less.  Few items: a larger share of the
   // pairs makes up for that.  More: the first of some larger shares with which the parts are no more than the blocks; or twice the share, where nothing else is.
-  const int share = paged_target(pairs, blocks, least);
+  const int blocks = blocks_of(pairs, items), share = paged_target(pairs, blocks, least);
   int target = 2 * share;
   auto cut = [&](int t) { return paged_parts(h.key_tiles, t, __builtin_amdgcn_rcpf((float)t), most(h.key_tiles)); };
   if (items * 16.0f <= (float)blocks) target = share + share / 16;
@@ -897,6 +897,13 @@ template <int HD, bool I8> struct PagedFew {
 __device__ __forceinline__ int chunk_parts(int tiles) { return (int)__builtin_amdgcn_sqrtf(2.0f * (float)tiles); }
 __device__ __forceinline__ int few_parts(int tiles) { return min(PF_MOST, (int)(2.0f * __builtin_amdgcn_sqrtf((float)tiles))); }
 
+// Parts for this many blocks.  Sequences with several q tiles come from L2, and where there are few tiles in all a second block to a unit only adds merges.  us, PF_BLOCKS | half of
+// them: int8, heads of 128, 128 rows behind 1024 (4608 pairs) 19.5 | 16.2, 10 behind 4000 17.5 | 15.0, 57 behind 1024 16.2 | 15.1, 64 behind 4000 (8192) 26.6 | 29.9; one row each of 16
+// sequences of up to 2000 (3000) 15.8 | 17.5; heads of 64, fp16, 13.2 | 9.9, 12.3 | 10.5, 11.5 | 10.6, 17.5 | 18.7; 13.5 | 14.1.
+__device__ __forceinline__ int few_blocks(const PagedAttnArgs &a, float pairs, float items) {
+  return items > (float)a.pb.n_seqs * (float)a.n_kv_heads.d && pairs <= 10.0f * PF_BLOCKS ? PF_BLOCKS / 2 : a.few_blocks;
+}
+
 // Every sequence by the few-row blocks: one new row each, on the whole, or little work all in all.
 template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4 : I8 ? 3 : 2) void attn_paged_few_kernel(PagedAttnArgs a) {
   typedef PagedFew<HD, I8> A;
@@ -904,7 +911,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4
   PagedItem it;
   const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
-  if (paged_item<PF_QROWS>(a, first, id, 1, 0x7fffffff, a.few_blocks, PF_LEAST, few_parts, it)) A::item(a, it, sm);
+  if (paged_item<PF_QROWS>(a, first, id, 1, 0x7fffffff, [&](float pairs, float items) { return few_blocks(a, pairs, items); }, PF_LEAST, few_parts, it)) A::item(a, it, sm);
 }
 
 // Chunks, and beside them the sequences that have PF_PAIRS and fewer: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
@@ -919,8 +926,10 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn
   const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
   const bool all = paged_little<PF_QROWS>(a, first, PF_PAIRS, PF_ALL<HD, I8>);
-  if (paged_item<PF_QROWS>(a, first, id, 1, all ? 0x7fffffff : PF_PAIRS, all ? a.few_blocks : PF_BLOCKS / 2, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
-  else if (!all && paged_item<PC_QROWS>(a, first, id, PF_PAIRS + 1, 0x7fffffff, id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
+  auto few = [&](float pairs, float items) { return all ? few_blocks(a, pairs, items) : PF_BLOCKS / 2; };
+  auto chunks = [&](float, float) { return id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS; };
+  if (paged_item<PF_QROWS>(a, first, id, 1, all ? 0x7fffffff : PF_PAIRS, few, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
+  else if (!all && paged_item<PC_QROWS>(a, first, id, PF_PAIRS + 1, 0x7fffffff, chunks, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
 }
 
 }  // namespace jsg
