@@ -149,6 +149,13 @@ __device__ __forceinline__ int page_uniform(const PagedBatch &p, int b, int pos)
   return id >= 0 && id < p.n_pages ? id : -1;
 }
 
+// The scale of V that an int8 row's weight has in the exponent.  The halves are weights times scales relative to the largest of these, so a row whose scale says more than its codes
+// would push the others out of fp16's range: one of zero codes, which is written with scale 1 and in a caller's own pages may have any.  It counts with 2^-60, and its weight 2^60 times that in the sum: it
+// is the largest only where it outweighs the others by so much that nothing of them is left in an fp16 result.  A scale below 2^-60 counts with that as well: values of 2^-53 and less are
+// nothing there either.  A scale that is not a number, or not finite, stays what it is.
+constexpr float PAGED_TINY = 0x1p-60f;
+__device__ __forceinline__ float scale_of_v(float v, bool zeros) { return v >= 0.0f && v < (zeros ? INFINITY : PAGED_TINY) ? PAGED_TINY : v; }
+
 // ---------------------------------------------------------------- chunks of new rows
 //
 // Block = 4 wavefronts = 128 (position, query head) pairs of one kv head of one sequence, keys in tiles of 64, as attn_prefill_kernel (prefill.hip) has it:
@@ -167,9 +174,9 @@ __device__ __forceinline__ int page_uniform(const PagedBatch &p, int b, int pos)
 constexpr int PC_THREADS = 256, PC_QROWS = 128;
 constexpr int PC_BLOCKS = 512, PC_LEAST = 4;               // two blocks to a compute unit; a tile takes 1.5 us, and a part some 5 us of its own
 constexpr int PC_SLOTS = 2 * PC_BLOCKS;
-// A row's weights are exp2(score - M) with a whole number M, which moves up only when a score is more than PC_SLACK above it: they are 2^7 and less, and their fp16 rounding is
-// relative to themselves all the same.  Sums are rescaled for nearly no tile then, and exactly, by a power of two.
-constexpr float PC_SLACK = 6.0f;
+// A row's weights are exp2(score - M) with a whole number M, PC_TOP below the maximum that it was last set to, and it moves up only when a score is more than PC_SLACK above that: they are 2^15 and
+// less, the largest 2^8 and more, and their fp16 rounding is relative to themselves, down to 2^-22 of the largest.  Sums are rescaled for nearly no tile then, and exactly, by a power of two.
+constexpr float PC_TOP = 9.0f, PC_SLACK = 6.0f;
 
 template <int HD, bool I8> struct PagedChunk {
   static constexpr int ROWB = HD * 2, PPR = HD / 8;                 // bytes and 16-byte pieces of a row of halves
@@ -259,12 +266,17 @@ template <int HD, bool I8> struct PagedChunk {
           *(u4_t *)(kt + r * ROWB + k_at(r, p) * 16) = k;
           *(u4_t *)(vt + r * ROWB + v_at(r, p) * 16) = v;
         }
+      uint32_t codes = 0;
+#pragma unroll
+      for (int c = 0; c < CPT; c++) codes |= vc[c][0] | vc[c][1] | vc[c][2] | vc[c][3];
+      const uint64_t some = __builtin_amdgcn_ballot_w64(codes != 0);   // four lanes to a row
       if (lane < 16) scl[buf][0][wave * 16 + lane] = sc * scale_log2;
       else if (lane < 32) {
         // A scale that is not a number makes the weights so, for the rows that see it.  Its reciprocal meets weights of zero as well, there and where
         // nothing was ever written, and has to be finite.
-        scl[buf][1][wave * 16 + lane - 16] = __builtin_amdgcn_logf(sc);
-        scl[buf][2][wave * 16 + lane - 16] = sc >= 1e-38f && sc < INFINITY ? __builtin_amdgcn_rcpf(sc) : 1.0f;
+        const float v = scale_of_v(sc, ((uint32_t)(some >> (lane - 16) * 4) & 15) == 0);
+        scl[buf][1][wave * 16 + lane - 16] = __builtin_amdgcn_logf(v);
+        scl[buf][2][wave * 16 + lane - 16] = v >= PAGED_TINY && v < INFINITY ? __builtin_amdgcn_rcpf(v) : 1.0f;
       }
     };
 
@@ -295,7 +307,7 @@ template <int HD, bool I8> struct PagedChunk {
 #pragma unroll
       for (int r = 0; r < 16; r++) o_acc[t][r] = 0.0f;
     // the maximum starts finite: a part of the keys may hold none that a row sees, and -inf minus -inf is not a number
-    float m_run = -1e30f, l_run = 0.0f;
+    float m_run = -1e30f, m_up = -1e30f, l_run = 0.0f;       // the weights' M, and the scores that move it
     const float unit = I8 ? 1.0f : scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
 
     // K fragment of key l32 (+ 32): chunk 2c + lg of its row; V: lane -> row (lane / 4 % 4) of its half's four keys, 8 bytes
@@ -369,18 +381,23 @@ template <int HD, bool I8> struct PagedChunk {
 #pragma unroll
         for (int r = 1; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
         mx = max_xor32(fmaxf(mx, s[15])) * unit;
-        if (__builtin_amdgcn_ballot_w64(mx > m_run + PC_SLACK)) {
-          const float m = fmaxf(m_run, __builtin_ceilf(mx)), alpha = __builtin_amdgcn_exp2f(m_run - m);   // first visible keys: 0
+        if (__builtin_amdgcn_ballot_w64(mx > m_up)) {
+          // scores so large that floats leave out whole numbers have no room for PC_TOP and PC_SLACK
+          const bool large = fabsf(fmaxf(mx, m_run)) >= 0x1p22f;
+          const float m = fmaxf(m_run, large ? mx : __builtin_ceilf(mx) - PC_TOP), by = m_run - m, alpha = __builtin_amdgcn_exp2f(by);   // first visible keys: 0
           m_run = m;
+          m_up = large ? m : m + (PC_TOP + PC_SLACK);
           l_run *= alpha;
 #pragma unroll
           for (int td = 0; td < NT; td++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
           if (tk == 1) {
-            const _Float16 h = (_Float16)alpha;
+            // in two steps: a half is no power of two below 2^-24, and 2^15 times that is a weight all the same
+            const float some = fmaxf(by, -14.0f);
+            const _Float16 a = (_Float16)__builtin_amdgcn_exp2f(some), b = (_Float16)__builtin_amdgcn_exp2f(by - some);
 #pragma unroll
-            for (int u = 0; u < 2; u++) pf[0][u] *= h8_t{h, h, h, h, h, h, h, h};
+            for (int u = 0; u < 2; u++) pf[0][u] = pf[0][u] * h8_t{a, a, a, a, a, a, a, a} * h8_t{b, b, b, b, b, b, b, b};
           }
         }
       };
@@ -564,6 +581,7 @@ template <int HD, bool I8> struct PagedChunk {
 constexpr int PF_THREADS = 256, PF_QROWS = 16;
 constexpr int PF_BLOCKS = 512, PF_LEAST = 2;
 constexpr int PF_SLOTS = 2 * PF_BLOCKS, PF_MOST = 64;      // parts of an item: a lane for each
+constexpr float PF_TOP = 15.0f;                            // a row's largest weight is 2^15: halves are normal numbers down to 2^-29 of it
 // Which sequences these blocks take.  A tile of 64 keys costs a compute unit 0.56 us for 16 pairs here and 1.4 for a chunk of 128 (int8 0.45 and 1.8; heads of 64 0.28 and 0.9,
 // 0.33 and 1.2), so that of up to 32 pairs their rows come cheaper: us, 16 pairs | 32 pairs, heads of 128, fp16 and int8: 30 sequences of up to 2300 with 32 pairs each 45 | 51 and
 // 49 | 34, behind 512 rows of another 72 | 67 and 87 | 75, four of 16000 76 | 60 and 80 | 49; 64 pairs: 30 sequences with 48 each 46 | 60 and 51 | 46.
@@ -691,6 +709,28 @@ template <int HD, bool I8> struct PagedFew {
       if constexpr (decltype(more)::value) load_k(st + NW, next);
       f4_t inv_v[2];
       if constexpr (I8) {
+        // scale_of_v, for which there is a reason in few steps: 16 codes of zero side by side, or a scale below PAGED_TINY
+        uint32_t codes = ~0u;
+        float least = INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int c = 0; c < GV; c++) codes = min(codes, vr[h][c][0] | vr[h][c][1] | vr[h][c][2] | vr[h][c][3]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) least = fminf(least, vs[h][e]);
+        }
+        if (__builtin_amdgcn_ballot_w64(codes == 0 || least < PAGED_TINY)) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            // lanes LPR * r and on have row r of the sixteen: LPR bits of each of these four rows
+            uint64_t some[GV];
+#pragma unroll
+            for (int c = 0; c < GV; c++) some[c] = __builtin_amdgcn_ballot_w64((vr[h][c][0] | vr[h][c][1] | vr[h][c][2] | vr[h][c][3]) != 0);
+            const uint32_t mine = (uint32_t)(some[lq * GV / 4] >> (lq * 4 % (64 / LPR)) * LPR);
+#pragma unroll
+            for (int e = 0; e < 4; e++) vs[h][e] = scale_of_v(vs[h][e], ((mine >> e * LPR) & ((1u << LPR) - 1)) == 0);
+          }
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -698,7 +738,7 @@ template <int HD, bool I8> struct PagedFew {
             // as in the chunk kernel: the scale of V in the exponent, its reciprocal finite whatever lies in a place that no row sees
             const float v = vs[h][e];
             s[h][e] = __builtin_fmaf(s[h][e], kscale[h][e], __builtin_amdgcn_logf(v));
-            inv_v[h][e] = v >= 1e-38f && v < INFINITY ? __builtin_amdgcn_rcpf(v) : 1.0f;
+            inv_v[h][e] = v >= PAGED_TINY && v < INFINITY ? __builtin_amdgcn_rcpf(v) : 1.0f;
           }
       }
       // value r of s[h] is key k0 + 16 h + 4 lq + r of row l16
@@ -721,13 +761,13 @@ template <int HD, bool I8> struct PagedFew {
 #pragma unroll
         for (int t = 0; t < NT; t++) o[t] *= alpha;
       }
-      const float mxs = m_run * unit;
       h8_t pf;
 #pragma unroll
       for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const float p = __builtin_amdgcn_exp2f(I8 ? s[h][r] - mxs : __builtin_fmaf(s[h][r], unit, -mxs));
+          // the difference first: it is never above zero, however large the scores are
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][r] - m_run, unit, PF_TOP));
           l_run = I8 ? __builtin_fmaf(p, inv_v[h][r], l_run) : l_run + p;
           pf[4 * h + r] = (_Float16)p;
         }

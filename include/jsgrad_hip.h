@@ -263,7 +263,7 @@ int jsgrad_hip_argmax_rows(const void *logits, int rows, int n, int32_t *tokens_
  *
  * A page holds page_size positions (a power of two from 16 to 256) of every kv head of one layer:
  *   pages_k, pages_v   [n_pages][n_kv_heads][page_size][head_dim], fp16 or int8 (kind JSGRAD_W_F16 / JSGRAD_W_I8), 16-byte aligned
- *   scales_k, scales_v float [n_pages][n_kv_heads][page_size] of int8 pages, 16-byte aligned: a row is code * scale, scale 1e-38 and more; NULL for fp16
+ *   scales_k, scales_v float [n_pages][n_kv_heads][page_size] of int8 pages, 16-byte aligned: a row is code * scale, scale 0 and more; NULL for fp16
  *   page_table         int32 [n_seqs][table_width]: the page of positions [i * page_size, (i + 1) * page_size) of the batch's sequence
  * An entry that is no page of the pool (below 0, or n_pages and more) is a page that is not there: nothing is written to its positions and
  * no query sees them, so that pages behind a window may be given away.  head_dim is 64 or 128.
