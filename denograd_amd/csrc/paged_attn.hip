@@ -174,9 +174,8 @@ __device__ __forceinline__ float scale_of_v(float v, bool zeros) { return v >= 0
 constexpr int PC_THREADS = 256, PC_QROWS = 128;
 constexpr int PC_BLOCKS = 512, PC_LEAST = 4;               // two blocks to a compute unit; a tile takes 1.5 us, and a part some 5 us of its own
 constexpr int PC_SLOTS = 2 * PC_BLOCKS;
-// A row's weights are exp2(score - M) with a whole number M, PC_TOP below the maximum that it was last set to, and it moves up only when a score is more than PC_SLACK above that: they are 2^15 and
-// less, the largest 2^8 and more, and their fp16 rounding is relative to themselves, down to 2^-22 of the largest.  Sums are rescaled for nearly no tile then, and exactly, by a power of two.
-constexpr float PC_TOP = 9.0f, PC_SLACK = 6.0f;
+// A row's weights are exp2(score - its maximum + PC_TOP): the largest is 2^15, which a half holds exactly, the others are rounded to 11 bits down to 2^-29 of it.
+constexpr float PC_TOP = 15.0f;
 
 template <int HD, bool I8> struct PagedChunk {
   static constexpr int ROWB = HD * 2, PPR = HD / 8;                 // bytes and 16-byte pieces of a row of halves
@@ -307,7 +306,7 @@ template <int HD, bool I8> struct PagedChunk {
 #pragma unroll
       for (int r = 0; r < 16; r++) o_acc[t][r] = 0.0f;
     // the maximum starts finite: a part of the keys may hold none that a row sees, and -inf minus -inf is not a number
-    float m_run = -1e30f, m_up = -1e30f, l_run = 0.0f;       // the weights' M, and the scores that move it
+    float m_run = -1e30f, l_run = 0.0f;                      // the maximum less PC_TOP
     const float unit = I8 ? 1.0f : scale_log2;               // of scores and their maximum: int8 ones have the factor in K's scale
 
     // K fragment of key l32 (+ 32): chunk 2c + lg of its row; V: lane -> row (lane / 4 % 4) of its half's four keys, 8 bytes
@@ -380,25 +379,21 @@ template <int HD, bool I8> struct PagedChunk {
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
-        mx = max_xor32(fmaxf(mx, s[15])) * unit;
-        if (__builtin_amdgcn_ballot_w64(mx > m_up)) {
-          // scores so large that floats leave out whole numbers have no room for PC_TOP and PC_SLACK
-          const bool large = fabsf(fmaxf(mx, m_run)) >= 0x1p22f;
-          const float m = fmaxf(m_run, large ? mx : __builtin_ceilf(mx) - PC_TOP), by = m_run - m, alpha = __builtin_amdgcn_exp2f(by);   // first visible keys: 0
+        return fmaxf(mx, s[15]);
+      };
+      // The sums are rescaled whenever some row's maximum has moved, so that the largest weight is not rounded, as in attn_prefill_kernel.  Off from float64 by 2.1e-4 with scores of
+      // deviation 3 (the result's own rounding) and 2.5e-4 with deviation 1, fp16 and int8 pages; rescaled only after growth by 2^6 it was 2.5e-4 and 2.7e-4, int8 2.9e-4, and 5 % faster.
+      auto raise = [&](float mx) {
+        mx = max_xor32(mx) * unit;
+        mx = fabsf(mx) < 0x1p22f ? mx - PC_TOP : mx;           // floats beyond have steps that the largest half has no room for beside PC_TOP
+        if (__builtin_amdgcn_ballot_w64(mx > m_run)) {
+          const float m = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m);   // first visible keys: 0
           m_run = m;
-          m_up = large ? m : m + (PC_TOP + PC_SLACK);
           l_run *= alpha;
 #pragma unroll
           for (int td = 0; td < NT; td++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o_acc[td][r] *= alpha;
-          if (tk == 1) {
-            // in two steps: a half is no power of two below 2^-24, and 2^15 times that is a weight all the same
-            const float some = fmaxf(by, -14.0f);
-            const _Float16 a = (_Float16)__builtin_amdgcn_exp2f(some), b = (_Float16)__builtin_amdgcn_exp2f(by - some);
-#pragma unroll
-            for (int u = 0; u < 2; u++) pf[0][u] = pf[0][u] * h8_t{a, a, a, a, a, a, a, a} * h8_t{b, b, b, b, b, b, b, b};
-          }
         }
       };
       auto weights = [&](const f16_t &s, int tk) {
@@ -449,10 +444,10 @@ template <int HD, bool I8> struct PagedChunk {
           }
       };
       f16_t s0 = score(0);
-      finish(s0, 0);
       f16_t s1 = score(1);
+      const float mx = finish(s0, 0);
+      raise(fmaxf(mx, finish(s1, 1)));
       weights(s0, 0);
-      finish(s1, 1);
       weigh(0);
       weights(s1, 1);
       weigh(1);
@@ -957,7 +952,7 @@ template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4
 // Chunks, and beside them the sequences that have PF_PAIRS and fewer: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
 // block for every compute unit, and the chunks' blocks beside them, as many again.  us, 512 rows behind 1792 and 30 sequences of up to 2304 with one each, heads of 128, fp16 | int8: chunks
 // alone 38 | 50, the others alone 40 | 25; chunks first, two blocks to a unit 84 | 71; the others first 66 | 71, and one block of each to a unit 57 | 64.
-template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, 2) void attn_paged_chunk_kernel(PagedAttnArgs a) {
+template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, HD == 128 ? 2 : I8 ? 3 : 4) void attn_paged_chunk_kernel(PagedAttnArgs a) {
   __shared__ union {
     typename PagedChunk<HD, I8>::Smem chunk;
     typename PagedFew<HD, I8>::Smem few;

@@ -94,3 +94,37 @@ def test_zero_codes_under_any_scale_and_scales_near_zero(hip, hd, chunks):
     for i, p in enumerate(range(1, 400, 49)):
         c.sv[ids[p], :, slots[p]] = [1e-38, 1e-30, 1e-25, 0.0][i % 4]
     check_case(hip, c, q, H, chunks)
+
+
+@pytest.mark.parametrize("kind", ["float16", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("chunks", [False, True])
+def test_the_largest_weight_of_a_row_is_not_rounded(hip, kind, hd, chunks):
+    """As with the contiguous cache.  Bound of one element: U16 |out| for the result; U16 w |V| for every key but the one with the largest weight (int8: weight times scale of V) and, as the
+    sum may be of the weights before or after their rounding, U16 w |out| for the same keys; scores are sums of four products, all others being zeros, so that
+    E = U32 (4 S + 8 max |s| + 16), twice for weights and sum each; float sums over n keys."""
+    rng = np.random.default_rng(hd)
+    KV, H, news, lens = 2, 8, [150], [190]
+    c = Case(rng, kind, hd, KV, 64, news, lens)
+    q = np.zeros((c.rows, H, hd))
+    q[..., 3::hd // 4] = 3 * np.sqrt(hd) / 2 * rng.standard_normal((c.rows, H, 4))
+    q = q.astype(np.float16)
+    got = run_attention(hip, *((lambda d: (d, padded(d, q)))(in_chunks(c, H)) if chunks else (c.device(), q)), H, 0, 0)
+    k, v = c.values("k"), c.values("v")
+    ids, slots = c.places(0, 0, lens[0])
+    worst = 0.0
+    for i in range(news[0]):
+        n = lens[0] - news[0] + i + 1
+        for h in range(H):
+            g, x = h // (H // KV), q[i, h].astype(np.float64)
+            kk, vv = k[ids[:n], g, slots[:n]], v[ids[:n], g, slots[:n]]
+            s = kk @ x / np.sqrt(hd)
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out, A = w @ vv, w @ np.abs(vv)
+            E = U32 * (4 * (np.abs(kk) @ np.abs(x)).max() / np.sqrt(hd) + 8 * np.abs(s).max() + 16)
+            top = (w * c.sv[ids[:n], g, slots[:n]] if kind == "int8" else w).argmax()
+            others = A - w[top] * np.abs(vv[top]) + (1 - w[top]) * np.abs(out)
+            tol = U16 * (np.abs(out) + others) + 2.0 ** -25 + (4 * E + U32 * n) * (A + np.abs(out)) + 2.0 ** -32 * n
+            worst = max(worst, (np.abs(got[i, h] - out) / tol).max())
+    assert worst <= 1, worst
