@@ -621,8 +621,8 @@ class Transformer:
         """Transformer.forward (llama.ts:201-213) for sequences of different lengths over a PagedCache: tokens[i] are the next token ids of sequence
         seqs[i], a prompt, a part of one, or the one token that the call before returned.  Returns the greedy next token of every sequence, an int32
         tensor in the order of seqs (Tensor.argmax of each, as forward_rows for several sequences).  window, sinks: as PagedBatch.attend has them.
-        A row of the model's own contiguous cache is neither read nor written.  fp16 activations; fp16 / int8 / NF4 weights."""
-        lib = ffi.load()
+        A row of the model's own contiguous cache is neither read nor written.  fp16 activations; fp16 / int8 / NF4 weights.  Where this raises, the
+        sequences are as they were."""
         if self.dtype != "float16":
             raise NotImplementedError("a paged cache is built for fp16 activations; float32 models take one position per call")
         if window < 0 or sinks < 0:
@@ -640,7 +640,15 @@ class Transformer:
         if any(cache.lengths[s] + t.size > 2 * self.max_context for s, t in zip(seqs, toks)):
             raise ValueError(f"positions beyond {2 * self.max_context}, where the rotary table ends")
         batch = cache.begin(seqs, [t.size for t in toks])
-        n, bsz = batch.rows, len(seqs)
+        try:
+            return self._run_paged(cache, batch, toks, flat, window, sinks)
+        except BaseException:
+            batch._cancel()
+            raise
+
+    def _run_paged(self, cache, batch: "PagedBatch", toks, flat: np.ndarray, window: int, sinks: int) -> Tensor:
+        lib, hd = ffi.load(), self.dim // self.n_heads
+        n, bsz = batch.rows, len(toks)
         if self._paged_rope is None or self._paged_rope.shape[1] < batch.width * cache.page_size:
             # the table reaches to the end of the last page of any sequence that may come
             self._paged_rope = precompute_freqs_cis(hd, 2 * self.max_context + cache.page_size, self.rope_theta, self.dtype, self.device)

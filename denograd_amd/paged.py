@@ -51,6 +51,17 @@ class PageTable:
             self.pages[s] += [self.free.pop() for _ in range(n)]
             self.lengths[s] += c
 
+    def _held(self, seqs) -> list[tuple[int, int, int]]:
+        return [(s, len(self.pages[s]), self.lengths[s]) for s in seqs]
+
+    def _put_back(self, held) -> None:
+        """Takes a grow back: held is what the sequences had before it."""
+        for s, n, length in reversed(held):
+            if s in self.pages:
+                self.free += [p for p in reversed(self.pages[s][n:]) if p >= 0]
+                del self.pages[s][n:]
+                self.lengths[s] = length
+
     def slide(self, seq: int, window: int, sinks: int = 0) -> int:
         """Gives away the pages that no later row of the sequence sees through this window; how many those were."""
         if window < 1 or sinks < 0:
@@ -83,11 +94,20 @@ class PagedCache(PageTable):
 
     def begin(self, seqs, counts) -> "PagedBatch":
         """A batch of counts[i] new rows of seqs[i], with pages for them.  The batch before it is over: they share the arrays that the device
-        reads, which move when a batch needs more room than any before it (a captured graph is of no more use then)."""
+        reads, which move when a batch needs more room than any before it (a captured graph is of no more use then).  Where this raises, no sequence has
+        changed."""
         seqs, counts = list(seqs), [int(c) for c in counts]
         if not 0 < len(seqs) <= 65535 or not 0 < sum(counts) < 1 << 24:
             raise ValueError(f"a batch has 1 to 65535 sequences and fewer than 2^24 rows, one at least: {len(seqs)} with {sum(counts)}")
+        held = self._held(seqs)
         self.grow(seqs, counts)
+        try:
+            return self._plan_batch(seqs, counts, held)
+        except BaseException:
+            self._put_back(held)
+            raise
+
+    def _plan_batch(self, seqs, counts, held) -> "PagedBatch":
         width = max(1, max(len(self.pages[s]) for s in seqs))
         n = len(seqs)
         plan = np.full(2 * n + 1 + n * width, -1, np.int32)
@@ -97,10 +117,11 @@ class PagedCache(PageTable):
         table = plan[2 * n + 1:].reshape(n, width)
         for i, s in enumerate(seqs):
             table[i, :len(self.pages[s])] = self.pages[s]
+        self._batches += 1                                    # in front of what ends the batch before it
         if self._plan is None or self._plan.numel < plan.size:
             self._plan = Tensor.empty((2 * plan.size,), "int32", self.device)
         self._plan.lazydata.view(plan.size, "int32", 0).ensure_allocated().copyin(plan)
-        return PagedBatch(self, n, int(plan[n]), width)
+        return PagedBatch(self, n, int(plan[n]), width, held)
 
     def workspace(self, n_heads: int) -> Tensor:
         if n_heads not in self._ws:
@@ -111,11 +132,16 @@ class PagedCache(PageTable):
 class PagedBatch:
     """The rows of one ragged batch, in the order of its sequences: row i of a sequence is its position length - count + i."""
 
-    def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int):
-        self.cache, self.n_seqs, self.rows, self.width = cache, n_seqs, rows, width
-        cache._batches += 1
+    def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int, held: list[tuple[int, int, int]]):
+        self.cache, self.n_seqs, self.rows, self.width, self._held = cache, n_seqs, rows, width, held
         self._number = cache._batches
         self._layers: dict[int, tuple] = {}                   # what the calls on a layer take
+
+    def _cancel(self) -> None:
+        """An error ended the batch between its layers: its sequences have the lengths and pages again that they had in front of it."""
+        if self._number == self.cache._batches:
+            self.cache._batches += 1
+            self.cache._put_back(self._held)
 
     def _args(self, layer: int) -> tuple:
         if self._number != self.cache._batches:
