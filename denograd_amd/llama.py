@@ -653,7 +653,10 @@ class Transformer:
             # the table reaches to the end of the last page of any sequence that may come
             self._paged_rope = precompute_freqs_cis(hd, 2 * self.max_context + cache.page_size, self.rope_theta, self.dtype, self.device)
         if self._paged is None or not self._paged.fits(bsz, n):
-            self._paged = _PagedScratch(bsz, n, self)
+            # a prompt has many rows of one sequence, a step one row of many: room for both
+            most = (bsz, n) if self._paged is None else (max(bsz, self._paged.bsz), max(n, self._paged.n))
+            self._paged = None                                # its buffers serve the new one where they are large enough
+            self._paged = _PagedScratch(*most, self)
         rows, sp = self._paged, lambda l: l.scale.ptr if l.scale is not None else None
         rows.tokens.lazydata.view(n, "int32", 0).ensure_allocated().copyin(flat)
         emb = self.tok_embeddings
