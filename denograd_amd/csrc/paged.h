@@ -48,7 +48,6 @@ JSG_BOTH size_t paged_row(const PagedBatch &p, int n_kv_heads, int id, int g, in
   return (((size_t)id * n_kv_heads + g) << p.page_shift) + (size_t)(pos & ((1 << p.page_shift) - 1));
 }
 
-
 constexpr int PAGED_GRID = 1 << 24;      // a launch has fewer blocks of 256 threads: it counts its threads in 32 bits
 
 // ---- the work of an attention launch
@@ -77,6 +76,15 @@ template <typename Div> JSG_BOTH PagedShare paged_share(const PagedSeq &s, int n
   h.key_tiles = s.n > 0 ? paged_keys(paged_pos(s, div((h.q_tiles - 1) * q_rows)), paged_pos(s, s.n - 1), room, window, sinks).n : 0;
   return h;
 }
+// q tiles per kv head that a batch of `rows` rows of `seqs` sequences has at most, however the rows are dealt out: of q_rows pairs, or of `least` where a sequence has no more than `few` of those.
+JSG_BOTH size_t paged_most_tiles(int rows, int n_rep, int seqs, int q_rows, int least, int few) {
+  const size_t by_pairs = (size_t)rows * n_rep / q_rows + (size_t)few * seqs, by_rows = (size_t)rows * ((n_rep + least - 1) / least);
+  return by_pairs < by_rows ? by_pairs : by_rows;
+}
+// Whether no such batch has a sequence of more than most_pairs pairs, or more than `little` pairs of a q tile and a key tile of all heads: few_items q tiles over room_tiles key tiles.
+JSG_BOTH bool paged_few_only(int rows, int n_rep, int most_pairs, size_t few_items, int room_tiles, float little) {
+  return (size_t)rows * n_rep <= (size_t)most_pairs || (double)few_items * room_tiles <= little;
+}
 // Key tiles of a part where `blocks` parts have the same share of the launch's pairs of a q tile and a key tile.  An item of key_tiles > target, for a target of that and more,
 // is cut into ceil(key_tiles / target) parts, one more at most, or fewer; the parts of cut items are no more than 2 * blocks, as each has half a target's pairs at least.
 JSG_BOTH int paged_target(float pairs, int blocks, int least) {
@@ -88,5 +96,7 @@ JSG_BOTH int paged_parts(int key_tiles, int target, float inv, int most) {
   const int n = key_tiles <= target ? 1 : (int)((float)(key_tiles - 1) * inv + 1e-3f) + 1;
   return n > most ? (most < 1 ? 1 : most) : n;
 }
+// No more blocks than this: an item's parts are one and less than one more for every target of its key tiles; the rest is for the rounding, there and here.
+JSG_BOTH float paged_most_blocks(float pairs, float items, float inv) { return 1.01f * (items + pairs * inv) + 8.0f; }
 
 }  // namespace jsg

@@ -60,47 +60,62 @@ __device__ __forceinline__ PagedSeq lane_seq(const PagedBatch &p, int b0) {
   return s;
 }
 
-// The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head: blocks_of(pairs of a q tile and a key tile, q tiles), least: see
-// paged_target; most(key tiles): parts of an item.  False, and id less these items' blocks, where it is none of them.
-template <int QROWS, typename Blocks, typename Most>
-__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSeq &first, int &id, int from, int to, Blocks blocks_of, int least, Most most, PagedItem &it) {
-  const int room = paged_room(a.pb), n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
+// Goes over the sequences, 64 at a time: look(first of them, this lane's) until it says true.  The next ones are asked for in front of it; sequences without new rows, as a batch that is filled up has many, are
+// passed over by the 64.
+template <typename Look> __device__ __forceinline__ bool paged_walk(const PagedBatch &p, const PagedSeq &first, Look look) {
+  PagedSeq s = first;
+  for (int b0 = 0; b0 < p.n_seqs; b0 += 64) {
+    PagedSeq next = {0, 0, 0};
+    if (b0 + 64 < p.n_seqs) next = lane_seq(p, b0 + 64);
+    if (__builtin_amdgcn_ballot_w64(s.n != 0) && look(b0, s)) return true;
+    s = next;
+  }
+  return false;
+}
+
+// q tiles of all heads, and pairs of these and a key tile, of some of a launch's sequences
+struct PagedSum {
+  float pairs, items;
+  __device__ void add(const PagedShare &h) { pairs += (float)h.q_tiles * (float)h.key_tiles; items += (float)h.q_tiles; }
+  __device__ void join(int KV) { pairs = wave_sum(pairs) * (float)KV; items = wave_sum(items) * (float)KV; }
+};
+
+template <int QROWS> __device__ __forceinline__ PagedShare share_of(const PagedAttnArgs &a, const PagedSeq &s) {
+  return paged_share(s, (int)a.n_rep.d, [&](int x) { return a.n_rep.div(x); }, QROWS, paged_room(a.pb), a.window, a.sinks);
+}
+
+// The item of block `id` among those of the sequences with `from` to `to` (position, query head) pairs per kv head, `sum` being these and share0 the first 64's: blocks: what they are shared among, least: see
+// paged_target; most(key tiles): parts of an item; last: none of other sequences come behind these.  False, and id less these items' blocks, where it is none of them.
+template <int QROWS, typename Most>
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSeq &first, const PagedShare &share0, int &id, int from, int to, const PagedSum &sum, int blocks, int least, Most most, bool last, PagedItem &it) {
+  const int n_rep = (int)a.n_rep.d, KV = (int)a.n_kv_heads.d;
   const uint32_t want = (uint32_t)a.n_kv_heads.div(id);
   it.g = id - (int)want * KV;
-  PagedSeq s;
-  PagedShare h;
-  auto look = [&](int b0) {
-    s = b0 ? lane_seq(a.pb, b0) : first;
-    h = {0, 0};
-    if (s.n * n_rep >= from && s.n * n_rep <= to) h = paged_share(s, n_rep, [&](int x) { return a.n_rep.div(x); }, QROWS, room, a.window, a.sinks);
+  const float pairs = sum.pairs, items = sum.items;
+  auto share_here = [&](int b0, const PagedSeq &s) {
+    const PagedShare h = b0 ? share_of<QROWS>(a, s) : share0;
+    return s.n * n_rep >= from && s.n * n_rep <= to ? h : PagedShare{0, 0};
   };
-  float pairs = 0.0f, items = 0.0f;
-  bool falls = false;
-  for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
-    look(b0);
-    falls |= s.n < 0;
-    pairs += (float)h.q_tiles * (float)h.key_tiles;
-    items += (float)h.q_tiles;
-  }
-  if (__builtin_amdgcn_ballot_w64(falls)) return false;      // no batch: there may be more parts than blocks, and what counts them would not get back to zero
-  pairs = wave_sum(pairs) * (float)KV;
-  items = wave_sum(items) * (float)KV;
   // A share of the pairs each.  An item has up to one part more than its pairs make whole, so that all come to blocks + items and less.  Few items: a larger share of the
   // pairs makes up for that.  More: the first of some larger shares with which the parts are no more than the blocks; or twice the share, where nothing else is.
-  const int blocks = blocks_of(pairs, items), share = paged_target(pairs, blocks, least);
+  const int share = paged_target(pairs, blocks, least);
   int target = 2 * share;
-  auto cut = [&](int t) { return paged_parts(h.key_tiles, t, __builtin_amdgcn_rcpf((float)t), most(h.key_tiles)); };
+  auto cut = [&](const PagedShare &h, int t) { return paged_parts(h.key_tiles, t, __builtin_amdgcn_rcpf((float)t), most(h.key_tiles)); };
   if (items * 16.0f <= (float)blocks) target = share + share / 16;
-  else if (a.pb.n_seqs <= 64 && items < (float)blocks)
+  else if (a.pb.n_seqs <= 64 && items < (float)blocks) {
+    const PagedShare h = share_here(0, first);
     for (int t = share; t < 2 * share; t += (share + 3) / 4)
-      if (wave_sum((float)h.q_tiles * (float)cut(t)) * (float)KV <= (float)blocks) {
+      if (wave_sum((float)h.q_tiles * (float)cut(h, t)) * (float)KV <= (float)blocks) {
         target = t;
         break;
       }
+  }
+  // a launch has blocks for the worst batch of its size, most of which are behind the last item of others
+  if (last && (float)id >= paged_most_blocks(pairs, items, __builtin_amdgcn_rcpf((float)target))) return false;
   uint32_t before = 0, slots = 0;
-  for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
-    if (a.pb.n_seqs > 64) look(b0);
-    const int parts = cut(target);
+  const bool found = paged_walk(a.pb, first, [&](int b0, const PagedSeq &s) {
+    const PagedShare h = share_here(b0, s);
+    const int parts = cut(h, target);
     const uint32_t mine = (uint32_t)min((uint64_t)h.q_tiles * parts, (uint64_t)PAGED_MOST);
     const uint32_t upto = scan64(mine), held = scan64(parts > 1 ? mine : 0);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(before + upto > want);
@@ -122,23 +137,10 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs &a, const PagedSe
     }
     before = min(before + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), PAGED_MOST);
     slots = min(slots + (uint32_t)__builtin_amdgcn_readlane((int)held, 63), PAGED_MOST);
-  }
-  id -= (int)before * KV;
-  return false;
-}
-
-// Whether no sequence has more than `few` (position, query head) pairs per kv head, or, with room for that (a.all_few), the batch is of no more than `little` pairs of a q
-// tile and a key tile, all heads.
-template <int QROWS> __device__ __forceinline__ bool paged_little(const PagedAttnArgs &a, const PagedSeq &first, int few, float little) {
-  float pairs = 0.0f;
-  bool more = false;
-  for (int b0 = 0; b0 < a.pb.n_seqs; b0 += 64) {
-    const PagedSeq s = b0 ? lane_seq(a.pb, b0) : first;
-    const PagedShare h = paged_share(s, (int)a.n_rep.d, [&](int x) { return a.n_rep.div(x); }, QROWS, paged_room(a.pb), a.window, a.sinks);
-    pairs += (float)h.q_tiles * (float)h.key_tiles;
-    more |= s.n * (int)a.n_rep.d > few;
-  }
-  return !__builtin_amdgcn_ballot_w64(more) || (a.all_few && wave_sum(pairs) * (float)a.n_kv_heads.d <= little);
+    return false;
+  });
+  if (!found) id -= (int)before * KV;
+  return found;
 }
 
 // paged_page for a position that all lanes share: through the scalar cache, sixteen entries to a line, and without a place among the vector loads, whose
@@ -946,7 +948,19 @@ template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4
   PagedItem it;
   const PagedSeq first = lane_seq(a.pb, 0);
   int id = blockIdx.x;
-  if (paged_item<PF_QROWS>(a, first, id, 1, 0x7fffffff, [&](float pairs, float items) { return few_blocks(a, pairs, items); }, PF_LEAST, few_parts, it)) A::item(a, it, sm);
+  PagedSum few = {0.0f, 0.0f};
+  PagedShare share0 = {0, 0};
+  bool falls = false;
+  paged_walk(a.pb, first, [&](int b0, const PagedSeq &s) {
+    falls |= s.n < 0;
+    const PagedShare h = share_of<PF_QROWS>(a, s);
+    if (!b0) share0 = h;
+    few.add(h);
+    return false;
+  });
+  if (__builtin_amdgcn_ballot_w64(falls)) return;            // no batch: there may be more parts than blocks, and what counts them would not get back to zero
+  few.join((int)a.n_kv_heads.d);
+  if (paged_item<PF_QROWS>(a, first, share0, id, 1, 0x7fffffff, few, few_blocks(a, few.pairs, few.items), PF_LEAST, few_parts, true, it)) A::item(a, it, sm);
 }
 
 // Chunks, and beside them the sequences that have PF_PAIRS and fewer: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
@@ -959,12 +973,36 @@ template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, HD == 128 ? 
   } sm;
   PagedItem it;
   const PagedSeq first = lane_seq(a.pb, 0);
+  const int n_rep = (int)a.n_rep.d;
   int id = blockIdx.x;
-  const bool all = paged_little<PF_QROWS>(a, first, PF_PAIRS, PF_ALL<HD, I8>);
-  auto few = [&](float pairs, float items) { return all ? few_blocks(a, pairs, items) : PF_BLOCKS / 2; };
-  auto chunks = [&](float, float) { return id < (int)blockIdx.x ? PC_BLOCKS / 2 : PC_BLOCKS; };
-  if (paged_item<PF_QROWS>(a, first, id, 1, all ? 0x7fffffff : PF_PAIRS, few, PF_LEAST, few_parts, it)) PagedFew<HD, I8>::item(a, it, sm.few);
-  else if (!all && paged_item<PC_QROWS>(a, first, id, PF_PAIRS + 1, 0x7fffffff, chunks, PC_LEAST, chunk_parts, it)) PagedChunk<HD, I8>::item(a, it, sm.chunk);
+  // small: all of the batch by the few-row blocks; few, chunk: its sequences of up to PF_PAIRS pairs, and of more
+  PagedSum small = {0.0f, 0.0f}, few = {0.0f, 0.0f}, chunk = {0.0f, 0.0f};
+  PagedShare few0 = {0, 0}, chunk0 = {0, 0};
+  bool falls = false;
+  paged_walk(a.pb, first, [&](int b0, const PagedSeq &s) {
+    falls |= s.n < 0;
+    const PagedShare h = share_of<PF_QROWS>(a, s);
+    const bool more = s.n * n_rep > PF_PAIRS;
+    if (!b0) few0 = h;
+    small.add(h);
+    if (!more) few.add(h);
+    if (__builtin_amdgcn_ballot_w64(more)) {
+      const PagedShare c = share_of<PC_QROWS>(a, s);
+      if (!b0) chunk0 = c;
+      if (more) chunk.add(c);
+    }
+    return false;
+  });
+  if (__builtin_amdgcn_ballot_w64(falls)) return;            // as in attn_paged_few_kernel
+  const int KV = (int)a.n_kv_heads.d;
+  small.join(KV); few.join(KV); chunk.join(KV);
+  // no sequence of more, or, with blocks enough for that, a batch of no more than PF_ALL pairs of a q tile and a key tile
+  const bool all = chunk.items == 0.0f || (a.all_few && small.pairs <= PF_ALL<HD, I8>);
+  if (all) few = small;
+  if (few.items > 0.0f && paged_item<PF_QROWS>(a, first, few0, id, 1, all ? 0x7fffffff : PF_PAIRS, few, all ? few_blocks(a, few.pairs, few.items) : PF_BLOCKS / 2, PF_LEAST, few_parts, all, it))
+    PagedFew<HD, I8>::item(a, it, sm.few);
+  else if (!all && paged_item<PC_QROWS>(a, first, chunk0, id, PF_PAIRS + 1, 0x7fffffff, chunk, few.items > 0.0f ? PC_BLOCKS / 2 : PC_BLOCKS, PC_LEAST, chunk_parts, true, it))
+    PagedChunk<HD, I8>::item(a, it, sm.chunk);
 }
 
 }  // namespace jsg
@@ -1012,13 +1050,14 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
   a.few_blocks = HD == 128 && !i8 ? PF_BLOCKS / 2 : PF_BLOCKS;
   // As many blocks as there may be items and parts: every sequence fills its last q tile at worst, PF_PAIRS make several of the small ones, and what is no longer than the least
   // part is not cut.  Where that is enough for items of PF_QROWS pairs alone, the device decides whether there are others (PF_ALL, and whether any sequence has more than
-  // PF_PAIRS).  Where rows or the table's room say so, the launch is of the smaller kernel: us, chunk kernel | that, 10 to 64 new rows alone, fp16 7.5 | 5.1, 100 sequences of up to 1500
-  // with one row each, int8 47 | 40.  More rows than sequences do not: 300 rows behind 3700 and 63 sequences with one, fp16 99 | 142, 200 behind 1000 75 | 80.
+  // PF_PAIRS).  The launch is of the smaller kernel where rows and the table's room say that there are none, however the rows are dealt out; us, chunk kernel | that, 10 to 64 new rows alone, fp16 7.5 | 5.1.
+  // As many rows as sequences say nothing: they may be one each, or one prompt among sequences without new rows.  us, heads of 128, fp16 and int8: 16 with one row each 36 | 36 and 23 | 23, 100 73 | 73 and
+  // 46 | 40 (three blocks to a unit), 256 111 | 110 and 83 | 72; 512 rows of one of 512 sequences 54 | 99 and 59 | 76, heads of 64 33 | 56 and 41 | 52.
   const int room_tiles = (paged_room(a.pb) + PAGED_KEYS - 1) / PAGED_KEYS, seqs = n_seqs < rows ? n_seqs : rows;
-  const size_t few_items = KV * ((size_t)rows * n_rep / PF_QROWS + seqs), few_slots = room_tiles > PF_LEAST ? PF_SLOTS : 0;
-  const size_t items = KV * ((size_t)rows * n_rep / PC_QROWS + (size_t)(PF_PAIRS / PF_QROWS) * seqs), slots = few_slots + (room_tiles > PC_LEAST ? PC_SLOTS : 0);
+  const size_t few_items = KV * paged_most_tiles(rows, n_rep, seqs, PF_QROWS, PF_QROWS, 1), few_slots = room_tiles > PF_LEAST ? PF_SLOTS : 0;
+  const size_t items = KV * paged_most_tiles(rows, n_rep, seqs, PC_QROWS, PF_QROWS, PF_PAIRS / PF_QROWS), slots = few_slots + (room_tiles > PC_LEAST ? PC_SLOTS : 0);
   const float all = HD == 64 ? (i8 ? PF_ALL<64, true> : PF_ALL<64, false>) : i8 ? PF_ALL<128, true> : PF_ALL<128, false>;
-  const bool few = rows <= n_seqs || (double)few_items * room_tiles <= all;
+  const bool few = paged_few_only(rows, n_rep, PF_PAIRS, few_items, room_tiles, all);
   const size_t blocks = few ? few_items + few_slots : items + slots;
   a.all_few = few_items + few_slots <= blocks;
   JSG_REQUIRE(blocks < (size_t)PAGED_GRID, "%s: %d rows of %d heads", who, rows, n_heads);
