@@ -330,13 +330,15 @@ class Llama3:
 
     def generate_paged(self, prompts, n_new: int, dtype: str = "float16", page_size: int = 64, window: int = 0, sinks: int = 0) -> np.ndarray:
         """Prompts of any lengths at once, greedily, over a paged cache made for them: fp16 pages, or int8 ones of half the size.  With a window a
-        sequence keeps the pages that it still sees.  Returns int32 [number of prompts, n_new]."""
+        sequence gives away the pages that it no longer sees, and the pool has no more than the prompts and those that are seen need.  Returns int32 [number of prompts, n_new]."""
         from .paged import PagedCache
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
         if not prompts or any(p.size == 0 for p in prompts) or n_new < 1:
             raise ValueError("one prompt and one new token at least, and no empty prompt")
         m = self.model
-        n_pages = sum(-(-(p.size + n_new - 1) // page_size) for p in prompts)
+        if window < 0 or sinks < 0 or page_size < 1:
+            raise ValueError(f"window {window}, sinks {sinks}, page_size {page_size}")
+        n_pages = PagedCache.pages_for([p.size for p in prompts], n_new, page_size, window, sinks)
         cache = PagedCache(len(m.layers), m.n_kv_heads, m.dim // m.n_heads, n_pages, page_size, dtype, self.device)
         seqs = [cache.add() for _ in prompts]
         out, toks = np.empty((len(prompts), n_new), np.int32), prompts

@@ -28,6 +28,17 @@ class PageTable:
         self.lengths: dict[int, int] = {}
         self._next = 0
 
+    @staticmethod
+    def pages_for(prompts, n_new: int, page_size: int, window: int = 0, sinks: int = 0) -> int:
+        """The most pages that sequences hold at a time which begin with these numbers of positions and grow by one n_new - 1 times, all at once; with a window,
+        `slide` comes behind every step."""
+        steps = np.asarray(prompts, np.int64)[:, None] + np.arange(n_new)
+        held = -(-steps // page_size)
+        if window:
+            given = np.maximum(steps[:, :-1] - window + 1, 0) // page_size - -(-sinks // page_size)
+            held[:, 1:] -= np.maximum(given, 0)
+        return int(held.sum(0).max())
+
     def add(self) -> int:
         """A new, empty sequence."""
         seq, self._next = self._next, self._next + 1
