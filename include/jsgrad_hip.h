@@ -284,7 +284,8 @@ typedef struct {
  * q [rows][n_heads][head_dim], whose rotated rows go to q_out (may be q; both NULL: no queries).  rope_table: [rope_rows][head_dim/2][2] as
  * jsgrad_hip_rope_table makes it, of at least table_width * page_size positions; NULL: no rotation.  Sums are float.  int8 pages: scale =
  * max |x| / 127 of a position's row of one head, code = rint(x / scale); a row of zeros has scale 1, one with a value that is not finite reads as
- * NaN.  Two rows of a batch on one place of one page: either may be the one that stays. */
+ * NaN.  Two rows of a batch on one place of one page (a page that the table names twice): what stays may be pieces of both, codes of one under the
+ * scale of the other among them. */
 int jsgrad_hip_paged_write(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q,
                            const void *k, const void *v, const void *rope_table, int rope_rows, void *q_out, int n_heads);
 
@@ -295,7 +296,7 @@ int jsgrad_hip_paged_read(const jsgrad_hip_pages_t *host_pages, const int32_t *r
 /* scaled_dot_product_attention (tensor.ts:3920-3934) of the batch's rows q [rows][n_heads][head_dim] over the pages, grouped-query: the row at
  * position p sees the positions j <= p that have a page and, with window > 0, j > p - window or j < sinks (the last `window` of them and the first
  * `sinks`).  out [rows][n_heads][head_dim], not q; zeros for a row that sees nothing.  What a row does not see does not reach its result, also where
- * it is not a number.  int8 pages count as code * scale in float.
+ * it is not a number.  int8 pages count as code * scale in float, a scale of V below 2^-60 as that.
  * workspace: jsgrad_hip_attn_paged_workspace_bytes() bytes, 16-byte aligned, zero-filled once before first use; any number of calls of these heads,
  * captured ones among them, may have the same one (they are ordered by the library's stream).  Results do not depend on the order in which
  * blocks run.  How the work is cut goes by the whole batch: a row's sums may come in another order in another batch, also beside other sequences. */
