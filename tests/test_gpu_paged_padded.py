@@ -1,5 +1,7 @@
 """Attention of batches with many sequences that have no new rows, as a captured graph's batch is filled up: groups of 64 of them in front of, between and behind the others, and no more rows
 than sequences."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -47,3 +49,39 @@ def test_row_starts_that_fall_behind_sequences_without_rows(hip):
     c, q = batch("float16", 64, {3: (40, 600)}, 300, 0)
     ref, tol = attention(c, q, 8)
     compare(run_attention(hip, c, q, 8, 0, 0, ws), ref, tol, 40)
+
+
+@pytest.mark.parametrize("kind,hd", [("float16", 64), ("int8", 64), ("float16", 128), ("int8", 128)])
+def test_a_captured_launch_serves_prompts_and_single_rows(hip, kind, hd):
+    """One graph for 130 sequences and 130 rows, replayed with a prompt, with a row each, with both and with nothing, another batch on the same workspace between the replays; each against an
+    eager call."""
+    n_seqs, rows, H = 130, 130, 8
+    rng = np.random.default_rng(hd)
+    lens = rng.integers(1, 200, n_seqs)
+    lens[[3, 70]] = 1500, 700
+    c = Case(rng, kind, hd, 2, 16, [1] * n_seqs, lens.tolist()).device()
+    other, oq = batch(kind, hd, {1: (90, 800)}, 70, 0)
+    q = rng.standard_normal((rows, H, hd)).astype(np.float16)
+    ws = [Tensor.zeros((hip.jsgrad_hip_attn_paged_workspace_bytes(H, 2, hd),), "uint8") for _ in range(2)]
+    tq, out, ref = Tensor(q), Tensor.full(q.shape, 7.0, "float16"), Tensor.full(q.shape, 7.0, "float16")
+    graph = C.c_void_p()
+    check(hip.jsgrad_hip_graph_begin())
+    try:
+        check(hip.jsgrad_hip_attn_paged(*c.batch, tq.ptr, out.ptr, H, 0, 0, ws[0].ptr))
+    finally:
+        check(hip.jsgrad_hip_graph_end(C.byref(graph)))
+    for news in ({3: 130}, {b: 1 for b in range(n_seqs)}, {3: 60, 70: 9, 71: 1, 129: 1}, {}, {70: 128}, {b: 1 for b in range(0, n_seqs, 2)}):
+        counts = [min(news.get(b, 0), int(lens[b])) for b in range(n_seqs)]
+        c.t["starts"].lazydata.copyin(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+        for t in (out, ref):
+            t.lazydata.copyin(np.full(q.shape, 7, np.float16))
+        check(hip.jsgrad_hip_graph_launch(graph))
+        got = out.numpy()
+        run_attention(hip, other, oq, H, 0, 0, ws[0])
+        check(hip.jsgrad_hip_attn_paged(*c.batch, tq.ptr, ref.ptr, H, 0, 0, ws[1].ptr))
+        assert np.array_equal(got, ref.numpy()) and np.all(got[sum(counts):] == 7) and not np.any(got[:sum(counts)] == 7)
+        if sum(counts) in (130, 128):
+            c.starts, c.news = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32), counts
+            want, tol = attention(c, q, H)
+            compare(got, want, tol, sum(counts))
+    check(hip.jsgrad_hip_graph_destroy(graph))
