@@ -165,16 +165,16 @@ __device__ __forceinline__ float scale_of_v(float v, bool zeros) { return v >= 0
 // wants them; V^T fragments by transposing LDS reads; one barrier per tile, tile t + 1 being asked for behind the barrier of tile t.
 // A page has 16 rows at least: the 16 rows of a tile that a wavefront brings lie on one page, whose number it asks for a tile ahead.
 // fp16 pages come by direct global-to-LDS loads.  int8 ones come through registers and become halves on their way into LDS (exact), once for the block;
-// K's scale multiplies the scores.  V's scale goes into the exponent, weight = exp2(score + log2(scale) - maximum of that), so that what is rounded to fp16 is at
-// most 1 and the largest contributions keep their bits whatever the scales are; the sum of the weights takes it out again, in float.
+// K's scale multiplies the scores.  V's scale goes into the exponent, weight = exp2(score + log2(scale) - maximum of that), so that the largest contributions
+// keep their bits whatever the scales are; the sum of the weights takes it out again, in float.
 // Tiles that hold keys which some row of the wavefront does not see (the diagonal, a window's edge, a missing page) take their V through a test: halves that are not
 // finite are left out of the product, where a weight of zero would not stop them, and added for the rows that see them.
 //
-// 16 x 2048 rows of 32 heads over 8, causal: heads of 128, fp16 757 us = 0.73 PFLOP/s, int8 820; heads of 64 395 and 525.  No unit is full: at the 1.7 GHz that the power limit leaves, the
-// matrix cores are busy 38 % of the time and the vector unit 46 (an exponential per score, and four more operations), LDS 19; a wavefront waits 29 % for memory and barriers and 29 % to issue, and
+// 16 x 2048 rows of 32 heads over 8, causal: heads of 128, fp16 735 us = 0.75 PFLOP/s, int8 808; heads of 64 407 and 498.  No unit is full: at the 1.8 GHz that the power limit leaves, the
+// matrix cores are busy 35 % of the time and the vector unit 51 (an exponential per score, and four more operations), LDS 18; a wavefront waits 26 % for memory and barriers and 30 % to issue, and
 // registers and LDS have room for two to a SIMD (heads of 64: three or four).
 constexpr int PC_THREADS = 256, PC_QROWS = 128;
-constexpr int PC_BLOCKS = 512, PC_LEAST = 4;               // two blocks to a compute unit; a tile takes 1.5 us, and a part some 5 us of its own
+constexpr int PC_BLOCKS = 512, PC_LEAST = 4;               // two blocks to a compute unit; a tile takes 1.4 us, and a part some 5 us of its own
 constexpr int PC_SLOTS = 2 * PC_BLOCKS;
 // A row's weights are exp2(score - its maximum + PC_TOP): the largest is 2^15, which a half holds exactly, the others are rounded to 11 bits down to 2^-29 of it.
 constexpr float PC_TOP = 15.0f;
@@ -573,20 +573,20 @@ template <int HD, bool I8> struct PagedChunk {
 // for as soon as the scores are made, its V rows as soon as those are in LDS, and nothing is waited for but that.  The wavefronts meet once, at the end.
 // The matrix instruction's 16 columns are the rows, so that a lane has four scores of each 16 keys of one row, and its weights are the operand of O^T = V^T . P^T as they lie.
 // Parts of an item are merged by the last of its blocks to arrive.
-// 3 sequences of 65000, 32 heads of 128 over 8, fp16: 117 us = 5.8 TB/s, as fast as a launch that only reads.  16 of 58 to 2304, int8 (81 MB) 20.9 us = 3.9 TB/s: 4 us of launch, some 3 each
+// 3 sequences of 65000, 32 heads of 128 over 8, fp16: 117 us = 5.8 TB/s, as fast as a launch that only reads.  16 of 435 to 4352, int8 (81 MB) 21.4 us = 3.8 TB/s: 4 us of launch, some 3 each
 // until the first keys are there and for the merge.
 constexpr int PF_THREADS = 256, PF_QROWS = 16;
 constexpr int PF_BLOCKS = 512, PF_LEAST = 2;
 constexpr int PF_SLOTS = 2 * PF_BLOCKS, PF_MOST = 64;      // parts of an item: a lane for each
 constexpr float PF_TOP = 15.0f;                            // a row's largest weight is 2^15: halves are normal numbers down to 2^-29 of it
-// Which sequences these blocks take.  A tile of 64 keys costs a compute unit 0.56 us for 16 pairs here and 1.4 for a chunk of 128 (int8 0.45 and 1.8; heads of 64 0.28 and 0.9,
-// 0.33 and 1.2), so that of up to 32 pairs their rows come cheaper: us, 16 pairs | 32 pairs, heads of 128, fp16 and int8: 30 sequences of up to 2300 with 32 pairs each 45 | 51 and
-// 49 | 34, behind 512 rows of another 72 | 67 and 87 | 75, four of 16000 76 | 60 and 80 | 49; 64 pairs: 30 sequences with 48 each 46 | 60 and 51 | 46.
+// Which sequences these blocks take.  A tile of 64 keys costs a compute unit 0.6 us for 16 pairs here and 1.4 for a chunk of 128 (int8 0.55 and 1.5; heads of 64 0.37 and 0.8, 0.35 and 0.95), so
+// that of up to 32 pairs their rows come cheaper: us, sequences of up to 16 pairs here | up to 32 | up to 64, heads of 128, fp16 and int8: 30 sequences of up to 2300 with 32 pairs each 56 | 55 | 56 and
+// 55 | 40 | 40, behind 512 rows of another 87 | 80 | 81 and 103 | 81 | 80, four of 16000 77 | 61 | 61 and 82 | 51 | 50; with 48 pairs each 51 | 51 | 69 and 58 | 58 | 59.
 constexpr int PF_PAIRS = 32;
 // And a batch with little work has all of its rows here: a few keys on each of many compute units are done before a chunk's blocks have started and merged.
-// us, one sequence, 32 heads of 128 over 8, chunks | these, new rows behind so many (tiles of 16 pairs and 64 keys): fp16, 64 behind 1024 (2176) 17.9 | 14.8, 128 behind 1024
-// (4608) 18.4 | 15.7, 10 behind 16000 (6024) 41 | 29, 256 behind 500 (6144) 18.7 | 21.0, 64 behind 4000 (8192) 25.6 | 28.9; int8, 10240 28.2 | 26.6, 16640 40 | 42; heads of 64,
-// 10240 16.9 | 15.4, 16640 23.2 | 26.6.
+// us, one sequence, 32 heads of 128 over 8, chunks | these, new rows behind so many (tiles of 16 pairs and 64 keys): fp16, 64 behind 1024 (2176) 17.7 | 14.3, 128 behind 1024
+// (4608) 18.6 | 15.0, 10 behind 16000 (6024) 41 | 29, 256 behind 500 (6144) 18.2 | 18.7, 64 behind 4000 (8192) 25.8 | 28.4; int8, 64 behind 4000 29.1 | 28.2, 128 behind 4000 (16640) 40 | 44; heads
+// of 64, 64 behind 4000 18.0 | 17.7 and 21.5 | 20.1, 128 behind 4000 24.7 | 26.9 and 26.8 | 31.8.  Few rows behind a long context would gain beyond that: 16 behind 65000, int8 99 | 85.
 template <int HD, bool I8> constexpr float PF_ALL = HD == 128 && !I8 ? 6100.0f : 12288.0f;
 
 template <int HD, bool I8> struct PagedFew {
@@ -965,7 +965,8 @@ template <int HD, bool I8> __global__ __launch_bounds__(PF_THREADS, HD == 64 ? 4
 
 // Chunks, and beside them the sequences that have PF_PAIRS and fewer: the ones are bound by the matrix cores and the vector unit, the others by memory.  Those come first, a
 // block for every compute unit, and the chunks' blocks beside them, as many again.  us, 512 rows behind 1792 and 30 sequences of up to 2304 with one each, heads of 128, fp16 | int8: chunks
-// alone 38 | 50, the others alone 40 | 25; chunks first, two blocks to a unit 84 | 71; the others first 66 | 71, and one block of each to a unit 57 | 64.
+// alone 36 | 43, the others alone 41 | 26, together 57 | 60.  (On an
+// earlier form of the kernels, with 57 | 64 like this: chunks first, two blocks to a unit 84 | 71; the others first 66 | 71.)
 template <int HD, bool I8> __global__ __launch_bounds__(PC_THREADS, HD == 128 ? 2 : I8 ? 3 : 4) void attn_paged_chunk_kernel(PagedAttnArgs a) {
   __shared__ union {
     typename PagedChunk<HD, I8>::Smem chunk;
