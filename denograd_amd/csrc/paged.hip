@@ -22,6 +22,8 @@ struct PagedArgs {
   const _Float16 *x[3];                  // k, v, q rows in
   _Float16 *y[3];                        // k, v, q rows out
   const _Float16 *rope;                  // [positions][HD/2][2] or null
+  const _Float16 *norm[3];               // k's weights [HD], none, q's
+  float eps;
   int n_kv_heads, n_heads;               // n_heads 0: no q
   Divisor pieces;                        // of a row that is read: 8 elements of a head each
 };
@@ -47,7 +49,9 @@ template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 
 // Bound by memory: 32768 rows of 32 and 8 heads of 128, fp16 159 us = 5.1 TB/s, int8 170 (the quotients are divided out, so that a code is the nearest one: fp16 rows have many
 // that lie in the middle).  One block per row of the batch, a thread per 8 elements of a head: its heads are n_kv_heads of k, as many of v, then n_heads of q.
-template <int HD, bool I8> __global__ __launch_bounds__(PR_THREADS) void paged_write_kernel(PagedArgs a) {
+// NORM: rows of k and q are RMSNorm'ed per head in front of the rotation, x / sqrt(mean x^2 + eps) * weight, all of it in float: the squares of a head are summed over the
+// lanes that hold it, so it costs no trip to memory beside that of the weights.
+template <int HD, bool I8, bool NORM> __global__ __launch_bounds__(PR_THREADS) void paged_write_kernel(PagedArgs a) {
   constexpr int G = HD / 8;
   const int r = blockIdx.x, KV = a.n_kv_heads, heads = 2 * KV + a.n_heads;
   const int b = paged_find(a.pb, r);
@@ -62,11 +66,23 @@ template <int HD, bool I8> __global__ __launch_bounds__(PR_THREADS) void paged_w
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) f[e] = (float)x[e];
+    if constexpr (NORM) {
+      if (which != 1) {
+        const h8_t w = *(const h8_t *)(a.norm[which] + e0);
+        float sq = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) sq = fmaf(f[e], f[e], sq);
+        sq = G == 8 ? row8_sum(sq) : row16_sum(sq);
+        const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fmul_rn(sq, 1.0f / HD), a.eps)));
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = f[e] * r * (float)w[e];
+      }
+    }
     if (which != 1 && a.rope) {
       const h8_t cs = *(const h8_t *)(a.rope + (size_t)pos * HD + e0);   // cos, sin of four pairs
 #pragma unroll
       for (int p = 0; p < 4; p++) {
-        const float ev = (float)x[2 * p], od = (float)x[2 * p + 1], c = (float)cs[2 * p], d = (float)cs[2 * p + 1];
+        const float ev = f[2 * p], od = f[2 * p + 1], c = (float)cs[2 * p], d = (float)cs[2 * p + 1];
         f[2 * p] = ev * c - od * d;
         f[2 * p + 1] = ev * d + od * c;
       }
@@ -226,6 +242,98 @@ int paged_check(const char *who, const jsgrad_hip_pages_t *pg, const int32_t *ro
 }
 static bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
+// ---- pages to other pages
+//
+// A move is {from, to, positions}: the first `positions` of every segment of page `from` to page `to`, in every pool.  Bound by memory: a block moves COPY_BYTES of one
+// move and pool, four 16-byte pieces to a thread in flight.  Pools travel in the kernel's arguments: 128 are the K, V and scales of 32 layers, and one launch.
+constexpr int COPY_POOLS = 128, COPY_MOVES = 32768, COPY_UNROLL = 4;
+constexpr size_t COPY_BYTES = PR_THREADS * 16 * COPY_UNROLL;
+struct CopyPool {
+  unsigned char *data;
+  int segments, positions, bytes;
+};
+struct CopyArgs {
+  CopyPool pool[COPY_POOLS];
+  const int32_t *moves;
+  int n_pages, parts;                    // parts of a page, COPY_BYTES each
+};
+
+template <typename U> __device__ __forceinline__ void copy_pieces(const unsigned char *from, unsigned char *to, uint32_t run, uint32_t seg, uint32_t total, uint32_t i0) {
+  // pieces of sizeof(U): `run` of every `seg`
+  U v[COPY_UNROLL];
+  uint32_t at[COPY_UNROLL];
+#pragma unroll
+  for (int u = 0; u < COPY_UNROLL; u++) {
+    const uint32_t i = min(i0 + u * PR_THREADS, total - 1), s = i / run;
+    at[u] = s * seg + (i - s * run);
+    v[u] = *as_global<U>(from + (size_t)at[u] * sizeof(U));
+  }
+#pragma unroll
+  for (int u = 0; u < COPY_UNROLL; u++)
+    if (i0 + u * PR_THREADS < total) *as_global_mut<U>(to + (size_t)at[u] * sizeof(U)) = v[u];
+}
+
+__global__ __launch_bounds__(PR_THREADS) void paged_copy_kernel(CopyArgs a) {
+  const int which = blockIdx.x / a.parts, part = blockIdx.x - which * a.parts;
+  const int32_t *const move = a.moves + (size_t)blockIdx.y * 3;
+  const int from = move[0], to = move[1];
+  const CopyPool &p = a.pool[which];
+  const int n = paged_clamp(move[2], 0, p.positions);
+  if (from < 0 || from >= a.n_pages || to < 0 || to >= a.n_pages || from == to || n == 0) return;
+  const uint32_t seg = (uint32_t)(p.positions * p.bytes), page = (uint32_t)p.segments * seg;
+  // whole pages are one run; a pool of whole 16 bytes per position (rows), or of pages of these, moves by 16, the others (scales) by 4
+  const bool all = n == p.positions;
+  const uint32_t run = all ? page : (uint32_t)(n * p.bytes), step = all ? page : seg, total = all ? page : (uint32_t)p.segments * run;
+  const unsigned char *const src = p.data + (size_t)from * page;
+  unsigned char *const dst = p.data + (size_t)to * page;
+  const uint32_t unit = page % 16 == 0 && run % 16 == 0 && step % 16 == 0 ? 16 : 4;
+  // COPY_BYTES are one turn of 16-byte pieces, or four of 4-byte ones
+  for (uint32_t turn = (uint32_t)part * (16 / unit), end = turn + 16 / unit; turn < end && turn * (PR_THREADS * COPY_UNROLL) < total / unit; turn++) {
+    const uint32_t i0 = turn * (PR_THREADS * COPY_UNROLL) + threadIdx.x;
+    if (unit == 16) copy_pieces<u4_t>(src, dst, run / 16, step / 16, total / 16, i0);
+    else copy_pieces<uint32_t>(src, dst, run / 4, step / 4, total / 4, i0);
+  }
+}
+
+// jsgrad_hip_paged_write and, with norm, jsgrad_hip_paged_write_norm
+static int paged_write(const char *who, const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, const void *k,
+                       const void *v, bool norm, const void *q_weight, const void *k_weight, float eps, const void *rope_table, int rope_rows, void *q_out, int n_heads) {
+  PagedArgs a = {};
+  if (int e = paged_check(who, host_pages, row_starts, lengths, n_seqs, rows, &a.pb)) return e;
+  JSG_REQUIRE(k && v, "%s: null pointer argument", who);
+  JSG_REQUIRE(!q == !q_out, "%s: q and q_out go together", who);
+  JSG_REQUIRE(!q || (n_heads > 0 && n_heads <= 65535), "%s: n_heads %d", who, n_heads);
+  JSG_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(rope_table) && aligned16(q_out), "%s: rows and the rope table must be 16-byte aligned", who);
+  JSG_REQUIRE(!rope_table || rope_rows >= paged_room(a.pb), "%s: a rope table of %d positions, the page table has %d", who, rope_rows, paged_room(a.pb));
+  if (norm) {
+    JSG_REQUIRE(k_weight && !q == !q_weight, "%s: k, and q where it is given, need the weights of their norms", who);
+    JSG_REQUIRE(aligned16(q_weight) && aligned16(k_weight), "%s: norm weights must be 16-byte aligned", who);
+    JSG_REQUIRE(eps >= 0.0f && eps < INFINITY, "%s: eps %g", who, (double)eps);
+  }
+  JSG_READY();
+  a.pages[0] = host_pages->pages_k; a.pages[1] = host_pages->pages_v;
+  a.scales[0] = (float *)host_pages->scales_k; a.scales[1] = (float *)host_pages->scales_v;
+  a.x[0] = (const _Float16 *)k; a.x[1] = (const _Float16 *)v; a.x[2] = (const _Float16 *)q;
+  a.y[2] = (_Float16 *)q_out;
+  a.rope = (const _Float16 *)rope_table;
+  a.norm[0] = (const _Float16 *)k_weight; a.norm[2] = (const _Float16 *)q_weight;
+  a.eps = eps;
+  a.n_kv_heads = host_pages->n_kv_heads; a.n_heads = q ? n_heads : 0;
+  const dim3 grid(rows), block(PR_THREADS);
+  const bool i8 = host_pages->kind == JSGRAD_W_I8;
+#define JSG_WRITE(HD, I8)                                                                                  \
+  do {                                                                                                     \
+    if (norm) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<HD, I8, true>), grid, block, 0, a);            \
+    else JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<HD, I8, false>), grid, block, 0, a);                \
+  } while (0)
+  if (host_pages->head_dim == 64 && i8) JSG_WRITE(64, true);
+  else if (host_pages->head_dim == 64) JSG_WRITE(64, false);
+  else if (i8) JSG_WRITE(128, true);
+  else JSG_WRITE(128, false);
+#undef JSG_WRITE
+  return 0;
+}
+
 }  // namespace jsg
 
 using namespace jsg;
@@ -234,27 +342,45 @@ extern "C" {
 
 int jsgrad_hip_paged_write(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q,
                            const void *k, const void *v, const void *rope_table, int rope_rows, void *q_out, int n_heads) {
-  const char *who = "jsgrad_hip_paged_write";
-  PagedArgs a = {};
-  if (int e = paged_check(who, host_pages, row_starts, lengths, n_seqs, rows, &a.pb)) return e;
-  JSG_REQUIRE(k && v, "%s: null pointer argument", who);
-  JSG_REQUIRE(!q == !q_out, "%s: q and q_out go together", who);
-  JSG_REQUIRE(!q || (n_heads > 0 && n_heads <= 65535), "%s: n_heads %d", who, n_heads);
-  JSG_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(rope_table) && aligned16(q_out), "%s: rows and the rope table must be 16-byte aligned", who);
-  JSG_REQUIRE(!rope_table || rope_rows >= paged_room(a.pb), "%s: a rope table of %d positions, the page table has %d", who, rope_rows, paged_room(a.pb));
+  return paged_write("jsgrad_hip_paged_write", host_pages, row_starts, lengths, n_seqs, rows, q, k, v, false, nullptr, nullptr, 0.0f, rope_table, rope_rows, q_out, n_heads);
+}
+
+int jsgrad_hip_paged_write_norm(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, const void *k,
+                                const void *v, const void *q_weight, const void *k_weight, float eps, const void *rope_table, int rope_rows, void *q_out, int n_heads) {
+  return paged_write("jsgrad_hip_paged_write_norm", host_pages, row_starts, lengths, n_seqs, rows, q, k, v, true, q_weight, k_weight, eps, rope_table, rope_rows, q_out, n_heads);
+}
+
+int jsgrad_hip_paged_copy(const jsgrad_hip_pool_t *host_pools, int n_pools, int n_pages, const int32_t *moves, int n_moves) {
+  const char *who = "jsgrad_hip_paged_copy";
+  JSG_REQUIRE(host_pools && moves, "%s: null pointer argument", who);
+  JSG_REQUIRE(n_pools > 0 && n_pages > 0 && n_moves > 0, "%s: %d pools of %d pages, %d moves", who, n_pools, n_pages, n_moves);
+  JSG_REQUIRE((uintptr_t)moves % 4 == 0, "%s: moves must be 4-byte aligned", who);
+  for (int i = 0; i < n_pools; i++) {
+    const jsgrad_hip_pool_t &p = host_pools[i];
+    JSG_REQUIRE(p.data, "%s: pool %d: null pointer", who, i);
+    JSG_REQUIRE(p.segments > 0 && p.positions > 0 && p.bytes > 0 && p.bytes % 4 == 0, "%s: pool %d: %d segments of %d positions of %d bytes (a multiple of 4)", who, i, p.segments, p.positions, p.bytes);
+    JSG_REQUIRE((size_t)p.positions * p.bytes < (size_t)1 << 30 && (size_t)p.segments * ((size_t)p.positions * p.bytes) < (size_t)1 << 30, "%s: pool %d: a page of 1 GiB or more", who, i);
+    JSG_REQUIRE((uintptr_t)p.data % 16 == 0, "%s: pool %d must be 16-byte aligned", who, i);
+  }
   JSG_READY();
-  a.pages[0] = host_pages->pages_k; a.pages[1] = host_pages->pages_v;
-  a.scales[0] = (float *)host_pages->scales_k; a.scales[1] = (float *)host_pages->scales_v;
-  a.x[0] = (const _Float16 *)k; a.x[1] = (const _Float16 *)v; a.x[2] = (const _Float16 *)q;
-  a.y[2] = (_Float16 *)q_out;
-  a.rope = (const _Float16 *)rope_table;
-  a.n_kv_heads = host_pages->n_kv_heads; a.n_heads = q ? n_heads : 0;
-  const dim3 grid(rows), block(PR_THREADS);
-  const bool i8 = host_pages->kind == JSGRAD_W_I8;
-  if (host_pages->head_dim == 64 && i8) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<64, true>), grid, block, 0, a);
-  else if (host_pages->head_dim == 64) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<64, false>), grid, block, 0, a);
-  else if (i8) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<128, true>), grid, block, 0, a);
-  else JSG_LAUNCH(PROF_PAGED_ROWS, (paged_write_kernel<128, false>), grid, block, 0, a);
+  for (int p0 = 0; p0 < n_pools; p0 += COPY_POOLS) {
+    CopyArgs a = {};
+    const int n = n_pools - p0 < COPY_POOLS ? n_pools - p0 : COPY_POOLS;
+    size_t most = 0;
+    for (int i = 0; i < n; i++) {
+      const jsgrad_hip_pool_t &p = host_pools[p0 + i];
+      a.pool[i] = {(unsigned char *)p.data, p.segments, p.positions, p.bytes};
+      const size_t page = (size_t)p.segments * p.positions * p.bytes;
+      most = most > page ? most : page;
+    }
+    a.n_pages = n_pages;
+    a.parts = (int)((most + COPY_BYTES - 1) / COPY_BYTES);
+    for (int m0 = 0; m0 < n_moves; m0 += COPY_MOVES) {
+      a.moves = moves + (size_t)m0 * 3;
+      // 2^16 parts of a page and COPY_POOLS are 2^23 blocks along x
+      JSG_LAUNCH(PROF_PAGED_ROWS, paged_copy_kernel, dim3((unsigned)(a.parts * n), (unsigned)(n_moves - m0 < COPY_MOVES ? n_moves - m0 : COPY_MOVES)), dim3(PR_THREADS), 0, a);
+    }
+  }
   return 0;
 }
 

@@ -30,6 +30,11 @@ class PagesDesc(C.Structure):
                 + [(n, C.c_void_p) for n in ("pages_k", "pages_v", "scales_k", "scales_v", "page_table")])
 
 
+class Pool(C.Structure):
+    """jsgrad_hip_pool_t"""
+    _fields_ = [("data", C.c_void_p)] + [(n, C.c_int) for n in ("segments", "positions", "bytes")]
+
+
 _pages = C.POINTER(PagesDesc)    # an instance may be passed as it is
 
 # name -> (argtypes, restype); every entry point declared in include/jsgrad_hip.h
@@ -94,6 +99,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "jsgrad_hip_attn_decode_batch": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32], _i32),
     "jsgrad_hip_argmax_rows": ([_vp, _i32, _i32, _vp], _i32),
     "jsgrad_hip_paged_write": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32], _i32),
+    "jsgrad_hip_paged_write_norm": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _i32, _vp, _i32], _i32),
+    "jsgrad_hip_paged_copy": ([C.POINTER(Pool), _i32, _i32, _vp, _i32], _i32),
     "jsgrad_hip_paged_read": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp], _i32),
     "jsgrad_hip_attn_paged_workspace_bytes": ([_i32, _i32, _i32], _sz),
     "jsgrad_hip_attn_paged": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp], _i32),

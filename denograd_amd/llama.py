@@ -32,7 +32,7 @@ def precompute_freqs_cis(dim: int, end: int, theta: float = 10000.0, dtype: str 
 
 
 class Attention:
-    def __init__(self, dim: int, n_heads: int, n_kv_heads: int | None, max_context: int, linear=Linear):
+    def __init__(self, dim: int, n_heads: int, n_kv_heads: int | None, max_context: int, linear=Linear, qk_norm_eps: float | None = None):
         self.n_heads = n_heads
         self.n_kv_heads = n_kv_heads if n_kv_heads is not None else n_heads
         self.head_dim = dim // n_heads
@@ -43,8 +43,14 @@ class Attention:
         self.wk = linear(dim, self.n_kv_heads * self.head_dim, False)
         self.wv = linear(dim, self.n_kv_heads * self.head_dim, False)
         self.wo = linear(self.n_heads * self.head_dim, dim, False)
+        if qk_norm_eps is not None:            # queries and keys are normed per head in front of the rotation: on a paged cache (call_paged)
+            self.q_norm, self.k_norm = RMSNorm(self.head_dim, qk_norm_eps), RMSNorm(self.head_dim, qk_norm_eps)
         self.cache_kv: Tensor | None = None
         self.layer_id: int | None = None   # set by Transformer: which layer of the model this is
+
+    @property
+    def qk_norms(self) -> "dict[str, RMSNorm]":
+        return {"q_norm": self.q_norm, "k_norm": self.k_norm} if hasattr(self, "q_norm") else {}
 
     def _ensure_cache(self, dtype: str, device: str, bsz: int = 1) -> None:
         # Tensor.zeros([2, bsz, max_context, n_kv_heads, head_dim]) (llama.ts:78-80); created for the batch size of the
@@ -86,7 +92,7 @@ class Attention:
             check(lib.jsgrad_hip_gemm_qkv_rope(*weights, *rest))
         else:
             check(lib.jsgrad_hip_gemm_qkv_rope_norm(*weights, norm.weight.ptr, norm.eps, rows.xn.ptr, *rest))
-        batch.write(layer, rows.k, rows.v, rows.q, freqs_cis, self.n_heads)
+        batch.write(layer, rows.k, rows.v, rows.q, freqs_cis, self.n_heads, **self.qk_norms)
         batch.attend(layer, rows.q, self.n_heads, rows.attn, window, sinks)
         check(lib.jsgrad_hip_gemm(self.wo.kind, self.wo.weight.ptr, sp(self.wo), self.dim, self.n_heads * self.head_dim, rows.attn.ptr, n, out.ptr, residual.ptr))
         return out
@@ -144,8 +150,9 @@ ATTENTION_ROWS, ATTENTION_PAGED, FEED_FORWARD_ROWS = Attention.call_rows, Attent
 
 
 class TransformerBlock:
-    def __init__(self, dim: int, hidden_dim: int, n_heads: int, n_kv_heads: int | None, norm_eps: float, max_context: int, linear=Linear, feed_forward=FeedForward):
-        self.attention = Attention(dim, n_heads, n_kv_heads, max_context, linear)
+    def __init__(self, dim: int, hidden_dim: int, n_heads: int, n_kv_heads: int | None, norm_eps: float, max_context: int, linear=Linear, feed_forward=FeedForward,
+                 qk_norm: bool = False):
+        self.attention = Attention(dim, n_heads, n_kv_heads, max_context, linear, norm_eps if qk_norm else None)
         self.feed_forward = feed_forward(dim, hidden_dim, linear)
         self.attention_norm = RMSNorm(dim, norm_eps)
         self.ffn_norm = RMSNorm(dim, norm_eps)
@@ -358,11 +365,12 @@ class TinyJit:
 class Transformer:
     def __init__(self, dim: int, hidden_dim: int, n_heads: int, n_layers: int, norm_eps: float, vocab_size: int, linear=Linear, embedding=Embedding,
                  n_kv_heads: int | None = None, rope_theta: float = 10000, max_context: int = 1024, jit: bool = True, feed_forward=FeedForward, device: str = "HIP",
-                 fused_step: bool = False, fuse_attn_wo: bool = True):
+                 fused_step: bool = False, fuse_attn_wo: bool = True, qk_norm: bool = False):
         self.dim, self.hidden_dim, self.n_heads, self.vocab_size, self.max_context = dim, hidden_dim, n_heads, vocab_size, max_context
         self.n_kv_heads = n_kv_heads if n_kv_heads is not None else n_heads
         self.rope_theta, self.device = rope_theta, device
-        self.layers = [TransformerBlock(dim, hidden_dim, n_heads, n_kv_heads, norm_eps, max_context, linear, feed_forward) for _ in range(n_layers)]
+        self.layers = [TransformerBlock(dim, hidden_dim, n_heads, n_kv_heads, norm_eps, max_context, linear, feed_forward, qk_norm) for _ in range(n_layers)]
+        self.qk_norm = qk_norm                        # RMSNorms of queries and keys per head: such a model runs on a paged cache
         self.norm = RMSNorm(dim, norm_eps)
         self.tok_embeddings = embedding(vocab_size, dim)
         self.output = Linear(dim, vocab_size, False) if embedding is Embedding else linear(dim, vocab_size, False)
@@ -433,6 +441,8 @@ class Transformer:
         return "stream" if self.fused_step == "stream" else "barrier"
 
     def _prepare(self) -> _Scratch:
+        if self.qk_norm:
+            raise NotImplementedError("a model that norms queries and keys per head runs on a paged cache (forward_paged)")
         if self._ctx is None:
             hd = self.dim // self.n_heads
             self._ctx = _Scratch(self.dim, self.hidden_dim, self.n_heads, self.n_kv_heads, hd, self.vocab_size, self.dtype, self.device)
@@ -741,6 +751,8 @@ def convert_from_huggingface(weights: dict, n_layers: int, n_heads: int, n_kv_he
     for l in range(n_layers):
         keymap[f"model.layers.{l}.input_layernorm.weight"] = f"layers.{l}.attention_norm.weight"
         keymap[f"model.layers.{l}.post_attention_layernorm.weight"] = f"layers.{l}.ffn_norm.weight"
+        for x in "qk":
+            keymap[f"model.layers.{l}.self_attn.{x}_norm.weight"] = f"layers.{l}.attention.{x}_norm.weight"
         for x in "qkvo":
             keymap[f"model.layers.{l}.self_attn.{x}_proj.weight"] = f"layers.{l}.attention.w{x}.weight"
             keymap[f"model.layers.{l}.self_attn.{x}_proj.bias"] = f"layers.{l}.attention.w{x}.bias"
@@ -760,6 +772,8 @@ def convert_from_huggingface(weights: dict, n_layers: int, n_heads: int, n_kv_he
             out = Tensor.empty(t.shape, t.dtype, device)
             check(lib.jsgrad_hip_hf_permute(t.ptr, out.ptr, t.shape[0], t.nbytes // t.shape[0], heads))
             t = out
+        if "self_attn" in k and permute_layers and ("q_norm" in k or "k_norm" in k):      # the weights of a head's features go the way of the features
+            t = Tensor(np.ascontiguousarray(t.numpy().reshape(2, -1).T).reshape(-1), dtype=t.dtype, device=device)
         sd[keymap[k]] = t
     return sd
 

@@ -127,7 +127,7 @@ class Llama3:
         self.params = params
         self.model = Transformer(params["dim"], params["hidden_dim"], params["n_heads"], params["n_layers"], params["norm_eps"], params["vocab_size"],
                                  self.linear, self.embedding, params.get("n_kv_heads"), params["rope_theta"], self.max_context, True, device=device,
-                                 fused_step=fused_step)
+                                 fused_step=fused_step, qk_norm=bool(params.get("qk_norm")))
         self.start_pos = 0
         self.tokenizer = None                  # set by load_tokenizer
         self.last_seen_toks: list[int] = []
@@ -141,6 +141,7 @@ class Llama3:
         """A model of a synthetic configuration (denograd_amd/synthetic.py).  Greedy unless told otherwise: the parity and
         benchmark runs compare argmax tokens; the constructor itself defaults to the reference's temperature 0.95 (llama3.ts:192)."""
         args = {k: cfg[k] for k in ("dim", "hidden_dim", "n_heads", "n_kv_heads", "n_layers", "norm_eps", "rope_theta", "vocab_size")}
+        args["qk_norm"] = cfg.get("qk_norm", False)
         q = cfg["quantize"] if cfg["quantize"] in ("int8", "nf4") else None
         return Llama3(quantize=q, device=device, max_context=cfg["max_context"], temperature=temperature, args=args, fused_step=fused_step)
 
@@ -214,6 +215,9 @@ class Llama3:
                 sd.update(quantise_one(f"layers.{l}.{name}.weight", randn(shp)))   # the fp16 source is freed right after
             sd[f"layers.{l}.attention_norm.weight"] = Tensor.ones((p["dim"],), "float16", self.device)
             sd[f"layers.{l}.ffn_norm.weight"] = Tensor.ones((p["dim"],), "float16", self.device)
+            if p.get("qk_norm"):
+                for x in "qk":
+                    sd[f"layers.{l}.attention.{x}_norm.weight"] = Tensor.ones((p["dim"] // p["n_heads"],), "float16", self.device)
         sd["norm.weight"] = Tensor.ones((p["dim"],), "float16", self.device)
         if self.quantize_embeds or tied:
             sd["output.weight"] = sd["tok_embeddings.weight"]

@@ -1,4 +1,5 @@
 """A paged KV cache: sequences of different lengths in pages of one pool, in fp16 or quantised to int8 as they are written.
+Sequences that begin alike may share pages (`fork`): whoever writes into a shared page gets a copy of it first.
 
 Stands beside the contiguous cache of `llama.Attention` (jsgrad/models/llama.ts:78-87), which holds equally long sequences at one
 position and reserves max_context positions for each.  `PageTable` is the bookkeeping, on the host alone; `PagedCache` has the pools of every
@@ -8,12 +9,16 @@ runs a model on it.
 from __future__ import annotations
 
 from math import prod
+from typing import TYPE_CHECKING
 
 import numpy as np
 
 from . import ffi
 from .ffi import check
 from .tensor import Tensor
+
+if TYPE_CHECKING:
+    from .nn import RMSNorm
 
 
 class PageTable:
@@ -26,6 +31,7 @@ class PageTable:
         self.free = list(range(n_pages - 1, -1, -1))
         self.pages: dict[int, list[int]] = {}                 # per sequence; -1: given away behind the window
         self.lengths: dict[int, int] = {}
+        self.shared: dict[int, int] = {}                      # pages with more than one holder: how many
         self._next = 0
 
     @staticmethod
@@ -45,33 +51,86 @@ class PageTable:
         self.pages[seq], self.lengths[seq] = [], 0
         return seq
 
+    def _let_go(self, pages) -> None:
+        """One holder less of each of these; those that had no other are free."""
+        for p in pages:
+            if p < 0:
+                continue
+            if p in self.shared:
+                self.shared[p] -= 1
+                if self.shared[p] == 1:
+                    del self.shared[p]
+            else:
+                self.free.append(p)
+
     def drop(self, seq: int) -> None:
-        """The sequence is over; its pages are free."""
-        self.free += [p for p in reversed(self.pages.pop(seq)) if p >= 0]
+        """The sequence is over; pages that no other one holds are free."""
+        self._let_go(reversed(self.pages.pop(seq)))
         del self.lengths[seq]
 
-    def grow(self, seqs, counts) -> None:
-        """Room for counts[i] more positions of seqs[i].  Nothing changes where the pool has too few pages left."""
+    def fork(self, seq: int, at: int | None = None) -> int:
+        """A new sequence that begins with the first `at` positions of this one (default: all), in the same pages."""
+        at = self.lengths[seq] if at is None else int(at)
+        if not 0 <= at <= self.lengths[seq]:
+            raise ValueError(f"a fork at position {at} of a sequence of {self.lengths[seq]}")
+        pages = self.pages[seq][:-(-at // self.page_size)]
+        if at % self.page_size and pages[-1] < 0:
+            raise ValueError(f"a fork at position {at}, in a page that was given away")
+        new = self.add()
+        self.pages[new], self.lengths[new] = list(pages), at
+        for p in pages:
+            if p >= 0:
+                self.shared[p] = self.shared.get(p, 1) + 1
+        return new
+
+    def grow(self, seqs, counts) -> list[tuple[int, int, int]]:
+        """Room for counts[i] more positions of seqs[i].  A begun last page that others hold as well is replaced by one of the sequence's own; returns what is to be copied
+        before anything is written, as (from, to, positions).  Nothing changes where the pool has too few pages left."""
         seqs, counts = list(seqs), [int(c) for c in counts]
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
             raise ValueError(f"sequences {seqs} with {counts} new positions: one count of 0 and more for each, no sequence twice")
         need = [-(-(self.lengths[s] + c) // self.page_size) - len(self.pages[s]) for s, c in zip(seqs, counts)]
-        if sum(need) > len(self.free):
-            raise MemoryError(f"{sum(need)} pages are needed and {len(self.free)} of {self.n_pages} are free")
-        for s, c, n in zip(seqs, counts, need):
+        holders, own = {}, []                                 # the last holder that is left writes into the page itself
+        for s, c in zip(seqs, counts):
+            last = self.pages[s][self.lengths[s] // self.page_size] if c and self.lengths[s] % self.page_size else -1
+            n = holders.get(last, self.shared.get(last, 1))
+            own.append(last if last >= 0 and n > 1 else -1)
+            if own[-1] >= 0:
+                holders[last] = n - 1
+        wanted = sum(need) + sum(p >= 0 for p in own)
+        if wanted > len(self.free):
+            raise MemoryError(f"{wanted} pages are needed and {len(self.free)} of {self.n_pages} are free")
+        moves = []
+        for s, c, n, old in zip(seqs, counts, need, own):
+            if old >= 0:
+                at = self.lengths[s] // self.page_size
+                self.pages[s][at] = self.free.pop()
+                self._let_go([old])
+                moves.append((old, self.pages[s][at], self.lengths[s] % self.page_size))
             self.pages[s] += [self.free.pop() for _ in range(n)]
             self.lengths[s] += c
+        return moves
 
-    def _held(self, seqs) -> list[tuple[int, int, int]]:
-        return [(s, len(self.pages[s]), self.lengths[s]) for s in seqs]
+    def _held(self, seqs) -> list[tuple[int, list[int], int]]:
+        return [(s, list(self.pages[s]), self.lengths[s]) for s in seqs]
 
     def _put_back(self, held) -> None:
         """Takes a grow back: held is what the sequences had before it."""
-        for s, n, length in reversed(held):
-            if s in self.pages:
-                self.free += [p for p in reversed(self.pages[s][n:]) if p >= 0]
-                del self.pages[s][n:]
-                self.lengths[s] = length
+        for s, pages, length in reversed(held):
+            if s not in self.pages:
+                continue
+            n = len(pages)
+            self._let_go(reversed(self.pages[s][n:]))
+            for at, (mine, old) in enumerate(zip(self.pages[s], pages)):
+                if mine == old or mine < 0:                   # a page that was given away in the meantime stays so
+                    pages[at] = mine
+                    continue
+                self._let_go([mine])
+                if old in self.free:                          # its other holders are gone
+                    self.free.remove(old)
+                else:
+                    self.shared[old] = self.shared.get(old, 1) + 1
+            self.pages[s], self.lengths[s] = pages, length
 
     def slide(self, seq: int, window: int, sinks: int = 0) -> int:
         """Gives away the pages that no later row of the sequence sees through this window; how many those were."""
@@ -81,9 +140,20 @@ class PageTable:
         # the next row is at position lengths[seq] and sees positions > lengths[seq] - window
         for i in range(-(-sinks // self.page_size), max(0, self.lengths[seq] - window + 1) // self.page_size):
             if pages[i] >= 0:
-                self.free.append(pages[i])
+                self._let_go([pages[i]])
                 pages[i], n = -1, n + 1
         return n
+
+    def _pack(self) -> list[tuple[int, int, int]]:
+        """Renumbers the pages so that those in use are the first ones; what has to be copied for that, from the upper ones to free lower ones."""
+        used = {p for pages in self.pages.values() for p in pages if p >= 0}
+        holes = [p for p in range(len(used)) if p not in used]
+        to = dict(zip(sorted(p for p in used if p >= len(used)), holes))
+        for pages in self.pages.values():
+            pages[:] = [to.get(p, p) for p in pages]
+        self.shared = {to.get(p, p): n for p, n in self.shared.items()}
+        self.free = list(range(self.n_pages - 1, len(used) - 1, -1))
+        return [(a, b, self.page_size) for a, b in to.items()]
 
 
 class PagedCache(PageTable):
@@ -99,6 +169,7 @@ class PagedCache(PageTable):
         rows = (2, n_pages, n_kv_heads, page_size)
         self.pools = [Tensor.zeros((*rows, head_dim), dtype, device) for _ in range(n_layers)]       # k, then v
         self.scales = [Tensor.ones(rows, "float32", device) if dtype == "int8" else None for _ in range(n_layers)]
+        self._moves: Tensor | None = None                     # what is copied next
         self._plan: Tensor | None = None                      # row_starts, lengths and page table of the batch last begun
         self._batches = 0
         self._ws: dict[int, Tensor] = {}
@@ -111,12 +182,45 @@ class PagedCache(PageTable):
         if not 0 < len(seqs) <= 65535 or not 0 < sum(counts) < 1 << 24:
             raise ValueError(f"a batch has 1 to 65535 sequences and fewer than 2^24 rows, one at least: {len(seqs)} with {sum(counts)}")
         held = self._held(seqs)
-        self.grow(seqs, counts)
+        moves = self.grow(seqs, counts)
         try:
+            if moves:
+                self._copy(moves)
             return self._plan_batch(seqs, counts, held)
         except BaseException:
             self._put_back(held)
             raise
+
+    def _page_pools(self) -> list[ffi.Pool]:
+        """Every pool of every layer."""
+        pools, row = [], self.head_dim * (2 if self.dtype == "float16" else 1)
+        for pool, scales in zip(self.pools, self.scales):
+            for i in (0, 1):
+                pools.append(ffi.Pool(pool.ptr + i * (pool.nbytes // 2), self.n_kv_heads, self.page_size, row))
+                if scales is not None:
+                    pools.append(ffi.Pool(scales.ptr + i * (scales.nbytes // 2), self.n_kv_heads, self.page_size, 4))
+        return pools
+
+    def _copy(self, moves) -> None:
+        moves = np.array(moves, np.int32).reshape(-1, 3)
+        if self._moves is None or self._moves.numel < moves.size:
+            self._moves = Tensor.empty((2 * moves.size,), "int32", self.device)
+        self._moves.lazydata.view(moves.size, "int32", 0).ensure_allocated().copyin(moves.reshape(-1))
+        pools = self._page_pools()
+        check(ffi.load().jsgrad_hip_paged_copy((ffi.Pool * len(pools))(*pools), len(pools), self.n_pages, self._moves.ptr, len(moves)))
+
+    def compact(self) -> int:
+        """Packs the pages in use into the first ones of the pools, in all layers; how many those are.  A batch that had begun is over."""
+        kept = {s: list(p) for s, p in self.pages.items()}, dict(self.shared), list(self.free)
+        moves = self._pack()
+        self._batches += 1
+        try:
+            if moves:
+                self._copy(moves)
+        except BaseException:
+            self.pages, self.shared, self.free = kept
+            raise
+        return self.n_pages - len(self.free)
 
     def _plan_batch(self, seqs, counts, held) -> "PagedBatch":
         width = max(1, max(len(self.pages[s]) for s in seqs))
@@ -143,7 +247,7 @@ class PagedCache(PageTable):
 class PagedBatch:
     """The rows of one ragged batch, in the order of its sequences: row i of a sequence is its position length - count + i."""
 
-    def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int, held: list[tuple[int, int, int]]):
+    def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int, held: list[tuple[int, list[int], int]]):
         self.cache, self.n_seqs, self.rows, self.width, self._held = cache, n_seqs, rows, width, held
         self._number = cache._batches
         self._layers: dict[int, tuple] = {}                   # what the calls on a layer take
@@ -172,8 +276,10 @@ class PagedBatch:
         if t.dtype != "float16" or prod(t.shape) < self.rows * heads * self.cache.head_dim:
             raise ValueError(f"{what}: {self.rows} float16 rows of {heads} heads of {self.cache.head_dim} are wanted, got {t.dtype} {t.shape}")
 
-    def write(self, layer: int, k: Tensor, v: Tensor, q: Tensor | None = None, freqs_cis: Tensor | None = None, n_heads: int = 0, q_out: Tensor | None = None) -> Tensor | None:
-        """Rotates k (and q, into q_out or in place) by freqs_cis, as precompute_freqs_cis makes it, and writes k and v into the pages."""
+    def write(self, layer: int, k: Tensor, v: Tensor, q: Tensor | None = None, freqs_cis: Tensor | None = None, n_heads: int = 0, q_out: Tensor | None = None,
+              q_norm: "RMSNorm | None" = None, k_norm: "RMSNorm | None" = None) -> Tensor | None:
+        """Rotates k (and q, into q_out or in place) by freqs_cis, as precompute_freqs_cis makes it, and writes k and v into the pages.  With k_norm and q_norm, the
+        RMSNorms of a model that norms keys and queries per head, these come in front of the rotation."""
         for what, t in (("k", k), ("v", v)):
             self._check(what, t, self.cache.n_kv_heads)
         if q is not None:
@@ -184,8 +290,16 @@ class PagedBatch:
         if freqs_cis is not None and (freqs_cis.dtype != "float16" or odd):
             raise ValueError(f"freqs_cis: float16 rows of {self.cache.head_dim} are wanted, got {freqs_cis.dtype} {freqs_cis.shape}")
         p = lambda t: t.ptr if t is not None else None
-        check(ffi.load().jsgrad_hip_paged_write(*self._args(layer), p(q), k.ptr, v.ptr, p(freqs_cis), positions,
-                                                p(q_out) if q is not None else None, n_heads))
+        norms = []
+        if k_norm is not None or q_norm is not None:
+            if k_norm is None or (q is None) != (q_norm is None) or (q is not None and q_norm.eps != k_norm.eps):
+                raise ValueError("the norms of q and k go together, with one eps")
+            for norm in (q_norm, k_norm):
+                if norm is not None and (norm.weight.dtype != "float16" or norm.weight.numel != self.cache.head_dim):
+                    raise ValueError(f"norms of q and k: {self.cache.head_dim} float16 weights are wanted, got {norm.weight.dtype} {norm.weight.shape}")
+            norms = [q_norm.weight.ptr if q_norm is not None else None, k_norm.weight.ptr, k_norm.eps]
+        call = ffi.load().jsgrad_hip_paged_write_norm if norms else ffi.load().jsgrad_hip_paged_write
+        check(call(*self._args(layer), p(q), k.ptr, v.ptr, *norms, p(freqs_cis), positions, p(q_out) if q is not None else None, n_heads))
         return q_out if q is not None else None
 
     def read(self, layer: int) -> tuple[Tensor, Tensor]:

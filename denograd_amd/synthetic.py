@@ -59,6 +59,9 @@ def random_state_dict(cfg: dict, seed: int = 0, std: float = 0.02) -> dict[str, 
             sd[f"layers.{l}.{name}.weight"] = randn(shp)
         sd[f"layers.{l}.attention_norm.weight"] = np.ones(cfg["dim"], wdt)
         sd[f"layers.{l}.ffn_norm.weight"] = np.ones(cfg["dim"], wdt)
+        if cfg.get("qk_norm"):                    # queries and keys normed per head
+            for x in "qk":
+                sd[f"layers.{l}.attention.{x}_norm.weight"] = np.ones(cfg["dim"] // cfg["n_heads"], wdt)
     sd["norm.weight"] = np.ones(cfg["dim"], wdt)
     sd["output.weight"] = sd["tok_embeddings.weight"] if cfg.get("tied") else randn((cfg["vocab_size"], cfg["dim"]))
     return sd

@@ -289,6 +289,23 @@ typedef struct {
 int jsgrad_hip_paged_write(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q,
                            const void *k, const void *v, const void *rope_table, int rope_rows, void *q_out, int n_heads);
 
+/* jsgrad_hip_paged_write behind an RMSNorm of every head's row of q and k (RMSNorm.call, nn/index.ts:586-588, over head_dim; models that norm queries and keys have no counterpart in
+ * the reference): x / sqrt(mean x^2 + eps) * weight, in float like the rotation that follows, rounded once.  q_weight, k_weight: float16 [head_dim], 16-byte aligned; q_weight NULL where q is.
+ * eps: 0 and more. */
+int jsgrad_hip_paged_write_norm(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, const void *k,
+                                const void *v, const void *q_weight, const void *k_weight, float eps, const void *rope_table, int rope_rows, void *q_out, int n_heads);
+
+/* A pool of a paged cache, as jsgrad_hip_paged_copy goes by it: its page is [segments][positions][bytes].  K or V: {pages_k, n_kv_heads, page_size, head_dim * 2} (int8: head_dim), scales
+ * {scales_k, n_kv_heads, page_size, 4}, what is kept once per page {p, 1, 1, its bytes}.  bytes: a multiple of 4; data: 16-byte aligned; a page below 1 GiB. */
+typedef struct {
+  void *data;
+  int segments, positions, bytes;
+} jsgrad_hip_pool_t;
+/* Pages to other pages, in all n_pools pools of n_pages pages (BufferCopy, engine/realize.ts:92-122, is the counterpart): moves is device memory, int32 [n_moves][3] = {from, to,
+ * positions}: the first `positions` of every segment (all that a segment has, where it has fewer).  A move from or to a page that is not in the pools, or to itself, is none.  Moves come in no
+ * order: a page that one of them writes must not be read or written by another. */
+int jsgrad_hip_paged_copy(const jsgrad_hip_pool_t *host_pools, int n_pools, int n_pages, const int32_t *moves, int n_moves);
+
 /* The batch's rows out of the pages: k_out, v_out [rows][n_kv_heads][head_dim], RN16(code * scale) of int8 pages, zeros where there is no
  * page.  A whole sequence: as many rows as positions. */
 int jsgrad_hip_paged_read(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, void *k_out, void *v_out);

@@ -67,6 +67,8 @@ const SYMBOLS = {
   jsgrad_hip_attn_decode_batch: { parameters: [P, P, P, P, P, P, I, I, I, I, I], result: I }, // q, cache_k, cache_v, state, out, workspace, batch, n_heads, n_kv_heads, head_dim, max_context
   jsgrad_hip_argmax_rows: { parameters: [P, I, I, P], result: I }, // logits, rows, n, tokens_out
   jsgrad_hip_paged_write: { parameters: [B, P, P, I, I, P, P, P, P, I, P, I], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, k, v, rope_table, rope_rows, q_out, n_heads
+  jsgrad_hip_paged_write_norm: { parameters: [B, P, P, I, I, P, P, P, P, P, F, P, I, P, I], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, k, v, q_weight, k_weight, eps, rope_table, rope_rows, q_out, n_heads
+  jsgrad_hip_paged_copy: { parameters: [B, I, I, P, I], result: I }, // host_pools, n_pools, n_pages, moves, n_moves
   jsgrad_hip_paged_read: { parameters: [B, P, P, I, I, P, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, k_out, v_out
   jsgrad_hip_attn_paged_workspace_bytes: { parameters: [I, I, I], result: U }, // n_heads, n_kv_heads, head_dim
   jsgrad_hip_attn_paged: { parameters: [B, P, P, I, I, P, P, I, I, I, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, out, n_heads, window, sinks, workspace
@@ -156,6 +158,18 @@ export const pack_pages = (d: PagesDesc): Uint8Array => {
   for (let i = 0; i < ints.length; i++) v.setInt32(4 * i, ints[i], true)
   const ptrs = [d.pages_k, d.pages_v, d.scales_k, d.scales_v, d.page_table]                                                        // 24..64
   for (let i = 0; i < ptrs.length; i++) v.setBigUint64(24 + 8 * i, ptrs[i] ?? 0n, true)
+  return new Uint8Array(buf)
+}
+export const POOL_BYTES = 24
+export type PoolDesc = { data: DevPtr, segments: number, positions: number, bytes: number }
+/** The host array handed to jsgrad_hip_paged_copy. */
+export const pack_pools = (pools: PoolDesc[]): Uint8Array => {
+  const buf = new ArrayBuffer(POOL_BYTES * pools.length), v = new DataView(buf)
+  pools.forEach((p, i) => {
+    v.setBigUint64(POOL_BYTES * i, p.data, true)
+    const ints = [p.segments, p.positions, p.bytes]
+    for (let j = 0; j < ints.length; j++) v.setInt32(POOL_BYTES * i + 8 + 4 * j, ints[j], true)
+  })
   return new Uint8Array(buf)
 }
 export const STEP_BYTES = 200
