@@ -113,6 +113,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "jsgrad_hip_read_probe": ([_vp, _sz, _vp], _i32),
     "jsgrad_hip_sample_workspace_bytes": ([_i32], _sz),
     "jsgrad_hip_sample": ([_vp, _i32, _i32, C.c_double, _i32, C.c_double, C.c_double, C.c_double, _vp, _vp, _vp, _vp, _i32, _i32, _vp], _i32),
+    "jsgrad_hip_sample_rows_workspace_bytes": ([_i32, _i32], _sz),
+    "jsgrad_hip_sample_rows": ([_vp, _i32, _i32, _sz, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], _i32),
     "jsgrad_hip_ggml_nbytes": ([_i32, _sz], _sz),
     "jsgrad_hip_ggml_dequant": ([_i32, _vp, _sz, _vp], _i32),
     "jsgrad_hip_cast": ([_vp, _i32, _vp, _i32, _sz], _i32),

@@ -22,6 +22,7 @@ from .tensor import Tensor
 
 if TYPE_CHECKING:
     from .paged import PagedBatch
+    from .sampling import RowSampler
 
 
 def precompute_freqs_cis(dim: int, end: int, theta: float = 10000.0, dtype: str = "float32", device: str = "HIP") -> Tensor:
@@ -627,10 +628,10 @@ class Transformer:
             check(lib.jsgrad_hip_argmax_rows(rows.logits.ptr, bsz, self.vocab_size, rows.next_tokens.ptr))
         return Tensor(buffer=rows.next_tokens.lazydata.view(bsz, "int32", 0), shape=(bsz,), dtype="int32", device=self.device)
 
-    def forward_paged(self, cache, seqs, tokens, window: int = 0, sinks: int = 0) -> Tensor:
+    def forward_paged(self, cache, seqs, tokens, window: int = 0, sinks: int = 0, sampler: "RowSampler | None" = None) -> Tensor:
         """Transformer.forward (llama.ts:201-213) for sequences of different lengths over a PagedCache: tokens[i] are the next token ids of sequence
-        seqs[i], a prompt, a part of one, or the one token that the call before returned.  Returns the greedy next token of every sequence, an int32
-        tensor in the order of seqs (Tensor.argmax of each, as forward_rows for several sequences).  window, sinks: as PagedBatch.attend has them.
+        seqs[i], a prompt, a part of one, or the one token that the call before returned.  Returns the next token of every sequence, an int32
+        tensor in the order of seqs: the greedy one (Tensor.argmax of each, as forward_rows for several sequences), or what the sampler picks.  window, sinks: as PagedBatch.attend has them.
         A row of the model's own contiguous cache is neither read nor written.  fp16 activations; fp16 / int8 / NF4 weights.  Where this raises, the
         sequences are as they were."""
         if self.dtype != "float16":
@@ -649,14 +650,16 @@ class Transformer:
             raise ValueError(f"a cache of {cache.n_layers} layers of {cache.n_kv_heads} heads of {cache.head_dim}, the model has {len(self.layers)} of {self.n_kv_heads} of {hd}")
         if any(cache.lengths[s] + t.size > 2 * self.max_context for s, t in zip(seqs, toks)):
             raise ValueError(f"positions beyond {2 * self.max_context}, where the rotary table ends")
+        if sampler is not None:
+            sampler.check(len(seqs))
         batch = cache.begin(seqs, [t.size for t in toks])
         try:
-            return self._run_paged(cache, batch, toks, flat, window, sinks)
+            return self._run_paged(cache, batch, toks, flat, window, sinks, sampler)
         except BaseException:
             batch._cancel()
             raise
 
-    def _run_paged(self, cache, batch: "PagedBatch", toks, flat: np.ndarray, window: int, sinks: int) -> Tensor:
+    def _run_paged(self, cache, batch: "PagedBatch", toks, flat: np.ndarray, window: int, sinks: int, sampler: "RowSampler | None") -> Tensor:
         lib, hd = ffi.load(), self.dim // self.n_heads
         n, bsz = batch.rows, len(toks)
         if self._paged_rope is None or self._paged_rope.shape[1] < batch.width * cache.page_size:
@@ -681,6 +684,8 @@ class Transformer:
                 check(lib.jsgrad_hip_copy(last.ptr + b * self.dim * 2, rows.h.ptr + int(i) * self.dim * 2, self.dim * 2))
         out = self.output
         check(lib.jsgrad_hip_gemm_norm(out.kind, out.weight.ptr, sp(out), self.vocab_size, self.dim, last.ptr, self.norm.weight.ptr, self.norm.eps, rows.xn.ptr, bsz, rows.logits.ptr))
+        if sampler is not None:
+            return sampler.pick(rows.logits, rows.next_tokens, bsz)
         check(lib.jsgrad_hip_argmax_rows(rows.logits.ptr, bsz, self.vocab_size, rows.next_tokens.ptr))
         return Tensor(buffer=rows.next_tokens.lazydata.view(bsz, "int32", 0), shape=(bsz,), dtype="int32", device=self.device)
 

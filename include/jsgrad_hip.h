@@ -414,6 +414,18 @@ size_t jsgrad_hip_sample_workspace_bytes(int n);
 int jsgrad_hip_sample(const void *logits, int n, int act, double temp, int k, double p, double af, double ap, int32_t *alpha_counter, uint32_t *rng,
                       int32_t *state, int32_t *tokens_out, int tokens_cap, int advance, void *workspace);
 
+/* A token for each of `rows` rows of logits (fp16 or float, row r at r * row_stride elements, n of them, 1 to 1048576), from given random numbers; stands beside `sample` (models/llama.ts:131-185), which
+ * draws for one sequence from a stream of its own.  temperature, top_k, top_p, min_p: one value per row on the device, so that a captured graph replays with what they hold then; NULL: 1, and none of the
+ * others.  With M the row's maximum and w = exp((x - M) / temperature): the entries with w >= min_p (above 1: 1); of these the first top_k (0 and less: all) in the order
+ * (x descending, index ascending); of these, in that order, those with less than top_p of their mass before them, the first at least (1 and more: all); the token is the first of what is left, by index, at which
+ * the running sum of w exceeds uniforms[r] (0 to below 1) of its total, probs_out[r] (or NULL) its share.  A temperature below 1e-6: the lowest index of the maximum, share 1.  What is not a number
+ * counts as minus infinity; a row with nothing above that: token -1, share 0.  Where infinity is the maximum, that alone has weight.  Sums are whole numbers of 2^-42 of the largest weight: results do not depend on
+ * the order in which blocks run, nor on the other rows.  workspace: jsgrad_hip_sample_rows_workspace_bytes() bytes, 16-byte aligned, whatever it holds; any number of calls of no more rows and
+ * logits may have the same one (they are ordered by the library's stream). */
+size_t jsgrad_hip_sample_rows_workspace_bytes(int rows, int n);
+int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                           const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace);
+
 /* Checkpoint formats on the way into the model.
  * ggml_dequant: ggml_data_to_tensor (nn/state.ts:192-223) for the quantised GGML types Q4_0 (2), Q4_1 (3), Q8_0 (8) and
  *   Q6_K (14): n elements (whole blocks) from the block bytes at `blocks` (2-byte aligned) to float32.

@@ -89,6 +89,8 @@ const SYMBOLS = {
   jsgrad_hip_nf4_dequant: { parameters: [P, P, U, P], result: I }, // packed, scale_f16, n, w16
   jsgrad_hip_sample_workspace_bytes: { parameters: [I], result: U }, // n
   jsgrad_hip_sample: { parameters: [P, I, I, D, I, D, D, D, P, P, P, P, I, I, P], result: I }, // logits, n, act, temp, k, p, af, ap, alpha_counter, rng, state, tokens_out, tokens_cap, advance, workspace
+  jsgrad_hip_sample_rows_workspace_bytes: { parameters: [I, I], result: U }, // rows, n
+  jsgrad_hip_sample_rows: { parameters: [P, I, I, U, I, P, P, P, P, P, P, P, P], result: I }, // logits, rows, n, row_stride, act, temperature, top_k, top_p, min_p, uniforms, tokens_out, probs_out, workspace
   jsgrad_hip_ggml_nbytes: { parameters: [I, U], result: U }, // ggml_type, n
   jsgrad_hip_ggml_dequant: { parameters: [I, P, U, P], result: I }, // ggml_type, blocks, n, out_f32
   jsgrad_hip_cast: { parameters: [P, I, P, I, U], result: I }, // src, src_dtype, dst, dst_dtype, n
