@@ -6,10 +6,7 @@
 // int8, for the row x of one position and head (keys behind the rotation, in float): scale = max |x| / 127, code = rint(x / scale), so that code * scale is
 // within scale / 2 of x.  A row of zeros has scale 1; one with a value that is not finite has scale NaN and reads as NaN.  Scales are float: an
 // fp16 one would be off by 2^-11 and would lose rows below 7.6e-6.
-#include <type_traits>
-
-#include "gemm.h"
-#include "paged.h"
+#include "paged_few.h"
 
 namespace jsg {
 
@@ -27,16 +24,6 @@ struct PagedArgs {
   int n_kv_heads, n_heads;               // n_heads 0: no q
   Divisor pieces;                        // of a row that is read: 8 elements of a head each
 };
-
-// Sequence of row r: the first one that ends behind it.  Called by whole wavefronts with a uniform r: 64 first rows at a time.
-__device__ __forceinline__ int paged_find(const PagedBatch &pb, int r) {
-  const int lane = threadIdx.x & 63;
-  for (int b0 = 0;; b0 += 64) {
-    const int b = b0 + lane;
-    const uint64_t behind = __builtin_amdgcn_ballot_w64(b >= pb.n_seqs || pb.row_starts[b + 1] > r);
-    if (behind) return b0 + __builtin_ctzll(behind);         // n_seqs: no sequence has the row
-  }
-}
 
 template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t v) {   // over 8 or 16 neighbouring lanes
   auto step = [&](auto c) { const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(c)::value, 0xf, 0xf, true); v = v > o ? v : o; };

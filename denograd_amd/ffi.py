@@ -104,6 +104,10 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "jsgrad_hip_paged_read": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp], _i32),
     "jsgrad_hip_attn_paged_workspace_bytes": ([_i32, _i32, _i32], _sz),
     "jsgrad_hip_attn_paged": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp], _i32),
+    "jsgrad_hip_paged_bounds": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp], _i32),
+    "jsgrad_hip_paged_select": ([_pages, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp], _i32),
+    "jsgrad_hip_attn_selected_workspace_bytes": ([_i32, _i32, _i32], _sz),
+    "jsgrad_hip_attn_selected": ([_pages, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp], _i32),
     "jsgrad_hip_step_workspace_bytes": ([_i32, _i32, _i32], _sz),
     "jsgrad_hip_decode_step": ([_vp], _i32),
     "jsgrad_hip_step_status": ([_vp, C.POINTER(_i32)], _i32),

@@ -82,8 +82,8 @@ class Attention:
         return out
 
     def call_paged(self, xn: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", residual: Tensor, out: Tensor, window: int = 0,
-                   sinks: int = 0, norm: RMSNorm | None = None) -> Tensor:
-        """The rows of a ragged batch over a paged cache: xn is the normed input, or what norm is to be applied to; out = residual + wo(attention)."""
+                   sinks: int = 0, norm: RMSNorm | None = None, choose: tuple[int, int, int] | None = None) -> Tensor:
+        """The rows of a ragged batch over a paged cache: xn is the normed input, or what norm is to be applied to; out = residual + wo(attention).  choose: as PagedBatch.choose has first, recent and top."""
         lib, n = ffi.load(), batch.rows
         sp = lambda l: l.scale.ptr if l.scale is not None else None
         weights = (self.wq.kind, self.wq.weight.ptr, sp(self.wq), self.wk.weight.ptr, sp(self.wk), self.wv.weight.ptr, sp(self.wv), xn.ptr)
@@ -94,7 +94,10 @@ class Attention:
         else:
             check(lib.jsgrad_hip_gemm_qkv_rope_norm(*weights, norm.weight.ptr, norm.eps, rows.xn.ptr, *rest))
         batch.write(layer, rows.k, rows.v, rows.q, freqs_cis, self.n_heads, **self.qk_norms)
-        batch.attend(layer, rows.q, self.n_heads, rows.attn, window, sinks)
+        if choose is not None:
+            batch.attend_chosen(layer, rows.q, self.n_heads, *choose, rows.attn)
+        else:
+            batch.attend(layer, rows.q, self.n_heads, rows.attn, window, sinks)
         check(lib.jsgrad_hip_gemm(self.wo.kind, self.wo.weight.ptr, sp(self.wo), self.dim, self.n_heads * self.head_dim, rows.attn.ptr, n, out.ptr, residual.ptr))
         return out
 
@@ -172,13 +175,14 @@ class TransformerBlock:
             h = attend(self._normed(x, self.attention_norm, rows, n), bsz, seqlen, start_pos, state, freqs_cis, rows, residual=x, out=rows.h2)
         return self._feed_rows(h, n, rows, x)
 
-    def call_paged(self, x: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", window: int = 0, sinks: int = 0) -> Tensor:
+    def call_paged(self, x: Tensor, layer: int, batch: "PagedBatch", freqs_cis: Tensor, rows: "_PagedScratch", window: int = 0, sinks: int = 0,
+                   choose: tuple[int, int, int] | None = None) -> Tensor:
         """TransformerBlock.call (llama.ts:124-127) on the rows x of a ragged batch over a paged cache; the result is written back into x."""
-        attend = self.attention.call_paged
+        attend, more = self.attention.call_paged, {} if choose is None else {"choose": choose}
         if getattr(attend, "__func__", None) is ATTENTION_PAGED:
-            h = attend(x, layer, batch, freqs_cis, rows, x, rows.h2, window, sinks, self.attention_norm)
+            h = attend(x, layer, batch, freqs_cis, rows, x, rows.h2, window, sinks, self.attention_norm, **more)
         else:
-            h = attend(self._normed(x, self.attention_norm, rows, batch.rows), layer, batch, freqs_cis, rows, x, rows.h2, window, sinks)
+            h = attend(self._normed(x, self.attention_norm, rows, batch.rows), layer, batch, freqs_cis, rows, x, rows.h2, window, sinks, **more)
         return self._feed_rows(h, batch.rows, rows, x)
 
     def _feed_rows(self, h: Tensor, n: int, rows, x: Tensor) -> Tensor:
@@ -628,16 +632,20 @@ class Transformer:
             check(lib.jsgrad_hip_argmax_rows(rows.logits.ptr, bsz, self.vocab_size, rows.next_tokens.ptr))
         return Tensor(buffer=rows.next_tokens.lazydata.view(bsz, "int32", 0), shape=(bsz,), dtype="int32", device=self.device)
 
-    def forward_paged(self, cache, seqs, tokens, window: int = 0, sinks: int = 0, sampler: "RowSampler | None" = None) -> Tensor:
+    def forward_paged(self, cache, seqs, tokens, window: int = 0, sinks: int = 0, sampler: "RowSampler | None" = None,
+                      choose: tuple[int, int, int] | None = None) -> Tensor:
         """Transformer.forward (llama.ts:201-213) for sequences of different lengths over a PagedCache: tokens[i] are the next token ids of sequence
         seqs[i], a prompt, a part of one, or the one token that the call before returned.  Returns the next token of every sequence, an int32
-        tensor in the order of seqs: the greedy one (Tensor.argmax of each, as forward_rows for several sequences), or what the sampler picks.  window, sinks: as PagedBatch.attend has them.
+        tensor in the order of seqs: the greedy one (Tensor.argmax of each, as forward_rows for several sequences), or what the sampler picks.  window, sinks: as PagedBatch.attend has them; choose:
+        first, recent and top of PagedBatch.choose, for attention over the pages that each row chooses (of a cache with bounds).
         A row of the model's own contiguous cache is neither read nor written.  fp16 activations; fp16 / int8 / NF4 weights.  Where this raises, the
         sequences are as they were."""
         if self.dtype != "float16":
             raise NotImplementedError("a paged cache is built for fp16 activations; float32 models take one position per call")
         if window < 0 or sinks < 0:
             raise ValueError(f"window {window}, sinks {sinks}")
+        if choose is not None and (window or not cache.bounds):
+            raise ValueError("pages are chosen of a cache with bounds=True, and without a window")
         toks = [np.asarray(t, np.int32).reshape(-1) for t in tokens]
         seqs = list(seqs)
         if len(toks) != len(seqs) or any(t.size == 0 for t in toks):
@@ -654,12 +662,13 @@ class Transformer:
             sampler.check(len(seqs))
         batch = cache.begin(seqs, [t.size for t in toks])
         try:
-            return self._run_paged(cache, batch, toks, flat, window, sinks, sampler)
+            return self._run_paged(cache, batch, toks, flat, window, sinks, sampler, choose)
         except BaseException:
             batch._cancel()
             raise
 
-    def _run_paged(self, cache, batch: "PagedBatch", toks, flat: np.ndarray, window: int, sinks: int, sampler: "RowSampler | None") -> Tensor:
+    def _run_paged(self, cache, batch: "PagedBatch", toks, flat: np.ndarray, window: int, sinks: int, sampler: "RowSampler | None",
+                   choose: tuple[int, int, int] | None) -> Tensor:
         lib, hd = ffi.load(), self.dim // self.n_heads
         n, bsz = batch.rows, len(toks)
         if self._paged_rope is None or self._paged_rope.shape[1] < batch.width * cache.page_size:
@@ -676,7 +685,7 @@ class Transformer:
         from .nn import _KIND
         check(lib.jsgrad_hip_embed_rows(_KIND[emb.weight.dtype], emb.weight.ptr, sp(emb), rows.tokens.ptr, n, rows.h.ptr, self.dim, self.vocab_size))
         for i, layer in enumerate(self.layers):
-            layer.call_paged(rows.h, i, batch, self._paged_rope, rows, window, sinks)
+            layer.call_paged(rows.h, i, batch, self._paged_rope, rows, window, sinks, *(() if choose is None else (choose,)))
         last = rows.h
         if n > bsz:
             last = rows.last

@@ -333,10 +333,10 @@ class Llama3:
         return hist.numpy().T.copy()
 
     def generate_paged(self, prompts, n_new: int, dtype: str = "float16", page_size: int = 64, window: int = 0, sinks: int = 0, samples: int = 1, temperature: float = 0.0,
-                       top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, seed: int = 0) -> np.ndarray:
+                       top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, seed: int = 0, choose: tuple[int, int, int] | None = None) -> np.ndarray:
         """Prompts of any lengths at once over a paged cache made for them: fp16 pages, or int8 ones of half the size.  With a window a
         sequence gives away the pages that it no longer sees, and the pool has no more than the prompts and those that are seen need.  Greedy, or drawn by these settings (RowSampler); `samples`
-        answers to each prompt share its pages.  Returns int32 [number of prompts * samples, n_new], the answers to a prompt side by side."""
+        answers to each prompt share its pages.  choose: attention over the pages that each row chooses, (first, recent, top) of PagedBatch.choose.  Returns int32 [number of prompts * samples, n_new], the answers to a prompt side by side."""
         from .paged import PagedCache
         from .sampling import RowSampler
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
@@ -352,18 +352,18 @@ class Llama3:
         n_pages = PagedCache.pages_for(sizes, n_new, page_size, window, sinks)
         if samples > 1 and not window:                        # whole pages of a prompt are there once
             n_pages -= sum((p.size - 1) // page_size for p in prompts) * (samples - 1)
-        cache = PagedCache(len(m.layers), m.n_kv_heads, m.dim // m.n_heads, n_pages, page_size, dtype, self.device)
+        cache = PagedCache(len(m.layers), m.n_kv_heads, m.dim // m.n_heads, n_pages, page_size, dtype, self.device, choose is not None)
         seqs = [cache.add() for _ in prompts]
         out, toks = np.empty((len(prompts) * samples, n_new), np.int32), prompts
         if samples > 1:
             # all but the last token once, the last one for each answer
             long = [(s, p) for s, p in zip(seqs, prompts) if p.size > 1]
             if long:
-                m.forward_paged(cache, [s for s, _ in long], [p[:-1] for _, p in long], window, sinks)
+                m.forward_paged(cache, [s for s, _ in long], [p[:-1] for _, p in long], window, sinks, choose=choose)
             seqs = [t for s in seqs for t in [s] + [cache.fork(s) for _ in range(samples - 1)]]
             toks = [p[-1:] for p in prompts for _ in range(samples)]
         for i in range(n_new):
-            toks = m.forward_paged(cache, seqs, toks, window, sinks, sampler).numpy()
+            toks = m.forward_paged(cache, seqs, toks, window, sinks, sampler, choose).numpy()
             out[:, i] = toks
             if window:
                 for s in seqs:

@@ -157,9 +157,10 @@ class PageTable:
 
 
 class PagedCache(PageTable):
-    """Pools of n_layers layers under one page table.  dtype: "float16", or "int8" with a float scale per position and head."""
+    """Pools of n_layers layers under one page table.  dtype: "float16", or "int8" with a float scale per position and head.  bounds: what PagedBatch.attend_chosen goes by is kept with
+    every write."""
 
-    def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, n_pages: int, page_size: int = 64, dtype: str = "float16", device: str = "HIP"):
+    def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, n_pages: int, page_size: int = 64, dtype: str = "float16", device: str = "HIP", bounds: bool = False):
         super().__init__(n_pages, page_size)
         if dtype not in ("float16", "int8"):
             raise ValueError(f"pages are float16 or int8, not {dtype}")
@@ -169,6 +170,9 @@ class PagedCache(PageTable):
         rows = (2, n_pages, n_kv_heads, page_size)
         self.pools = [Tensor.zeros((*rows, head_dim), dtype, device) for _ in range(n_layers)]       # k, then v
         self.scales = [Tensor.ones(rows, "float32", device) if dtype == "int8" else None for _ in range(n_layers)]
+        # per layer: the least and largest of each feature of a page's keys, as whole numbers, and their unit
+        self.bounds = [(Tensor.zeros((n_pages, n_kv_heads, 2, head_dim), "int8", device), Tensor.ones((n_pages, n_kv_heads), "float32", device)) for _ in range(n_layers)] if bounds else []
+        self._chosen: Tensor | None = None
         self._moves: Tensor | None = None                     # what is copied next
         self._plan: Tensor | None = None                      # row_starts, lengths and page table of the batch last begun
         self._batches = 0
@@ -199,6 +203,8 @@ class PagedCache(PageTable):
                 pools.append(ffi.Pool(pool.ptr + i * (pool.nbytes // 2), self.n_kv_heads, self.page_size, row))
                 if scales is not None:
                     pools.append(ffi.Pool(scales.ptr + i * (scales.nbytes // 2), self.n_kv_heads, self.page_size, 4))
+        for codes, scales in self.bounds:
+            pools += [ffi.Pool(codes.ptr, 1, 1, codes.nbytes // self.n_pages), ffi.Pool(scales.ptr, 1, 1, scales.nbytes // self.n_pages)]
         return pools
 
     def _copy(self, moves) -> None:
@@ -238,10 +244,12 @@ class PagedCache(PageTable):
         self._plan.lazydata.view(plan.size, "int32", 0).ensure_allocated().copyin(plan)
         return PagedBatch(self, n, int(plan[n]), width, held)
 
-    def workspace(self, n_heads: int) -> Tensor:
-        if n_heads not in self._ws:
-            self._ws[n_heads] = Tensor.zeros((ffi.load().jsgrad_hip_attn_paged_workspace_bytes(n_heads, self.n_kv_heads, self.head_dim),), "uint8", self.device)
-        return self._ws[n_heads]
+    def workspace(self, n_heads: int, chosen: bool = False) -> Tensor:
+        key = -n_heads if chosen else n_heads
+        if key not in self._ws:
+            call = ffi.load().jsgrad_hip_attn_selected_workspace_bytes if chosen else ffi.load().jsgrad_hip_attn_paged_workspace_bytes
+            self._ws[key] = Tensor.zeros((call(n_heads, self.n_kv_heads, self.head_dim),), "uint8", self.device)
+        return self._ws[key]
 
 
 class PagedBatch:
@@ -300,6 +308,9 @@ class PagedBatch:
             norms = [q_norm.weight.ptr if q_norm is not None else None, k_norm.weight.ptr, k_norm.eps]
         call = ffi.load().jsgrad_hip_paged_write_norm if norms else ffi.load().jsgrad_hip_paged_write
         check(call(*self._args(layer), p(q), k.ptr, v.ptr, *norms, p(freqs_cis), positions, p(q_out) if q is not None else None, n_heads))
+        if self.cache.bounds:
+            codes, scales = self.cache.bounds[layer]
+            check(ffi.load().jsgrad_hip_paged_bounds(*self._args(layer), codes.ptr, scales.ptr))
         return q_out if q is not None else None
 
     def read(self, layer: int) -> tuple[Tensor, Tensor]:
@@ -317,3 +328,32 @@ class PagedBatch:
         self._check("out", out, n_heads)
         check(ffi.load().jsgrad_hip_attn_paged(*self._args(layer), q.ptr, out.ptr, n_heads, window, sinks, self.cache.workspace(n_heads).ptr))
         return out
+
+    def choose(self, layer: int, q: Tensor, n_heads: int, first: int, recent: int, top: int) -> Tensor:
+        """The pages of each row of q [rows, n_heads, head_dim] per kv head, by the bounds of their keys: int32 [rows, n_kv_heads, top], rising, -1 behind the last.  The first `first` and the last `recent` ones,
+        the row's own among them, and of the others those on which its queries may score most."""
+        self._check("q", q, n_heads)
+        c = self.cache
+        if not c.bounds:
+            raise ValueError("pages are chosen by their bounds: a cache with bounds=True is wanted")
+        n = self.rows * c.n_kv_heads * max(top, 1)
+        if c._chosen is None or c._chosen.numel < n:
+            c._chosen = Tensor.empty((n,), "int32", c.device)
+        codes, scales = c.bounds[layer]
+        check(ffi.load().jsgrad_hip_paged_select(*self._args(layer), q.ptr, n_heads, codes.ptr, scales.ptr, first, recent, top, c._chosen.ptr))
+        return Tensor(buffer=c._chosen.lazydata.view(n, "int32", 0), shape=(self.rows, c.n_kv_heads, top), dtype="int32", device=c.device)
+
+    def attend_pages(self, layer: int, q: Tensor, n_heads: int, chosen: Tensor, out: Tensor | None = None) -> Tensor:
+        """Attention of q [rows, n_heads, head_dim] over the positions up to a row's own on the pages in chosen [rows, n_kv_heads, any number]."""
+        self._check("q", q, n_heads)
+        c = self.cache
+        if chosen.dtype != "int32" or len(chosen.shape) != 3 or chosen.shape[0] < self.rows or chosen.shape[1] != c.n_kv_heads:
+            raise ValueError(f"chosen: int32 [{self.rows}, {c.n_kv_heads}, pages] are wanted, got {chosen.dtype} {chosen.shape}")
+        out = out if out is not None else Tensor.empty((self.rows, n_heads, c.head_dim), "float16", c.device)
+        self._check("out", out, n_heads)
+        check(ffi.load().jsgrad_hip_attn_selected(*self._args(layer), q.ptr, out.ptr, n_heads, chosen.ptr, chosen.shape[2], c.workspace(n_heads, True).ptr))
+        return out
+
+    def attend_chosen(self, layer: int, q: Tensor, n_heads: int, first: int, recent: int, top: int, out: Tensor | None = None) -> Tensor:
+        """Attention over the pages that `choose` names."""
+        return self.attend_pages(layer, q, n_heads, self.choose(layer, q, n_heads, first, recent, top), out)

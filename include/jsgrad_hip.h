@@ -321,6 +321,25 @@ size_t jsgrad_hip_attn_paged_workspace_bytes(int n_heads, int n_kv_heads, int he
 int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out,
                           int n_heads, int window, int sinks, void *workspace);
 
+/* Attention over the pages that each row chooses, for contexts too long to look at whole (no counterpart in the reference): a step calls _paged_write, _paged_bounds, _paged_select and _attn_selected.
+ *
+ * _paged_bounds: the bounds of every page that the batch's rows are on, of all the positions that its sequence has there: bounds int8 [n_pages][n_kv_heads][2][head_dim], 16-byte aligned, and bound_scales float
+ * [n_pages][n_kv_heads], a pool that belongs to the layer's K pool.  scale = the smallest power of two, 2^-126 and more, that 127 times is max |k| and more (1 for zeros), bounds[0] = floor(min k / scale), bounds[1] =
+ * ceil(max k / scale), k of int8 pages being the float product code * scale.  A page with a key that is not finite: scale infinity, bounds 0. */
+int jsgrad_hip_paged_bounds(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, int8_t *bounds, float *bound_scales);
+/* _paged_select: selected int32 [rows][n_kv_heads][top], the pages (columns of the page table) of the row at position p, rising, -1 behind the last: those among the first `first` and the last `recent` of the columns
+ * [0, p / page_size] that have a page, and of the others with one the best, up to `top` in all.  A page's score: with the row's query heads of the kv head as whole numbers c = rint(q / 2^e), 2^e as the scale above
+ * of their largest |q|, scale * max over these heads of sum_d c_d * bounds[c_d > 0][d], which no key of the page exceeds; infinity where the scale is.  It is exact, equal ones go to the lower page.  Queries that are not all finite
+ * count as zeros.  Rows behind row_starts[n_seqs] are left as they are; rows at positions below 0 choose none.  top: 1 to 1024, first 0 and more, recent 1 and more, both together no more than top; at most 64 query
+ * heads to a kv head, and 32768 columns. */
+int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, int n_heads,
+                            const int8_t *bounds, const float *bound_scales, int first, int recent, int top, int32_t *selected);
+/* _attn_selected: jsgrad_hip_attn_paged where the row at position p sees the positions j <= p of the pages in its selected [n_kv_heads][top], whoever made them, in any order; an entry that is no column of the
+ * table, or one without a page, is none, one that comes twice counts twice.  workspace: jsgrad_hip_attn_selected_workspace_bytes() bytes, otherwise as that call's. */
+size_t jsgrad_hip_attn_selected_workspace_bytes(int n_heads, int n_kv_heads, int head_dim);
+int jsgrad_hip_attn_selected(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out, int n_heads,
+                             const int32_t *selected, int top, void *workspace);
+
 /* ---------------------------------------------------------------------------------
  * The whole decode step as ONE kernel.
  *

@@ -72,6 +72,10 @@ const SYMBOLS = {
   jsgrad_hip_paged_read: { parameters: [B, P, P, I, I, P, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, k_out, v_out
   jsgrad_hip_attn_paged_workspace_bytes: { parameters: [I, I, I], result: U }, // n_heads, n_kv_heads, head_dim
   jsgrad_hip_attn_paged: { parameters: [B, P, P, I, I, P, P, I, I, I, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, out, n_heads, window, sinks, workspace
+  jsgrad_hip_paged_bounds: { parameters: [B, P, P, I, I, P, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, bounds, bound_scales
+  jsgrad_hip_paged_select: { parameters: [B, P, P, I, I, P, I, P, P, I, I, I, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, n_heads, bounds, bound_scales, first, recent, top, selected
+  jsgrad_hip_attn_selected_workspace_bytes: { parameters: [I, I, I], result: U }, // n_heads, n_kv_heads, head_dim
+  jsgrad_hip_attn_selected: { parameters: [B, P, P, I, I, P, P, I, P, I, P], result: I }, // host_pages, row_starts, lengths, n_seqs, rows, q, out, n_heads, selected, top, workspace
   jsgrad_hip_step_workspace_bytes: { parameters: [I, I, I], result: U }, // n_heads, n_kv_heads, head_dim
   jsgrad_hip_decode_step: { parameters: [B], result: I }, // host_desc
   jsgrad_hip_step_status: { parameters: [P, B], result: I }, // workspace, host_out_error
