@@ -8,6 +8,7 @@
 
 namespace jsg {
 
+typedef int i4v __attribute__((ext_vector_type(4)));
 constexpr int PS_THREADS = 256, PS_MOST = 1024, PS_WIDTH = 32768;      // pages that a row chooses, columns of the table
 
 struct PagedSelectArgs {
@@ -18,6 +19,7 @@ struct PagedSelectArgs {
   int8_t *bounds;                        // [n_pages][KV][lo, hi][HD]
   float *bound_scales;                   // [n_pages][KV]
   int n_kv_heads, n_rep, first, recent, top;
+  int tile, heads_log, stride;           // rows of a block, columns of queries to a row as a power of two, keys of a row
   int32_t *selected;                     // [rows][KV][top]
 };
 
@@ -106,107 +108,281 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
-// Block = (row, kv head).
-template <int HD> __global__ __launch_bounds__(PS_THREADS) void paged_select_kernel(PagedSelectArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int r = blockIdx.x, g = blockIdx.y, KV = a.n_kv_heads, n_rep = a.n_rep, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = paged_find(a.pb, r);
-  if (b >= a.pb.n_seqs) return;
-  const PagedSeq s = paged_seq(a.pb, b);
-  const int pos = paged_pos(s, r - s.start);
-  if (r < s.start) return;
-  int32_t *const out = a.selected + ((size_t)r * KV + g) * a.top;
-  const int last = pos < 0 ? -1 : pos >> a.pb.page_shift, n = min(last + 1, a.pb.width);
-  // the group's queries as whole numbers: positive parts, then negative ones
-  int8_t *const qc = (int8_t *)smem;                         // [n_rep][2][HD]
-  uint32_t *const keys = (uint32_t *)(smem + (size_t)n_rep * 2 * HD);
-  __shared__ float red[PS_THREADS / 64];
-  __shared__ int count[2][PS_THREADS / 64];
-  const _Float16 *const q = a.q + ((size_t)r * KV + g) * n_rep * HD;
-  float most = 0.0f;
-  for (int i = tid; i < n_rep * HD; i += PS_THREADS) {
-    const float f = fabsf((float)q[i]);
-    most = f < INFINITY ? fmaxf(most, f) : INFINITY;
-    if (!(f < INFINITY)) break;
+constexpr uint32_t KEY_ALWAYS = 0xffffffffu;               // of a page that is among the first or the recent ones; 0: of one that is not there
+
+// over the lanes, for all of them: a value from the lanes below, row by row, then from row to row; the last lane has everything
+template <typename Op> __device__ __forceinline__ uint32_t wave_all(uint32_t v, Op op) {
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, false));     // quad_perm [1,0,3,2], [2,3,0,1], then the halves of a row and the row mirrored
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xf, 0xf, false));
+  auto row = [&](int r) { return (uint32_t)__builtin_amdgcn_readlane((int)v, r * 16); };
+  return op(op(row(0), row(1)), op(row(2), row(3)));
+}
+// sums of a lane's value and those of the lanes below
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// The first `top` of n keys in the order (key descending, index ascending), those above 0, written as rising indexes with -1 behind.  By one wavefront, or (NW > 1) by a block of NW, each with a stretch of
+// the keys.  What lies between the least and the largest is counted in 256 parts, then the part with the border in 256 again, until a part is wanted whole or its keys are all alike: two or
+// three turns, four at most.  (Halving a threshold takes some 15: 33000 positions in pages of 64, 4.3 us of them.)
+template <int NW> struct KeyChoice {
+  static constexpr int TURNS = NW == 1 ? 1 : 4;              // counts that stay zero until their turn; one wavefront clears its own
+  __align__(16) uint32_t hist[TURNS][256];
+  uint32_t least[NW], most[NW], real[NW], always[NW], above[NW], tied[NW];
+
+  __device__ __forceinline__ void operator()(const uint32_t *keys, int n, int top, int32_t *out, int wave) {
+    const int per = NW == 1 ? n : ((n + NW - 1) / NW + 63) & ~63, lo = min(wave * per, n), hi = min(lo + per, n);
+    if (per <= 4 * 64) choose<4>(keys, lo, hi, n, top, out, wave);
+    else if (per <= 16 * 64) choose<16>(keys, lo, hi, n, top, out, wave);
+    else choose<0>(keys, lo, hi, n, top, out, wave);
   }
-  most = wave_max(most);
-  if (lane == 0) red[wave] = most;
-  __syncthreads();
-  for (int w = 0; w < PS_THREADS / 64; w++) most = fmaxf(most, red[w]);
-  const float step = most < INFINITY ? bound_step(most) : 0.0f;   // queries that are not finite say nothing
-  for (int i = tid; i < n_rep * HD; i += PS_THREADS) {
-    const int c = step > 0.0f ? (int)rintf(__fdiv_rn((float)q[i], step)) : 0, h = i / HD, d = i % HD;
-    qc[(h * 2) * HD + d] = (int8_t)max(c, 0);
-    qc[(h * 2 + 1) * HD + d] = (int8_t)min(c, 0);
-  }
-  __syncthreads();
-  for (int i = tid; i < n; i += PS_THREADS) {
-    const int id = paged_page(a.pb, b, i << a.pb.page_shift);
-    uint32_t key = 0;                                        // no page
-    if (id >= 0) {
-      if (i < a.first || i > last - a.recent) {
-        key = 0xffffffffu;
+  // K: keys of a lane; 0: any number, from where they are
+  template <int K> __device__ void choose(const uint32_t *keys, int lo, int hi, int n, int top, int32_t *out, int wave) {
+    const int lane = threadIdx.x & 63;
+    uint32_t mine[K ? K : 1];
+#pragma unroll
+    for (int u = 0; u < K; u++) mine[u] = lo + u * 64 + lane < hi ? keys[lo + u * 64 + lane] : 0;
+    auto each = [&](auto f) {                                // f(key, its index less the lane), 64 side by side; 0 past the end
+      if constexpr (K > 0) {
+#pragma unroll
+        for (int u = 0; u < K; u++) f(mine[u], lo + u * 64);
       } else {
-        const int *const lo = (const int *)(a.bounds + ((size_t)id * KV + g) * 2 * HD), *const hi = lo + HD / 4;
-        int best = -0x7fffffff;
-        for (int h = 0; h < n_rep; h++) {
-          const int *const up = (const int *)(qc + h * 2 * HD), *const down = up + HD / 4;
-          int sum = 0;
-          for (int d = 0; d < HD / 4; d++) sum = __builtin_amdgcn_sdot4(hi[d], up[d], __builtin_amdgcn_sdot4(lo[d], down[d], sum, false), false);
-          best = max(best, sum);
-        }
-        const float scale = a.bound_scales[(size_t)id * KV + g];
-        key = min(score_key(scale < INFINITY ? (float)best * scale : INFINITY), 0xfffffffeu);
+        for (int i = lo; i < hi; i += 64) f(i + lane < hi ? keys[i + lane] : 0u, i);
+      }
+    };
+    auto join = [&](uint32_t (&of)[NW], uint32_t v, auto op) {   // over the block, behind a barrier
+      if constexpr (NW == 1) return v;
+      uint32_t all = of[0];
+#pragma unroll
+      for (int w = 1; w < NW; w++) all = op(all, of[w]);
+      return all;
+    };
+    auto sum = [](uint32_t x, uint32_t y) { return x + y; };
+    auto lower = [](uint32_t x, uint32_t y) { return min(x, y); };
+    auto upper = [](uint32_t x, uint32_t y) { return max(x, y); };
+    uint32_t a = ~0u, b = 0, n_real = 0, n_always = 0;       // of the keys between 0 and KEY_ALWAYS
+    each([&](uint32_t k, int) {
+      const bool some = k - 1 < KEY_ALWAYS - 1;
+      a = min(a, some ? k : ~0u);
+      b = max(b, some ? k : 0u);
+      n_real += some;
+      n_always += k == KEY_ALWAYS;
+    });
+    a = wave_all(a, lower);
+    b = wave_all(b, upper);
+    n_real = wave_all(n_real, sum);
+    n_always = wave_all(n_always, sum);
+    if constexpr (NW > 1) {
+      if (lane == 0) { least[wave] = a; most[wave] = b; real[wave] = n_real; always[wave] = n_always; }
+      for (int i = threadIdx.x; i < TURNS * 256; i += NW * 64) hist[0][i] = 0;
+      lds_barrier();
+      a = join(least, a, lower);
+      b = join(most, b, upper);
+      n_real = join(real, n_real, sum);
+      n_always = join(always, n_always, sum);
+    }
+    uint32_t t = 1;                                          // what is chosen reaches it; of the keys that are t, the first `ties`
+    int ties = n;
+    uint32_t need = (uint32_t)top - min(n_always, (uint32_t)top);
+    if (need == 0) t = KEY_ALWAYS;
+    else if (n_real > need)
+      for (int turn = 0;; turn++) {
+        const uint32_t span = b - a;
+        const int shift = span < 256 ? 0 : 24 - __builtin_clz(span);
+        uint32_t *const h = hist[NW == 1 ? 0 : turn];
+        if constexpr (NW == 1) *(uint4 *)&h[lane * 4] = make_uint4(0, 0, 0, 0);
+        each([&](uint32_t k, int) {
+          if (k - a <= span) atomicAdd(&h[(k - a) >> shift], 1u);
+        });
+        if constexpr (NW > 1) lds_barrier();
+        const uint4 c = *(const uint4 *)&h[252 - 4 * lane];  // from the largest down
+        const uint32_t four = c.x + c.y + c.z + c.w, upto = wave_upto(four);
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto >= need));
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+        uint32_t before = of(upto - four), bin = 255 - 4 * l, held = of(c.w);
+        if (before + held < need) { before += held; held = of(c.z); bin--; }
+        if (before + held < need) { before += held; held = of(c.y); bin--; }
+        if (before + held < need) { before += held; held = of(c.x); bin--; }
+        need -= before;
+        a += bin << shift;
+        t = a;
+        if (held == need) break;
+        if (shift == 0) { ties = (int)need; break; }
+        b = min(b, a + ((1u << shift) - 1));
+      }
+    int at = 0, left = ties;
+    if constexpr (NW > 1) {
+      uint32_t over = 0, equal = 0;
+      each([&](uint32_t k, int) { over += k > t; equal += k == t; });
+      over = wave_all(over, sum);
+      equal = wave_all(equal, sum);
+      if (lane == 0) { above[wave] = over; tied[wave] = equal; }
+      lds_barrier();
+      for (int w = 0; w < wave; w++) {
+        const int held = min(left, (int)tied[w]);
+        at += (int)above[w] + held;
+        left -= held;
       }
     }
-    keys[i] = key;
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    each([&](uint32_t k, int i) {
+      const uint64_t tie = __builtin_amdgcn_ballot_w64(k == t);
+      const bool take = k > t || (k == t && (int)__builtin_popcountll(tie & below) < left);
+      left -= min(left, (int)__builtin_popcountll(tie));
+      const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
+      const int place = at + (int)__builtin_popcountll(taken & below);
+      if (take && place < top) out[place] = i + lane;
+      at += (int)__builtin_popcountll(taken);
+    });
+    if (NW == 1 || wave == NW - 1)
+      for (int i = at + lane; i < top; i += 64) out[i] = -1;
   }
-  __syncthreads();
-  auto block_count = [&](int mine, int turn) {               // over the block; `turn` alternates
-    const int c = (int)wave_sum((float)mine);
-    if (lane == 0) count[turn][wave] = c;
-    __syncthreads();
-    return count[turn][0] + count[turn][1] + count[turn][2] + count[turn][3];
-  };
-  // the largest threshold that `top` keys reach; 1 where there are fewer
-  uint32_t t = 0;
-  for (int bit = 31; bit >= 0; bit--) {
-    const uint32_t up = t | 1u << bit;
-    int mine = 0;
-    for (int i = tid; i < n; i += PS_THREADS) mine += keys[i] >= up;
-    if (block_count(mine, bit & 1) >= a.top) t = up;
-  }
-  int more = 0;
-  for (int i = tid; i < n; i += PS_THREADS) more += keys[i] > t;
-  more = block_count(more, 1);
-  int ties = t ? a.top - more : 0, at = 0;                   // of the keys at the threshold, the first so many
-  __syncthreads();
-  // in the order of the pages, 256 at a time
-  for (int i0 = 0; i0 < n; i0 += PS_THREADS) {
-    const int i = i0 + tid;
-    const uint32_t key = i < n ? keys[i] : 0;
-    const bool tie = key == t && key;
-    const uint64_t tied = __builtin_amdgcn_ballot_w64(tie), above = (uint64_t)1 << lane;
-    if (lane == 0) count[0][wave] = __popcll(tied);
-    __syncthreads();
-    int before = __popcll(tied & (above - 1)), all = 0;
-    for (int w = 0; w < PS_THREADS / 64; w++) {
-      if (w < wave) before += count[0][w];
-      all += count[0][w];
+};
+
+// Block = some rows of a sequence, side by side, and a kv head.  Scores on the matrix cores: 16 pages' bounds against 16 columns of queries, the heads of a row next to each other, so that a lane has
+// four columns' scores of its page.  Bound by what waits for what: batch, page numbers, bounds, then the turns of the choice.  (us, 33000 positions, pages of 64, 32 heads of 128 over 8, a page to
+// a thread with dot products and 32 turns through LDS 22; 16 rows of up to 32768, pages of 32, 30; 2048 rows behind 14336, heads of 64, 138.)
+// HT tiles of 16 columns: of more heads of the rows (HEADS), or of more rows, for which the bounds are loaded once.
+template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, NW == 4 ? 4 : 2) void paged_select_kernel(PagedSelectArgs a) {
+  extern __shared__ __align__(16) uint32_t keys[];           // [rows of a block][stride]
+  __shared__ union {
+    KeyChoice<NW> block;
+    KeyChoice<1> wave[NW];
+  } choice;
+  constexpr int KS = 2 * HD / 64;                            // steps of 64 bytes: the lower bounds, then the upper ones
+  const int g = blockIdx.y, KV = a.n_kv_heads, n_rep = a.n_rep, lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hp = 1 << a.heads_log, shift = a.pb.page_shift;
+  const int r_end = min((int)(blockIdx.x + 1) * a.tile, a.pb.rows);
+  for (int r0 = blockIdx.x * a.tile; r0 < r_end;) {
+    const int b = paged_find(a.pb, r0);
+    if (b >= a.pb.n_seqs) return;
+    const PagedSeq s = paged_seq(a.pb, b);
+    const int n_rows = min(s.start + s.n, r_end) - r0;
+    if (r0 < s.start) { r0++; continue; }                    // no sequence has it
+    const int p0 = paged_pos(s, r0 - s.start), last_page = p0 + n_rows - 1 < 0 ? -1 : (p0 + n_rows - 1) >> shift, n = min(last_page + 1, a.pb.width);
+    // U tiles at a time: their page numbers in one trip to memory, asked for ahead, their bounds in the next.  The numbers without a branch: behind one, each would be waited for.
+    constexpr int U = HT > 1 ? 2 : NW == 8 ? 8 : 4;
+    const int32_t *const table = a.pb.table + (size_t)b * a.pb.width;
+    int id[U];
+    auto pages_of = [&](int t0) {
+#pragma unroll
+      for (int u = 0; u < U; u++) id[u] = *as_global<int>(table + max(min((t0 + u * NW) * 16 + l16, n - 1), 0));
+    };
+    pages_of(wave);
+    // column l16 of a tile: a head of a row; those past the last repeat it
+    u4_t q[HT][HD / 64][2];
+    float most[HT];
+#pragma unroll
+    for (int h = 0; h < HT; h++) {
+      const int row = min((HEADS ? 0 : h * (16 >> a.heads_log)) + (l16 >> a.heads_log), n_rows - 1), head = min((HEADS ? h * 16 : 0) + (l16 & (hp - 1)), n_rep - 1);
+      const _Float16 *const qp = a.q + (((size_t)(r0 + row) * KV + g) * n_rep + head) * HD + lq * 16;
+      uint32_t bits = 0;                                     // of the largest |q|, in both halves
+#pragma unroll
+      for (int c = 0; c < HD / 64; c++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          q[h][c][u] = *as_global<u4_t>(qp + c * 64 + u * 8);
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            typedef uint16_t us2_t __attribute__((ext_vector_type(2)));
+            const us2_t v = __builtin_bit_cast(us2_t, q[h][c][u][w] & 0x7fff7fffu), m = __builtin_bit_cast(us2_t, bits);
+            bits = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(v, m));
+          }
+        }
+      bits = max(bits & 0xffff, bits >> 16);                 // halves without their sign are in the order of their bits
+      most[h] = bits < 0x7c00 ? h2f(__builtin_bit_cast(_Float16, (uint16_t)bits)) : INFINITY;
+      most[h] = max_xor32(max_xor16(most[h]));
+      for (int off = 1; off < hp; off <<= 1) most[h] = fmaxf(most[h], __shfl_xor(most[h], off));
     }
-    const bool take = key > t || (tie && before < ties);
-    ties -= min(ties, all);
-    const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
-    if (lane == 0) count[1][wave] = __popcll(taken);
-    __syncthreads();
-    int place = at + __popcll(taken & (above - 1));
-    for (int w = 0; w < PS_THREADS / 64; w++) {
-      if (w < wave) place += count[1][w];
-      at += count[1][w];
+    if (HEADS)
+#pragma unroll
+      for (int h = 0; h < HT; h++) most[0] = fmaxf(most[0], most[h]);
+    i4v qf[HT][KS];                                          // negative parts against lower bounds, positive ones against upper
+#pragma unroll
+    for (int h = 0; h < HT; h++) {
+      const bool says = most[HEADS ? 0 : h] < INFINITY;      // queries that are not finite say nothing
+      const float per_step = says ? 1.0f / bound_step(most[HEADS ? 0 : h]) : 0.0f;   // of a power of two: exact
+#pragma unroll
+      for (int c = 0; c < HD / 64; c++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          uint32_t v[4];                                     // the addition rounds to a whole number, whose last byte is the code
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const h2_t p = as_h2(q[h][c][w / 2][w % 2 * 2 + e / 2]);
+            v[e] = __float_as_uint(__builtin_fmaf((float)p[e % 2], per_step, 12582912.0f));
+          }
+          const uint32_t code = says ? __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u), __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), 0x05040100u) : 0;
+          const uint32_t sign = (code >> 7) & 0x01010101u, minus = (sign << 8) - sign;
+          qf[h][c][w] = (int)(code & minus);
+          qf[h][HD / 64 + c][w] = (int)(code & ~minus);
+        }
     }
-    if (take && place < a.top) out[place] = i;
+    for (int t0 = wave; t0 * 16 < n; t0 += U * NW) {
+      i4v bf[U][KS];
+      float scale[U];
+      bool held[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if ((t0 + u * NW) * 16 + l16 >= n || id[u] >= a.pb.n_pages) id[u] = -1;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const size_t at = (size_t)max(id[u], 0) * KV + g;
+        const int8_t *const box = a.bounds + at * 2 * HD + lq * 16;
+#pragma unroll
+        for (int k = 0; k < KS; k++) bf[u][k] = *as_global<i4v>(box + k * 64);
+        scale[u] = *as_global<float>(a.bound_scales + at);
+        held[u] = id[u] >= 0;
+      }
+      pages_of(t0 + U * NW);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int i = (t0 + u * NW) * 16 + l16;
+        if (i - l16 >= n) break;
+        float v[4];
+#pragma unroll
+        for (int h = 0; h < HT; h++) {
+          i4v acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[h][k], bf[u][k], acc, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = HEADS && h ? fmaxf(v[e], (float)acc[e]) : (float)acc[e];   // column 4 lq + e, page l16
+        if (HEADS && h < HT - 1) continue;
+        // over a row's columns
+        if (a.heads_log >= 1) { v[0] = fmaxf(v[0], v[1]); v[2] = fmaxf(v[2], v[3]); }
+        if (a.heads_log >= 2) v[0] = fmaxf(v[0], v[2]);
+        if (a.heads_log >= 3) v[0] = max_xor16(v[0]);
+        if (a.heads_log >= 4) v[0] = max_xor32(v[0]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int at = (HEADS ? 0 : h * (16 >> a.heads_log)) + ((4 * lq + e) >> a.heads_log);
+          if ((e & (hp - 1)) != 0 || at >= n_rows || i >= n) continue;
+          const int last = p0 + at < 0 ? -1 : (p0 + at) >> shift;
+          uint32_t key = min(score_key(scale[u] < INFINITY ? v[e] * scale[u] : INFINITY), KEY_ALWAYS - 1);
+          if (i < a.first || i > last - a.recent) key = KEY_ALWAYS;
+          if (!held[u] || i > last) key = 0;
+          keys[at * a.stride + i] = key;
+        }
+        }
+      }
+    }
+    __syncthreads();
+    auto place = [&](int at) { return a.selected + ((size_t)(r0 + at) * KV + g) * a.top; };
+    auto pages = [&](int at) { return p0 + at < 0 ? 0 : min(((p0 + at) >> shift) + 1, a.pb.width); };
+    if (a.tile == 1) choice.block(keys, n, a.top, place(0), wave);
+    else
+      for (int at = wave; at < n_rows; at += NW) choice.wave[wave](keys + at * a.stride, pages(at), a.top, place(at), 0);
+    r0 += n_rows;
+    if (r0 < r_end) __syncthreads();
   }
-  for (int i = at + tid; i < a.top; i += PS_THREADS) out[i] = -1;
 }
 
 // ---------------------------------------------------------------- attention over the chosen pages
@@ -331,15 +507,33 @@ int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t 
   a.n_kv_heads = host_pages->n_kv_heads; a.n_rep = n_rep;
   a.first = first; a.recent = recent; a.top = top;
   a.selected = selected;
-  const dim3 grid((unsigned)rows, (unsigned)a.n_kv_heads), block(PS_THREADS);
-  const size_t lds = (size_t)n_rep * 2 * HD + (size_t)host_pages->table_width * 4;
-  if (HD == 64) {
-    if (lds > 64 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<64>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    JSG_LAUNCH(PROF_ATTN_PAGED, paged_select_kernel<64>, grid, block, lds, a);
-  } else {
-    if (lds > 64 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<128>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    JSG_LAUNCH(PROF_ATTN_PAGED, paged_select_kernel<128>, grid, block, lds, a);
-  }
+  while ((1 << a.heads_log) < (n_rep < 16 ? n_rep : 16)) a.heads_log++;
+  a.stride = (host_pages->table_width + 15) & ~15;
+  // Rows of a sequence share its bounds; where rows are one to a sequence, a block of eight wavefronts is done sooner with one.
+  const bool many = n_rep > 16;
+  int tile = 16 >> a.heads_log, tiles = 1;
+  if (!many && rows >= 8 * tile * n_seqs && (size_t)rows * a.n_kv_heads >= (size_t)tile * 4096 && (size_t)tile * 4 * a.stride * 4 <= 64 * 1024) tiles = 4;
+  a.tile = rows > n_seqs && (size_t)tile * tiles * a.stride * 4 <= 64 * 1024 ? tile * tiles : 1;
+  const bool wide = a.tile == 1 && (size_t)rows * a.n_kv_heads <= 1024;
+  const dim3 grid((unsigned)((rows + a.tile - 1) / a.tile), (unsigned)a.n_kv_heads);
+  const size_t lds = (size_t)a.tile * a.stride * 4;
+#define JSG_SELECT(HD, NW, HT, HEADS)                                                                                                                                        \
+  do {                                                                                                                                                                        \
+    if (lds > 48 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<HD, NW, HT, HEADS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));              \
+    JSG_LAUNCH(PROF_ATTN_PAGED, (paged_select_kernel<HD, NW, HT, HEADS>), grid, dim3(NW * 64), lds, a);                                                                          \
+  } while (0)
+#define JSG_SELECT_HD(HD)                                \
+  do {                                                   \
+    if (many && wide) JSG_SELECT(HD, 8, 4, true);          \
+    else if (many) JSG_SELECT(HD, 4, 4, true);             \
+    else if (wide) JSG_SELECT(HD, 8, 1, false);            \
+    else if (tiles > 1) JSG_SELECT(HD, 4, 4, false);       \
+    else JSG_SELECT(HD, 4, 1, false);                      \
+  } while (0)
+  if (HD == 64) JSG_SELECT_HD(64);
+  else JSG_SELECT_HD(128);
+#undef JSG_SELECT_HD
+#undef JSG_SELECT
   return 0;
 }
 
