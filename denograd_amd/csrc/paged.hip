@@ -6,7 +6,9 @@
 // int8, for the row x of one position and head (keys behind the rotation, in float): scale = max |x| / 127, code = rint(x / scale), so that code * scale is
 // within scale / 2 of x.  A row of zeros has scale 1; one with a value that is not finite has scale NaN and reads as NaN.  Scales are float: an
 // fp16 one would be off by 2^-11 and would lose rows below 7.6e-6.
-#include "paged_few.h"
+#include <type_traits>
+
+#include "paged_device.h"
 
 namespace jsg {
 

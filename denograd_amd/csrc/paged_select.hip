@@ -4,7 +4,9 @@
 // No key of a page scores more with a query than sum_d q_d (q_d > 0 ? hi_d : lo_d), lo and hi being the least and the largest of each feature.  Both are kept as whole numbers, rounded outwards, times one power of
 // two per page and head; a row's queries are rounded to whole numbers times one power of two as well.  So scores are whole numbers below 2^21 times a power of two, exact however they are summed, and
 // which pages are chosen is a question of the inputs alone: with float sums two scores that are nearly the same would fall either way.
-#include "paged_few.h"
+#include <type_traits>
+
+#include "paged_device.h"
 
 namespace jsg {
 
@@ -251,7 +253,7 @@ template <int NW> struct KeyChoice {
 // four columns' scores of its page.  Bound by what waits for what: batch, page numbers, bounds, then the turns of the choice.  (us, 33000 positions, pages of 64, 32 heads of 128 over 8, a page to
 // a thread with dot products and 32 turns through LDS 22; 16 rows of up to 32768, pages of 32, 30; 2048 rows behind 14336, heads of 64, 138.)
 // HT tiles of 16 columns: of more heads of the rows (HEADS), or of more rows, for which the bounds are loaded once.
-template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, NW == 4 ? 4 : 2) void paged_select_kernel(PagedSelectArgs a) {
+template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, NW == 8 || HT == 1 ? 2 : HD == 64 && !HEADS ? 3 : 2) void paged_select_kernel(PagedSelectArgs a) {
   extern __shared__ __align__(16) uint32_t keys[];           // [rows of a block][stride]
   __shared__ union {
     KeyChoice<NW> block;
@@ -387,67 +389,450 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
 
 // ---------------------------------------------------------------- attention over the chosen pages
 
+// Block = 4 wavefronts, one row, up to 16 of its query heads of a kv head (usually four), and a part of its chosen pages.  Each wavefront walks its own steps of 64 keys: K rows to
+// registers as they are the matrix operand, V rows through registers into the wavefront's own LDS, from where the transposing reads take them; the next step's rows are asked for as soon as the registers are free.
+//
+// A matrix instruction scores 16 keys for 16 columns, and a row has few heads: with four, three columns of four would score the same again, and the vector unit would make the exponentials of
+// all.  So the columns are heads times groups of keys: column c of what a lane keeps has head c % HP over the keys of group c / HP of the step's four, each picked from that group's scores
+// (a selection per value), and holds its own running maximum, sum and share of the output; its weights are the operand of O^T = V^T . P^T with zeros at the other groups' keys.  The columns of a
+// head meet at the end, with the wavefronts.  A: accumulators that are left, 1 where a row has up to 4 heads, 2 up to 8, 4 beyond.
+constexpr int PA_THREADS = 256, PA_QROWS = 16, PA_MOST = 64;           // parts of a row: a lane for each
+constexpr int PA_SLOTS = 1024, PA_BLOCKS = 512;
+constexpr float PA_TOP = 15.0f;                            // a column's largest weight is 2^15: halves are normal numbers down to 2^-29 of it
+
 struct SelectedArgs {
-  PagedAttnArgs at;
+  PagedBatch pb;
+  const void *pages_k, *pages_v;
+  const float *scales_k, *scales_v;
+  const _Float16 *q;                     // [rows][H][HD]
+  _Float16 *out;
   const int32_t *selected;               // [rows][KV][top]
-  int top, parts, q_tiles;
+  int n_heads, n_rep, heads_log, top, parts, q_tiles;
+  Divisor n_kv_heads;
+  float scale_log2;                      // float(1 / sqrt(HD)) * log2(e)
+  int *counters;                         // zero, and zero again afterwards
+  float *ws;
 };
 
-// The keys of chosen pages: a list of {page, first position} in LDS.
-struct SelectedKeys {
-  const int2 *list;
-  __device__ void find(const PagedBatch &pb, int st, FewStep &s) const {
+template <int HD, bool I8, int A> struct SelectedRow {
+  static constexpr int NW = 4, KEYS = 64, ROWB = HD * 2;
+  static constexpr int VROW = ROWB + 32;                     // bytes between V rows in LDS: eight banks further each, so that the reads of 16 rows by 32 bytes meet all banks alike
+  static constexpr int NT = HD / 16, KS = HD / 32;           // 16-feature tiles of the output, matrix instructions per 16 keys
+  static constexpr int OROW = HD + 4;                        // floats between rows of a wavefront's sums in LDS
+  static constexpr int GK = KS / (I8 ? 2 : 1), LPR = HD / (I8 ? 16 : 8), GV = LPR / 4;   // 16-byte loads of 16 keys' K and V; lanes per V row
+  static constexpr int SLOT = PA_QROWS * (HD + 4);           // floats of a part: the heads' sums, then (m, l, -, -) of each
+  struct Smem {
+    union {
+      unsigned char v[32 * VROW];
+      float o[16 * OROW];
+    } wave[NW];
+    float m[NW][16], l[NW][16];
+    float w[PA_QROWS][PA_MOST], inv[PA_QROWS];
+    f4_t fold[PA_THREADS];
+    int2 list[PS_MOST + 4];                                  // the row's pages: number, first position
+    int most[NW], is_last;
+  };
+
+  // Must be called by every thread of the block (it contains barriers).  r, pos: the row and its position.
+  static __device__ void run(const SelectedArgs &a, int r, int g, int qt, int part, int b, int pos, Smem &sm) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+    const int n_rep = a.n_rep, KV = (int)a.n_kv_heads.d, hp = 1 << a.heads_log, shift = a.pb.page_shift, q0 = qt * PA_QROWS, nr = min(PA_QROWS, n_rep - q0);
+    const int cg = l16 >> a.heads_log;                       // this lane's group
+    const size_t q_off = ((size_t)r * a.n_heads + g * n_rep + q0) * HD;
+    h8_t qf[KS];                                             // the features that the K fragments have: fp16 8 (4 s + lq) .., int8 16 (lq + 4 c) + 8 u .., s = 2 c + u
+    {
+      const _Float16 *const qp = a.q + q_off + (size_t)min(l16 & (hp - 1), nr - 1) * HD;   // columns past the last head repeat it and are never stored
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int at = st * 32 + 16 * h;
-      const int2 e = list[at >> pb.page_shift];
-      s.id[h] = __builtin_amdgcn_readfirstlane(e.x);
-      s.key[h] = __builtin_amdgcn_readfirstlane(e.y) + (at & ((1 << pb.page_shift) - 1));
+      for (int s = 0; s < KS; s++) qf[s] = *as_global<h8_t>(qp + (I8 ? 16 * (lq + 4 * (s / 2)) + 8 * (s % 2) : 8 * (4 * s + lq)));
+    }
+    // the list, up to the last entry that names a page
+    const int32_t *const sel = a.selected + ((size_t)r * KV + g) * a.top;
+    const int last = pos < 0 ? -1 : pos >> shift;
+    int n = 0;
+    for (int i = tid; i < a.top + 4; i += PA_THREADS) {
+      const int page = i < a.top ? sel[i] : -1, held = page >= 0 && page <= last && page < a.pb.width ? paged_page(a.pb, b, page << shift) : -1;
+      sm.list[i] = make_int2(held, held >= 0 ? page << shift : 0);
+      if (held >= 0) n = i + 1;
+    }
+    for (int d = 32; d > 0; d >>= 1) n = max(n, __shfl_xor(n, d));
+    if (lane == 0) sm.most[wave] = n;
+    lds_barrier();
+    n = max(max(sm.most[0], sm.most[1]), max(sm.most[2], sm.most[3]));
+    const int steps = ((n << shift) + KEYS - 1) / KEYS, per = (steps + a.parts - 1) / a.parts, st_lo = min(part * per, steps), st_end = min(st_lo + per, steps);
+
+    struct Step {
+      int id[4], key[4];                                     // of the four groups: page, first position
+    };
+    auto find = [&](int st, Step &to) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int at = st * KEYS + 16 * j;
+        const int2 e = sm.list[min(at >> shift, a.top)];     // behind the last: none
+        to.id[j] = st < st_end ? __builtin_amdgcn_readfirstlane(e.x) : -1;
+        to.key[j] = __builtin_amdgcn_readfirstlane(e.y) + (at & ((1 << shift) - 1));
+      }
+    };
+    u4_t kr[4][GK], vr[4][GV];
+    f4_t ks[A], vs[A];                                       // of the keys that this lane keeps
+    auto row_of = [&](const Step &to, int j) { return paged_row(a.pb, KV, max(to.id[j], 0), g, to.key[j]); };   // a missing page: page 0, masked
+    auto mine = [&](auto v0, auto v1, auto v2, auto v3, int at) {   // of the four groups' values, that of this lane's accumulator `at`
+      if constexpr (A == 1) return cg == 0 ? v0 : cg == 1 ? v1 : cg == 2 ? v2 : v3;
+      else if constexpr (A == 2) return at == 0 ? (cg == 0 ? v0 : v1) : (cg == 0 ? v2 : v3);
+      else return at == 0 ? v0 : at == 1 ? v1 : at == 2 ? v2 : v3;
+    };
+    // a group's rows lie side by side: a base that all lanes share, and a lane's place from there
+    constexpr int KROW = I8 ? HD : ROWB;
+    const uint32_t k_at = l16 * KROW + lq * 16, v_at = lane / LPR * KROW + lane % LPR * 16;
+    auto load_k = [&](const Step &to) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const JSG_GLOBAL unsigned char *const from = as_global<unsigned char>(a.pages_k) + row_of(to, j) * KROW;
+#pragma unroll
+        for (int c = 0; c < GK; c++) kr[j][c] = *(const JSG_GLOBAL u4_t *)(from + (k_at + c * 64));
+      }
+      if constexpr (I8)
+#pragma unroll
+        for (int s = 0; s < A; s++) ks[s] = *as_global<f4_t>(a.scales_k + mine(row_of(to, 0), row_of(to, 1), row_of(to, 2), row_of(to, 3), s) + 4 * lq);
+    };
+    auto load_v = [&](const Step &to, int u) {               // groups 2 u and 2 u + 1
+#pragma unroll
+      for (int j = 2 * u; j < 2 * u + 2; j++) {
+        const JSG_GLOBAL unsigned char *const from = as_global<unsigned char>(a.pages_v) + row_of(to, j) * KROW;
+#pragma unroll
+        for (int c = 0; c < GV; c++) vr[j][c] = *(const JSG_GLOBAL u4_t *)(from + (v_at + c * (64 / LPR) * KROW));
+      }
+    };
+    auto load_vs = [&](const Step &to) {
+      if constexpr (I8)
+#pragma unroll
+        for (int s = 0; s < A; s++) vs[s] = *as_global<f4_t>(a.scales_v + mine(row_of(to, 0), row_of(to, 1), row_of(to, 2), row_of(to, 3), s) + 4 * lq);
+    };
+
+    int st;
+    Step at, next;
+    f4_t o[NT];
+    float m_run, l_run;
+    const float unit = I8 ? 1.0f : a.scale_log2;
+    unsigned char *const vl = sm.wave[wave].v;
+
+    // more: there is another step; careful: V may hold halves that are not finite
+    auto step = [&](auto more, auto careful) {
+      constexpr bool MORE = decltype(more)::value, CAREFUL = decltype(careful)::value;
+      find(st + NW, next);
+      f4_t d[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        d[j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < GK; c++)
+#pragma unroll
+          for (int u = 0; u < KS / GK; u++) {
+            u4_t k = kr[j][c];
+            if constexpr (I8) {
+              uint32_t w[4];
+              i8x4_to_h2x2(kr[j][c][2 * u], w[0], w[1]);
+              i8x4_to_h2x2(kr[j][c][2 * u + 1], w[2], w[3]);
+              k = u4_t{w[0], w[1], w[2], w[3]};
+            }
+            d[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, k), qf[c * (KS / GK) + u], d[j], 0, 0, 0);
+          }
+      }
+      f4_t s[A];
+#pragma unroll
+      for (int x = 0; x < A; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[x][e] = mine(d[0][e], d[1][e], d[2][e], d[3][e], x);
+      f4_t kscale[A], inv_v[A];
+      if constexpr (I8)
+#pragma unroll
+        for (int x = 0; x < A; x++) kscale[x] = ks[x] * a.scale_log2;
+      if constexpr (MORE) load_k(next);
+      if constexpr (I8) {
+        // scale_of_v, for which there is a reason in few steps: 16 codes of zero side by side, or a scale below PAGED_TINY
+        uint32_t codes = ~0u;
+        float least = INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int c = 0; c < GV; c++) codes = min(codes, vr[j][c][0] | vr[j][c][1] | vr[j][c][2] | vr[j][c][3]);
+#pragma unroll
+        for (int x = 0; x < A; x++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) least = fminf(least, vs[x][e]);
+        if (__builtin_amdgcn_ballot_w64(codes == 0 || least < PAGED_TINY)) {
+          uint32_t zeros[4];                                 // of rows 4 lq .. of each group: which are all zero
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint64_t some[GV];                               // lanes LPR * r and on have row r of the sixteen: LPR bits of each of these four rows
+#pragma unroll
+            for (int c = 0; c < GV; c++) some[c] = __builtin_amdgcn_ballot_w64((vr[j][c][0] | vr[j][c][1] | vr[j][c][2] | vr[j][c][3]) != 0);
+            const uint64_t held = GV == 1 || lq * GV / 4 == 0 ? some[0] : some[GV - 1];
+            const uint32_t rows = (uint32_t)(held >> (lq * 4 % (64 / LPR)) * LPR);
+            zeros[j] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) zeros[j] |= (uint32_t)(((rows >> e * LPR) & ((1u << LPR) - 1)) == 0) << e;
+          }
+#pragma unroll
+          for (int x = 0; x < A; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vs[x][e] = scale_of_v(vs[x][e], mine(zeros[0], zeros[1], zeros[2], zeros[3], x) >> e & 1);
+        }
+#pragma unroll
+        for (int x = 0; x < A; x++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            // the scale of V in the exponent, its reciprocal finite whatever lies in a place that no row sees
+            const float v = vs[x][e];
+            s[x][e] = __builtin_fmaf(s[x][e], kscale[x][e], __builtin_amdgcn_logf(v));
+            inv_v[x][e] = v >= PAGED_TINY && v < INFINITY ? __builtin_amdgcn_rcpf(v) : 1.0f;
+          }
+      }
+      // value e of s[x] is key 4 lq + e of this lane's group
+      const bool masked = (at.id[0] | at.id[1] | at.id[2] | at.id[3]) < 0 || max(max(at.key[0], at.key[1]), max(at.key[2], at.key[3])) + 15 > pos;
+      if (masked)
+#pragma unroll
+        for (int x = 0; x < A; x++) {
+          const int seen = pos - mine(at.key[0], at.key[1], at.key[2], at.key[3], x) - 4 * lq, id = mine(at.id[0], at.id[1], at.id[2], at.id[3], x);
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[x][e] = id >= 0 && e <= seen ? s[x][e] : -INFINITY;
+        }
+      if (A == 1 && a.heads_log < 2)                         // more groups of columns than of keys
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[0][e] = cg < 4 ? s[0][e] : -INFINITY;
+      float mx = m_run;
+#pragma unroll
+      for (int x = 0; x < A; x++) mx = fmaxf(fmaxf(fmaxf(mx, s[x][0]), fmaxf(s[x][1], s[x][2])), s[x][3]);
+      mx = max_xor32(max_xor16(mx));
+      if (__builtin_amdgcn_ballot_w64(mx > m_run)) {
+        const float alpha = __builtin_amdgcn_exp2f((m_run - mx) * unit);
+        m_run = mx;
+        l_run *= alpha;
+#pragma unroll
+        for (int t = 0; t < NT; t++) o[t] *= alpha;
+      }
+      uint32_t pk[A][2];
+#pragma unroll
+      for (int x = 0; x < A; x++) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          // the difference first: it is never above zero, however large the scores are
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e] - m_run, unit, PA_TOP));
+          l_run = I8 ? __builtin_fmaf(p[e], inv_v[x][e], l_run) : l_run + p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) pk[x][e] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)p[2 * e], (_Float16)p[2 * e + 1]});
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {                          // 32 keys: groups 2 u and 2 u + 1
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int c = 0; c < GV; c++) {
+            const int row = 16 * h + c * (64 / LPR) + lane / LPR, piece = lane % LPR;
+            const u4_t v = vr[2 * u + h][c];
+            if constexpr (I8) {
+#pragma unroll
+              for (int x = 0; x < 2; x++) {
+                uint32_t w[4];
+                i8x4_to_h2x2(v[2 * x], w[0], w[1]);
+                i8x4_to_h2x2(v[2 * x + 1], w[2], w[3]);
+                *(u4_t *)(vl + row * VROW + (2 * piece + x) * 16) = u4_t{w[0], w[1], w[2], w[3]};
+              }
+            } else {
+              *(u4_t *)(vl + row * VROW + piece * 16) = v;
+            }
+          }
+        if constexpr (MORE) {
+          load_v(next, u);
+          if (u == 1) load_vs(next);
+        }
+        u4_t pw;                                             // this column's weights, zero at the other groups' keys
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int x = A == 1 ? 0 : A == 2 ? u : 2 * u + h;
+          const bool own = A == 4 || cg == (A == 1 ? 2 * u + h : h);
+#pragma unroll
+          for (int e = 0; e < 2; e++) pw[2 * h + e] = own ? pk[x][e] : 0;
+        }
+        const h8_t pf = __builtin_bit_cast(h8_t, pw);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          s4_t v[2];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int row = 16 * h + 4 * lq + (l16 >> 2), c = t * 32 + (l16 & 3) * 8;
+            v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t *)(vl + row * VROW + c));
+          }
+          u4_t w = __builtin_bit_cast(u4_t, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (CAREFUL) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t x = ((w[e] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;   // the sign bit of halves that are not finite
+              w[e] &= ~(x | (x - (x >> 15)));
+            }
+          }
+          o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w), pf, o[t], 0, 0, 0);
+        }
+        if constexpr (CAREFUL) {
+          // those are left out of the product, where a weight of zero would not stop them, and added once for each head that sees them
+          for (int key = 0; key < 32; key++) {
+            const bool upper = key >= 16;
+            const int id = upper ? at.id[2 * u + 1] : at.id[2 * u], first = upper ? at.key[2 * u + 1] : at.key[2 * u];
+            const bool seen = id >= 0 && first + (key & 15) <= pos && (A == 4 || cg == (A == 1 ? 2 * u : 0) + upper);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              const uint2 w = *(const uint2 *)(vl + key * VROW + t * 32 + 8 * lq);
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const uint32_t x = (e < 2 ? w.x : w.y) >> (16 * (e & 1)) & 0xffffu;
+                o[t][e] += seen && (x & 0x7c00u) == 0x7c00u ? (float)__builtin_bit_cast(_Float16, (uint16_t)x) : 0.0f;
+              }
+            }
+          }
+        }
+      }
+      at = next;
+    };
+    auto walk = [&](auto careful) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) o[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      m_run = -1e30f;                                        // finite: a step may hold no key that a column sees
+      l_run = 0.0f;
+      st = st_lo + wave;
+      find(st, at);
+      if (st >= st_end) return;
+      load_k(at);
+      load_v(at, 0);
+      load_v(at, 1);
+      load_vs(at);
+      // the last step by itself: behind a branch around its loads every wait would be for all of them
+      for (; st + NW < st_end; st += NW) step(std::true_type(), careful);
+      step(std::false_type(), careful);
+    };
+    walk(std::false_type());
+    if constexpr (!I8) {
+      // Halves of V that are not finite make sums so that are not finite, also where their weight is zero.  It is seen here, and then the walk is made once more with a look at every half: that look in
+      // every walk is a quarter of the vector unit's work.
+      bool bad = false;
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) bad |= !(fabsf(o[t][e]) < INFINITY);
+      if (__builtin_amdgcn_ballot_w64(bad)) walk(std::true_type());
+    }
+
+    // the block's wavefronts and columns: value e of o[t] is feature 16 t + 4 lq + e of column l16
+    l_run = add_xor32(add_xor16(l_run));
+#pragma unroll
+    for (int t = 0; t < NT; t++) *(f4_t *)&sm.wave[wave].o[l16 * OROW + t * 16 + 4 * lq] = o[t];
+    if (lq == 0) { sm.m[wave][l16] = m_run; sm.l[wave][l16] = l_run; }
+    lds_barrier();
+    constexpr int GROUPS = 4 / A;                            // columns of a head
+    auto block_sum = [&](int h, int c, f4_t &sum, float &M, float &L) {   // features 4 c .. of head h
+      M = -1e30f;
+#pragma unroll
+      for (int w = 0; w < NW; w++)
+#pragma unroll
+        for (int j = 0; j < GROUPS; j++) M = fmaxf(M, sm.m[w][j * hp + h]);
+      sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; w++)
+#pragma unroll
+        for (int j = 0; j < GROUPS; j++) {
+          const int col = j * hp + h;
+          const float e = __builtin_amdgcn_exp2f((sm.m[w][col] - M) * unit);
+          L = __builtin_fmaf(sm.l[w][col], e, L);
+          const f4_t v = *(const f4_t *)&sm.wave[w].o[col * OROW + 4 * c];
+#pragma unroll
+          for (int x = 0; x < 4; x++) sum[x] = __builtin_fmaf(v[x], e, sum[x]);
+        }
+    };
+    auto put = [&](int h, int c, f4_t sum, float inv) {
+      const h2_t lo = {(_Float16)(sum[0] * inv), (_Float16)(sum[1] * inv)}, hi = {(_Float16)(sum[2] * inv), (_Float16)(sum[3] * inv)};
+      *(uint2 *)(a.out + q_off + (size_t)h * HD + 4 * c) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+    };
+    const int pieces = nr * (HD / 4);
+    if (a.parts == 1) {
+      for (int i = tid; i < pieces; i += PA_THREADS) {
+        f4_t sum;
+        float M, L;
+        block_sum(i / (HD / 4), i % (HD / 4), sum, M, L);
+        put(i / (HD / 4), i % (HD / 4), sum, L == 0.0f ? 0.0f : 1.0f / L);   // 0: the row sees nothing
+      }
+      return;
+    }
+    // Parts: sums through memory at device scope (cache policy 16), counted once they are acknowledged; the last block of the row and heads folds them in order.
+    const int slot = (r * a.q_tiles + qt) * a.parts * KV + g;
+    const uint32_t part_bytes = (uint32_t)KV * SLOT * 4;
+    const __amdgpu_buffer_rsrc_t rw = wave_buffer(a.ws + (size_t)slot * SLOT, (uint32_t)(a.parts - 1) * part_bytes + SLOT * 4);
+    for (int i = tid; i < pieces; i += PA_THREADS) {
+      f4_t sum;
+      float M, L;
+      const int h = i / (HD / 4), c = i % (HD / 4);
+      block_sum(h, c, sum, M, L);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, sum), rw, (uint32_t)part * part_bytes + i * 16, 0, 16);
+      if (c == 0) {
+        const f4_t ml = {M, L, 0.0f, 0.0f};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, ml), rw, (uint32_t)part * part_bytes + (PA_QROWS * HD + h * 4) * 4, 0, 16);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) sm.is_last = __hip_atomic_fetch_add(&a.counters[slot], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+    __syncthreads();
+    if (!sm.is_last) return;
+    if (tid == 0) __hip_atomic_store(&a.counters[slot], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+    // weights of the parts: a wavefront per head, a part per lane
+    for (int h = wave; h < nr; h += NW) {
+      const f4_t ml = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, (uint32_t)min(lane, a.parts - 1) * part_bytes + (PA_QROWS * HD + h * 4) * 4, 0, 16));
+      const float m = lane < a.parts ? ml[0] : -1e30f, M = wave_max(m), e = lane < a.parts ? __builtin_amdgcn_exp2f((m - M) * unit) : 0.0f;
+      const float L = wave_sum(lane < a.parts ? ml[1] * e : 0.0f);
+      sm.w[h][lane] = e;
+      if (lane == 0) sm.inv[h] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+    lds_barrier();
+    // a thread per four features of a head; where those are fewer than threads, teams of threads share the parts
+    const int teams = pieces < PA_THREADS ? PA_THREADS / pieces : 1, team = teams > 1 ? tid / pieces : 0;
+    for (int i0 = teams > 1 ? tid - team * pieces : tid; i0 < pieces; i0 += PA_THREADS) {
+      const int h = i0 / (HD / 4), c = i0 % (HD / 4);
+      f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (team < teams)
+        for (int f = team; f < a.parts; f += teams * 8) {
+          f4_t v[8];
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            v[u] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, (uint32_t)min(f + u * teams, a.parts - 1) * part_bytes + i0 * 16, 0, 16));
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            if (f + u * teams < a.parts)
+#pragma unroll
+              for (int x = 0; x < 4; x++) sum[x] = __builtin_fmaf(v[u][x], sm.w[h][f + u * teams], sum[x]);
+        }
+      if (teams == 1) put(h, c, sum, sm.inv[h]);
+      else sm.fold[tid] = sum;
+    }
+    if (teams > 1) {
+      lds_barrier();
+      if (tid < pieces) {
+        f4_t sum = sm.fold[tid];
+        for (int u = 1; u < teams; u++) sum += sm.fold[tid + u * pieces];
+        put(tid / (HD / 4), tid % (HD / 4), sum, sm.inv[tid / (HD / 4)]);
+      }
     }
   }
-  __device__ bool masks(const int (&k)[2], int pos_lo, int) const { return max(k[0], k[1]) + 15 > pos_lo; }
-  __device__ bool sees(int key, int pos) const { return key <= pos; }
 };
 
-// Block = 16 of a row's query heads of one kv head, and a part of the row's chosen pages: PagedFew's work on one position.
-constexpr int PA_SLOTS = 1024, PA_BLOCKS = 512;
-template <int HD, bool I8> __global__ __launch_bounds__(FEW_THREADS, HD == 64 ? 4 : I8 ? 3 : 2) void attn_selected_kernel(SelectedArgs sa) {
-  typedef PagedFew<HD, I8> A;
-  __shared__ typename A::Smem sm;
-  __shared__ int2 list[PS_MOST + 1];
-  const PagedAttnArgs &a = sa.at;
-  const int KV = (int)a.n_kv_heads.d;
-  int id = blockIdx.x;
-  PagedItem it;
-  it.g = id % KV;
-  id /= KV;
-  it.part = id % sa.parts;
-  id /= sa.parts;
-  it.qt = id % sa.q_tiles;
-  const int r = id / sa.q_tiles, b = paged_find(a.pb, r);
+// Block numbers have the kv heads innermost: blocks are dealt to the eight XCDs in turn, so that with eight kv heads each XCD has one, all rows of which share its K and V in that L2.
+template <int HD, bool I8, int A> __global__ __launch_bounds__(PA_THREADS, HD == 64 ? (I8 || A > 1 ? 3 : 4) : 2) void attn_selected_kernel(SelectedArgs a) {
+  __shared__ typename SelectedRow<HD, I8, A>::Smem sm;
+  const int id = blockIdx.x, KV = (int)a.n_kv_heads.d, rest = a.n_kv_heads.div(id), g = id - rest * KV;
+  const int part = rest % a.parts, tile = rest / a.parts, qt = tile % a.q_tiles, r = tile / a.q_tiles, b = paged_find(a.pb, r);
   if (b >= a.pb.n_seqs) return;
   const PagedSeq s = paged_seq(a.pb, b);
   if (r < s.start) return;
-  const int pos = paged_pos(s, r - s.start);
-  it.b = b;
-  it.s = {r, 1, pos + 1};                                    // the one row, at its position
-  it.parts = sa.parts;
-  it.slot = (r * sa.q_tiles + it.qt) * sa.parts * KV + it.g;
-  const int32_t *const sel = sa.selected + ((size_t)r * KV + it.g) * sa.top;
-  const int last = pos < 0 ? -1 : pos >> a.pb.page_shift;
-  int n = 0;                                                 // behind the last entry that names a page
-  for (int i = threadIdx.x; i <= sa.top; i += FEW_THREADS) {
-    const int page = i < sa.top ? sel[i] : -1, held = page >= 0 && page <= last && page < a.pb.width ? paged_page(a.pb, b, page << a.pb.page_shift) : -1;
-    list[i] = make_int2(held, held >= 0 ? page << a.pb.page_shift : 0);
-    if (held >= 0) n = i + 1;
-  }
-  for (int d = 32; d > 0; d >>= 1) n = max(n, __shfl_xor(n, d));
-  __shared__ int most[FEW_THREADS / 64];
-  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = n;
-  __syncthreads();
-  n = max(max(most[0], most[1]), max(most[2], most[3]));
-  const int steps = ((n << a.pb.page_shift) + 31) / 32, per = (steps + sa.parts - 1) / sa.parts, lo = min(it.part * per, steps);
-  A::walk(a, it, SelectedKeys{list}, lo, min(lo + per, steps), sm);
+  SelectedRow<HD, I8, A>::run(a, r, g, qt, part, b, paged_pos(s, r - s.start), sm);
 }
 
 // Argument checks that the calls here share
@@ -539,14 +924,13 @@ int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t 
 
 size_t jsgrad_hip_attn_selected_workspace_bytes(int n_heads, int n_kv_heads, int head_dim) {
   (void)n_heads, (void)n_kv_heads;
-  return PA_SLOTS * sizeof(int) + (size_t)PA_SLOTS * FEW_QROWS * (head_dim + 4) * sizeof(float);
+  return PA_SLOTS * sizeof(int) + (size_t)PA_SLOTS * PA_QROWS * (head_dim + 4) * sizeof(float);
 }
 
 int jsgrad_hip_attn_selected(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, void *out, int n_heads,
                              const int32_t *selected, int top, void *workspace) {
   const char *who = "jsgrad_hip_attn_selected";
-  SelectedArgs sa = {};
-  PagedAttnArgs &a = sa.at;
+  SelectedArgs a = {};
   if (int e = paged_check(who, host_pages, row_starts, lengths, n_seqs, rows, &a.pb)) return e;
   if (int e = heads_check(who, host_pages, q, rows, n_heads)) return e;
   JSG_REQUIRE(out && selected && workspace, "%s: null pointer argument", who);
@@ -557,27 +941,36 @@ int jsgrad_hip_attn_selected(const jsgrad_hip_pages_t *host_pages, const int32_t
   a.pages_k = host_pages->pages_k; a.pages_v = host_pages->pages_v;
   a.scales_k = (const float *)host_pages->scales_k; a.scales_v = (const float *)host_pages->scales_v;
   a.q = (const _Float16 *)q; a.out = (_Float16 *)out;
-  a.n_heads = n_heads;
-  a.n_rep = divisor(n_rep); a.n_kv_heads = divisor(KV);
+  a.n_heads = n_heads; a.n_rep = n_rep;
+  while ((1 << a.heads_log) < (n_rep < PA_QROWS ? n_rep : PA_QROWS)) a.heads_log++;
+  a.n_kv_heads = divisor(KV);
   a.scale_log2 = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
-  a.few_counters = (int *)workspace;
-  a.few_ws = (float *)((char *)workspace + PA_SLOTS * sizeof(int));
-  sa.selected = selected; sa.top = top;
-  sa.q_tiles = (n_rep + FEW_QROWS - 1) / FEW_QROWS;
-  const size_t items = (size_t)rows * sa.q_tiles * KV;
+  a.counters = (int *)workspace;
+  a.ws = (float *)((char *)workspace + PA_SLOTS * sizeof(int));
+  a.selected = selected; a.top = top;
+  a.q_tiles = (n_rep + PA_QROWS - 1) / PA_QROWS;
+  const size_t items = (size_t)rows * a.q_tiles * KV;
   JSG_REQUIRE(items < (size_t)PAGED_GRID, "%s: %d rows of %d heads", who, rows, n_heads);
-  const int steps = (int)(((size_t)(top < a.pb.width ? top : a.pb.width) << a.pb.page_shift) / 32) + 1;
+  // parts of a row where there are few: two blocks to a unit, each wavefront with two steps at least
+  const int steps = (int)(((size_t)(top < a.pb.width ? top : a.pb.width) << a.pb.page_shift) / 64);
   int parts = items * 2 <= PA_BLOCKS ? (int)(PA_BLOCKS / items) : 1;
-  parts = parts < FEW_MOST ? parts : FEW_MOST;
-  parts = parts < steps / 8 ? parts : steps / 8;
-  sa.parts = parts > 1 ? parts : 1;
+  parts = parts < PA_MOST ? parts : PA_MOST;
+  parts = parts < steps / 4 ? parts : steps / 4;
+  a.parts = parts > 1 ? parts : 1;
   JSG_READY();
-  const dim3 grid((unsigned)(items * sa.parts)), block(FEW_THREADS);
+  const dim3 grid((unsigned)(items * a.parts)), block(PA_THREADS);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
-  if (HD == 64 && i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<64, true>), grid, block, 0, sa);
-  else if (HD == 64) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<64, false>), grid, block, 0, sa);
-  else if (i8) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<128, true>), grid, block, 0, sa);
-  else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<128, false>), grid, block, 0, sa);
+#define JSG_SELECTED(HD, I8)                                                                                    \
+  do {                                                                                                          \
+    if (a.heads_log <= 2) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, 1>), grid, block, 0, a);      \
+    else if (a.heads_log == 3) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, 2>), grid, block, 0, a); \
+    else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, 4>), grid, block, 0, a);                       \
+  } while (0)
+  if (HD == 64 && i8) JSG_SELECTED(64, true);
+  else if (HD == 64) JSG_SELECTED(64, false);
+  else if (i8) JSG_SELECTED(128, true);
+  else JSG_SELECTED(128, false);
+#undef JSG_SELECTED
   return 0;
 }
 
