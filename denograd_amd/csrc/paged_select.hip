@@ -25,6 +25,31 @@ struct PagedSelectArgs {
   int32_t *selected;                     // [rows][KV][top]
 };
 
+// sums of a lane's value and those of the lanes below
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// The sequence of a row, and its number; n_seqs where none has it.  As paged_find and paged_seq, for a uniform r, but in one trip to memory for up to 64 sequences: it is in front of everything else.
+__device__ __forceinline__ int find_row(const PagedBatch &pb, int r, PagedSeq &s) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < pb.n_seqs; b0 += 64) {
+    const int b = min(b0 + lane, pb.n_seqs - 1), start = pb.row_starts[b], end = pb.row_starts[b + 1], len = pb.lengths[b];
+    const uint64_t behind = __builtin_amdgcn_ballot_w64(end > r);
+    if (!behind) continue;
+    const int l = __builtin_ctzll(behind);
+    s = paged_seq(__builtin_amdgcn_readlane(start, l), __builtin_amdgcn_readlane(end, l), __builtin_amdgcn_readlane(len, l), pb.rows);
+    return b0 + l;
+  }
+  return pb.n_seqs;
+}
+
 // The smallest power of two, 2^-126 and more, that 127 times is `most` (finite) and more; 1 for 0.
 __device__ __forceinline__ float bound_step(float most) {
   if (most == 0.0f) return 1.0f;
@@ -33,21 +58,40 @@ __device__ __forceinline__ float bound_step(float most) {
   return __builtin_amdgcn_ldexpf(1.0f, max(e - 7 + (f > 127.0f / 128.0f), -126));
 }
 
-// Block = (row, kv head), at work where the row is the first of the batch on its page: the whole page is looked at, so bounds do not depend on how its rows came.
-// Bound by memory: HD / 8 lanes a row, 16 bytes (int8: 8) each.
+// The t-th page that the batch's rows are on, sequence by sequence: its sequence (n_seqs: there are not so many) and the page's first position.  A sequence to a lane.
+__device__ __forceinline__ int find_touched(const PagedBatch &pb, uint32_t t, PagedSeq &s, int &first) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < pb.n_seqs; b0 += 64) {
+    const int b = min(b0 + lane, pb.n_seqs - 1), start = pb.row_starts[b], end = pb.row_starts[b + 1], len = pb.lengths[b];
+    const PagedSeq mine = paged_seq(start, end, len, pb.rows);
+    const int p0 = max(paged_pos(mine, 0), 0) >> pb.page_shift;
+    const uint32_t n = b0 + lane < pb.n_seqs && mine.n > 0 && mine.len > 0 ? (uint32_t)(((mine.len - 1) >> pb.page_shift) - p0 + 1) : 0, upto = wave_upto(n);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(upto > t);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      s = {__builtin_amdgcn_readlane(mine.start, l), __builtin_amdgcn_readlane(mine.n, l), __builtin_amdgcn_readlane(mine.len, l)};
+      first = (__builtin_amdgcn_readlane(p0, l) + (int)(t - (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), l))) << pb.page_shift;
+      return b0 + l;
+    }
+    t -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  }
+  return pb.n_seqs;
+}
+
+// Block = (page that the batch's rows are on, kv head): the whole page is looked at, so bounds do not depend on how its rows came.  Bound by memory: HD / 8 lanes a row, 16 bytes (int8: 8) each.
+// (A block for every row, most of which have nothing to do: 2048 rows, heads of 64, 27 us.)
 template <int HD, bool I8> __global__ __launch_bounds__(PS_THREADS) void paged_bounds_kernel(PagedSelectArgs a) {
   constexpr int G = HD / 8, RPB = PS_THREADS / G;
   __shared__ float lo_sh[PS_THREADS / 64][HD], hi_sh[PS_THREADS / 64][HD];
   __shared__ float most_sh[PS_THREADS / 64];
-  const int r = blockIdx.x, g = blockIdx.y, KV = a.n_kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = paged_find(a.pb, r);
+  const int g = blockIdx.y, KV = a.n_kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  PagedSeq s;
+  int first;
+  const int b = find_touched(a.pb, blockIdx.x, s, first);
   if (b >= a.pb.n_seqs) return;
-  const PagedSeq s = paged_seq(a.pb, b);
-  const int pos = paged_pos(s, r - s.start), P = 1 << a.pb.page_shift;
-  if (r < s.start || pos < 0 || (r > s.start && pos > 0 && (pos & (P - 1)) != 0)) return;
-  const int id = paged_page(a.pb, b, pos);
+  const int id = paged_page(a.pb, b, first);
   if (id < 0) return;
-  const int first = pos & ~(P - 1), n = min(P, s.len - first);
+  const int n = min(1 << a.pb.page_shift, s.len - first);
   const size_t row0 = paged_row(a.pb, KV, id, g, first);
   const int e0 = threadIdx.x % G * 8;
   float lo[8], hi[8];
@@ -121,17 +165,6 @@ template <typename Op> __device__ __forceinline__ uint32_t wave_all(uint32_t v, 
   auto row = [&](int r) { return (uint32_t)__builtin_amdgcn_readlane((int)v, r * 16); };
   return op(op(row(0), row(1)), op(row(2), row(3)));
 }
-// sums of a lane's value and those of the lanes below
-__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
-  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 // The first `top` of n keys in the order (key descending, index ascending), those above 0, written as rising indexes with -1 behind.  By one wavefront, or (NW > 1) by a block of NW, each with a stretch of
 // the keys.  What lies between the least and the largest is counted in 256 parts, then the part with the border in 256 again, until a part is wanted whole or its keys are all alike: two or
 // three turns, four at most.  (Halving a threshold takes some 15: 33000 positions in pages of 64, 4.3 us of them.)
@@ -143,7 +176,6 @@ template <int NW> struct KeyChoice {
   __device__ __forceinline__ void operator()(const uint32_t *keys, int n, int top, int32_t *out, int wave) {
     const int per = NW == 1 ? n : ((n + NW - 1) / NW + 63) & ~63, lo = min(wave * per, n), hi = min(lo + per, n);
     if (per <= 4 * 64) choose<4>(keys, lo, hi, n, top, out, wave);
-    else if (per <= 16 * 64) choose<16>(keys, lo, hi, n, top, out, wave);
     else choose<0>(keys, lo, hi, n, top, out, wave);
   }
   // K: keys of a lane; 0: any number, from where they are
@@ -157,7 +189,13 @@ template <int NW> struct KeyChoice {
 #pragma unroll
         for (int u = 0; u < K; u++) f(mine[u], lo + u * 64);
       } else {
-        for (int i = lo; i < hi; i += 64) f(i + lane < hi ? keys[i + lane] : 0u, i);
+        for (int i = lo; i < hi; i += 256) {
+          uint32_t k[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) k[u] = i + u * 64 + lane < hi ? keys[i + u * 64 + lane] : 0u;
+#pragma unroll
+          for (int u = 0; u < 4; u++) f(k[u], i + u * 64);
+        }
       }
     };
     auto join = [&](uint32_t (&of)[NW], uint32_t v, auto op) {   // over the block, behind a barrier
@@ -264,9 +302,9 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hp = 1 << a.heads_log, shift = a.pb.page_shift;
   const int r_end = min((int)(blockIdx.x + 1) * a.tile, a.pb.rows);
   for (int r0 = blockIdx.x * a.tile; r0 < r_end;) {
-    const int b = paged_find(a.pb, r0);
+    PagedSeq s;
+    const int b = find_row(a.pb, r0, s);
     if (b >= a.pb.n_seqs) return;
-    const PagedSeq s = paged_seq(a.pb, b);
     const int n_rows = min(s.start + s.n, r_end) - r0;
     if (r0 < s.start) { r0++; continue; }                    // no sequence has it
     const int p0 = paged_pos(s, r0 - s.start), last_page = p0 + n_rows - 1 < 0 ? -1 : (p0 + n_rows - 1) >> shift, n = min(last_page + 1, a.pb.width);
@@ -389,8 +427,10 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
 
 // ---------------------------------------------------------------- attention over the chosen pages
 
-// Block = 4 wavefronts, one row, up to 16 of its query heads of a kv head (usually four), and a part of its chosen pages.  Each wavefront walks its own steps of 64 keys: K rows to
-// registers as they are the matrix operand, V rows through registers into the wavefront's own LDS, from where the transposing reads take them; the next step's rows are asked for as soon as the registers are free.
+// Block = 4 wavefronts.  Where there are few rows, one row, up to 16 of its query heads of a kv head (usually four), and a part of its chosen pages, each wavefront with steps of its own; else (SOLO) four
+// rows, a wavefront to each, which neither wait for one another nor start anew every few steps.  A step is 64 keys: rows of K and V
+// come through registers into the wavefront's own LDS, 32 at a time, V's for the transposing reads; the next step's rows are asked for as soon as the registers are free.  K straight to registers, as the
+// matrix operand has it, would put the lanes of a quarter on different rows, and the L1 cache would be asked 64 times for what it gives in 16: 2048 rows, heads of 64, 305 us.
 //
 // A matrix instruction scores 16 keys for 16 columns, and a row has few heads: with four, three columns of four would score the same again, and the vector unit would make the exponentials of
 // all.  So the columns are heads times groups of keys: column c of what a lane keeps has head c % HP over the keys of group c / HP of the step's four, each picked from that group's scores
@@ -414,12 +454,13 @@ struct SelectedArgs {
   float *ws;
 };
 
-template <int HD, bool I8, int A> struct SelectedRow {
-  static constexpr int NW = 4, KEYS = 64, ROWB = HD * 2;
+template <int HD, bool I8, int A, bool SOLO> struct SelectedRow {
+  static constexpr int NW = 4, ROW_WAVES = SOLO ? 1 : NW, ROW_THREADS = ROW_WAVES * 64, KEYS = 64, ROWB = HD * 2;
   static constexpr int VROW = ROWB + 32;                     // bytes between V rows in LDS: eight banks further each, so that the reads of 16 rows by 32 bytes meet all banks alike
   static constexpr int NT = HD / 16, KS = HD / 32;           // 16-feature tiles of the output, matrix instructions per 16 keys
   static constexpr int OROW = HD + 4;                        // floats between rows of a wavefront's sums in LDS
-  static constexpr int GK = KS / (I8 ? 2 : 1), LPR = HD / (I8 ? 16 : 8), GV = LPR / 4;   // 16-byte loads of 16 keys' K and V; lanes per V row
+  static constexpr int KROW = ROWB + 16;                     // and K rows in LDS: eight rows' 16 bytes meet all banks alike
+  static constexpr int LPR = HD / (I8 ? 16 : 8), GV = LPR / 4;   // lanes to a row, 16-byte loads of 16 keys' rows
   static constexpr int SLOT = PA_QROWS * (HD + 4);           // floats of a part: the heads' sums, then (m, l, -, -) of each
   struct Smem {
     union {
@@ -427,38 +468,46 @@ template <int HD, bool I8, int A> struct SelectedRow {
       float o[16 * OROW];
     } wave[NW];
     float m[NW][16], l[NW][16];
-    float w[PA_QROWS][PA_MOST], inv[PA_QROWS];
-    f4_t fold[PA_THREADS];
-    int2 list[PS_MOST + 4];                                  // the row's pages: number, first position
+    float w[SOLO ? 1 : PA_QROWS][PA_MOST], inv[PA_QROWS];
+    f4_t fold[SOLO ? 1 : PA_THREADS];
+    int2 list[SOLO ? 1 : PS_MOST + 4];                       // the row's pages: number, first position; SOLO: in the lanes
     int most[NW], is_last;
   };
 
-  // Must be called by every thread of the block (it contains barriers).  r, pos: the row and its position.
-  static __device__ void run(const SelectedArgs &a, int r, int g, int qt, int part, int b, int pos, Smem &sm) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lq = lane >> 4;
+  // Must be called by every thread of the block (it contains barriers; SOLO: of the wavefront, and none).  r, pos: the row and its position; chosen: this thread's entry of its list.
+  static __device__ void run(const SelectedArgs &a, int r, int g, int qt, int part, int b, int pos, int chosen, Smem &sm) {
+    const int lane = threadIdx.x & 63, tid = SOLO ? lane : threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, lq = lane >> 4;
     const int n_rep = a.n_rep, KV = (int)a.n_kv_heads.d, hp = 1 << a.heads_log, shift = a.pb.page_shift, q0 = qt * PA_QROWS, nr = min(PA_QROWS, n_rep - q0);
     const int cg = l16 >> a.heads_log;                       // this lane's group
     const size_t q_off = ((size_t)r * a.n_heads + g * n_rep + q0) * HD;
-    h8_t qf[KS];                                             // the features that the K fragments have: fp16 8 (4 s + lq) .., int8 16 (lq + 4 c) + 8 u .., s = 2 c + u
+    h8_t qf[KS];                                             // the features that the K fragments have: 8 (4 s + lq) ..
     {
       const _Float16 *const qp = a.q + q_off + (size_t)min(l16 & (hp - 1), nr - 1) * HD;   // columns past the last head repeat it and are never stored
 #pragma unroll
-      for (int s = 0; s < KS; s++) qf[s] = *as_global<h8_t>(qp + (I8 ? 16 * (lq + 4 * (s / 2)) + 8 * (s % 2) : 8 * (4 * s + lq)));
+      for (int s = 0; s < KS; s++) qf[s] = *as_global<h8_t>(qp + 8 * (4 * s + lq));
     }
     // the list, up to the last entry that names a page
     const int32_t *const sel = a.selected + ((size_t)r * KV + g) * a.top;
     const int last = pos < 0 ? -1 : pos >> shift;
-    int n = 0;
-    for (int i = tid; i < a.top + 4; i += PA_THREADS) {
-      const int page = i < a.top ? sel[i] : -1, held = page >= 0 && page <= last && page < a.pb.width ? paged_page(a.pb, b, page << shift) : -1;
-      sm.list[i] = make_int2(held, held >= 0 ? page << shift : 0);
-      if (held >= 0) n = i + 1;
+    auto held_by = [&](int page) { return page >= 0 && page <= last && page < a.pb.width ? paged_page(a.pb, b, page << shift) : -1; };
+    int n = 0, my_id = -1, my_first = 0;
+    if constexpr (SOLO) {
+      my_id = held_by(chosen);
+      my_first = my_id >= 0 ? chosen << shift : 0;
+      const uint64_t held = __builtin_amdgcn_ballot_w64(my_id >= 0);
+      n = held ? 64 - __builtin_clzll(held) : 0;
+    } else {
+      for (int i = tid; i < a.top + 4; i += PA_THREADS) {
+        const int page = i < PA_THREADS ? chosen : i < a.top ? sel[i] : -1, held = held_by(page);
+        sm.list[i] = make_int2(held, held >= 0 ? page << shift : 0);
+        if (held >= 0) n = i + 1;
+      }
+      for (int d = 32; d > 0; d >>= 1) n = max(n, __shfl_xor(n, d));
+      if (lane == 0) sm.most[wave] = n;
+      lds_barrier();
+      n = max(max(sm.most[0], sm.most[1]), max(sm.most[2], sm.most[3]));
     }
-    for (int d = 32; d > 0; d >>= 1) n = max(n, __shfl_xor(n, d));
-    if (lane == 0) sm.most[wave] = n;
-    lds_barrier();
-    n = max(max(sm.most[0], sm.most[1]), max(sm.most[2], sm.most[3]));
-    const int steps = ((n << shift) + KEYS - 1) / KEYS, per = (steps + a.parts - 1) / a.parts, st_lo = min(part * per, steps), st_end = min(st_lo + per, steps);
+    const int steps = ((n << shift) + KEYS - 1) / KEYS, per = SOLO ? steps : (steps + a.parts - 1) / a.parts, st_lo = SOLO ? 0 : min(part * per, steps), st_end = min(st_lo + per, steps);
 
     struct Step {
       int id[4], key[4];                                     // of the four groups: page, first position
@@ -466,13 +515,18 @@ template <int HD, bool I8, int A> struct SelectedRow {
     auto find = [&](int st, Step &to) {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int at = st * KEYS + 16 * j;
-        const int2 e = sm.list[min(at >> shift, a.top)];     // behind the last: none
-        to.id[j] = st < st_end ? __builtin_amdgcn_readfirstlane(e.x) : -1;
-        to.key[j] = __builtin_amdgcn_readfirstlane(e.y) + (at & ((1 << shift) - 1));
+        const int at = st * KEYS + 16 * j, i = at >> shift;
+        if constexpr (SOLO) {
+          to.id[j] = i < 64 ? __builtin_amdgcn_readlane(my_id, i) : -1;
+          to.key[j] = (i < 64 ? __builtin_amdgcn_readlane(my_first, i) : 0) + (at & ((1 << shift) - 1));
+        } else {
+          const int2 e = sm.list[min(i, a.top)];             // behind the last: none
+          to.id[j] = st < st_end ? __builtin_amdgcn_readfirstlane(e.x) : -1;
+          to.key[j] = __builtin_amdgcn_readfirstlane(e.y) + (at & ((1 << shift) - 1));
+        }
       }
     };
-    u4_t kr[4][GK], vr[4][GV];
+    u4_t kr[4][GV], vr[4][GV];
     f4_t ks[A], vs[A];                                       // of the keys that this lane keeps
     auto row_of = [&](const Step &to, int j) { return paged_row(a.pb, KV, max(to.id[j], 0), g, to.key[j]); };   // a missing page: page 0, masked
     auto mine = [&](auto v0, auto v1, auto v2, auto v3, int at) {   // of the four groups' values, that of this lane's accumulator `at`
@@ -481,26 +535,40 @@ template <int HD, bool I8, int A> struct SelectedRow {
       else return at == 0 ? v0 : at == 1 ? v1 : at == 2 ? v2 : v3;
     };
     // a group's rows lie side by side: a base that all lanes share, and a lane's place from there
-    constexpr int KROW = I8 ? HD : ROWB;
-    const uint32_t k_at = l16 * KROW + lq * 16, v_at = lane / LPR * KROW + lane % LPR * 16;
+    constexpr int HELD = I8 ? HD : ROWB;
+    const uint32_t lane_at = lane / LPR * HELD + lane % LPR * 16;
+    auto load_rows = [&](const void *pages, const Step &to, int j, u4_t (&r)[GV]) {
+      const JSG_GLOBAL unsigned char *const from = as_global<unsigned char>(pages) + row_of(to, j) * HELD;
+#pragma unroll
+      for (int c = 0; c < GV; c++) r[c] = *(const JSG_GLOBAL u4_t *)(from + (lane_at + c * (64 / LPR) * HELD));
+    };
+    auto store_rows = [&](const u4_t (&r)[GV], int h, int row_bytes) {   // 16 rows to LDS as halves, behind h * 16 others
+#pragma unroll
+      for (int c = 0; c < GV; c++) {
+        unsigned char *const to = sm.wave[wave].v + (16 * h + c * (64 / LPR) + lane / LPR) * row_bytes + lane % LPR * (I8 ? 32 : 16);
+        if constexpr (I8) {
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            uint32_t w[4];
+            i8x4_to_h2x2(r[c][2 * x], w[0], w[1]);
+            i8x4_to_h2x2(r[c][2 * x + 1], w[2], w[3]);
+            *(u4_t *)(to + x * 16) = u4_t{w[0], w[1], w[2], w[3]};
+          }
+        } else {
+          *(u4_t *)to = r[c];
+        }
+      }
+    };
     auto load_k = [&](const Step &to) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const JSG_GLOBAL unsigned char *const from = as_global<unsigned char>(a.pages_k) + row_of(to, j) * KROW;
-#pragma unroll
-        for (int c = 0; c < GK; c++) kr[j][c] = *(const JSG_GLOBAL u4_t *)(from + (k_at + c * 64));
-      }
+      for (int j = 0; j < 4; j++) load_rows(a.pages_k, to, j, kr[j]);
       if constexpr (I8)
 #pragma unroll
         for (int s = 0; s < A; s++) ks[s] = *as_global<f4_t>(a.scales_k + mine(row_of(to, 0), row_of(to, 1), row_of(to, 2), row_of(to, 3), s) + 4 * lq);
     };
     auto load_v = [&](const Step &to, int u) {               // groups 2 u and 2 u + 1
 #pragma unroll
-      for (int j = 2 * u; j < 2 * u + 2; j++) {
-        const JSG_GLOBAL unsigned char *const from = as_global<unsigned char>(a.pages_v) + row_of(to, j) * KROW;
-#pragma unroll
-        for (int c = 0; c < GV; c++) vr[j][c] = *(const JSG_GLOBAL u4_t *)(from + (v_at + c * (64 / LPR) * KROW));
-      }
+      for (int j = 2 * u; j < 2 * u + 2; j++) load_rows(a.pages_v, to, j, vr[j]);
     };
     auto load_vs = [&](const Step &to) {
       if constexpr (I8)
@@ -518,24 +586,19 @@ template <int HD, bool I8, int A> struct SelectedRow {
     // more: there is another step; careful: V may hold halves that are not finite
     auto step = [&](auto more, auto careful) {
       constexpr bool MORE = decltype(more)::value, CAREFUL = decltype(careful)::value;
-      find(st + NW, next);
+      find(st + ROW_WAVES, next);
       f4_t d[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        d[j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < 2; u++) {
+        store_rows(kr[2 * u], 0, KROW);
+        store_rows(kr[2 * u + 1], 1, KROW);
 #pragma unroll
-        for (int c = 0; c < GK; c++)
+        for (int h = 0; h < 2; h++) {
+          f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int u = 0; u < KS / GK; u++) {
-            u4_t k = kr[j][c];
-            if constexpr (I8) {
-              uint32_t w[4];
-              i8x4_to_h2x2(kr[j][c][2 * u], w[0], w[1]);
-              i8x4_to_h2x2(kr[j][c][2 * u + 1], w[2], w[3]);
-              k = u4_t{w[0], w[1], w[2], w[3]};
-            }
-            d[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, k), qf[c * (KS / GK) + u], d[j], 0, 0, 0);
-          }
+          for (int c = 0; c < KS; c++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const h8_t *)(vl + (16 * h + l16) * KROW + (4 * c + lq) * 16), qf[c], acc, 0, 0, 0);
+          d[2 * u + h] = acc;
+        }
       }
       f4_t s[A];
 #pragma unroll
@@ -625,24 +688,8 @@ template <int HD, bool I8, int A> struct SelectedRow {
       }
 #pragma unroll
       for (int u = 0; u < 2; u++) {                          // 32 keys: groups 2 u and 2 u + 1
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int c = 0; c < GV; c++) {
-            const int row = 16 * h + c * (64 / LPR) + lane / LPR, piece = lane % LPR;
-            const u4_t v = vr[2 * u + h][c];
-            if constexpr (I8) {
-#pragma unroll
-              for (int x = 0; x < 2; x++) {
-                uint32_t w[4];
-                i8x4_to_h2x2(v[2 * x], w[0], w[1]);
-                i8x4_to_h2x2(v[2 * x + 1], w[2], w[3]);
-                *(u4_t *)(vl + row * VROW + (2 * piece + x) * 16) = u4_t{w[0], w[1], w[2], w[3]};
-              }
-            } else {
-              *(u4_t *)(vl + row * VROW + piece * 16) = v;
-            }
-          }
+        store_rows(vr[2 * u], 0, VROW);
+        store_rows(vr[2 * u + 1], 1, VROW);
         if constexpr (MORE) {
           load_v(next, u);
           if (u == 1) load_vs(next);
@@ -699,7 +746,7 @@ template <int HD, bool I8, int A> struct SelectedRow {
       for (int t = 0; t < NT; t++) o[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
       m_run = -1e30f;                                        // finite: a step may hold no key that a column sees
       l_run = 0.0f;
-      st = st_lo + wave;
+      st = st_lo + (SOLO ? 0 : wave);
       find(st, at);
       if (st >= st_end) return;
       load_k(at);
@@ -707,7 +754,7 @@ template <int HD, bool I8, int A> struct SelectedRow {
       load_v(at, 1);
       load_vs(at);
       // the last step by itself: behind a branch around its loads every wait would be for all of them
-      for (; st + NW < st_end; st += NW) step(std::true_type(), careful);
+      for (; st + ROW_WAVES < st_end; st += ROW_WAVES) step(std::true_type(), careful);
       step(std::false_type(), careful);
     };
     walk(std::false_type());
@@ -727,21 +774,22 @@ template <int HD, bool I8, int A> struct SelectedRow {
 #pragma unroll
     for (int t = 0; t < NT; t++) *(f4_t *)&sm.wave[wave].o[l16 * OROW + t * 16 + 4 * lq] = o[t];
     if (lq == 0) { sm.m[wave][l16] = m_run; sm.l[wave][l16] = l_run; }
-    lds_barrier();
+    if constexpr (SOLO) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // of this wavefront, in order
+    else lds_barrier();
     constexpr int GROUPS = 4 / A;                            // columns of a head
     auto block_sum = [&](int h, int c, f4_t &sum, float &M, float &L) {   // features 4 c .. of head h
       M = -1e30f;
 #pragma unroll
-      for (int w = 0; w < NW; w++)
+      for (int w = 0; w < ROW_WAVES; w++)
 #pragma unroll
-        for (int j = 0; j < GROUPS; j++) M = fmaxf(M, sm.m[w][j * hp + h]);
+        for (int j = 0; j < GROUPS; j++) M = fmaxf(M, sm.m[SOLO ? wave : w][j * hp + h]);
       sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
       L = 0.0f;
 #pragma unroll
-      for (int w = 0; w < NW; w++)
+      for (int w0 = 0; w0 < ROW_WAVES; w0++)
 #pragma unroll
         for (int j = 0; j < GROUPS; j++) {
-          const int col = j * hp + h;
+          const int col = j * hp + h, w = SOLO ? wave : w0;
           const float e = __builtin_amdgcn_exp2f((sm.m[w][col] - M) * unit);
           L = __builtin_fmaf(sm.l[w][col], e, L);
           const f4_t v = *(const f4_t *)&sm.wave[w].o[col * OROW + 4 * c];
@@ -754,8 +802,8 @@ template <int HD, bool I8, int A> struct SelectedRow {
       *(uint2 *)(a.out + q_off + (size_t)h * HD + 4 * c) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
     };
     const int pieces = nr * (HD / 4);
-    if (a.parts == 1) {
-      for (int i = tid; i < pieces; i += PA_THREADS) {
+    if (SOLO || a.parts == 1) {
+      for (int i = tid; i < pieces; i += ROW_THREADS) {
         f4_t sum;
         float M, L;
         block_sum(i / (HD / 4), i % (HD / 4), sum, M, L);
@@ -763,6 +811,12 @@ template <int HD, bool I8, int A> struct SelectedRow {
       }
       return;
     }
+    if constexpr (!SOLO) join(a, r, g, qt, part, pieces, nr, unit, block_sum, put, sm);
+  }
+
+  template <typename Sum, typename Put>
+  static __device__ void join(const SelectedArgs &a, int r, int g, int qt, int part, int pieces, int nr, float unit, Sum block_sum, Put put, Smem &sm) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), KV = (int)a.n_kv_heads.d;
     // Parts: sums through memory at device scope (cache policy 16), counted once they are acknowledged; the last block of the row and heads folds them in order.
     const int slot = (r * a.q_tiles + qt) * a.parts * KV + g;
     const uint32_t part_bytes = (uint32_t)KV * SLOT * 4;
@@ -825,14 +879,25 @@ template <int HD, bool I8, int A> struct SelectedRow {
 };
 
 // Block numbers have the kv heads innermost: blocks are dealt to the eight XCDs in turn, so that with eight kv heads each XCD has one, all rows of which share its K and V in that L2.
-template <int HD, bool I8, int A> __global__ __launch_bounds__(PA_THREADS, HD == 64 ? (I8 || A > 1 ? 3 : 4) : 2) void attn_selected_kernel(SelectedArgs a) {
-  __shared__ typename SelectedRow<HD, I8, A>::Smem sm;
+template <int HD, bool I8, int A, bool SOLO> __global__ __launch_bounds__(PA_THREADS, HD == 64 ? (I8 || A > 1 ? 3 : 4) : 2) void attn_selected_kernel(SelectedArgs a) {
+  typedef SelectedRow<HD, I8, A, SOLO> Row;
+  __shared__ typename Row::Smem sm;
   const int id = blockIdx.x, KV = (int)a.n_kv_heads.d, rest = a.n_kv_heads.div(id), g = id - rest * KV;
-  const int part = rest % a.parts, tile = rest / a.parts, qt = tile % a.q_tiles, r = tile / a.q_tiles, b = paged_find(a.pb, r);
-  if (b >= a.pb.n_seqs) return;
-  const PagedSeq s = paged_seq(a.pb, b);
-  if (r < s.start) return;
-  SelectedRow<HD, I8, A>::run(a, r, g, qt, part, b, paged_pos(s, r - s.start), sm);
+  int part = 0, tile = rest;
+  if constexpr (SOLO) {
+    tile = rest * Row::NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  } else {
+    tile = rest / a.parts;
+    part = rest - tile * a.parts;
+  }
+  const int r = tile / a.q_tiles, qt = tile - r * a.q_tiles;
+  if (r >= a.pb.rows) return;
+  // the row's first pages are asked for beside its sequence
+  const int first = SOLO ? threadIdx.x & 63 : threadIdx.x, chosen = first < a.top ? a.selected[((size_t)r * KV + g) * a.top + first] : -1;
+  PagedSeq s;
+  const int b = find_row(a.pb, r, s);
+  if (b >= a.pb.n_seqs || r < s.start) return;
+  Row::run(a, r, g, qt, part, b, paged_pos(s, r - s.start), chosen, sm);
 }
 
 // Argument checks that the calls here share
@@ -865,7 +930,8 @@ int jsgrad_hip_paged_bounds(const jsgrad_hip_pages_t *host_pages, const int32_t 
   a.scales_k = (const float *)host_pages->scales_k;
   a.bounds = bounds; a.bound_scales = bound_scales;
   a.n_kv_heads = host_pages->n_kv_heads;
-  const dim3 grid((unsigned)rows, (unsigned)a.n_kv_heads), block(PS_THREADS);
+  // a sequence's rows begin and end inside pages
+  const dim3 grid((unsigned)(rows / host_pages->page_size + 2 * (n_seqs < rows ? n_seqs : rows)), (unsigned)a.n_kv_heads), block(PS_THREADS);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
   if (host_pages->head_dim == 64 && i8) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_bounds_kernel<64, true>), grid, block, 0, a);
   else if (host_pages->head_dim == 64) JSG_LAUNCH(PROF_PAGED_ROWS, (paged_bounds_kernel<64, false>), grid, block, 0, a);
@@ -958,19 +1024,26 @@ int jsgrad_hip_attn_selected(const jsgrad_hip_pages_t *host_pages, const int32_t
   parts = parts < steps / 4 ? parts : steps / 4;
   a.parts = parts > 1 ? parts : 1;
   JSG_READY();
-  const dim3 grid((unsigned)(items * a.parts)), block(PA_THREADS);
+  const bool solo = a.parts == 1 && top <= 64 && items >= 4096;
+  const dim3 grid((unsigned)(solo ? ((size_t)rows * a.q_tiles + 3) / 4 * KV : items * a.parts)), block(PA_THREADS);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
-#define JSG_SELECTED(HD, I8)                                                                                    \
-  do {                                                                                                          \
-    if (a.heads_log <= 2) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, 1>), grid, block, 0, a);      \
-    else if (a.heads_log == 3) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, 2>), grid, block, 0, a); \
-    else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, 4>), grid, block, 0, a);                       \
+#define JSG_SELECTED_A(HD, I8, A)                                                                            \
+  do {                                                                                                       \
+    if (solo) JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, A, true>), grid, block, 0, a);         \
+    else JSG_LAUNCH(PROF_ATTN_PAGED, (attn_selected_kernel<HD, I8, A, false>), grid, block, 0, a);             \
+  } while (0)
+#define JSG_SELECTED(HD, I8)                              \
+  do {                                                    \
+    if (a.heads_log <= 2) JSG_SELECTED_A(HD, I8, 1);        \
+    else if (a.heads_log == 3) JSG_SELECTED_A(HD, I8, 2);   \
+    else JSG_SELECTED_A(HD, I8, 4);                         \
   } while (0)
   if (HD == 64 && i8) JSG_SELECTED(64, true);
   else if (HD == 64) JSG_SELECTED(64, false);
   else if (i8) JSG_SELECTED(128, true);
   else JSG_SELECTED(128, false);
 #undef JSG_SELECTED
+#undef JSG_SELECTED_A
   return 0;
 }
 
