@@ -41,62 +41,80 @@ template <int LANES> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 // NORM: rows of k and q are RMSNorm'ed per head in front of the rotation, x / sqrt(mean x^2 + eps) * weight, all of it in float: the squares of a head are summed over the
 // lanes that hold it, so it costs no trip to memory beside that of the weights.
 template <int HD, bool I8, bool NORM> __global__ __launch_bounds__(PR_THREADS) void paged_write_kernel(PagedArgs a) {
-  constexpr int G = HD / 8;
-  const int r = blockIdx.x, KV = a.n_kv_heads, heads = 2 * KV + a.n_heads;
+  constexpr int G = HD / 8, U = NORM ? 3 : 1;                // pieces of a thread whose loads are on their way together
+  const int r = blockIdx.x, KV = a.n_kv_heads, heads = 2 * KV + a.n_heads, total = heads * G, e0 = threadIdx.x % G * 8;
+  h8_t x[U], weight[2];                                      // NORM: of k and of q
+  auto ask = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int h = min(i0 + u * PR_THREADS, total - 1) / G, which = h < KV ? 0 : h < 2 * KV ? 1 : 2, n = which == 2 ? a.n_heads : KV;
+      x[u] = *(const h8_t *)(a.x[which] + ((size_t)r * n + h - which * KV) * HD + e0);
+    }
+  };
+  if constexpr (NORM) {                                      // in front of the trips that find the row's place
+    ask(threadIdx.x);
+    weight[0] = *(const h8_t *)(a.norm[0] + e0);
+    weight[1] = *(const h8_t *)((a.n_heads ? a.norm[2] : a.norm[0]) + e0);
+  }
   const int b = paged_find(a.pb, r);
   if (b >= a.pb.n_seqs) return;
   const PagedSeq s = paged_seq(a.pb, b);
   const int pos = paged_pos(s, r - s.start);
   if (r < s.start || pos < 0 || pos >= paged_room(a.pb)) return;
   const int id = paged_page(a.pb, b, pos);
-  for (int i = threadIdx.x; i < heads * G; i += PR_THREADS) {        // heads * G is a multiple of G: the lanes of a head stay together
-    const int h = i / G, e0 = i % G * 8, which = h < KV ? 0 : h < 2 * KV ? 1 : 2, n = which == 2 ? a.n_heads : KV, g = h - which * KV;
-    const h8_t x = *(const h8_t *)(a.x[which] + ((size_t)r * n + g) * HD + e0);
-    float f[8];
+  for (int i0 = threadIdx.x; i0 < total; i0 += U * PR_THREADS) {
+    if (!NORM || i0 >= U * PR_THREADS) ask(i0);
 #pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = (float)x[e];
-    if constexpr (NORM) {
-      if (which != 1) {
-        const h8_t w = *(const h8_t *)(a.norm[which] + e0);
-        float sq = 0.0f;
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * PR_THREADS;                       // total is a multiple of G: the lanes of a head stay together
+      if (i >= total) break;
+      const int h = i / G, which = h < KV ? 0 : h < 2 * KV ? 1 : 2, n = which == 2 ? a.n_heads : KV, g = h - which * KV;
+      float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) sq = fmaf(f[e], f[e], sq);
-        sq = G == 8 ? row8_sum(sq) : row16_sum(sq);
-        const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fmul_rn(sq, 1.0f / HD), a.eps)));
+      for (int e = 0; e < 8; e++) f[e] = (float)x[u][e];
+      if constexpr (NORM) {
+        if (which != 1) {
+          const h8_t w = which == 0 ? weight[0] : weight[1];
+          float sq = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = f[e] * r * (float)w[e];
+          for (int e = 0; e < 8; e++) sq = fmaf(f[e], f[e], sq);
+          sq = G == 8 ? row8_sum(sq) : row16_sum(sq);
+          const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fmul_rn(sq, 1.0f / HD), a.eps)));
+#pragma unroll
+          for (int e = 0; e < 8; e++) f[e] = f[e] * r * (float)w[e];
+        }
       }
-    }
-    if (which != 1 && a.rope) {
-      const h8_t cs = *(const h8_t *)(a.rope + (size_t)pos * HD + e0);   // cos, sin of four pairs
+      if (which != 1 && a.rope) {
+        const h8_t cs = *(const h8_t *)(a.rope + (size_t)pos * HD + e0);   // cos, sin of four pairs
 #pragma unroll
-      for (int p = 0; p < 4; p++) {
-        const float ev = f[2 * p], od = f[2 * p + 1], c = (float)cs[2 * p], d = (float)cs[2 * p + 1];
-        f[2 * p] = ev * c - od * d;
-        f[2 * p + 1] = ev * d + od * c;
+        for (int p = 0; p < 4; p++) {
+          const float ev = f[2 * p], od = f[2 * p + 1], c = (float)cs[2 * p], d = (float)cs[2 * p + 1];
+          f[2 * p] = ev * c - od * d;
+          f[2 * p + 1] = ev * d + od * c;
+        }
       }
-    }
-    h8_t o;
+      h8_t o;
 #pragma unroll
-    for (int e = 0; e < 8; e++) o[e] = (_Float16)f[e];
-    if (which == 2) {
-      *(h8_t *)(a.y[2] + ((size_t)r * n + g) * HD + e0) = o;
-    } else if (id >= 0) {
-      const size_t row = paged_row(a.pb, KV, id, g, pos);
-      if constexpr (!I8) {
-        *(h8_t *)((_Float16 *)a.pages[which] + row * HD + e0) = o;
-      } else {
-        uint32_t top = 0;                                     // as bits: what is not a number is above infinity, and that above everything else
+      for (int e = 0; e < 8; e++) o[e] = (_Float16)f[e];
+      if (which == 2) {
+        *(h8_t *)(a.y[2] + ((size_t)r * n + g) * HD + e0) = o;
+      } else if (id >= 0) {
+        const size_t row = paged_row(a.pb, KV, id, g, pos);
+        if constexpr (!I8) {
+          *(h8_t *)((_Float16 *)a.pages[which] + row * HD + e0) = o;
+        } else {
+          uint32_t top = 0;                                     // as bits: what is not a number is above infinity, and that above everything else
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-        top = group_max<G>(top);
-        const bool finite = top < 0x7f800000u;
-        const float amax = __uint_as_float(top), scale = top == 0 ? 1.0f : finite ? __fdiv_rn(amax, 127.0f) : NAN;
-        uint32_t c[2] = {0, 0};
+          for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+          top = group_max<G>(top);
+          const bool finite = top < 0x7f800000u;
+          const float amax = __uint_as_float(top), scale = top == 0 ? 1.0f : finite ? __fdiv_rn(amax, 127.0f) : NAN;
+          uint32_t c[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; e++) c[e / 4] |= (uint32_t)((finite ? (int)rintf(__fdiv_rn(f[e], scale)) : 0) & 255) << (e % 4 * 8);
-        *(uint2 *)((int8_t *)a.pages[which] + row * HD + e0) = make_uint2(c[0], c[1]);
-        if (e0 == 0) a.scales[which][row] = scale;
+          for (int e = 0; e < 8; e++) c[e / 4] |= (uint32_t)((finite ? (int)rintf(__fdiv_rn(f[e], scale)) : 0) & 255) << (e % 4 * 8);
+          *(uint2 *)((int8_t *)a.pages[which] + row * HD + e0) = make_uint2(c[0], c[1]);
+          if (e0 == 0) a.scales[which][row] = scale;
+        }
       }
     }
   }
