@@ -68,13 +68,43 @@ def choose(case, q, H, codes, scales, first, recent, top, before):
     return out
 
 
-def attention(case, q, H, selected):
-    """(result, bound) as tests.paged_ref.attention has them, over the positions of the chosen pages."""
+def choose_many(case, q, H, codes, scales, first, recent, top, before):
+    """choose() for many rows at once, each sequence's as one array."""
+    out, rep = before.copy(), H // case.KV
+    for b, (n, l) in enumerate(zip(case.news, case.lens)):
+        if not n:
+            continue
+        rows, cols = slice(case.starts[b], case.starts[b] + n), np.arange(case.table.shape[1])
+        last = np.arange(l - n, l) // case.page
+        ids, _ = case.places(b, 0, cols.size * case.page)
+        ids = ids[::case.page]
+        for g in range(case.KV):
+            x = q[rows, g * rep:(g + 1) * rep].astype(np.float64)
+            top_of = np.abs(x).max((1, 2))
+            fine = np.isfinite(top_of)
+            c = np.where(fine[:, None, None], np.rint(x / step(np.where(fine, top_of, 0))[:, None, None]), 0.0)
+            lo, hi = (codes[np.maximum(ids, 0), g, i].astype(np.float64) for i in range(2))
+            scale = scales[np.maximum(ids, 0), g].astype(np.float64)
+            always = (cols < first) | (cols > last[:, None] - recent)
+            with np.errstate(invalid="ignore"):
+                score = (np.maximum(c, 0) @ hi.T + np.minimum(c, 0) @ lo.T).max(1) * scale
+            rank = np.where(always, 0, np.where(np.isinf(scale), 1, 2))
+            score = np.where(rank == 2, score, 0.0)
+            rank = np.where((ids < 0) | (cols > last[:, None]), 3, rank)
+            order = np.lexsort((np.broadcast_to(cols, rank.shape), -score, rank))[:, :top]
+            mine = np.sort(np.where(np.take_along_axis(rank, order, 1) < 3, order, 1 << 30), 1)
+            out[rows, g] = -1
+            out[rows, g, :mine.shape[1]] = np.where(mine < 1 << 30, mine, -1)
+    return out
+
+
+def attention(case, q, H, selected, every=1):
+    """(result, bound) as tests.paged_ref.attention has them, over the positions of the chosen pages; of each `every`-th row of a sequence alone, where that is more than 1."""
     k, v = case.values("k"), case.values("v")
     out, tol = np.zeros((case.rows, H, case.hd)), np.zeros((case.rows, H, case.hd))
     rep = H // case.KV
     for b, (n, l) in enumerate(zip(case.news, case.lens)):
-        for i in range(n):
+        for i in range(0, n, every):
             p, r = l - n + i, case.starts[b] + i
             for g in range(case.KV):
                 j = np.concatenate([np.arange(c * case.page, (c + 1) * case.page) for c in selected[r, g] if 0 <= c < case.table.shape[1]] + [np.zeros(0, int)]).astype(int)

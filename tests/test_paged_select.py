@@ -46,3 +46,18 @@ def test_references_against_each_other():
     for most, want in ((127.0, 1.0), (127.0625, 2.0), (128.0, 2.0), (63.5, 0.5), (0.0, 1.0), (6e-8, 2.0 ** -30), (65504.0, 1024.0), (1e-42, 2.0 ** -126)):
         assert step(most) == want
         assert most == 0 or want == 2.0 ** -126 or np.float64(127) * want >= most > 127 * want / 2
+
+
+def test_the_choice_for_many_rows_at_once():
+    from tests import select_ref as ref
+    from tests.paged_ref import Case
+    rng = np.random.default_rng(0)
+    c = Case(rng, "float16", 64, 2, 16, [60, 0, 7], [300, 5, 7])
+    c.table[0, 4] = -1
+    codes, scales = ref.bounds(c, np.zeros((c.n_pages, 2, 2, 64), np.int8), np.ones((c.n_pages, 2), np.float32))
+    scales[c.table[0, 16]] = np.inf
+    q = rng.standard_normal((67, 8, 64)).astype(np.float16)
+    q[3, 2, 1], q[4] = np.nan, 0
+    for top in (3, 30):
+        before = np.full((67, 2, top), 77, np.int32)
+        assert np.array_equal(ref.choose(c, q, 8, codes, scales, 1, 2, top, before), ref.choose_many(c, q, 8, codes, scales, 1, 2, top, before))
