@@ -21,6 +21,9 @@ constexpr int SR_FINE = 256, SR_STEP = 32, SR_STEPS = 345, SR_STEPS_UP = 352, SR
 constexpr int SR_FEW = 256, SR_HELD = 256;                   // a top_k that goes by candidates, and how many of these a part may have
 constexpr int SR_GROUPS = 2048, SR_LIST = 2048;              // groups whose maxima say where candidates begin; candidates of a row
 constexpr int SR_ROOM = 8192;                                // entries of a step that are listed
+// A call's parts are as short as leaves it at most SR_BLOCKS of them: two a CU.  With 1024, whose joins are longer, 16 rows of 128256 took 29 us
+// with top_k = 200, 56 with top_k = 1000 and top_p = 0.9 and 45 with top_p = 0.95 alone; with 512 they take 27, 52 and 43.
+constexpr size_t SR_BLOCKS = 512;
 
 struct SampleRowsArgs {
   const void *logits;
@@ -858,7 +861,7 @@ template <typename AT, bool VEC> __global__ __launch_bounds__(SR_THREADS) void s
 // Entries of a part: enough blocks for the chip where there are few rows, fewer and longer parts where there are many.
 static int sample_part(int rows, int n) {
   for (int g = 1; g < 4; g *= 2)
-    if ((size_t)rows * ((n + SR_PART * g - 1) / (SR_PART * g)) <= 1024) return SR_PART * g;
+    if ((size_t)rows * ((n + SR_PART * g - 1) / (SR_PART * g)) <= SR_BLOCKS) return SR_PART * g;
   return SR_PART * 4;
 }
 
@@ -870,9 +873,9 @@ extern "C" {
 
 size_t jsgrad_hip_sample_rows_workspace_bytes(int rows, int n) {
   if (rows <= 0 || n <= 0 || n > SR_MOST) return 0;
-  // of all numbers of rows up to this: fewer rows have shorter parts, up to 1024 of them
+  // of all numbers of rows up to this: fewer rows have shorter parts, up to SR_BLOCKS of them
   const size_t longest = (size_t)rows * ((n + 4 * SR_PART - 1) / (4 * SR_PART)), shortest = (size_t)rows * ((n + SR_PART - 1) / SR_PART);
-  return (size_t)rows * sizeof(SampleFound) + sizeof(SamplePart) * (shortest < 1024 ? shortest : longest < 1024 ? 1024 : longest);
+  return (size_t)rows * sizeof(SampleFound) + sizeof(SamplePart) * (shortest < SR_BLOCKS ? shortest : longest < SR_BLOCKS ? SR_BLOCKS : longest);
 }
 
 int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
