@@ -79,7 +79,7 @@ __device__ __forceinline__ int find_touched(const PagedBatch &pb, uint32_t t, Pa
 }
 
 // Block = (page that the batch's rows are on, kv head): the whole page is looked at, so bounds do not depend on how its rows came.  Bound by memory: HD / 8 lanes a row, 16 bytes (int8: 8) each.
-// (A block for every row, most of which have nothing to do: 2048 rows, heads of 64, 27 us.)
+// One row behind 33000 positions takes 4.5 us, 16 of 16 sequences 4.5, most of it a launch; 2048 rows on 32 pages 5.4.  (A block for every row, most of which have nothing to do: 27.)
 template <int HD, bool I8> __global__ __launch_bounds__(PS_THREADS) void paged_bounds_kernel(PagedSelectArgs a) {
   constexpr int G = HD / 8, RPB = PS_THREADS / G;
   __shared__ float lo_sh[PS_THREADS / 64][HD], hi_sh[PS_THREADS / 64][HD];
@@ -165,7 +165,7 @@ template <typename Op> __device__ __forceinline__ uint32_t wave_all(uint32_t v, 
   auto row = [&](int r) { return (uint32_t)__builtin_amdgcn_readlane((int)v, r * 16); };
   return op(op(row(0), row(1)), op(row(2), row(3)));
 }
-// The first `top` of n keys in the order (key descending, index ascending), those above 0, written as rising indexes with -1 behind.  By one wavefront, or (NW > 1) by a block of NW, each with a stretch of
+// The first `top` of n keys in the order (key descending, index ascending), those above 0, written as rising indexes with -1 behind.  By one wavefront, or by a block of NW, each with a stretch of
 // the keys.  What lies between the least and the largest is counted in 256 parts, then the part with the border in 256 again, until a part is wanted whole or its keys are all alike: two or
 // three turns, four at most.  (Halving a threshold takes some 15: 33000 positions in pages of 64, 4.3 us of them.)
 template <int NW> struct KeyChoice {
@@ -288,10 +288,12 @@ template <int NW> struct KeyChoice {
 };
 
 // Block = some rows of a sequence, side by side, and a kv head.  Scores on the matrix cores: 16 pages' bounds against 16 columns of queries, the heads of a row next to each other, so that a lane has
-// four columns' scores of its page.  Bound by what waits for what: batch, page numbers, bounds, then the turns of the choice.  (us, 33000 positions, pages of 64, 32 heads of 128 over 8, a page to
-// a thread with dot products and 32 turns through LDS 22; 16 rows of up to 32768, pages of 32, 30; 2048 rows behind 14336, heads of 64, 138.)
+// four columns' scores of its page.  Few rows are bound by what waits for what: batch, page numbers, bounds, then the turns of the choice; many by the vector unit, which makes keys of scores and counts them.
+// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 10.5; 16 rows of up to 32768, pages of 32: 14; 2048 rows behind 14336, heads of 64: 34.  (A page to a thread with dot products and 32 turns
+// through LDS: 22, 30 and 138.  Blocks of eight wavefronts where rows are one to a sequence: 11.5 and 15, 64 sequences of 8192 positions 16 instead of 8.)
 // HT tiles of 16 columns: of more heads of the rows (HEADS), or of more rows, for which the bounds are loaded once.
-template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, NW == 8 || HT == 1 ? 2 : HD == 64 && !HEADS ? 3 : 2) void paged_select_kernel(PagedSelectArgs a) {
+template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2) void paged_select_kernel(PagedSelectArgs a) {
+  constexpr int NW = PS_THREADS / 64;
   extern __shared__ __align__(16) uint32_t keys[];           // [rows of a block][stride]
   __shared__ union {
     KeyChoice<NW> block;
@@ -309,7 +311,7 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
     if (r0 < s.start) { r0++; continue; }                    // no sequence has it
     const int p0 = paged_pos(s, r0 - s.start), last_page = p0 + n_rows - 1 < 0 ? -1 : (p0 + n_rows - 1) >> shift, n = min(last_page + 1, a.pb.width);
     // U tiles at a time: their page numbers in one trip to memory, asked for ahead, their bounds in the next.  The numbers without a branch: behind one, each would be waited for.
-    constexpr int U = HT > 1 ? 2 : NW == 8 ? 8 : 4;
+    constexpr int U = HT > 1 ? 2 : 4;
     const int32_t *const table = a.pb.table + (size_t)b * a.pb.width;
     int id[U];
     auto pages_of = [&](int t0) {
@@ -431,6 +433,10 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
 // rows, a wavefront to each, which neither wait for one another nor start anew every few steps.  A step is 64 keys: rows of K and V
 // come through registers into the wavefront's own LDS, 32 at a time, V's for the transposing reads; the next step's rows are asked for as soon as the registers are free.  K straight to registers, as the
 // matrix operand has it, would put the lanes of a quarter on different rows, and the L1 cache would be asked 64 times for what it gives in 16: 2048 rows, heads of 64, 305 us.
+//
+// us, 32 heads over 8: one row, 32 pages of 64, heads of 128, 9.6, of which 4 go by until the first keys are there and 4 in the join of the parts; 16 rows, 64 int8 pages of 32, heads of 128, 21: memory, 4 TB/s and start
+// and join; 2048 rows, 16 pages of 64, heads of 64, 195: every row gathers 2 MB of its own, 4.3 GB in all, at 64 % of what L1 gives and as much of LDS's rate (each byte goes in once and out once), 20 TB/s of it
+// from L2, with the vector unit at 32 %.
 //
 // A matrix instruction scores 16 keys for 16 columns, and a row has few heads: with four, three columns of four would score the same again, and the vector unit would make the exponentials of
 // all.  So the columns are heads times groups of keys: column c of what a lane keeps has head c % HP over the keys of group c / HP of the step's four, each picked from that group's scores
@@ -960,30 +966,25 @@ int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t 
   a.selected = selected;
   while ((1 << a.heads_log) < (n_rep < 16 ? n_rep : 16)) a.heads_log++;
   a.stride = (host_pages->table_width + 15) & ~15;
-  // Rows of a sequence share its bounds; where rows are one to a sequence, a block of eight wavefronts is done sooner with one.
+  // Rows of a sequence share its bounds: the columns of a matrix instruction are theirs, and with heads of 128 four such tiles where enough blocks are left.  us, one tile | four, 32 heads of 128 over
+  // 8: 1024 rows behind 15360 27 | 20, 2048 behind 14336 48 | 37, 2048 behind 2048 29 | 28, 700 behind 9000 16.5 | 18, 128 behind 16256 7.4 | 15.  Heads of 64, whose bounds are half as long:
+  // 2048 behind 14336 31 | 29, behind 2048 21 | 23, 4096 from the start 35 | 38.
   const bool many = n_rep > 16;
-  int tile = 16 >> a.heads_log, tiles = 1;
-  if (!many && rows >= 8 * tile * n_seqs && (size_t)rows * a.n_kv_heads >= (size_t)tile * 4096 && (size_t)tile * 4 * a.stride * 4 <= 64 * 1024) tiles = 4;
-  a.tile = rows > n_seqs && (size_t)tile * tiles * a.stride * 4 <= 64 * 1024 ? tile * tiles : 1;
-  const bool wide = a.tile == 1 && (size_t)rows * a.n_kv_heads <= 1024;
+  const int tile = 16 >> a.heads_log;
+  const bool four = HD == 128 && !many && (size_t)rows >= (size_t)8 * tile * n_seqs && (size_t)rows * a.n_kv_heads >= (size_t)tile * 2048 && (size_t)tile * 4 * a.stride * 4 <= 64 * 1024;
+  a.tile = rows > n_seqs && (size_t)tile * a.stride * 4 <= 64 * 1024 ? tile * (four ? 4 : 1) : 1;
   const dim3 grid((unsigned)((rows + a.tile - 1) / a.tile), (unsigned)a.n_kv_heads);
   const size_t lds = (size_t)a.tile * a.stride * 4;
-#define JSG_SELECT(HD, NW, HT, HEADS)                                                                                                                                        \
-  do {                                                                                                                                                                        \
-    if (lds > 48 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<HD, NW, HT, HEADS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));              \
-    JSG_LAUNCH(PROF_ATTN_PAGED, (paged_select_kernel<HD, NW, HT, HEADS>), grid, dim3(NW * 64), lds, a);                                                                          \
+#define JSG_SELECT(HD, HT, HEADS)                                                                                                                                    \
+  do {                                                                                                                                                                \
+    if (lds > 48 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<HD, HT, HEADS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));          \
+    JSG_LAUNCH(PROF_ATTN_PAGED, (paged_select_kernel<HD, HT, HEADS>), grid, dim3(PS_THREADS), lds, a);                                                                   \
   } while (0)
-#define JSG_SELECT_HD(HD)                                \
-  do {                                                   \
-    if (many && wide) JSG_SELECT(HD, 8, 4, true);          \
-    else if (many) JSG_SELECT(HD, 4, 4, true);             \
-    else if (wide) JSG_SELECT(HD, 8, 1, false);            \
-    else if (tiles > 1) JSG_SELECT(HD, 4, 4, false);       \
-    else JSG_SELECT(HD, 4, 1, false);                      \
-  } while (0)
-  if (HD == 64) JSG_SELECT_HD(64);
-  else JSG_SELECT_HD(128);
-#undef JSG_SELECT_HD
+  if (HD == 64 && many) JSG_SELECT(64, 4, true);
+  else if (HD == 64) JSG_SELECT(64, 1, false);
+  else if (many) JSG_SELECT(128, 4, true);
+  else if (a.tile > tile) JSG_SELECT(128, 4, false);
+  else JSG_SELECT(128, 1, false);
 #undef JSG_SELECT
   return 0;
 }
@@ -1017,14 +1018,17 @@ int jsgrad_hip_attn_selected(const jsgrad_hip_pages_t *host_pages, const int32_t
   a.q_tiles = (n_rep + PA_QROWS - 1) / PA_QROWS;
   const size_t items = (size_t)rows * a.q_tiles * KV;
   JSG_REQUIRE(items < (size_t)PAGED_GRID, "%s: %d rows of %d heads", who, rows, n_heads);
-  // parts of a row where there are few: two blocks to a unit, each wavefront with two steps at least
+  // Parts of a row where there are few: two blocks to a unit, each wavefront with one step at least.  us, 256 | 512 | 1024 blocks: one row, 32 pages of 64, 9.3 | 9.5 | 9.4; 16 rows of 64 pages fp16 44 | 46 | 47, int8 31 | 31 | -;
+  // with 128 these take 9.4, 44 and 48.
   const int steps = (int)(((size_t)(top < a.pb.width ? top : a.pb.width) << a.pb.page_shift) / 64);
   int parts = items * 2 <= PA_BLOCKS ? (int)(PA_BLOCKS / items) : 1;
   parts = parts < PA_MOST ? parts : PA_MOST;
   parts = parts < steps / 4 ? parts : steps / 4;
   a.parts = parts > 1 ? parts : 1;
   JSG_READY();
-  const bool solo = a.parts == 1 && top <= 64 && items >= 4096;
+  // A row to a wavefront where each has one and the chip is full.  us, a row to a block | to a wavefront, 16 pages of 64 for each of n rows, 32 heads over 8: heads of 64 fp16 n = 128 18 | 24, 256 32 | 32, 512
+  // 58 | 52, 1024 110 | 96, int8 256 37 | 41, 512 69 | 63; heads of 128 fp16 128 33 | 35, 256 61 | 54, 1024 228 | 193, int8 256 74 | 67, 1024 280 | 238.
+  const bool solo = a.parts == 1 && top <= 64 && items * HD >= (size_t)4096 * 64;
   const dim3 grid((unsigned)(solo ? ((size_t)rows * a.q_tiles + 3) / 4 * KV : items * a.parts)), block(PA_THREADS);
   const bool i8 = host_pages->kind == JSGRAD_W_I8;
 #define JSG_SELECTED_A(HD, I8, A)                                                                            \

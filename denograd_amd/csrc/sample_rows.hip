@@ -6,6 +6,11 @@
 // Which entry a sum ends at is a question of borders: with float sums, off by 1e-7, one draw in a hundred over a flat vocabulary would fall to a neighbour.  So a weight is
 // made in 64 bits and held as a whole number of 2^-42: sums of up to 2^20 of them are exact and come out alike in any order, and the borders p Z and u Z are
 // multiplied out in full.  What the rounding to 2^-42 leaves is a chance of some 1e-10 to land on another side than real numbers would.
+//
+// Three launches, as the maximum has to be known before a weight is, and masses before a border: maxima of parts of the rows; per part the candidates of the first top_k (k up to SR_FEW), or its mass by steps
+// of an eighth of an octave below the maximum; one block a row for what lies on the step with a border.  One row of 128256 halves 18 us: 3.6, 6.3 and 8.5, launches and trips that wait for each other.  Sixteen
+// rows with settings of their own 47 to 53, of which 41 are the last block of a row with top_k = 1000 and top_p: 13 for each border.  256 rows with top_p = 0.95 (66 MB) 83: 14 (4.7 TB/s), 39 (33 million
+// weights in 64 bits; histograms in several copies change nothing) and 34.
 #include "common.h"
 #include "sample_rows.h"
 

@@ -8,7 +8,7 @@ from tests.test_gpu_paged_select import arrays, everything, run_attend, run_boun
 
 pytestmark = pytest.mark.gpu
 
-BATCHES = [  # kind, hd, H, KV, page, new rows, lengths, first, recent, top; the choice has tiles of 16 / (H / KV) rows and takes four at a time from 4096 tiles over the kv heads on
+BATCHES = [  # kind, hd, H, KV, page, new rows, lengths, first, recent, top; the choice has tiles of 16 / (H / KV) rows, and with heads of 128 takes four of them at a time
     ("float16", 64, 32, 8, 16, [1500, 0, 33, 567], [2000, 100, 33, 5000], 1, 2, 12), ("int8", 128, 16, 2, 64, [4023, 77], [4023, 4999], 1, 1, 5),
     ("float16", 128, 16, 1, 32, [3001, 1100], [3001, 1900], 0, 1, 9), ("int8", 64, 6, 2, 16, [8201], [8300], 2, 3, 20), ("float16", 128, 16, 8, 256, [4099], [4200], 0, 1, 3),
     ("float16", 64, 16, 16, 128, [4001, 1, 95], [4001, 700, 800], 1, 1, 4), ("int8", 128, 20, 1, 16, [2050], [2100], 1, 1, 17), ("float16", 64, 40, 1, 16, [1400], [1500], 1, 1, 7),
