@@ -347,7 +347,8 @@ class Llama3:
             raise ValueError(f"window {window}, sinks {sinks}, page_size {page_size}")
         if samples < 1:
             raise ValueError(f"{samples} answers to a prompt")
-        sampler = RowSampler(temperature, top_k, top_p, min_p, seed, self.device) if temperature >= 1e-6 else None
+        sampler = RowSampler(temperature, top_k, top_p, min_p, seed, self.device)
+        sampler = sampler if temperature >= 1e-6 else None
         sizes = np.repeat([p.size for p in prompts], samples)
         n_pages = PagedCache.pages_for(sizes, n_new, page_size, window, sinks)
         if samples > 1 and not window:                        # whole pages of a prompt are there once

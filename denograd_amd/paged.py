@@ -329,19 +329,20 @@ class PagedBatch:
         check(ffi.load().jsgrad_hip_attn_paged(*self._args(layer), q.ptr, out.ptr, n_heads, window, sinks, self.cache.workspace(n_heads).ptr))
         return out
 
-    def choose(self, layer: int, q: Tensor, n_heads: int, first: int, recent: int, top: int) -> Tensor:
+    def choose(self, layer: int, q: Tensor, n_heads: int, first: int, recent: int, top: int, out: Tensor | None = None) -> Tensor:
         """The pages of each row of q [rows, n_heads, head_dim] per kv head, by the bounds of their keys: int32 [rows, n_kv_heads, top], rising, -1 behind the last.  The first `first` and the last `recent` ones,
         the row's own among them, and of the others those on which its queries may score most."""
         self._check("q", q, n_heads)
         c = self.cache
         if not c.bounds:
             raise ValueError("pages are chosen by their bounds: a cache with bounds=True is wanted")
-        n = self.rows * c.n_kv_heads * max(top, 1)
-        if c._chosen is None or c._chosen.numel < n:
-            c._chosen = Tensor.empty((n,), "int32", c.device)
+        shape = (self.rows, c.n_kv_heads, top)
+        out = out if out is not None else Tensor.empty((self.rows, c.n_kv_heads, max(top, 1)), "int32", c.device)
+        if out.dtype != "int32" or out.numel < prod(shape):
+            raise ValueError(f"out: int32 {shape} are wanted, got {out.dtype} {out.shape}")
         codes, scales = c.bounds[layer]
-        check(ffi.load().jsgrad_hip_paged_select(*self._args(layer), q.ptr, n_heads, codes.ptr, scales.ptr, first, recent, top, c._chosen.ptr))
-        return Tensor(buffer=c._chosen.lazydata.view(n, "int32", 0), shape=(self.rows, c.n_kv_heads, top), dtype="int32", device=c.device)
+        check(ffi.load().jsgrad_hip_paged_select(*self._args(layer), q.ptr, n_heads, codes.ptr, scales.ptr, first, recent, top, out.ptr))
+        return out if out.shape == shape else Tensor(buffer=out.lazydata.view(prod(shape), "int32", 0), shape=shape, dtype="int32", device=c.device)
 
     def attend_pages(self, layer: int, q: Tensor, n_heads: int, chosen: Tensor, out: Tensor | None = None) -> Tensor:
         """Attention of q [rows, n_heads, head_dim] over the positions up to a row's own on the pages in chosen [rows, n_kv_heads, any number]."""
@@ -355,5 +356,8 @@ class PagedBatch:
         return out
 
     def attend_chosen(self, layer: int, q: Tensor, n_heads: int, first: int, recent: int, top: int, out: Tensor | None = None) -> Tensor:
-        """Attention over the pages that `choose` names."""
-        return self.attend_pages(layer, q, n_heads, self.choose(layer, q, n_heads, first, recent, top), out)
+        """Attention over the pages that `choose` names, in a list that the cache keeps for every layer and batch."""
+        c, n = self.cache, self.rows * self.cache.n_kv_heads * max(top, 1)
+        if c._chosen is None or c._chosen.numel < n:
+            c._chosen = Tensor.empty((n,), "int32", c.device)
+        return self.attend_pages(layer, q, n_heads, self.choose(layer, q, n_heads, first, recent, top, c._chosen), out)

@@ -322,6 +322,7 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
                           int n_heads, int window, int sinks, void *workspace);
 
 /* Attention over the pages that each row chooses, for contexts too long to look at whole (no counterpart in the reference): a step calls _paged_write, _paged_bounds, _paged_select and _attn_selected.
+ * Which rows these work on where row_starts fall is not promised.
  *
  * _paged_bounds: the bounds of every page that the batch's rows are on, of all the positions that its sequence has there: bounds int8 [n_pages][n_kv_heads][2][head_dim], 16-byte aligned, and bound_scales float
  * [n_pages][n_kv_heads], a pool that belongs to the layer's K pool.  scale = the smallest power of two, 2^-126 and more, that 127 times is max |k| and more (1 for zeros), bounds[0] = floor(min k / scale), bounds[1] =
