@@ -111,8 +111,13 @@ template <int HD, bool I8, bool NORM> __global__ __launch_bounds__(PR_THREADS) v
           const bool finite = top < 0x7f800000u;
           const float amax = __uint_as_float(top), scale = top == 0 ? 1.0f : finite ? __fdiv_rn(amax, 127.0f) : NAN;
           uint32_t c[2] = {0, 0};
+          // NORM: 127 x / max |x| in 64 bits.  Where x is half the maximum, as in one row of forty of halves, that is 63.5, and the float quotient by a float scale falls to either side of it.
+          const double per = NORM && finite && top ? 127.0 / (double)amax : 0.0;
 #pragma unroll
-          for (int e = 0; e < 8; e++) c[e / 4] |= (uint32_t)((finite ? (int)rintf(__fdiv_rn(f[e], scale)) : 0) & 255) << (e % 4 * 8);
+          for (int e = 0; e < 8; e++) {
+            const int code = NORM ? (int)rint((double)f[e] * per) : finite ? (int)rintf(__fdiv_rn(f[e], scale)) : 0;
+            c[e / 4] |= (uint32_t)((finite ? code : 0) & 255) << (e % 4 * 8);
+          }
           *(uint2 *)((int8_t *)a.pages[which] + row * HD + e0) = make_uint2(c[0], c[1]);
           if (e0 == 0) a.scales[which][row] = scale;
         }

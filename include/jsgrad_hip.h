@@ -290,7 +290,7 @@ int jsgrad_hip_paged_write(const jsgrad_hip_pages_t *host_pages, const int32_t *
                            const void *k, const void *v, const void *rope_table, int rope_rows, void *q_out, int n_heads);
 
 /* jsgrad_hip_paged_write behind an RMSNorm of every head's row of q and k (RMSNorm.call, nn/index.ts:586-588, over head_dim; models that norm queries and keys have no counterpart in
- * the reference): x / sqrt(mean x^2 + eps) * weight, in float like the rotation that follows, rounded once.  q_weight, k_weight: float16 [head_dim], 16-byte aligned; q_weight NULL where q is.
+ * the reference): x / sqrt(mean x^2 + eps) * weight, in float like the rotation that follows, rounded once; codes of int8 pages are the whole numbers nearest to 127 x / max |x|.  q_weight, k_weight: float16 [head_dim], 16-byte aligned; q_weight NULL where q is.
  * eps: 0 and more. */
 int jsgrad_hip_paged_write_norm(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, const void *k,
                                 const void *v, const void *q_weight, const void *k_weight, float eps, const void *rope_table, int rope_rows, void *q_out, int n_heads);

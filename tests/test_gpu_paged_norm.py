@@ -170,3 +170,20 @@ def test_a_checkpoint_with_norms_in_rotate_half_order(hip):
         assert np.array_equal(got, np.stack([w[:32], w[32:]], -1).reshape(-1))
     kept = convert_from_huggingface({"model.layers.0.self_attn.q_norm.weight": w}, 1, 4, 2, permute_layers=False)
     assert np.array_equal(kept["layers.0.attention.q_norm.weight"].numpy(), w)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_codes_are_the_nearest_whole_numbers(hip, hd):
+    """Of v, whose rows are not changed: to 127 x / max |x| in 64 bits (three roundings of 2^-53 there, of at most 127); halves have many quotients in the middle between two."""
+    rng = np.random.default_rng(hd)
+    c = Case(rng, "int8", hd, 8, 64, [2000], [2000]).device()
+    v = rng.standard_normal((2000, 8, hd)).astype(np.float16)
+    v[::3] = (v[::3] * 16).round() / 16                       # few values: ties in most rows
+    v[0, 0], v[1, 1] = 0, 6e-8
+    k, tv, w = Tensor(rng.standard_normal((2000, 8, hd)).astype(np.float16)), Tensor(v), Tensor(np.ones(hd, np.float16))
+    check(hip.jsgrad_hip_paged_write_norm(*c.batch, None, k.ptr, tv.ptr, None, w.ptr, EPS, None, 0, None, 0))
+    ids, slots = c.places(0, 0, 2000)
+    codes = c.t["v"].numpy()[ids, :, slots].astype(np.float64)
+    most = np.abs(v.astype(np.float64)).max(-1, keepdims=True)
+    exact = 127 * v.astype(np.float64) / np.where(most == 0, 1, most)
+    assert np.all(np.abs(codes - exact) <= 0.5 + 4 * 127 * 2.0 ** -53)
