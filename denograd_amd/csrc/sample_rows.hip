@@ -9,8 +9,10 @@
 //
 // Three launches, as the maximum has to be known before a weight is, and masses before a border: maxima of parts of the rows; per part the candidates of the first top_k (k up to SR_FEW), or its mass by steps
 // of an eighth of an octave below the maximum; one block a row for what lies on the step with a border.  One row of 128256 halves 18 us: 3.6, 6.3 and 8.5, launches and trips that wait for each other.  Sixteen
-// rows with settings of their own 47 to 53, of which 41 are the last block of a row with top_k = 1000 and top_p: 13 for each border.  256 rows with top_p = 0.95 (66 MB) 83: 14 (4.7 TB/s), 39 (33 million
-// weights in 64 bits; histograms in several copies change nothing) and 34.
+// rows with settings of their own 44, of which 32 are the last block of a row with top_k = 1000 and top_p: 8 to get the row from beyond the unit's L2 and look it over, 5 for the parts' sums, 3 for the draw
+// (52 with a look for each of the two borders).  256 rows with top_p = 0.95 (66 MB) 83: 14 (4.7 TB/s), 39 (33 million weights in 64 bits; histograms in several copies change nothing) and 34.
+#include <type_traits>
+
 #include "common.h"
 #include "sample_rows.h"
 
@@ -27,7 +29,7 @@ constexpr int SR_FEW = 256, SR_HELD = 256;                   // a top_k that goe
 constexpr int SR_GROUPS = 2048, SR_LIST = 2048;              // groups whose maxima say where candidates begin; candidates of a row
 constexpr int SR_ROOM = 8192;                                // entries of a step that are listed
 // A call's parts are as short as leaves it at most SR_BLOCKS of them: two a CU.  With 1024, whose joins are longer, 16 rows of 128256 took 29 us
-// with top_k = 200, 56 with top_k = 1000 and top_p = 0.9 and 45 with top_p = 0.95 alone; with 512 they take 27, 52 and 43.
+// with top_k = 200, 56 with top_k = 1000 and top_p = 0.9 and 45 with top_p = 0.95 alone; with 512 they took 27, 52 and 43.
 constexpr size_t SR_BLOCKS = 512;
 
 struct SampleRowsArgs {
@@ -633,11 +635,13 @@ template <typename AT, bool VEC> struct SampleLast {
     return true;
   }
 
-  int listed;                                                // the step whose entries `entries` goes over, and whether they are all in the list
+  int list_lo, list_hi;                                      // the steps whose entries were listed, and whether they are all in the list
   bool fits;
-  // f(entry, index) for all of the row that are on a step
-  template <typename F> __device__ __forceinline__ void on_step(int step, F f) {
-    const float from = sample_value(row.edge((step + 1) * SR_STEP)), to = step ? sample_value(row.edge(step * SR_STEP) - 1) : row.top;
+  __device__ float least_of(int step) const { return sample_value(row.edge((step + 1) * SR_STEP)); }
+  __device__ float most_of(int step) const { return step ? sample_value(row.edge(step * SR_STEP) - 1) : row.top; }
+  // f(entry, index) for all of the row that are on these steps
+  template <typename F> __device__ __forceinline__ void on_steps(int lo, int hi, F f) {
+    const float from = least_of(hi), to = most_of(lo);
     constexpr int U = sizeof(AT) == 2 ? 4 : 2;
     for (int i0 = threadIdx.x * 8; i0 < a.n; i0 += U * SR_THREADS * 8) {
       float v[U][8];
@@ -654,33 +658,42 @@ template <typename AT, bool VEC> struct SampleLast {
       }
     }
   }
-  template <typename F> __device__ __forceinline__ void entries(F f) {
-    if (!fits) return on_step(listed, f);
+  // Lists the entries of steps; between barriers.
+  __device__ void list(int lo, int hi) {
+    on_steps(lo, hi, [&](float v, int i) {
+      const int slot = atomicAdd(&l.n, 1);
+      if (slot < SR_ROOM) l.place[slot] = sample_place(v, i);
+    });
+    __syncthreads();
+    list_lo = lo;
+    list_hi = hi;
+    fits = l.n <= SR_ROOM;
+  }
+  // f(key, index, weight, depth) for all entries of a step, one of those listed
+  template <typename F> __device__ __forceinline__ void entries(int step, F f) {
+    auto take = [&](float v, int i) {
+      int d;
+      const uint64_t w = row.weight(v, table, d);
+      if (d / SR_STEP == step) f(sample_key(v), i, w, d);
+    };
+    if (!fits) return on_steps(step, step, take);
     for (int i = threadIdx.x; i < l.n; i += SR_THREADS) {
       const uint64_t p = l.place[i];
-      f(place_value(p), place_at(p));
+      take(place_value(p), place_at(p));
     }
   }
-  // The cut among the entries of a step that `within` keeps at which their counts (MASS: weights) reach `target`, 1 and more, and the weight up to it; false where too many are on one depth.
-  template <bool MASS> __device__ bool border(int step, uint64_t target, SampleCut within, SampleCut &cut, uint64_t &mass) {
+  // The cut among the entries of a step that `within` keeps at which their counts (MASS: weights) reach `target`, 1 and more, and the weight up to it; false where too many are on one depth.  Where the row has to be
+  // gone over for that, everything from the step `first` on is listed.
+  template <bool MASS> __device__ bool border(int step, int first, uint64_t target, SampleCut within, SampleCut &cut, uint64_t &mass) {
     const int tid = threadIdx.x, lane = tid & 63;
     __syncthreads();
     if (tid < SR_STEP) { l.fine_mass[tid] = 0; l.fine_count[tid] = 0; }
-    if (tid == 0) { l.n_near = 0; if (listed != step) l.n = 0; }
+    const bool again = step < list_lo || step > list_hi;
+    if (tid == 0) { l.n_near = 0; if (again) l.n = 0; }
     __syncthreads();
-    if (listed != step) {
-      on_step(step, [&](float v, int i) {
-        const int slot = atomicAdd(&l.n, 1);
-        if (slot < SR_ROOM) l.place[slot] = sample_place(v, i);
-      });
-      __syncthreads();
-      listed = step;
-      fits = l.n <= SR_ROOM;
-    }
-    entries([&](float v, int i) {
-      if (!within.keeps(sample_key(v), i)) return;
-      int d;
-      const uint64_t w = row.weight(v, table, d);
+    if (again) list(first, step);
+    entries(step, [&](uint32_t key, int i, uint64_t w, int d) {
+      if (!within.keeps(key, i)) return;
       atomicAdd((unsigned long long *)&l.fine_mass[(uint32_t)d % SR_STEP], (unsigned long long)w);
       atomicAdd(&l.fine_count[(uint32_t)d % SR_STEP], 1u);
     });
@@ -694,12 +707,10 @@ template <typename AT, bool VEC> struct SampleLast {
     auto at_on = [&](uint64_t v) { return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), on) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, on); };
     sum = at_on(sum - m);
     count = at_on(count - n);
-    entries([&](float v, int i) {
-      int d;
-      const uint64_t w = row.weight(v, table, d);
-      if ((int)((uint32_t)d % SR_STEP) != on || !within.keeps(sample_key(v), i)) return;
+    entries(step, [&](uint32_t key, int i, uint64_t w, int d) {
+      if ((int)((uint32_t)d % SR_STEP) != on || !within.keeps(key, i)) return;
       const int slot = atomicAdd(&l.n_near, 1);
-      if (slot < SR_LIST) { l.near[slot] = sample_place(v, i); l.near_w[slot] = w; }
+      if (slot < SR_LIST) { l.near[slot] = sample_place(sample_value(key), i); l.near_w[slot] = w; }
     });
     __syncthreads();
     if (l.n_near > SR_LIST) return false;
@@ -722,19 +733,35 @@ template <typename AT, bool VEC> struct SampleLast {
     uint64_t z = 0, extra = 0;                               // mass that is kept, and how much of it is on `step`
     if (row.way == SAMPLE_STEPS) {
       for (int s = tid; s < SR_STEPS_UP; s += SR_THREADS) { l.mass[s] = 0; l.count[s] = 0; }
-      listed = -1;
+      list_lo = 1;
+      list_hi = 0;
       __syncthreads();
       constexpr int E = (SR_STEPS + 63) / 64;                // a wavefront to a part, steps to its lanes
       uint64_t m[E] = {};
       uint32_t c[E] = {};
-#pragma unroll 2
-      for (int p = wave; p < a.parts; p += SR_THREADS / 64)
+      auto sum = [&](auto &to, auto of, auto together) {     // so many parts at once; behind the last part: that one, and not counted
+        constexpr int U = decltype(together)::value;
+        for (int p0 = wave; p0 < a.parts; p0 += U * (SR_THREADS / 64)) {
+          std::remove_reference_t<decltype(to[0])> v[U][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-          const int s = min(e * 64 + lane, SR_STEPS_UP - 1);
-          m[e] += ws[p].mass[s];
-          if (row.top_k) c[e] += ws[p].count[s];
+          for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[u][e] = of(ws[min(p0 + u * (SR_THREADS / 64), a.parts - 1)])[min(e * 64 + lane, SR_STEPS_UP - 1)];
+#pragma unroll
+          for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) to[e] += p0 + u * (SR_THREADS / 64) < a.parts ? v[u][e] : 0;
         }
+      };
+      auto masses = [](const SamplePart &p) { return p.mass; };
+      auto counts = [](const SamplePart &p) { return p.count; };
+      if (a.parts > 2 * (SR_THREADS / 64)) {
+        sum(m, masses, std::integral_constant<int, 4>());
+        if (row.top_k) sum(c, counts, std::integral_constant<int, 4>());
+      } else {
+        sum(m, masses, std::integral_constant<int, 1>());
+        if (row.top_k) sum(c, counts, std::integral_constant<int, 1>());
+      }
 #pragma unroll
       for (int e = 0; e < E; e++) {
         const int s = e * 64 + lane;
@@ -747,7 +774,8 @@ template <typename AT, bool VEC> struct SampleLast {
         uint64_t before;
         const int s = reach(l.count, (uint64_t)row.top_k, before);
         if (s < SR_STEPS && before + l.count[s] > (uint64_t)row.top_k) {
-          if (!border<false>(s, (uint64_t)row.top_k - before, cut, cut, extra)) return false;
+          // all that the first top_k are among, where it fits: a border by top_p is there too
+          if (!border<false>(s, row.top_p < 1.0f && before + l.count[s] <= SR_ROOM ? 0 : s, (uint64_t)row.top_k - before, cut, cut, extra)) return false;
           step = s;
         } else if (s < SR_STEPS) {
           step = s + 1;
@@ -764,7 +792,7 @@ template <typename AT, bool VEC> struct SampleLast {
         const uint64_t target = max(sample_share(__float_as_uint(row.top_p), z, true), (uint64_t)1);
         const int s = reach(l.mass, target, before);
         if (before + l.mass[s] > target) {
-          if (!border<true>(s, target - before, s == step ? cut : SampleCut{0, 0x7fffffff}, cut, extra)) return false;
+          if (!border<true>(s, s, target - before, s == step ? cut : SampleCut{0, 0x7fffffff}, cut, extra)) return false;
           step = s;
         } else if (s != step) {                              // the whole step, which is none that a cut went through
           step = s + 1;
@@ -782,8 +810,8 @@ template <typename AT, bool VEC> struct SampleLast {
       }
       __syncthreads();
       if (extra)
-        entries([&](float v, int i) {
-          if (cut.keeps(sample_key(v), i)) atomicAdd((unsigned long long *)&l.part[i / a.part], (unsigned long long)row.weight(v, table));
+        entries(step, [&](uint32_t key, int i, uint64_t w, int) {
+          if (cut.keeps(key, i)) atomicAdd((unsigned long long *)&l.part[i / a.part], (unsigned long long)w);
         });
     } else {
       for (int p = tid; p < a.parts; p += SR_THREADS) l.part[p] = ws[p].total;
@@ -844,7 +872,7 @@ template <typename AT, bool VEC> __global__ __launch_bounds__(SR_THREADS) void s
     prob = 0.0f;
   } else if (row.way != SAMPLE_GREEDY) {
     __syncthreads();
-    SampleLast<AT, VEC> last = {a, row, found, ws, x, sm, sm.list, table, -1, false};
+    SampleLast<AT, VEC> last = {a, row, found, ws, x, sm, sm.list, table, 1, 0, false};
     uint64_t w, total;
     if (!(row.way == SAMPLE_FEW ? last.few(n_found, vs, indexes, token, w, total) : last.steps(token, w, total))) {
       // many entries side by side in the order, where the cut is: digit by digit over the whole row

@@ -59,6 +59,18 @@ def test_rows_with_settings_of_their_own(hip, n, dtype):
     agree(hip, logits(rng, R, n, dtype), **mixed(rng, R))
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("n", [20011, 128256, 1 << 19])
+def test_borders_by_number_and_by_mass_in_one_row(hip, n, dtype):
+    """Both on one step, on steps far apart, with all that is in front of the first in a list or too much for one, and entries that are alike at them."""
+    rng = np.random.default_rng(n)
+    ks, ps = [257, 1000, 5000, 8190, 9000, 19000], [1e-3, 0.3, 0.9, 0.999, 1 - 1e-6]
+    R = len(ks) * len(ps)
+    x = logits(rng, R, n, dtype)
+    x[::3] = (x[::3] * 8).round() / 8
+    agree(hip, x, temperature=rng.choice([0.5, 1, 1.5], R), top_k=np.repeat(ks, len(ps)), top_p=np.tile(ps, len(ks)), min_p=rng.choice([0, 0, 1e-5], R), uniforms=rng.random(R))
+
+
 @pytest.mark.parametrize("alone", ["temperature", "top_k", "top_p", "min_p", None])
 def test_settings_alone(hip, alone):
     rng = np.random.default_rng(1)
