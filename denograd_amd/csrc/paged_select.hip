@@ -289,17 +289,17 @@ template <int NW> struct KeyChoice {
 
 // Block = some rows of a sequence, side by side, and a kv head.  Scores on the matrix cores: 16 pages' bounds against 16 columns of queries, the heads of a row next to each other, so that a lane has
 // four columns' scores of its page.  Few rows are bound by what waits for what: batch, page numbers, bounds, then the turns of the choice; many by the vector unit, which makes keys of scores and counts them.
-// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 10.5; 16 rows of up to 32768, pages of 32: 14; 2048 rows behind 14336, heads of 64: 34.  (A page to a thread with dot products and 32 turns
-// through LDS: 22, 30 and 138.  Blocks of eight wavefronts where rows are one to a sequence: 11.5 and 15, 64 sequences of 8192 positions 16 instead of 8.)
+// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 8.3; 16 rows of up to 32768, pages of 32: 11.3; 2048 rows behind 14336, heads of 64: 27.  (A page to a thread with dot products and 32 turns
+// through LDS: 22, 30 and 138.)
 // HT tiles of 16 columns: of more heads of the rows (HEADS), or of more rows, for which the bounds are loaded once.
-template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2) void paged_select_kernel(PagedSelectArgs a) {
-  constexpr int NW = PS_THREADS / 64;
+template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, 2) void paged_select_kernel(PagedSelectArgs a) {
   extern __shared__ __align__(16) uint32_t keys[];           // [rows of a block][stride]
   __shared__ union {
     KeyChoice<NW> block;
     KeyChoice<1> wave[NW];
-  } choice;
-  constexpr int KS = 2 * HD / 64;                            // steps of 64 bytes: the lower bounds, then the upper ones
+    unsigned char box[NW][16 * (2 * HD + 16)];               // each wavefront's tile of bounds, a page to a row; sixteen bytes between them, so that 16 rows' pieces meet all banks alike
+  } sm;
+  constexpr int KS = 2 * HD / 64, LPP = 2 * HD / 16, ROW = 2 * HD + 16;   // steps of 64 bytes (the lower bounds, then the upper ones), lanes to a page, bytes between pages
   const int g = blockIdx.y, KV = a.n_kv_heads, n_rep = a.n_rep, lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hp = 1 << a.heads_log, shift = a.pb.page_shift;
   const int r_end = min((int)(blockIdx.x + 1) * a.tile, a.pb.rows);
@@ -311,7 +311,7 @@ template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2
     if (r0 < s.start) { r0++; continue; }                    // no sequence has it
     const int p0 = paged_pos(s, r0 - s.start), last_page = p0 + n_rows - 1 < 0 ? -1 : (p0 + n_rows - 1) >> shift, n = min(last_page + 1, a.pb.width);
     // U tiles at a time: their page numbers in one trip to memory, asked for ahead, their bounds in the next.  The numbers without a branch: behind one, each would be waited for.
-    constexpr int U = HT > 1 ? 2 : 4;
+    constexpr int U = HT > 1 || NW == 8 ? 2 : 4;
     const int32_t *const table = a.pb.table + (size_t)b * a.pb.width;
     int id[U];
     auto pages_of = [&](int t0) {
@@ -369,7 +369,9 @@ template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2
         }
     }
     for (int t0 = wave; t0 * 16 < n; t0 += U * NW) {
-      i4v bf[U][KS];
+      // As they lie, neighbouring lanes on one page, and through LDS into the operand, whose lanes of a quarter are on different pages: straight from there, L1 is asked 64 times for what it gives in 16
+      // (2048 rows behind 14336, heads of 64, 31 us instead of 27, 512 of 128 17 instead of 14).
+      i4v box[U][KS];
       float scale[U];
       bool held[U];
 #pragma unroll
@@ -378,9 +380,11 @@ template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const size_t at = (size_t)max(id[u], 0) * KV + g;
-        const int8_t *const box = a.bounds + at * 2 * HD + lq * 16;
 #pragma unroll
-        for (int k = 0; k < KS; k++) bf[u][k] = *as_global<i4v>(box + k * 64);
+        for (int k = 0; k < KS; k++) {
+          const int of = max(__shfl(id[u], k * (64 / LPP) + lane / LPP), 0);
+          box[u][k] = *as_global<i4v>(a.bounds + ((size_t)of * KV + g) * 2 * HD + lane % LPP * 16);
+        }
         scale[u] = *as_global<float>(a.bound_scales + at);
         held[u] = id[u] >= 0;
       }
@@ -389,12 +393,17 @@ template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2
       for (int u = 0; u < U; u++) {
         const int i = (t0 + u * NW) * 16 + l16;
         if (i - l16 >= n) break;
+        i4v bf[KS];
+#pragma unroll
+        for (int k = 0; k < KS; k++) *(i4v *)(sm.box[wave] + (k * (64 / LPP) + lane / LPP) * ROW + lane % LPP * 16) = box[u][k];
+#pragma unroll
+        for (int k = 0; k < KS; k++) bf[k] = *(const i4v *)(sm.box[wave] + l16 * ROW + k * 64 + lq * 16);
         float v[4];
 #pragma unroll
         for (int h = 0; h < HT; h++) {
           i4v acc = {0, 0, 0, 0};
 #pragma unroll
-          for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[h][k], bf[u][k], acc, 0, 0, 0);
+          for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[h][k], bf[k], acc, 0, 0, 0);
 #pragma unroll
           for (int e = 0; e < 4; e++) v[e] = HEADS && h ? fmaxf(v[e], (float)acc[e]) : (float)acc[e];   // column 4 lq + e, page l16
         if (HEADS && h < HT - 1) continue;
@@ -419,9 +428,9 @@ template <int HD, int HT, bool HEADS> __global__ __launch_bounds__(PS_THREADS, 2
     __syncthreads();
     auto place = [&](int at) { return a.selected + ((size_t)(r0 + at) * KV + g) * a.top; };
     auto pages = [&](int at) { return p0 + at < 0 ? 0 : min(((p0 + at) >> shift) + 1, a.pb.width); };
-    if (a.tile == 1) choice.block(keys, n, a.top, place(0), wave);
+    if (a.tile == 1) sm.block(keys, n, a.top, place(0), wave);
     else
-      for (int at = wave; at < n_rows; at += NW) choice.wave[wave](keys + at * a.stride, pages(at), a.top, place(at), 0);
+      for (int at = wave; at < n_rows; at += NW) sm.wave[wave](keys + at * a.stride, pages(at), a.top, place(at), 0);
     r0 += n_rows;
     if (r0 < r_end) __syncthreads();
   }
@@ -974,17 +983,22 @@ int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t 
   const bool four = HD == 128 && !many && (size_t)rows >= (size_t)8 * tile * n_seqs && (size_t)rows * a.n_kv_heads >= (size_t)tile * 2048 && (size_t)tile * 4 * a.stride * 4 <= 64 * 1024;
   a.tile = rows > n_seqs && (size_t)tile * a.stride * 4 <= 64 * 1024 ? tile * (four ? 4 : 1) : 1;
   const dim3 grid((unsigned)((rows + a.tile - 1) / a.tile), (unsigned)a.n_kv_heads);
+  // Eight wavefronts where a unit has no more than one block.  us, four | eight: one row behind 33000 positions, pages of 64, 9.4 | 8.1, of 16 25 | 17; 16 rows of up to 32768, pages of 32, 13.3 | 10.8; 64 rows of
+  // 64 sequences of 8192 7.6 | 9.9; 128 rows behind 16256 (256 blocks) 7.0 | 6.5, 512 14.4 | 15.
   const size_t lds = (size_t)a.tile * a.stride * 4;
-#define JSG_SELECT(HD, HT, HEADS)                                                                                                                                    \
-  do {                                                                                                                                                                \
-    if (lds > 48 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<HD, HT, HEADS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));          \
-    JSG_LAUNCH(PROF_ATTN_PAGED, (paged_select_kernel<HD, HT, HEADS>), grid, dim3(PS_THREADS), lds, a);                                                                   \
+  const bool wide = !many && !four && (size_t)grid.x * grid.y <= 256 && lds <= 64 * 1024;   // the tiles of eight have 34 KB of LDS
+#define JSG_SELECT(HD, NW, HT, HEADS)                                                                                                                                        \
+  do {                                                                                                                                                                        \
+    if (lds > 48 * 1024) JSG_HIP(hipFuncSetAttribute((const void *)paged_select_kernel<HD, NW, HT, HEADS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));              \
+    JSG_LAUNCH(PROF_ATTN_PAGED, (paged_select_kernel<HD, NW, HT, HEADS>), grid, dim3(NW * 64), lds, a);                                                                          \
   } while (0)
-  if (HD == 64 && many) JSG_SELECT(64, 4, true);
-  else if (HD == 64) JSG_SELECT(64, 1, false);
-  else if (many) JSG_SELECT(128, 4, true);
-  else if (a.tile > tile) JSG_SELECT(128, 4, false);
-  else JSG_SELECT(128, 1, false);
+  if (HD == 64 && many) JSG_SELECT(64, 4, 4, true);
+  else if (HD == 64 && wide) JSG_SELECT(64, 8, 1, false);
+  else if (HD == 64) JSG_SELECT(64, 4, 1, false);
+  else if (many) JSG_SELECT(128, 4, 4, true);
+  else if (wide) JSG_SELECT(128, 8, 1, false);
+  else if (a.tile > tile) JSG_SELECT(128, 4, 4, false);
+  else JSG_SELECT(128, 4, 1, false);
 #undef JSG_SELECT
   return 0;
 }

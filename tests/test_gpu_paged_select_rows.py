@@ -100,3 +100,19 @@ def test_more_rows_than_positions(hip):
     out = run_attend(hip, c, q, 8, sel)
     exact, tol = ref.attention(c, q, 8, sel, 3)
     assert np.all(out[:100] == 0) and np.all(np.abs(out[::3].astype(np.float64) - exact[::3]) <= tol[::3])
+
+
+@pytest.mark.parametrize("hd,H,width", [(128, 4, 32768), (128, 20, 32768), (128, 4, 16385), (128, 4, 16384), (64, 4, 16400)])
+def test_the_widest_tables(hip, hd, H, width):
+    """As many columns as a choice takes, and those at which a block has fewer rows and wavefronts; pages come again and again, ties go to the lower column."""
+    rng = np.random.default_rng(width + H)
+    for rows in (1, 3):
+        c = Case(rng, "int8", hd, 1, 16, [rows], [1000])
+        c.table = np.resize(c.table[0, :62], width).astype(np.int32)[None]
+        c.lens = [width * 16 - 5]
+        c.device()
+        codes, scales = arrays(c, rng)
+        q = rng.standard_normal((rows, H, hd)).astype(np.float16)
+        for top in (5, 1024):
+            sel = run_choose(hip, c, q, H, codes, scales, 2, 3, top)
+            assert np.array_equal(sel, ref.choose_many(c, q, H, codes, scales, 2, 3, top, np.full(sel.shape, 77, np.int32)))
