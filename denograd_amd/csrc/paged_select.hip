@@ -289,7 +289,7 @@ template <int NW> struct KeyChoice {
 
 // Block = some rows of a sequence, side by side, and a kv head.  Scores on the matrix cores: 16 pages' bounds against 16 columns of queries, the heads of a row next to each other, so that a lane has
 // four columns' scores of its page.  Few rows are bound by what waits for what: batch, page numbers, bounds, then the turns of the choice; many by the vector unit, which makes keys of scores and counts them.
-// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 8.3; 16 rows of up to 32768, pages of 32: 11.3; 2048 rows behind 14336, heads of 64: 27.  (A page to a thread with dot products and 32 turns
+// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 8.9; 16 rows of up to 32768, pages of 32: 12; 2048 rows behind 14336, heads of 64: 31.  (A page to a thread with dot products and 32 turns
 // through LDS: 22, 30 and 138.)
 // HT tiles of 16 columns: of more heads of the rows (HEADS), or of more rows, for which the bounds are loaded once.
 template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, 2) void paged_select_kernel(PagedSelectArgs a) {
@@ -975,9 +975,9 @@ int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t 
   a.selected = selected;
   while ((1 << a.heads_log) < (n_rep < 16 ? n_rep : 16)) a.heads_log++;
   a.stride = (host_pages->table_width + 15) & ~15;
-  // Rows of a sequence share its bounds: the columns of a matrix instruction are theirs, and with heads of 128 four such tiles where enough blocks are left.  us, one tile | four, 32 heads of 128 over
-  // 8: 1024 rows behind 15360 27 | 20, 2048 behind 14336 48 | 37, 2048 behind 2048 29 | 28, 700 behind 9000 16.5 | 18, 128 behind 16256 7.4 | 15.  Heads of 64, whose bounds are half as long:
-  // 2048 behind 14336 31 | 29, behind 2048 21 | 23, 4096 from the start 35 | 38.
+  // Rows of a sequence share its bounds: the columns of a matrix instruction are theirs, and with heads of 128 four such tiles where enough blocks are left.  us, one tile | four: 2048 rows behind 14336, 16 heads of
+  // 128 over 1 23 | 15, 16 over 2 20 | 17, 64 over 8 70 | 60, 32 over 8 39 | 37.5, 1024 of these behind 15360 22 | 20, 700 behind 9000 14 | 18, 256 behind 16128 8 | 16.  Heads of 64, whose bounds are half as
+  // long: 2048 behind 14336 31 | 29, behind 2048 21 | 23, 4096 from the start 35 | 38 (with the bounds straight to the operand).
   const bool many = n_rep > 16;
   const int tile = 16 >> a.heads_log;
   const bool four = HD == 128 && !many && (size_t)rows >= (size_t)8 * tile * n_seqs && (size_t)rows * a.n_kv_heads >= (size_t)tile * 2048 && (size_t)tile * 4 * a.stride * 4 <= 64 * 1024;
