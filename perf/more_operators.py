@@ -1,6 +1,6 @@
 """What the speed of a serving step's further operators is measured on, beside those of `perf/operators.py`.
 
-* `sample`: a token for every row of logits by temperature, min-p, top-k and top-p from given random numbers, and the probability that it had among those that
+* `sample`: a token for every row of logits by temperature, top-k, top-p and min-p from given random numbers, and the probability that it had among those that
   were left (`jsgrad_hip_sample_rows`).
 * `copy`: pages of all layers copied to other pages, where a prompt gets several answers or a pool is packed (`jsgrad_hip_paged_copy`).
 * `norm`: the new rows of a ragged batch, q and k normed per head and rotated, and written into the pages (`jsgrad_hip_paged_write_norm`); int8 rows are read
@@ -144,7 +144,7 @@ def _rng(seed: int) -> torch.Generator:
 
 
 def _settings(case: dict, g: torch.Generator):
-    """temperature, top_k, top_p and min_p of every row; min-p comes first, then top-k, then top-p."""
+    """temperature, top_k, top_p and min_p of every row."""
     n = case["rows"]
     if case["settings"] == "usual":
         rows = [(0.7, 50, 0.9, 0.0)] * n
@@ -315,10 +315,10 @@ def _sample(s: dict) -> dict:
     w = torch.where(top == top[:, :1], 1.0, w)
     rank = torch.arange(x.shape[1], device="cuda")
     k = s["top_k"].unsqueeze(1)
-    w = torch.where(((rank < k) | (k <= 0)) & (w >= col("min_p").clamp(max=1.0)), w, 0.0)
+    w = torch.where((rank < k) | (k <= 0), w, 0.0)
     before = w.cumsum(1) - w
     keep = (before < col("top_p") * w.sum(1, keepdim=True)) | (rank == 0) | (col("top_p") >= 1.0)
-    w = torch.where(keep, w, 0.0)
+    w = torch.where(keep & (w >= col("min_p").clamp(max=1.0)), w, 0.0)
     w = torch.zeros_like(w).scatter_(1, order, w)
     run = w.cumsum(1)
     drawn = (run > col("uniforms") * run[:, -1:]).to(torch.uint8).argmax(1)
@@ -470,13 +470,12 @@ def _exact_sample(s: dict) -> dict:
         with np.errstate(invalid="ignore"):
             w = np.where(v == v[best], 1.0, np.exp((v - v[best]) / T[r]))
         order = np.argsort(-v, kind="stable")
-        order = order[w[order] >= min(M[r], 1.0)]
         if K[r] > 0:
             order = order[:int(K[r])]
         if P[r] < 1.0:
             mass = np.cumsum(w[order])
             order = order[:1 + int(np.count_nonzero(mass[:-1] < P[r] * mass[-1]))]
-        order = np.sort(order)
+        order = np.sort(order[w[order] >= min(M[r], 1.0)])
         run_ = np.cumsum(w[order])
         out.append(int(order[np.searchsorted(run_, U[r] * run_[-1], side="right")]))
         probs.append(w[out[-1]] / run_[-1])
