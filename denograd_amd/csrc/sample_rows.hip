@@ -1,7 +1,8 @@
 // A token for every row of logits, by the row's own temperature, min-p, top-k and top-p and a given uniform number (jsgrad_hip_sample_rows).
 //
 // With M the row's maximum, w = exp((x - M) / T); the entries with w >= min_p; of these the first top_k in the order (x descending, index ascending); of these the first whose mass
-// reaches top_p of them all; the token is the first, by index, at which the running sum of what is left exceeds u times its total.
+// reaches top_p of them all; the token is the first, by index, at which the running sum of what is left exceeds u times its total.  Or min_p last (jsgrad_hip_sample_rows_ordered): the mass that top_p is a share of
+// counts entries that min_p drops afterwards.  Where top_p is 1 the place makes no difference, as w falls along the order.
 //
 // Which entry a sum ends at is a question of borders: with float sums, off by 1e-7, one draw in a hundred over a flat vocabulary would fall to a neighbour.  So a weight is
 // made in 64 bits and held as a whole number of 2^-42: sums of up to 2^20 of them are exact and come out alike in any order, and the borders p Z and u Z are
@@ -40,6 +41,7 @@ struct SampleRowsArgs {
   const int32_t *top_k;
   int32_t *tokens;
   float *probs;
+  int order;                                                 // JSGRAD_MIN_P_FIRST or _LAST
   int parts, part, lanes;                                    // of a row, entries of one, and threads that share a group
   struct SampleFound *found;                                 // [rows]
   struct SamplePart *ws;                                     // [rows][parts]
@@ -67,12 +69,12 @@ struct SampleRow {
   float top;                                                 // M
   bool infinite;                                             // M is: it alone has weight
   double from, scale;                                        // M again, log2(e) / T
-  uint64_t least;                                            // weight that min_p asks for
+  uint64_t least, late;                                      // weight that min_p asks for in front of the others, and behind them
   float top_p, u;
   int top_k;                                                 // 0: all
   SampleWay way;
 
-  __device__ SampleRow(const SampleRowsArgs &a, int r, float best) {
+  __device__ __forceinline__ SampleRow(const SampleRowsArgs &a, int r, float best) {
     // an array that is not given is another one in its place: five loads at once, without branches
     const float *const ts = a.temperature ? a.temperature : a.uniforms, *const ps = a.top_p ? a.top_p : a.uniforms, *const ms = a.min_p ? a.min_p : a.uniforms;
     const int32_t *const ks = a.top_k ? a.top_k : (const int32_t *)a.uniforms;
@@ -84,11 +86,13 @@ struct SampleRow {
     infinite = best == INFINITY;
     from = infinite ? 0.0 : (double)best;
     scale = 1.4426950408889634 / (double)temperature;
-    least = m > 0.0f ? (uint64_t)ceil((double)fminf(m, 1.0f) * (double)(1ull << SR_BITS)) : 0;
+    const uint64_t asked = m > 0.0f ? (uint64_t)ceil((double)fminf(m, 1.0f) * (double)(1ull << SR_BITS)) : 0;
     top_p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;
     u = v > 0.0f ? fminf(v, 0x1.fffffep-1f) : 0.0f;
     top_k = k > 0 && k < a.n ? k : 0;
     way = !(best > -INFINITY) || !(temperature >= 1e-6f) ? SAMPLE_GREEDY : top_k > 0 && top_k <= SR_FEW ? SAMPLE_FEW : top_k > 0 || top_p < 1.0f ? SAMPLE_STEPS : SAMPLE_WHOLE;
+    late = a.order == JSGRAD_MIN_P_LAST && way != SAMPLE_WHOLE ? asked : 0;
+    least = late ? 0 : asked;
   }
   static constexpr double MAGIC = 6755399441055744.0;        // 1.5 * 2^52: what it is added to comes out rounded to a whole number
   // log2 of an entry's weight: x - M is exact in 64 bits, the product off by 2^-52 of itself.  Entries that are not numbers are minus infinity, and that has no weight.
@@ -132,6 +136,8 @@ struct SampleRow {
     int unused;
     return weight(x, table, unused);
   }
+  // The step on which weights fall below `late`, 1 and more: rounded they reach it from half a unit less on.
+  __device__ int late_step() const { return -(int)rint((log2((double)late - 0.5) - SR_BITS) * SR_FINE) / SR_STEP; }
 };
 // 2^(i / 256), filled by the first 256 threads
 __device__ __forceinline__ void sample_table(double *table) {
@@ -219,7 +225,7 @@ template <typename AT> struct SampleBlock {
   __device__ float at(int i) const { return sample_clean((float)x[i]); }
 
   // The cut behind the first entries, in the row's order, that `within` keeps and whose counts (or, MASS, weights) together reach `target`, 1 and more; everything where they do not.
-  template <bool MASS> __device__ SampleCut cut(uint64_t target, SampleCut within) {
+  template <bool MASS> __device__ __forceinline__ SampleCut cut(uint64_t target, SampleCut within) {
     uint32_t prefix = 0;
     int shift = 32;
     uint64_t above = 0;                                      // of the keys above the prefix
@@ -293,7 +299,7 @@ template <typename AT> struct SampleBlock {
     return c;
   }
 
-  __device__ uint64_t mass(SampleCut c) {
+  __device__ __forceinline__ uint64_t mass(SampleCut c) {
     uint64_t s = 0, total;
     for (int i = threadIdx.x; i < n; i += SR_THREADS) {
       const float v = at(i);
@@ -303,19 +309,20 @@ template <typename AT> struct SampleBlock {
     return total;
   }
 
-  // The first entry at which the running sum of what c keeps exceeds u of it all.
-  __device__ int draw(SampleCut c, float u, uint64_t &weight, uint64_t &total) {
+  // The first entry at which the running sum of what c, and min_p behind it, keep exceeds u of it all.
+  __device__ uint64_t kept(SampleCut c, int i) const {
+    const float v = at(i);
+    const uint64_t w = c.keeps(sample_key(v), i) ? row.weight(v, table) : 0;
+    return w < row.late ? 0 : w;
+  }
+  __device__ __forceinline__ int draw(SampleCut c, float u, uint64_t &weight, uint64_t &total) {
     const int tiles = (n + SR_TILE - 1) / SR_TILE;
     __syncthreads();
     for (int t = threadIdx.x; t < SR_MOST / SR_TILE; t += SR_THREADS) sm.hist.mass[t] = 0;
     __syncthreads();
     for (int t = 0; t < tiles; t++) {
       const int i = t * SR_TILE + threadIdx.x;
-      uint64_t w = 0;
-      if (i < n) {
-        const float v = at(i);
-        if (c.keeps(sample_key(v), i)) w = row.weight(v, table);
-      }
+      const uint64_t w = i < n ? kept(c, i) : 0;
       if (w) atomicAdd((unsigned long long *)&sm.hist.mass[t], (unsigned long long)w);
     }
     __syncthreads();
@@ -328,11 +335,8 @@ template <typename AT> struct SampleBlock {
     __syncthreads();
     const int t = (int)sm.result[0], i = t * SR_TILE + threadIdx.x;
     const uint64_t base = sm.result[1];
-    uint64_t w = 0, all;
-    if (i < n) {
-      const float v = at(i);
-      if (c.keeps(sample_key(v), i)) w = row.weight(v, table);
-    }
+    uint64_t all;
+    const uint64_t w = i < n ? kept(c, i) : 0;
     const uint64_t run = base + block_scan(w, all, sm);
     if (run <= target && run + w > target) {
       sm.result[0] = i;
@@ -594,7 +598,7 @@ template <typename AT, bool VEC> struct SampleLast {
   }
 
   // Of the first top_k among the candidates; false where there are more than the list has room for.
-  __device__ bool few(int c, const float (&v)[2], const int (&index)[2], int &token, uint64_t &weight, uint64_t &total) {
+  __device__ __forceinline__ bool few(int c, const float (&v)[2], const int (&index)[2], int &token, uint64_t &weight, uint64_t &total) {
     const int tid = threadIdx.x;
     if (c > SR_LIST) return false;
 #pragma unroll
@@ -617,7 +621,7 @@ template <typename AT, bool VEC> struct SampleLast {
     const uint64_t target = row.top_p < 1.0f ? max(sample_share(__float_as_uint(row.top_p), z, true), (uint64_t)1) : z;
     uint64_t left = 0;
     for (int i = tid; i < c; i += SR_THREADS) {
-      const uint64_t w = l.near[i] < target ? l.w[i] : 0;
+      const uint64_t w = l.near[i] < target && l.w[i] >= row.late ? l.w[i] : 0;
       l.near_w[i] = w;
       left += w;
     }
@@ -659,7 +663,7 @@ template <typename AT, bool VEC> struct SampleLast {
     }
   }
   // Lists the entries of steps; between barriers.
-  __device__ void list(int lo, int hi) {
+  __device__ __forceinline__ void list(int lo, int hi) {
     on_steps(lo, hi, [&](float v, int i) {
       const int slot = atomicAdd(&l.n, 1);
       if (slot < SR_ROOM) l.place[slot] = sample_place(v, i);
@@ -684,7 +688,7 @@ template <typename AT, bool VEC> struct SampleLast {
   }
   // The cut among the entries of a step that `within` keeps at which their counts (MASS: weights) reach `target`, 1 and more, and the weight up to it; false where too many are on one depth.  Where the row has to be
   // gone over for that, everything from the step `first` on is listed.
-  template <bool MASS> __device__ bool border(int step, int first, uint64_t target, SampleCut within, SampleCut &cut, uint64_t &mass) {
+  template <bool MASS> __device__ __forceinline__ bool border(int step, int first, uint64_t target, SampleCut within, SampleCut &cut, uint64_t &mass) {
     const int tid = threadIdx.x, lane = tid & 63;
     __syncthreads();
     if (tid < SR_STEP) { l.fine_mass[tid] = 0; l.fine_count[tid] = 0; }
@@ -726,7 +730,7 @@ template <typename AT, bool VEC> struct SampleLast {
   }
 
   // By masses and counts of the steps: those above one step are kept whole, of that one what the cut keeps.  False where a step holds too many entries.
-  __device__ bool steps(int &token, uint64_t &weight, uint64_t &total) {
+  __device__ __forceinline__ bool steps(int &token, uint64_t &weight, uint64_t &total) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     SampleCut cut = {0, 0x7fffffff};
     int step = SR_STEPS;                                     // kept whole: the steps before this one
@@ -800,6 +804,13 @@ template <typename AT, bool VEC> struct SampleLast {
           extra = 0;
         }
       }
+      if (row.late)
+        if (const int s = row.late_step(); s < step) {         // steps above this one are kept whole, of those below nothing is; it is looked for once, so not listed
+          step = s;
+          cut = SampleCut{0, 0x7fffffff};
+          extra = 1;
+          fits = false;
+        }
       // what of every part is kept: whole steps, sixteen threads to a part, then those of the step with the cut
       for (int p = tid / 16; p < a.parts; p += SR_THREADS / 16) {
         uint64_t m = 0;
@@ -811,7 +822,7 @@ template <typename AT, bool VEC> struct SampleLast {
       __syncthreads();
       if (extra)
         entries(step, [&](uint32_t key, int i, uint64_t w, int) {
-          if (cut.keeps(key, i)) atomicAdd((unsigned long long *)&l.part[i / a.part], (unsigned long long)w);
+          if (cut.keeps(key, i) && w >= row.late) atomicAdd((unsigned long long *)&l.part[i / a.part], (unsigned long long)w);
         });
     } else {
       for (int p = tid; p < a.parts; p += SR_THREADS) l.part[p] = ws[p].total;
@@ -833,7 +844,7 @@ template <typename AT, bool VEC> struct SampleLast {
         const float v = sample_clean((float)x[i]);
         int d;
         const uint64_t m = row.weight(v, table, d);
-        if (d < step * SR_STEP || (d < (step + 1) * SR_STEP && extra && cut.keeps(sample_key(v), i))) w[e] = m;
+        if (d < step * SR_STEP || (d < (step + 1) * SR_STEP && extra && cut.keeps(sample_key(v), i) && m >= row.late)) w[e] = m;
       }
       sum += w[e];
     }
@@ -898,22 +909,9 @@ static int sample_part(int rows, int n) {
   return SR_PART * 4;
 }
 
-}  // namespace jsg
-
-using namespace jsg;
-
-extern "C" {
-
-size_t jsgrad_hip_sample_rows_workspace_bytes(int rows, int n) {
-  if (rows <= 0 || n <= 0 || n > SR_MOST) return 0;
-  // of all numbers of rows up to this: fewer rows have shorter parts, up to SR_BLOCKS of them
-  const size_t longest = (size_t)rows * ((n + 4 * SR_PART - 1) / (4 * SR_PART)), shortest = (size_t)rows * ((n + SR_PART - 1) / SR_PART);
-  return (size_t)rows * sizeof(SampleFound) + sizeof(SamplePart) * (shortest < SR_BLOCKS ? shortest : longest < SR_BLOCKS ? SR_BLOCKS : longest);
-}
-
-int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
-                           const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace) {
-  const char *who = "jsgrad_hip_sample_rows";
+// jsgrad_hip_sample_rows and _sample_rows_ordered
+static int sample_rows(const char *who, const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                       int order, const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace) {
   JSG_REQUIRE(logits && uniforms && tokens_out && workspace, "%s: null pointer argument", who);
   JSG_REQUIRE(act == JSGRAD_F16 || act == JSGRAD_F32, "%s: unknown activation dtype %d", who, act);
   JSG_REQUIRE(rows > 0 && rows <= 65535, "%s: %d rows (1 to 65535)", who, rows);
@@ -923,8 +921,9 @@ int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_strid
   JSG_REQUIRE(((uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)uniforms | (uintptr_t)tokens_out | (uintptr_t)probs_out) % 4 == 0,
               "%s: the rows' arrays must be 4-byte aligned", who);
   JSG_REQUIRE((uintptr_t)workspace % 16 == 0, "%s: workspace must be 16-byte aligned", who);
+  JSG_REQUIRE(order == JSGRAD_MIN_P_FIRST || order == JSGRAD_MIN_P_LAST, "%s: order %d (min-p first or last)", who, order);
   JSG_READY();
-  SampleRowsArgs a = {logits, row_stride, n, temperature, top_p, min_p, uniforms, top_k, tokens_out, probs_out};
+  SampleRowsArgs a = {logits, row_stride, n, temperature, top_p, min_p, uniforms, top_k, tokens_out, probs_out, order};
   a.part = sample_part(rows, n);
   a.parts = (n + a.part - 1) / a.part;
   a.lanes = 1;                                               // of the groups, as many as are no more than four times SR_FEW
@@ -946,6 +945,29 @@ int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_strid
   else JSG_SAMPLE(float, false);
 #undef JSG_SAMPLE
   return 0;
+}
+
+}  // namespace jsg
+
+using namespace jsg;
+
+extern "C" {
+
+size_t jsgrad_hip_sample_rows_workspace_bytes(int rows, int n) {
+  if (rows <= 0 || n <= 0 || n > SR_MOST) return 0;
+  // of all numbers of rows up to this: fewer rows have shorter parts, up to SR_BLOCKS of them
+  const size_t longest = (size_t)rows * ((n + 4 * SR_PART - 1) / (4 * SR_PART)), shortest = (size_t)rows * ((n + SR_PART - 1) / SR_PART);
+  return (size_t)rows * sizeof(SampleFound) + sizeof(SamplePart) * (shortest < SR_BLOCKS ? shortest : longest < SR_BLOCKS ? SR_BLOCKS : longest);
+}
+
+int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                           const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace) {
+  return sample_rows("jsgrad_hip_sample_rows", logits, rows, n, row_stride, act, temperature, top_k, top_p, min_p, JSGRAD_MIN_P_FIRST, uniforms, tokens_out, probs_out, workspace);
+}
+
+int jsgrad_hip_sample_rows_ordered(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                                   int order, const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace) {
+  return sample_rows("jsgrad_hip_sample_rows_ordered", logits, rows, n, row_stride, act, temperature, top_k, top_p, min_p, order, uniforms, tokens_out, probs_out, workspace);
 }
 
 }  // extern "C"

@@ -333,7 +333,7 @@ class Llama3:
         return hist.numpy().T.copy()
 
     def generate_paged(self, prompts, n_new: int, dtype: str = "float16", page_size: int = 64, window: int = 0, sinks: int = 0, samples: int = 1, temperature: float = 0.0,
-                       top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, seed: int = 0, choose: tuple[int, int, int] | None = None) -> np.ndarray:
+                       top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, seed: int = 0, choose: tuple[int, int, int] | None = None, min_p_last: bool = False) -> np.ndarray:
         """Prompts of any lengths at once over a paged cache made for them: fp16 pages, or int8 ones of half the size.  With a window a
         sequence gives away the pages that it no longer sees, and the pool has no more than the prompts and those that are seen need.  Greedy, or drawn by these settings (RowSampler); `samples`
         answers to each prompt share its pages.  choose: attention over the pages that each row chooses, (first, recent, top) of PagedBatch.choose.  Returns int32 [number of prompts * samples, n_new], the answers to a prompt side by side."""
@@ -347,7 +347,7 @@ class Llama3:
             raise ValueError(f"window {window}, sinks {sinks}, page_size {page_size}")
         if samples < 1:
             raise ValueError(f"{samples} answers to a prompt")
-        sampler = RowSampler(temperature, top_k, top_p, min_p, seed, self.device)
+        sampler = RowSampler(temperature, top_k, top_p, min_p, seed, self.device, min_p_last)
         sampler = sampler if temperature >= 1e-6 else None
         sizes = np.repeat([p.size for p in prompts], samples)
         n_pages = PagedCache.pages_for(sizes, n_new, page_size, window, sinks)

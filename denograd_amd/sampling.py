@@ -14,9 +14,11 @@ from .tensor import Tensor
 
 
 class RowSampler:
-    """Settings of the rows of a batch: a number for all of them, or one for each.  min_p comes first, then top_k (0: all), then top_p; a temperature of 0 is the greedy token."""
+    """Settings of the rows of a batch: a number for all of them, or one for each.  min_p comes first, then top_k (0: all), then top_p; or,
+    min_p_last, on what these two leave, whose mass then counts for top_p; a temperature of 0 is the greedy token."""
 
-    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0, device: str = "HIP"):
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0, device: str = "HIP", min_p_last: bool = False):
+        self.order = ffi.MIN_P_LAST if min_p_last else ffi.MIN_P_FIRST
         self.device, self.rng = device, np.random.default_rng(seed)
         self.settings = [np.atleast_1d(np.asarray(x, t)) for x, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
         temperature, top_k, top_p, min_p = self.settings
@@ -56,6 +58,6 @@ class RowSampler:
         need = lib.jsgrad_hip_sample_rows_workspace_bytes(rows, n)
         if self._ws is None or self._ws.nbytes < need:
             self._ws = Tensor.empty((need,), "uint8", self.device)
-        check(lib.jsgrad_hip_sample_rows(logits.ptr, rows, n, n, act_code(logits.dtype), at[0], at[1], at[2], at[3], at[4], tokens_out.ptr, at[5], self._ws.ptr))
+        check(lib.jsgrad_hip_sample_rows_ordered(logits.ptr, rows, n, n, act_code(logits.dtype), at[0], at[1], at[2], at[3], self.order, at[4], tokens_out.ptr, at[5], self._ws.ptr))
         self.probs = Tensor(buffer=self._held.lazydata.view(rows, "float32", 20 * rows), shape=(rows,), dtype="float32", device=self.device)
         return Tensor(buffer=tokens_out.lazydata if tokens_out.shape == (rows,) else tokens_out.lazydata.view(rows, "int32", 0), shape=(rows,), dtype="int32", device=self.device)

@@ -441,10 +441,15 @@ int jsgrad_hip_sample(const void *logits, int n, int act, double temp, int k, do
  * the running sum of w exceeds uniforms[r] (0 to below 1) of its total, probs_out[r] (or NULL) its share.  A temperature below 1e-6: the lowest index of the maximum, share 1.  What is not a number
  * counts as minus infinity; a row with nothing above that: token -1, share 0.  Where infinity is the maximum, that alone has weight.  Sums are whole numbers of 2^-42 of the largest weight: results do not depend on
  * the order in which blocks run, nor on the other rows.  workspace: jsgrad_hip_sample_rows_workspace_bytes() bytes, 16-byte aligned, whatever it holds; any number of calls of no more rows and
- * logits may have the same one (they are ordered by the library's stream). */
+ * logits may have the same one (they are ordered by the library's stream).
+ * _sample_rows_ordered: the same with JSGRAD_MIN_P_FIRST; with JSGRAD_MIN_P_LAST the first top_k of all entries, of these those with less than top_p of their mass before them, and of these the entries with w >= min_p,
+ * which is another set, or another total, where top_p is below 1. */
+enum { JSGRAD_MIN_P_FIRST = 0, JSGRAD_MIN_P_LAST = 1 };
 size_t jsgrad_hip_sample_rows_workspace_bytes(int rows, int n);
 int jsgrad_hip_sample_rows(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                            const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace);
+int jsgrad_hip_sample_rows_ordered(const void *logits, int rows, int n, size_t row_stride, int act, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                                   int order, const float *uniforms, int32_t *tokens_out, float *probs_out, void *workspace);
 
 /* Checkpoint formats on the way into the model.
  * ggml_dequant: ggml_data_to_tensor (nn/state.ts:192-223) for the quantised GGML types Q4_0 (2), Q4_1 (3), Q8_0 (8) and

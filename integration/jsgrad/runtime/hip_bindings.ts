@@ -95,6 +95,7 @@ const SYMBOLS = {
   jsgrad_hip_sample: { parameters: [P, I, I, D, I, D, D, D, P, P, P, P, I, I, P], result: I }, // logits, n, act, temp, k, p, af, ap, alpha_counter, rng, state, tokens_out, tokens_cap, advance, workspace
   jsgrad_hip_sample_rows_workspace_bytes: { parameters: [I, I], result: U }, // rows, n
   jsgrad_hip_sample_rows: { parameters: [P, I, I, U, I, P, P, P, P, P, P, P, P], result: I }, // logits, rows, n, row_stride, act, temperature, top_k, top_p, min_p, uniforms, tokens_out, probs_out, workspace
+  jsgrad_hip_sample_rows_ordered: { parameters: [P, I, I, U, I, P, P, P, P, I, P, P, P, P], result: I }, // logits, rows, n, row_stride, act, temperature, top_k, top_p, min_p, order, uniforms, tokens_out, probs_out, workspace
   jsgrad_hip_ggml_nbytes: { parameters: [I, U], result: U }, // ggml_type, n
   jsgrad_hip_ggml_dequant: { parameters: [I, P, U, P], result: I }, // ggml_type, blocks, n, out_f32
   jsgrad_hip_cast: { parameters: [P, I, P, I, U], result: I }, // src, src_dtype, dst, dst_dtype, n
@@ -118,6 +119,7 @@ export const check = (rc: number): void => {
 
 // include/jsgrad_hip.h: activation dtypes, weight formats, cast sources, profile kinds
 export const JSGRAD_F32 = 0, JSGRAD_F16 = 1, JSGRAD_BF16 = 2
+export const JSGRAD_MIN_P_FIRST = 0, JSGRAD_MIN_P_LAST = 1
 export const JSGRAD_W_F32 = 0, JSGRAD_W_F16 = 1, JSGRAD_W_I8 = 2, JSGRAD_W_NF4 = 3
 export const PROF = ['EMBED', 'RMSNORM', 'LINEAR', 'QKV_ROPE', 'ATTN', 'FFN_GATE', 'ARGMAX', 'STEP', 'GEMM', 'ATTN_PREFILL', 'ATTN_WO', 'READ', 'SAMPLE', 'PAGED_ROWS', 'ATTN_PAGED'] as const
 
