@@ -280,8 +280,8 @@ def _own(s: dict):
                                       ptr(s["pages_k"]), ptr(s["pages_v"]), ptr(s["scales_k"]), ptr(s["scales_v"]), ptr(s["table"]))
     if case["kind"] == "sample":
         ws = _workspace(("sample", case["rows"], case["n"]), lib.jsgrad_hip_sample_rows_workspace_bytes(case["rows"], case["n"]))
-        check(lib.jsgrad_hip_sample_rows(ptr(s["logits"]), case["rows"], case["n"], case["n"] + case["pad"], ffi.F16 if case["act"] == "f16" else ffi.F32, ptr(s["temperature"]),
-                                         ptr(s["top_k"]), ptr(s["top_p"]), ptr(s["min_p"]), ptr(s["uniforms"]), ptr(s["tokens"]), ptr(s["probs"]), ws))
+        check(lib.jsgrad_hip_sample_rows_ordered(ptr(s["logits"]), case["rows"], case["n"], case["n"] + case["pad"], ffi.F16 if case["act"] == "f16" else ffi.F32, ptr(s["temperature"]),
+                                                 ptr(s["top_k"]), ptr(s["top_p"]), ptr(s["min_p"]), ffi.MIN_P_LAST, ptr(s["uniforms"]), ptr(s["tokens"]), ptr(s["probs"]), ws))
         return {"tokens": s["tokens"], "probs": s["probs"]}
     if case["kind"] == "copy":
         check(lib.jsgrad_hip_paged_copy(s["host_pools"], len(s["host_pools"]), case["pool"], ptr(s["moves"]), case["moves"]))
