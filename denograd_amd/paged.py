@@ -90,13 +90,16 @@ class PageTable:
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
             raise ValueError(f"sequences {seqs} with {counts} new positions: one count of 0 and more for each, no sequence twice")
         need = [-(-(self.lengths[s] + c) // self.page_size) - len(self.pages[s]) for s, c in zip(seqs, counts)]
-        holders, own = {}, []                                 # the last holder that is left writes into the page itself
-        for s, c in zip(seqs, counts):
-            last = self.pages[s][self.lengths[s] // self.page_size] if c and self.lengths[s] % self.page_size else -1
-            n = holders.get(last, self.shared.get(last, 1))
-            own.append(last if last >= 0 and n > 1 else -1)
-            if own[-1] >= 0:
-                holders[last] = n - 1
+        # Holders of one page who all write: the longest of them into the page itself, behind what the others have there, so that a batch which is taken back leaves every one's rows.
+        writers: dict[int, list[int]] = {}
+        for i, (s, c) in enumerate(zip(seqs, counts)):
+            if c and self.lengths[s] % self.page_size:
+                writers.setdefault(self.pages[s][self.lengths[s] // self.page_size], []).append(i)
+        own = [-1] * len(seqs)
+        for page, held_by in writers.items():
+            stays = max(held_by, key=lambda i: (self.lengths[seqs[i]], i)) if len(held_by) == self.shared.get(page, 1) else -1
+            for i in held_by:
+                own[i] = page if i != stays else -1
         wanted = sum(need) + sum(p >= 0 for p in own)
         if wanted > len(self.free):
             raise MemoryError(f"{wanted} pages are needed and {len(self.free)} of {self.n_pages} are free")
