@@ -141,13 +141,21 @@ class Llama3:
         """A model of a synthetic configuration (denograd_amd/synthetic.py).  Greedy unless told otherwise: the parity and
         benchmark runs compare argmax tokens; the constructor itself defaults to the reference's temperature 0.95 (llama3.ts:192)."""
         args = {k: cfg[k] for k in ("dim", "hidden_dim", "n_heads", "n_kv_heads", "n_layers", "norm_eps", "rope_theta", "vocab_size")}
-        args["qk_norm"] = cfg.get("qk_norm", False)
+        args["qk_norm"] = cfg.get("qk_norm")
         q = cfg["quantize"] if cfg["quantize"] in ("int8", "nf4") else None
         return Llama3(quantize=q, device=device, max_context=cfg["max_context"], temperature=temperature, args=args, fused_step=fused_step)
 
     def load_weights(self, weights: dict, quantized: bool = False) -> "Llama3":
         """llama3.ts:233-255: `weights` holds unquantised Meta-style tensors (host arrays or device Tensors) unless
-        `quantized` says the codes and scales are already there; quantise per self.quantize, then load."""
+        `quantized` says the codes and scales are already there; quantise per self.quantize, then load.  Norms of queries and keys per head belong to a model whose args have
+        qk_norm=True; with qk_norm=False weights that have them are loaded without."""
+        norms = {k for k in weights if k.endswith((".attention.q_norm.weight", ".attention.k_norm.weight"))}
+        if norms and self.params.get("qk_norm") is None:
+            raise KeyError(f"{min(norms)}: the weights have norms of queries and keys per head, and the model's args say nothing of them (qk_norm=True: with them, False: without)")
+        if self.params.get("qk_norm"):
+            missing = {f"layers.{l}.attention.{x}_norm.weight" for l in range(self.params["n_layers"]) for x in "qk"} - norms
+            if missing:
+                raise KeyError(f"{min(missing)} missing from the weights of a model with qk_norm=True")
         dev = {k: (v if isinstance(v, Tensor) else Tensor(np.ascontiguousarray(v), device=self.device)) for k, v in weights.items()}
         if not quantized:
             if self.quantize == "int8":
