@@ -417,7 +417,8 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
           const int at = (HEADS ? 0 : h * (16 >> a.heads_log)) + ((4 * lq + e) >> a.heads_log);
           if ((e & (hp - 1)) != 0 || at >= n_rows || i >= n) continue;
           const int last = p0 + at < 0 ? -1 : (p0 + at) >> shift;
-          uint32_t key = min(score_key(scale[u] < INFINITY ? v[e] * scale[u] : INFINITY), KEY_ALWAYS - 1);
+          // in units 2^-15 as large: 2^21 times the largest, 2^122, is a float then, and a whole number of the smallest, 2^-126, still one (below the normal ones)
+          uint32_t key = min(score_key(scale[u] < INFINITY ? v[e] * (scale[u] * 0x1p-15f) : INFINITY), KEY_ALWAYS - 1);
           if (i < a.first || i > last - a.recent) key = KEY_ALWAYS;
           if (!held[u] || i > last) key = 0;
           keys[at * a.stride + i] = key;

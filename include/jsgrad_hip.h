@@ -330,7 +330,7 @@ int jsgrad_hip_attn_paged(const jsgrad_hip_pages_t *host_pages, const int32_t *r
 int jsgrad_hip_paged_bounds(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, int8_t *bounds, float *bound_scales);
 /* _paged_select: selected int32 [rows][n_kv_heads][top], the pages (columns of the page table) of the row at position p, rising, -1 behind the last: those among the first `first` and the last `recent` of the columns
  * [0, p / page_size] that have a page, and of the others with one the best, up to `top` in all.  A page's score: with the row's query heads of the kv head as whole numbers c = rint(q / 2^e), 2^e as the scale above
- * of their largest |q|, scale * max over these heads of sum_d c_d * bounds[c_d > 0][d], which no key of the page exceeds; infinity where the scale is.  It is exact, equal ones go to the lower page.  Queries that are not all finite
+ * of their largest |q|, scale * max over these heads of sum_d c_d * bounds[c_d > 0][d], which no key of the page exceeds; infinity where the scale is.  It is exact for scales as _paged_bounds makes them, 2^-126 to 2^122; equal ones go to the lower page.  Queries that are not all finite
  * count as zeros.  Rows behind row_starts[n_seqs] are left as they are; rows at positions below 0 choose none.  top: 1 to 1024, first 0 and more, recent 1 and more, both together no more than top; at most 64 query
  * heads to a kv head, and 32768 columns. */
 int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t *row_starts, const int32_t *lengths, int n_seqs, int rows, const void *q, int n_heads,
