@@ -142,8 +142,10 @@ template <int HD, bool I8> __global__ __launch_bounds__(PS_THREADS) void paged_b
   const float step = bad ? INFINITY : bound_step(most);      // of a page with a key that is not finite: no bound
   if (threadIdx.x < HD) {
     int8_t *const to = a.bounds + ((size_t)id * KV + g) * 2 * HD + d;
-    to[0] = bad ? 0 : (int8_t)(int)floorf(__fdiv_rn(l, step));
-    to[HD] = bad ? 0 : (int8_t)(int)ceilf(__fdiv_rn(h, step));
+    // outwards also where the quotient is nothing that a float holds
+    const float lower = floorf(__fdiv_rn(l, step)), upper = ceilf(__fdiv_rn(h, step));
+    to[0] = bad ? 0 : (int8_t)(int)(l < 0.0f ? fminf(lower, -1.0f) : lower);
+    to[HD] = bad ? 0 : (int8_t)(int)(h > 0.0f ? fmaxf(upper, 1.0f) : upper);
     if (d == 0) a.bound_scales[(size_t)id * KV + g] = step;
   }
 }

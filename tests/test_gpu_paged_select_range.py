@@ -46,3 +46,20 @@ def test_from_keys_to_choices(hip, hd):
     q = rng.standard_normal((300, 8, hd)).astype(np.float16)
     sel = run_choose(hip, c, q, 8, *got, 1, 1, 5)
     assert np.array_equal(sel, ref.choose(c, q, 8, *want, 1, 1, 5, np.full(sel.shape, 77, np.int32)))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_keys_far_apart_on_one_page(hip, hd):
+    """A key that is less than the last bit of a float in the page's unit is rounded outwards all the same: to -1 below zero, to 1 above it."""
+    rng = np.random.default_rng(hd + 1)
+    c = Case(rng, "int8", hd, 2, 16, [160], [160])
+    c.sk = (2.0 ** rng.integers(-149, 119, c.sk.shape)).astype(np.float32)
+    c.sk[c.table[0, 0], :, 0], c.sk[c.table[0, 0], :, 1:] = 2.0 ** 100, 2.0 ** -140
+    c.ck[c.table[0, 0], :, 0, 0], c.ck[c.table[0, 0], :, 1:, 1], c.ck[c.table[0, 0], :, 1:, 2] = 64, 3, -3
+    c.ck[c.table[0, 0], :, 0, 1:] = 0
+    c.device()
+    none = np.zeros((c.n_pages, 2, 2, hd), np.int8), np.ones((c.n_pages, 2), np.float32)
+    got, want = run_bounds(hip, c, *none), ref.bounds(c, *none)
+    at = c.table[0, 0]
+    assert want[0][at, 0, :, 1].tolist() == [0, 1] and want[0][at, 0, :, 2].tolist() == [-1, 0] and want[1][at, 0] == 2.0 ** 100
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
