@@ -69,7 +69,7 @@ class PageTable:
         del self.lengths[seq]
 
     def fork(self, seq: int, at: int | None = None) -> int:
-        """A new sequence that begins with the first `at` positions of this one (default: all), in the same pages."""
+        """A new sequence that begins with the first `at` positions of this one (default: all), in the same pages; those that were given away behind a window it does not have either."""
         at = self.lengths[seq] if at is None else int(at)
         if not 0 <= at <= self.lengths[seq]:
             raise ValueError(f"a fork at position {at} of a sequence of {self.lengths[seq]}")
@@ -245,7 +245,7 @@ class PagedCache(PageTable):
         if self._plan is None or self._plan.numel < plan.size:
             self._plan = Tensor.empty((2 * plan.size,), "int32", self.device)
         self._plan.lazydata.view(plan.size, "int32", 0).ensure_allocated().copyin(plan)
-        return PagedBatch(self, n, int(plan[n]), width, held)
+        return PagedBatch(self, n, int(plan[n]), width, held, counts)
 
     def workspace(self, n_heads: int, chosen: bool = False) -> Tensor:
         key = -n_heads if chosen else n_heads
@@ -258,8 +258,10 @@ class PagedCache(PageTable):
 class PagedBatch:
     """The rows of one ragged batch, in the order of its sequences: row i of a sequence is its position length - count + i."""
 
-    def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int, held: list[tuple[int, list[int], int]]):
+    def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int, held: list[tuple[int, list[int], int]], counts: list[int]):
         self.cache, self.n_seqs, self.rows, self.width, self._held = cache, n_seqs, rows, width, held
+        # what pages behind a window were given away of the sequences that have new rows: seldom any
+        self._gaps = [(s, pages, length) for (s, pages, length), n in zip(held, counts) if n and -1 in pages]
         self._number = cache._batches
         self._layers: dict[int, tuple] = {}                   # what the calls on a layer take
 
@@ -286,6 +288,14 @@ class PagedBatch:
     def _check(self, what: str, t: Tensor, heads: int) -> None:
         if t.dtype != "float16" or prod(t.shape) < self.rows * heads * self.cache.head_dim:
             raise ValueError(f"{what}: {self.rows} float16 rows of {heads} heads of {self.cache.head_dim} are wanted, got {t.dtype} {t.shape}")
+
+    def _check_seen(self, window: int, sinks: int) -> None:
+        """Raises where a row's window reaches positions that were given away, as those of a fork behind the window of the sequence it comes from: they would be left out in silence."""
+        size = self.cache.page_size
+        for s, pages, length in self._gaps:
+            seen = pages[max(0, length - window + 1) // size if window else 0:] + (pages[:-(-min(sinks, length) // size)] if window else [])
+            if -1 in seen:
+                raise ValueError(f"sequence {s} has given away pages that its row at position {length} sees with window {window} and sinks {sinks}")
 
     def write(self, layer: int, k: Tensor, v: Tensor, q: Tensor | None = None, freqs_cis: Tensor | None = None, n_heads: int = 0, q_out: Tensor | None = None,
               q_norm: "RMSNorm | None" = None, k_norm: "RMSNorm | None" = None) -> Tensor | None:
@@ -325,8 +335,9 @@ class PagedBatch:
 
     def attend(self, layer: int, q: Tensor, n_heads: int, out: Tensor | None = None, window: int = 0, sinks: int = 0) -> Tensor:
         """Attention of q [rows, n_heads, head_dim] over the pages: everything up to a row's own position or, with window > 0, the last
-        `window` positions of that and the first `sinks`."""
+        `window` positions of that and the first `sinks`; these have to be there still (PageTable.slide)."""
         self._check("q", q, n_heads)
+        self._check_seen(window, sinks)
         out = out if out is not None else Tensor.empty((self.rows, n_heads, self.cache.head_dim), "float16", self.cache.device)
         self._check("out", out, n_heads)
         check(ffi.load().jsgrad_hip_attn_paged(*self._args(layer), q.ptr, out.ptr, n_heads, window, sinks, self.cache.workspace(n_heads).ptr))

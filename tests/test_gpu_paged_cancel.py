@@ -36,3 +36,23 @@ def test_rows_of_forks_behind_a_step_that_failed(hip, dtype, order):
         m.forward_paged(cache, seqs, more[:, :1] + 1)
         after.append(logits(m, 3))
     assert np.array_equal(*after)
+
+
+def test_a_fork_behind_a_window(hip):
+    """What its next row would see was given away: refused, with the sequences as they were; a fork that has it goes on as the sequence does."""
+    cfg, llm = model()
+    m, rng = llm.model, np.random.default_rng(9)
+    cache = cache_for(llm, 16)
+    a = cache.add()
+    m.forward_paged(cache, [a], [rng.integers(0, cfg["vocab_size"], 160).astype(np.int32)], 40)
+    cache.slide(a, 40)
+    back, beside = cache.fork(a, 80), cache.fork(a, 160)
+    before = {s: list(p) for s, p in cache.pages.items()}, dict(cache.lengths), list(cache.free)
+    for seqs, window in (([back], 40), ([a, back], 40), ([a], 60), ([a], 0)):
+        with pytest.raises(ValueError, match="given away"):
+            m.forward_paged(cache, seqs, [np.array([1])] * len(seqs), window)
+        assert before == (cache.pages, cache.lengths, cache.free)
+    m.forward_paged(cache, [a], [np.array([1])], 40)
+    want = logits(m, 1)
+    m.forward_paged(cache, [beside], [np.array([1])], 40)
+    assert np.array_equal(want, logits(m, 1))
