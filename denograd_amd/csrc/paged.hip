@@ -391,7 +391,7 @@ int jsgrad_hip_paged_copy(const jsgrad_hip_pool_t *host_pools, int n_pools, int 
     a.parts = (int)((most + COPY_BYTES - 1) / COPY_BYTES);
     for (int m0 = 0; m0 < n_moves; m0 += COPY_MOVES) {
       a.moves = moves + (size_t)m0 * 3;
-      // 2^16 parts of a page and COPY_POOLS are 2^23 blocks along x
+      // pages below 2^30 bytes have up to 2^15 parts: with COPY_POOLS 2^22 blocks along x
       JSG_LAUNCH(PROF_PAGED_ROWS, paged_copy_kernel, dim3((unsigned)(a.parts * n), (unsigned)(n_moves - m0 < COPY_MOVES ? n_moves - m0 : COPY_MOVES)), dim3(PR_THREADS), 0, a);
     }
   }

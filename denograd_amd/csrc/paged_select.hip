@@ -4,6 +4,8 @@
 // No key of a page scores more with a query than sum_d q_d (q_d > 0 ? hi_d : lo_d), lo and hi being the least and the largest of each feature.  Both are kept as whole numbers, rounded outwards, times one power of
 // two per page and head; a row's queries are rounded to whole numbers times one power of two as well.  So scores are whole numbers below 2^21 times a power of two, exact however they are summed, and
 // which pages are chosen is a question of the inputs alone: with float sums two scores that are nearly the same would fall either way.
+//
+// Figures: us a call, 300 of them with the same inputs one after another, unless they are said to be a profiler's.
 #include <type_traits>
 
 #include "paged_device.h"
@@ -79,7 +81,7 @@ __device__ __forceinline__ int find_touched(const PagedBatch &pb, uint32_t t, Pa
 }
 
 // Block = (page that the batch's rows are on, kv head): the whole page is looked at, so bounds do not depend on how its rows came.  Bound by memory: HD / 8 lanes a row, 16 bytes (int8: 8) each.
-// One row behind 33000 positions takes 4.5 us, 16 of 16 sequences 4.5, most of it a launch; 2048 rows on 32 pages 5.4.  (A block for every row, most of which have nothing to do: 27.)
+// One row behind 33000 positions takes 4.5 us, 16 of 16 sequences 4.5, most of it a launch; 2048 rows on 32 pages 5.1.  (A block for every row, most of which have nothing to do: 27.)
 template <int HD, bool I8> __global__ __launch_bounds__(PS_THREADS) void paged_bounds_kernel(PagedSelectArgs a) {
   constexpr int G = HD / 8, RPB = PS_THREADS / G;
   __shared__ float lo_sh[PS_THREADS / 64][HD], hi_sh[PS_THREADS / 64][HD];
@@ -290,9 +292,10 @@ template <int NW> struct KeyChoice {
 };
 
 // Block = some rows of a sequence, side by side, and a kv head.  Scores on the matrix cores: 16 pages' bounds against 16 columns of queries, the heads of a row next to each other, so that a lane has
-// four columns' scores of its page.  Few rows are bound by what waits for what: batch, page numbers, bounds, then the turns of the choice; many by the vector unit, which makes keys of scores and counts them.
-// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 8.9; 16 rows of up to 32768, pages of 32: 12; 2048 rows behind 14336, heads of 64: 31.  (A page to a thread with dot products and 32 turns
-// through LDS: 22, 30 and 138.)
+// four columns' scores of its page.  Few rows are bound by what waits for what: batch, page numbers, bounds, then the turns of the choice.  Of many, the vector unit, which makes keys of scores and counts them, has half
+// of the time (11.0 M instructions, 43 of 87 thousand cycles of each), and wavefronts wait for 44 % of theirs.
+// us, one row of 33000 positions, pages of 64, 32 heads of 128 over 8: 8.4; 16 rows of up to 32768, pages of 32: 11; 2048 rows behind 14336, heads of 64: 26.  (A page to a thread with dot products and 32 turns
+// through LDS, by the profiler: 22, 30 and 138, where these take 9, 12 and 30.)
 // HT tiles of 16 columns: of more heads of the rows (HEADS), or of more rows, for which the bounds are loaded once.
 template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 64, 2) void paged_select_kernel(PagedSelectArgs a) {
   extern __shared__ __align__(16) uint32_t keys[];           // [rows of a block][stride]
@@ -372,7 +375,7 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
     }
     for (int t0 = wave; t0 * 16 < n; t0 += U * NW) {
       // As they lie, neighbouring lanes on one page, and through LDS into the operand, whose lanes of a quarter are on different pages: straight from there, L1 is asked 64 times for what it gives in 16
-      // (2048 rows behind 14336, heads of 64, 31 us instead of 27, 512 of 128 17 instead of 14).
+      // (2048 rows behind 14336, heads of 64, 30.7 us instead of 26.4, one row of 33000 9.7 instead of 8.4 together with the four more wavefronts that it has).
       i4v box[U][KS];
       float scale[U];
       bool held[U];
@@ -444,11 +447,11 @@ template <int HD, int NW, int HT, bool HEADS> __global__ __launch_bounds__(NW * 
 // Block = 4 wavefronts.  Where there are few rows, one row, up to 16 of its query heads of a kv head (usually four), and a part of its chosen pages, each wavefront with steps of its own; else (SOLO) four
 // rows, a wavefront to each, which neither wait for one another nor start anew every few steps.  A step is 64 keys: rows of K and V
 // come through registers into the wavefront's own LDS, 32 at a time, V's for the transposing reads; the next step's rows are asked for as soon as the registers are free.  K straight to registers, as the
-// matrix operand has it, would put the lanes of a quarter on different rows, and the L1 cache would be asked 64 times for what it gives in 16: 2048 rows, heads of 64, 305 us.
+// matrix operand has it, would put the lanes of a quarter on different rows, and the L1 cache would be asked 64 times for what it gives in 16: 2048 rows, heads of 64, 305 us by the profiler.
 //
-// us, 32 heads over 8: one row, 32 pages of 64, heads of 128, 9.6, of which 4 go by until the first keys are there and 4 in the join of the parts; 16 rows, 64 int8 pages of 32, heads of 128, 21: memory, 4 TB/s and start
-// and join; 2048 rows, 16 pages of 64, heads of 64, 195: every row gathers 2 MB of its own, 4.3 GB in all, at 64 % of what L1 gives and as much of LDS's rate (each byte goes in once and out once), 20 TB/s of it
-// from L2, with the vector unit at 32 %.
+// us, 32 heads over 8: one row, 32 pages of 64, heads of 128, 9.8, of which 4 go by until the first keys are there and 4 in the join of the parts; 16 rows, 64 int8 pages of 32, heads of 128, 21: memory, 4 TB/s and start
+// and join; 2048 rows, 16 pages of 64, heads of 64, 168 (the profiler says 195): every row gathers 2 MB of its own, 4.3 GB in all, in the profile at 64 % of what L1 gives and as much of LDS's rate (each byte goes in
+// once and out once), 20 TB/s of it from L2, with the vector unit at 32 %.
 //
 // A matrix instruction scores 16 keys for 16 columns, and a row has few heads: with four, three columns of four would score the same again, and the vector unit would make the exponentials of
 // all.  So the columns are heads times groups of keys: column c of what a lane keeps has head c % HP over the keys of group c / HP of the step's four, each picked from that group's scores
@@ -986,8 +989,8 @@ int jsgrad_hip_paged_select(const jsgrad_hip_pages_t *host_pages, const int32_t 
   const bool four = HD == 128 && !many && (size_t)rows >= (size_t)8 * tile * n_seqs && (size_t)rows * a.n_kv_heads >= (size_t)tile * 2048 && (size_t)tile * 4 * a.stride * 4 <= 64 * 1024;
   a.tile = rows > n_seqs && (size_t)tile * a.stride * 4 <= 64 * 1024 ? tile * (four ? 4 : 1) : 1;
   const dim3 grid((unsigned)((rows + a.tile - 1) / a.tile), (unsigned)a.n_kv_heads);
-  // Eight wavefronts where a unit has no more than one block.  us, four | eight: one row behind 33000 positions, pages of 64, 9.4 | 8.1, of 16 25 | 17; 16 rows of up to 32768, pages of 32, 13.3 | 10.8; 64 rows of
-  // 64 sequences of 8192 7.6 | 9.9; 128 rows behind 16256 (256 blocks) 7.0 | 6.5, 512 14.4 | 15.
+  // Eight wavefronts where a unit has no more than one block.  us, four | eight: one row behind 33000 positions, pages of 64, 9.6 | 8.4, of 16 24 | 17.5; 16 rows of up to 32768, pages of 32, 13.2 | 11.3; 128
+  // rows behind 16256 (256 blocks) 7.2 | 7.1; with more blocks, 64 rows of 64 sequences of 8192 7.6 | 9.9, 512 behind 15872 14.4 | 15.
   const size_t lds = (size_t)a.tile * a.stride * 4;
   const bool wide = !many && !four && (size_t)grid.x * grid.y <= 256 && lds <= 64 * 1024;   // the tiles of eight have 34 KB of LDS
 #define JSG_SELECT(HD, NW, HT, HEADS)                                                                                                                                        \

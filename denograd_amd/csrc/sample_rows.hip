@@ -10,7 +10,7 @@
 //
 // Three launches, as the maximum has to be known before a weight is, and masses before a border: maxima of parts of the rows; per part the candidates of the first top_k (k up to SR_FEW), or its mass by steps
 // of an eighth of an octave below the maximum; one block a row for what lies on the step with a border.  One row of 128256 halves 18 us: 3.6, 6.3 and 8.5, launches and trips that wait for each other.  Sixteen
-// rows with settings of their own 44, of which 32 are the last block of a row with top_k = 1000 and top_p: 8 to get the row from beyond the unit's L2 and look it over, 5 for the parts' sums, 3 for the draw
+// rows with settings of their own 43 (44 with min-p last), of which 32 are the last block of a row with top_k = 1000 and top_p: 8 to get the row from beyond the unit's L2 and look it over, 5 for the parts' sums, 3 for the draw
 // (52 with a look for each of the two borders).  256 rows with top_p = 0.95 (66 MB) 83: 14 (4.7 TB/s), 39 (33 million weights in 64 bits; histograms in several copies change nothing) and 34.
 #include <type_traits>
 
