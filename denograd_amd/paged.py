@@ -32,6 +32,7 @@ class PageTable:
         self.pages: dict[int, list[int]] = {}                 # per sequence; -1: given away behind the window
         self.lengths: dict[int, int] = {}
         self.shared: dict[int, int] = {}                      # pages with more than one holder: how many
+        self.gaps: set[int] = set()                           # sequences with pages that were given away
         self._next = 0
 
     @staticmethod
@@ -67,6 +68,7 @@ class PageTable:
         """The sequence is over; pages that no other one holds are free."""
         self._let_go(reversed(self.pages.pop(seq)))
         del self.lengths[seq]
+        self.gaps.discard(seq)
 
     def fork(self, seq: int, at: int | None = None) -> int:
         """A new sequence that begins with the first `at` positions of this one (default: all), in the same pages; those that were given away behind a window it does not have either."""
@@ -78,6 +80,8 @@ class PageTable:
             raise ValueError(f"a fork at position {at}, in a page that was given away")
         new = self.add()
         self.pages[new], self.lengths[new] = list(pages), at
+        if seq in self.gaps:
+            self.gaps.add(new)
         for p in pages:
             if p >= 0:
                 self.shared[p] = self.shared.get(p, 1) + 1
@@ -145,6 +149,8 @@ class PageTable:
             if pages[i] >= 0:
                 self._let_go([pages[i]])
                 pages[i], n = -1, n + 1
+        if n:
+            self.gaps.add(seq)
         return n
 
     def _pack(self) -> list[tuple[int, int, int]]:
@@ -260,8 +266,8 @@ class PagedBatch:
 
     def __init__(self, cache: PagedCache, n_seqs: int, rows: int, width: int, held: list[tuple[int, list[int], int]], counts: list[int]):
         self.cache, self.n_seqs, self.rows, self.width, self._held = cache, n_seqs, rows, width, held
-        # what pages behind a window were given away of the sequences that have new rows: seldom any
-        self._gaps = [(s, pages, length) for (s, pages, length), n in zip(held, counts) if n and -1 in pages]
+        self._gaps = [h for h, n in zip(held, counts) if n and h[0] in cache.gaps]     # what _check_seen looks at
+        self._seen: set[tuple[int, int]] = set()              # windows and sinks that it has looked at
         self._number = cache._batches
         self._layers: dict[int, tuple] = {}                   # what the calls on a layer take
 
@@ -291,11 +297,14 @@ class PagedBatch:
 
     def _check_seen(self, window: int, sinks: int) -> None:
         """Raises where a row's window reaches positions that were given away, as those of a fork behind the window of the sequence it comes from: they would be left out in silence."""
+        if (window, sinks) in self._seen:
+            return
         size = self.cache.page_size
         for s, pages, length in self._gaps:
             seen = pages[max(0, length - window + 1) // size if window else 0:] + (pages[:-(-min(sinks, length) // size)] if window else [])
             if -1 in seen:
                 raise ValueError(f"sequence {s} has given away pages that its row at position {length} sees with window {window} and sinks {sinks}")
+        self._seen.add((window, sinks))
 
     def write(self, layer: int, k: Tensor, v: Tensor, q: Tensor | None = None, freqs_cis: Tensor | None = None, n_heads: int = 0, q_out: Tensor | None = None,
               q_norm: "RMSNorm | None" = None, k_norm: "RMSNorm | None" = None) -> Tensor | None:
