@@ -10,7 +10,7 @@
 //
 // Three launches, as the maximum has to be known before a weight is, and masses before a border: maxima of parts of the rows; per part the candidates of the first top_k (k up to SR_FEW), or its mass by steps
 // of an eighth of an octave below the maximum; one block a row for what lies on the step with a border.  One row of 128256 halves 18 us: 3.6, 6.3 and 8.5, launches and trips that wait for each other.  Sixteen
-// rows with settings of their own 43 (44 with min-p last), of which 32 are the last block of a row with top_k = 1000 and top_p: 8 to get the row from beyond the unit's L2 and look it over, 5 for the parts' sums, 3 for the draw
+// rows with settings of their own 38 to 42, by inputs, of which up to 32 are the last block of a row with top_k = 1000 and top_p: 8 to get the row from beyond the unit's L2 and look it over, 5 for the parts' sums, 3 for the draw
 // (52 with a look for each of the two borders).  256 rows with top_p = 0.95 (66 MB) 83: 14 (4.7 TB/s), 39 (33 million weights in 64 bits; histograms in several copies change nothing) and 34.
 #include <type_traits>
 
@@ -735,6 +735,7 @@ template <typename AT, bool VEC> struct SampleLast {
     SampleCut cut = {0, 0x7fffffff};
     int step = SR_STEPS;                                     // kept whole: the steps before this one
     uint64_t z = 0, extra = 0;                               // mass that is kept, and how much of it is on `step`
+    const int late = row.late ? row.late_step() : SR_STEPS;  // a last border that is further down is not looked for: nothing of its step is left
     if (row.way == SAMPLE_STEPS) {
       for (int s = tid; s < SR_STEPS_UP; s += SR_THREADS) { l.mass[s] = 0; l.count[s] = 0; }
       list_lo = 1;
@@ -779,7 +780,9 @@ template <typename AT, bool VEC> struct SampleLast {
         const int s = reach(l.count, (uint64_t)row.top_k, before);
         if (s < SR_STEPS && before + l.count[s] > (uint64_t)row.top_k) {
           // all that the first top_k are among, where it fits: a border by top_p is there too
-          if (!border<false>(s, row.top_p < 1.0f && before + l.count[s] <= SR_ROOM ? 0 : s, (uint64_t)row.top_k - before, cut, cut, extra)) return false;
+          if ((row.top_p < 1.0f || s <= late) &&
+              !border<false>(s, row.top_p < 1.0f && before + l.count[s] <= SR_ROOM ? 0 : s, (uint64_t)row.top_k - before, cut, cut, extra))
+            return false;
           step = s;
         } else if (s < SR_STEPS) {
           step = s + 1;
@@ -796,7 +799,7 @@ template <typename AT, bool VEC> struct SampleLast {
         const uint64_t target = max(sample_share(__float_as_uint(row.top_p), z, true), (uint64_t)1);
         const int s = reach(l.mass, target, before);
         if (before + l.mass[s] > target) {
-          if (!border<true>(s, s, target - before, s == step ? cut : SampleCut{0, 0x7fffffff}, cut, extra)) return false;
+          if (s <= late && !border<true>(s, s, target - before, s == step ? cut : SampleCut{0, 0x7fffffff}, cut, extra)) return false;
           step = s;
         } else if (s != step) {                              // the whole step, which is none that a cut went through
           step = s + 1;
@@ -804,13 +807,12 @@ template <typename AT, bool VEC> struct SampleLast {
           extra = 0;
         }
       }
-      if (row.late)
-        if (const int s = row.late_step(); s < step) {         // steps above this one are kept whole, of those below nothing is; it is looked for once, so not listed
-          step = s;
-          cut = SampleCut{0, 0x7fffffff};
-          extra = 1;
-          fits = false;
-        }
+      if (late < step) {                                     // steps above this one are kept whole, of those below nothing is
+        if (late < list_lo || late > list_hi) fits = false;    // looked for once, so not listed
+        step = late;
+        cut = SampleCut{0, 0x7fffffff};
+        extra = 1;
+      }
       // what of every part is kept: whole steps, sixteen threads to a part, then those of the step with the cut
       for (int p = tid / 16; p < a.parts; p += SR_THREADS / 16) {
         uint64_t m = 0;
